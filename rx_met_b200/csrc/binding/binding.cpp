@@ -20,6 +20,7 @@
 
 #include "rxmet_b200.h"
 #include "rxmet_b200_lstm.h"
+#include "rxmet_b200_mixer.h"
 
 namespace {
 
@@ -341,7 +342,7 @@ std::pair<int, std::vector<Tensor>> lstmBackwardQat(const std::vector<Tensor> &m
 
 // ---- learned-grid quantize-dequantize -----------------------------------------------------------------------------
 
-void checkQdq(int status, const char *what) {
+void checkStatus(int status, const char *what) {
     if (status == RXMET_OK) return;
     const std::string message = std::string(what) + ": " + rxmet_last_error();
     if (status == RXMET_ERR_INVALID_ARGUMENT) throw pybind11::value_error(message);
@@ -357,7 +358,7 @@ struct QuantDequant : torch::autograd::Function<QuantDequant> {
         const c10::cuda::CUDAGuard guard(tensor.device());   // launch on the tensor's device, whatever device is current
         const Tensor x = tensor.contiguous(), s = gridValues(scale), o = gridValues(offset);
         Tensor y = at::empty_like(x);
-        checkQdq(rxmet_affine_qdq_forward(x.const_data_ptr<float>(), outer, channels, inner, s.const_data_ptr<float>(),
+        checkStatus(rxmet_affine_qdq_forward(x.const_data_ptr<float>(), outer, channels, inner, s.const_data_ptr<float>(),
                                           o.const_data_ptr<float>(), static_cast<int>(qmin), static_cast<int>(qmax), reciprocal,
                                           y.mutable_data_ptr<float>(), nullptr, streamOf(x)),
                  "affine_qdq.forward");
@@ -386,7 +387,7 @@ struct QuantDequant : torch::autograd::Function<QuantDequant> {
             if (bytes > 0) ws = emptyLike(x, {static_cast<int64_t>(bytes)}, at::kByte);
         }
         auto raw = [](const Tensor &t) { return t.defined() ? static_cast<float *>(t.data_ptr()) : nullptr; };
-        checkQdq(rxmet_affine_qdq_backward(raw(g), raw(x), outer, channels, inner, raw(s), raw(o), static_cast<int>(plan[0]),
+        checkStatus(rxmet_affine_qdq_backward(raw(g), raw(x), outer, channels, inner, raw(s), raw(o), static_cast<int>(plan[0]),
                                            static_cast<int>(plan[1]), static_cast<int>(plan[2]), raw(out[0]), raw(out[1]),
                                            raw(out[2]), ws.defined() ? ws.data_ptr() : nullptr, bytes, streamOf(x)),
                  "affine_qdq.backward");
@@ -399,6 +400,291 @@ Tensor quantizeDequantize(const Tensor &tensor, const Tensor &scale, const Tenso
     return QuantDequant::apply(tensor, scale, offset, qmin, qmax, reciprocal, outer, channels, inner);
 }
 
+// ---- token mixer: residual norm, product of codes, linear attention with decays ---------------------------------------------
+
+int typeOf(const Tensor &t, const char *name) {
+    if (t.scalar_type() == at::kFloat) return RXMET_TYPE_F32;
+    if (t.scalar_type() == at::kBFloat16) return RXMET_TYPE_BF16;
+    TORCH_CHECK(t.scalar_type() == at::kHalf, name, " must be a float32, bfloat16 or float16 tensor");
+    return RXMET_TYPE_F16;
+}
+
+void sameDevice(const Tensor &t, const Tensor &like, const char *name) {
+    TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be a CUDA tensor on ", like.device());
+}
+
+// [rows][width] with neighbouring elements, a view where the strides allow one; the distance of its rows.
+Tensor asRows(const Tensor &t) {
+    const Tensor flat = t.reshape({t.numel() / t.size(-1), t.size(-1)});
+    return flat.stride(1) == 1 || flat.size(1) == 1 ? flat : flat.contiguous();
+}
+int64_t pitchOf(const Tensor &rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
+
+// Codes of rows that start on 16 bytes, as the products read them; the padding is not part of the tensor and holds nothing.
+Tensor emptyCodes(const Tensor &like, at::IntArrayRef shape) {
+    const int64_t width = shape.back(), pitch = (width + 15) / 16 * 16;
+    Shape padded = shape.vec();
+    padded.back() = pitch;
+    const Tensor held = emptyLike(like, padded, at::kChar);
+    return pitch == width ? held : held.narrow(-1, 0, width);
+}
+
+struct NormArguments {
+    Tensor x, residual, weight;
+    int type, weightType;
+    int64_t rows, width;
+    NormArguments(const Tensor &input, const MaybeTensor &added, const MaybeTensor &weights, const char *what) {
+        TORCH_CHECK(input.is_cuda() && input.dim() >= 1 && input.size(-1) > 0, what, ": x must be a CUDA tensor with a last dimension");
+        type = typeOf(input, "x");
+        width = input.size(-1);
+        x = asRows(input);
+        rows = x.size(0);
+        if (added) {
+            sameDevice(*added, input, "residual");
+            TORCH_CHECK(added->sizes() == input.sizes() && added->scalar_type() == input.scalar_type(), what,
+                        ": residual must have the shape and type of x");
+            residual = asRows(*added);
+        }
+        weightType = type;
+        if (weights) {
+            sameDevice(*weights, input, "weight");
+            weightType = typeOf(*weights, "weight");
+            TORCH_CHECK(weights->dim() == 1 && weights->size(0) == width, what, ": weight must have shape [", width, "]");
+            weight = weights->contiguous();
+        }
+    }
+};
+
+const void *dataOf(const Tensor &t) { return t.defined() && t.numel() > 0 ? t.const_data_ptr() : nullptr; }
+void *mutableOf(const Tensor &t) { return t.defined() && t.numel() > 0 ? t.mutable_data_ptr() : nullptr; }
+
+// The outputs are y and, with a residual, total.
+struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &weight,
+                                                  const MaybeTensor &residual, double eps) {
+        const NormArguments a(x, residual, weight, "add_rms_norm");
+        const c10::cuda::CUDAGuard guard(x.device());
+        Tensor y = emptyLike(x, x.sizes(), x.scalar_type()), total;
+        if (residual) total = emptyLike(x, x.sizes(), x.scalar_type());
+        const Tensor rms = emptyLike(x, {a.rows});
+        checkStatus(rxmet_add_rms_norm(a.rows, static_cast<int>(a.width), a.type, dataOf(a.x), pitchOf(a.x), dataOf(a.residual),
+                                       residual ? pitchOf(a.residual) : 0, dataOf(a.weight), a.weightType, static_cast<float>(eps),
+                                       mutableOf(total), mutableOf(y), pointer<float>(rms), streamOf(x)),
+                    "add_rms_norm");
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({x, rms, weight, residual ? *residual : Tensor()});
+        if (residual) return {y, total};
+        return {y};
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        torch::autograd::variable_list out(4);
+        const at::NoGradGuard noGrad;
+        const Tensor given = saved[0], rms = saved[1], weight = saved[2].contiguous();
+        const c10::cuda::CUDAGuard guard(given.device());
+        const Tensor dtotal = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : Tensor();
+        if (!grads[0].defined()) {
+            if (dtotal.defined()) out[0] = out[2] = dtotal;
+            return out;
+        }
+        const Tensor dy = grads[0].contiguous(), x = asRows(given), residual = saved[3].defined() ? asRows(saved[3]) : Tensor();
+        const int type = typeOf(given, "x"), weightType = typeOf(weight, "weight"), width = static_cast<int>(given.size(-1));
+        const Tensor dx = emptyLike(given, given.sizes(), given.scalar_type());
+        Tensor ws;
+        size_t bytes = 0;
+        if (ctx->needs_input_grad(1)) {
+            out[1] = emptyLike(given, {width}, weight.scalar_type());
+            bytes = rxmet_add_rms_norm_backward_workspace_bytes(x.size(0), width, type);
+            ws = emptyLike(given, {static_cast<int64_t>(bytes)}, at::kByte);
+        }
+        checkStatus(rxmet_add_rms_norm_backward(x.size(0), width, type, dataOf(dy), dataOf(dtotal), dataOf(x), pitchOf(x), dataOf(residual),
+                                                residual.defined() ? pitchOf(residual) : 0, pointer<float>(rms),
+                                                dataOf(weight), weightType, mutableOf(dx), mutableOf(out[1]), mutableOf(ws), bytes, streamOf(given)),
+                    "add_rms_norm backward");
+        out[0] = dx;
+        if (ctx->needs_input_grad(2)) out[2] = dx;
+        return out;
+    }
+};
+
+std::vector<Tensor> addRmsNorm(const Tensor &x, const Tensor &weight, const MaybeTensor &residual, double eps) {
+    return AddRmsNorm::apply(x, weight, residual, eps);
+}
+
+// Codes, scales and (with a residual) total.
+std::vector<Tensor> addRmsNormCodes(const Tensor &x, const MaybeTensor &weight, const MaybeTensor &residual, double eps) {
+    const NormArguments a(x, residual, weight, "add_rms_norm_codes");
+    const c10::cuda::CUDAGuard guard(x.device());
+    std::vector<Tensor> out{emptyCodes(x, x.sizes()), emptyLike(x, x.sizes().slice(0, x.dim() - 1))};
+    if (residual) out.push_back(emptyLike(x, x.sizes(), x.scalar_type()));
+    checkStatus(rxmet_add_rms_norm_codes(a.rows, static_cast<int>(a.width), a.type, dataOf(a.x), pitchOf(a.x), dataOf(a.residual),
+                                         residual ? pitchOf(a.residual) : 0, dataOf(a.weight), a.weightType, static_cast<float>(eps),
+                                         residual ? mutableOf(out[2]) : nullptr, static_cast<int8_t *>(mutableOf(out[0])), (a.width + 15) / 16 * 16,
+                                         pointer<float>(out[1]), streamOf(x)),
+                "add_rms_norm_codes");
+    return out;
+}
+
+Tensor codedLinear(const Tensor &codes, const Tensor &scale, const Tensor &weight, const Tensor &weightScale, const MaybeTensor &bias,
+                   int activation, const MaybeTensor &residual, int outType) {
+    constexpr at::ScalarType kTypes[] = {at::kFloat, at::kBFloat16, at::kHalf};
+    TORCH_CHECK(outType >= 0 && outType <= 2, "coded_linear: unknown output type");
+    TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kChar && codes.dim() >= 1, "codes must be a CUDA int8 tensor");
+    sameDevice(weight, codes, "weight codes");
+    TORCH_CHECK(weight.scalar_type() == at::kChar && weight.dim() == 2, "weight codes must be an int8 tensor of two dimensions");
+    const int64_t inner = weight.size(1), outer = weight.size(0);
+    TORCH_CHECK(inner > 0 && outer > 0 && codes.size(-1) == inner, "coded_linear: codes of ", codes.size(-1), " elements for a weight of shape ", listText(weight.sizes()));
+    sameDevice(scale, codes, "scale");
+    TORCH_CHECK(scale.scalar_type() == at::kFloat && scale.sizes() == codes.sizes().slice(0, codes.dim() - 1), "scale must be float32 with the shape of codes but its last dimension");
+    sameDevice(weightScale, codes, "weight scale");
+    TORCH_CHECK(weightScale.scalar_type() == at::kFloat && weightScale.dim() == 1 && weightScale.size(0) == outer, "weight scale must be float32 of shape [", outer, "]");
+    Shape shape = codes.sizes().vec();
+    shape.back() = outer;
+    const c10::cuda::CUDAGuard guard(codes.device());
+    const Tensor rows = asRows(codes), weights = asRows(weight), scales = scale.contiguous(), weightScales = weightScale.contiguous();
+    Tensor added, biases;
+    if (bias) {
+        sameDevice(*bias, codes, "bias");
+        TORCH_CHECK(bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == outer, "bias must be float32 of shape [", outer, "]");
+        biases = bias->contiguous();
+    }
+    if (residual) {
+        sameDevice(*residual, codes, "residual");
+        TORCH_CHECK(residual->scalar_type() == kTypes[outType] && residual->sizes() == at::IntArrayRef(shape), "residual must have the type and shape of the output, ", listText(shape));
+        added = asRows(*residual);
+    }
+    const Tensor out = emptyLike(codes, shape, kTypes[outType]);
+    checkStatus(rxmet_coded_linear(rows.size(0), static_cast<int>(inner), static_cast<int>(outer), static_cast<const int8_t *>(dataOf(rows)), pitchOf(rows),
+                                   pointer<float>(scales), static_cast<const int8_t *>(dataOf(weights)), pitchOf(weights), pointer<float>(weightScales),
+                                   pointer<float>(biases), activation, dataOf(added), residual ? pitchOf(added) : 0, outType, mutableOf(out), streamOf(codes)),
+                "coded_linear");
+    return out;
+}
+
+// Arguments of linear attention as the C ABI takes them; tensors of three dimensions are single tokens.
+struct AttentionArguments {
+    Tensor q, k, v, logDecay, lengths, state;
+    rxmet_decayed_attention problem{};
+    Shape stateShape;
+
+    static rxmet_head_tensor view(const Tensor &t) {
+        const bool step = t.dim() == 3;
+        return {dataOf(t), t.stride(0), step ? 0 : t.stride(1), t.stride(step ? 1 : 2), static_cast<int32_t>(t.size(step ? 1 : 2))};
+    }
+    static Tensor rowsOf(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+
+    AttentionArguments(const Tensor &queries, const Tensor &keys, const Tensor &values, const Tensor &decays, const MaybeTensor &start,
+                       const MaybeTensor &counts, double scale, int64_t dims) {
+        TORCH_CHECK(queries.is_cuda() && queries.dim() == dims, "q must be a CUDA tensor of ", dims, " dimensions");
+        problem.type = typeOf(queries, "q");
+        for (const auto &[t, name] : {std::pair<const Tensor &, const char *>{keys, "k"}, {values, "v"}}) {
+            sameDevice(t, queries, name);
+            TORCH_CHECK(t.dim() == dims && t.scalar_type() == queries.scalar_type(), name, " must have the dimensions and type of q");
+            for (int64_t i = 0; i < dims - 2; ++i) TORCH_CHECK(t.size(i) == queries.size(i), name, " must have batch and tokens of q");
+        }
+        TORCH_CHECK(keys.size(-1) == queries.size(-1), "q and k must have heads of one size");
+        sameDevice(decays, queries, "log_decay");
+        TORCH_CHECK(decays.scalar_type() == at::kFloat && decays.dim() == 1 && decays.size(0) > 0, "log_decay must be a float32 tensor of one dimension, the heads");
+        TORCH_CHECK(!decays.requires_grad(), "log_decay is a constant of the layer: it has no gradient");
+        q = rowsOf(queries);
+        k = rowsOf(keys);
+        v = rowsOf(values);
+        logDecay = decays.contiguous();
+        problem.batch = static_cast<int32_t>(q.size(0));
+        problem.tokens = dims == 3 ? 1 : static_cast<int32_t>(q.size(1));
+        problem.heads = static_cast<int32_t>(logDecay.size(0));
+        problem.key_dim = static_cast<int32_t>(q.size(-1));
+        problem.value_dim = static_cast<int32_t>(v.size(-1));
+        stateShape = {problem.batch, problem.heads, problem.key_dim, problem.value_dim};
+        if (start) state = checkedState(*start, "state").contiguous();
+        if (counts) {
+            sameDevice(*counts, queries, "lengths");
+            TORCH_CHECK(counts->dim() == 1 && counts->size(0) == problem.batch && at::isIntegralType(counts->scalar_type(), true), "lengths must be integers of shape [", problem.batch, "]");
+            lengths = counts->to(at::kInt).contiguous();
+        }
+        problem.q = view(q);
+        problem.k = view(k);
+        problem.v = view(v);
+        problem.log_decay = logDecay.const_data_ptr<float>();
+        problem.lengths = lengths.defined() ? lengths.const_data_ptr<int32_t>() : nullptr;
+        problem.scale = static_cast<float>(scale);
+    }
+    const Tensor &checkedState(const Tensor &t, const char *name) const {
+        sameDevice(t, q, name);
+        TORCH_CHECK(t.scalar_type() == at::kFloat && t.sizes() == at::IntArrayRef(stateShape), name, " must be float32 of shape ", listText(stateShape));
+        return t;
+    }
+    Tensor workspaceFor(bool backward, size_t &bytes) const {
+        bytes = rxmet_decayed_attention_workspace_bytes(&problem, backward);
+        return bytes > 0 ? emptyLike(q, {static_cast<int64_t>(bytes)}, at::kByte) : Tensor();
+    }
+    void forward(const Tensor &out, const Tensor &last) const {
+        size_t bytes;
+        const Tensor ws = workspaceFor(false, bytes);
+        checkStatus(rxmet_decayed_attention_forward(&problem, pointer<float>(state), mutableOf(out), pointer<float>(last), mutableOf(ws), bytes, streamOf(q)), "decayed_attention");
+    }
+};
+
+struct DecayedAttention : torch::autograd::Function<DecayedAttention> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &logDecay,
+                                                  const MaybeTensor &state, const MaybeTensor &lengths, double scale) {
+        const AttentionArguments a(q, k, v, logDecay, state, lengths, scale, 4);
+        const c10::cuda::CUDAGuard guard(q.device());
+        const Tensor out = emptyLike(q, {q.size(0), q.size(1), logDecay.size(0), v.size(3)}, q.scalar_type()), last = emptyLike(q, a.stateShape);
+        a.forward(out, last);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({q, k, v, a.logDecay, state ? *state : Tensor(), a.lengths});
+        ctx->saved_data["scale"] = scale;
+        return {out, last};
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        torch::autograd::variable_list out(7);
+        if (!grads[0].defined() && !grads[1].defined()) return out;
+        const at::NoGradGuard noGrad;
+        auto maybe = [](const Tensor &t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); };
+        const Tensor q = saved[0];
+        const AttentionArguments a(q.detach(), saved[1].detach(), saved[2].detach(), saved[3], maybe(saved[4]), maybe(saved[5]), ctx->saved_data["scale"].toDouble(), 4);
+        const c10::cuda::CUDAGuard guard(q.device());
+        const Tensor dout = grads[0].defined() ? AttentionArguments::rowsOf(grads[0])
+                                               : at::zeros({q.size(0), q.size(1), a.problem.heads, a.problem.value_dim}, q.options());
+        const Tensor dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+        for (int i = 0; i < 3; ++i)
+            if (ctx->needs_input_grad(i)) out[i] = emptyLike(q, saved[i].sizes(), q.scalar_type());
+        if (saved[4].defined() && ctx->needs_input_grad(4)) out[4] = emptyLike(q, a.stateShape);
+        size_t bytes;
+        const Tensor ws = a.workspaceFor(true, bytes);
+        const rxmet_head_tensor d = AttentionArguments::view(dout);
+        checkStatus(rxmet_decayed_attention_backward(&a.problem, pointer<float>(a.state), &d, pointer<float>(dlast), mutableOf(out[0]), mutableOf(out[1]),
+                                                     mutableOf(out[2]), pointer<float>(out[4]), mutableOf(ws), bytes, streamOf(q)),
+                    "decayed_attention backward");
+        return out;
+    }
+};
+
+std::vector<Tensor> decayedAttention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &logDecay, const MaybeTensor &state,
+                                     const MaybeTensor &lengths, double scale) {
+    return DecayedAttention::apply(q, k, v, logDecay, state, lengths, scale);
+}
+
+// One token for each row; the states go to `newState`, which may be `state` itself.
+Tensor decayedAttentionStep(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &logDecay, const Tensor &state, const Tensor &newState,
+                            const MaybeTensor &active, double scale) {
+    if (at::GradMode::is_enabled())
+        for (const Tensor *t : {&q, &k, &v, &state, &newState})
+            TORCH_CHECK(!t->requires_grad(), "decayed_attention_step has no gradient: use decayed_attention, or no_grad");
+    const AttentionArguments a(q, k, v, logDecay, state, active, scale, 3);
+    a.checkedState(newState, "new_state");
+    TORCH_CHECK(newState.is_contiguous(), "new_state must be contiguous");
+    const c10::cuda::CUDAGuard guard(q.device());
+    const Tensor out = emptyLike(q, {q.size(0), logDecay.size(0), v.size(2)}, q.scalar_type());
+    a.forward(out, newState);
+    newState.unsafeGetTensorImpl()->bump_version();
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_binding, m) {
@@ -407,5 +693,10 @@ PYBIND11_MODULE(_binding, m) {
     m.def("gru_backward_quant", &gruBackwardQuant);
     m.def("lstm_forward_quant", &lstmForwardQuant);
     m.def("lstm_backward_qat", &lstmBackwardQat);
+    m.def("add_rms_norm", &addRmsNorm, pybind11::call_guard<pybind11::gil_scoped_release>());
+    m.def("add_rms_norm_codes", &addRmsNormCodes, pybind11::call_guard<pybind11::gil_scoped_release>());
+    m.def("coded_linear", &codedLinear, pybind11::call_guard<pybind11::gil_scoped_release>());
+    m.def("decayed_attention", &decayedAttention, pybind11::call_guard<pybind11::gil_scoped_release>());
+    m.def("decayed_attention_step", &decayedAttentionStep, pybind11::call_guard<pybind11::gil_scoped_release>());
     m.def("quantize_dequantize", &quantizeDequantize, pybind11::call_guard<pybind11::gil_scoped_release>());
 }

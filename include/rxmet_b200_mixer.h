@@ -18,6 +18,10 @@ extern "C" {
 /* Element types of activations. */
 enum { RXMET_TYPE_F32 = 0, RXMET_TYPE_BF16 = 1, RXMET_TYPE_F16 = 2 };
 
+/* 1 in *gave_up once a bounded device-side wait of one of these operators' kernels has run out on the current device (its output is incomplete),
+ * else 0.  Synchronises the device.  No wait runs out in a working program. */
+RXMET_API int rxmet_wait_status(int *gave_up);
+
 /* ---- residual addition and root-mean-square norm -----------------------------------------------
  * total = x + residual;  y = total * rsqrt(mean(total^2) + eps) * weight, row by row, sums in 32 bits; y is taken from the unrounded
  * total.  Rows of x and residual start `*_pitch` elements apart; total and y are contiguous.  residual may be null (total is x then and

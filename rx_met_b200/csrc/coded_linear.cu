@@ -95,6 +95,7 @@ extern "C" int rxmet_coded_linear(int64_t rows, int inner, int outer, const int8
         RXMET_REQUIRE((rows == 1 || codes_pitch >= inner) && (outer == 1 || weight_pitch >= inner), "coded_linear: rows overlap");
         const codedlinear::Problem p{rows, inner, outer, codes_dev, codes_pitch, scale_dev, weight_dev, weight_pitch, weight_scale_dev, bias_dev, activation,
                                      residual_dev, residual_pitch, out_type, out_dev};
-        codedlinear::launchBytes(p, static_cast<cudaStream_t>(stream));
+        if (codedlinear::takesTensorCores(p)) codedlinear::launchTensorCores(p, static_cast<cudaStream_t>(stream));
+        else codedlinear::launchBytes(p, static_cast<cudaStream_t>(stream));
     });
 }

@@ -23,5 +23,9 @@ struct Problem {
     void *out;                   // [rows][outer]
 };
 
+// Operands whose rows start on 16 bytes.
+bool takesTensorCores(const Problem &p);
+void launchTensorCores(const Problem &p, cudaStream_t st);
+
 }  // namespace codedlinear
 }  // namespace rxmet

@@ -53,13 +53,16 @@ __global__ void __launch_bounds__(kThreads) codedLinearBytes(const __grid_consta
         const int n = col0 + tx + 16 * j;
         if (n >= p.outer) continue;
         const Channel channel(p, n);
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = channel.value(acc[i][j], p.scale[min(row0 + ty + 16 * i, p.rows - 1)]);
+        activate(v, p.activation);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int64_t m = row0 + ty + 16 * i;
             if (m >= p.rows) continue;
-            float v = channel.value(acc[i][j], p.scale[m], p.activation);
-            if (p.residual) v += toFloat(static_cast<const T *>(p.residual)[m * p.residualPitch + n]);
-            static_cast<T *>(p.out)[m * p.outer + n] = fromFloat<T>(v);
+            if (p.residual) v[i] += toFloat(static_cast<const T *>(p.residual)[m * p.residualPitch + n]);
+            static_cast<T *>(p.out)[m * p.outer + n] = fromFloat<T>(v[i]);
         }
     }
 }
@@ -93,6 +96,8 @@ extern "C" int rxmet_coded_linear(int64_t rows, int inner, int outer, const int8
         if (rows == 0) return;
         RXMET_REQUIRE(codes_dev && scale_dev && weight_dev && weight_scale_dev && out_dev, "coded_linear: null tensor");
         RXMET_REQUIRE((rows == 1 || codes_pitch >= inner) && (outer == 1 || weight_pitch >= inner), "coded_linear: rows overlap");
+        if (rows == 1) codes_pitch = static_cast<int64_t>(alignUp(inner, 16));   // the distance of a single row's next one does not matter
+        if (outer == 1) weight_pitch = static_cast<int64_t>(alignUp(inner, 16));
         const codedlinear::Problem p{rows, inner, outer, codes_dev, codes_pitch, scale_dev, weight_dev, weight_pitch, weight_scale_dev, bias_dev, activation,
                                      residual_dev, residual_pitch, out_type, out_dev};
         if (codedlinear::takesTensorCores(p)) codedlinear::launchTensorCores(p, static_cast<cudaStream_t>(stream));

@@ -35,27 +35,43 @@ constexpr int kChunk = 128;                  // codes of K in a stage
 constexpr int kChannels = 128;               // channels of a CTA's accumulator
 constexpr uint32_t kWeightBytes = kChannels * kChunk;
 
-// Sixteen rows of the accumulator, one channel: epilogue and stores of those below `count`.
-template <class T, class Sums>
-__device__ __forceinline__ void storeRows(const Problem &p, const Channel &channel, int n, int64_t row0, int count, Sums sums) {
-    float v[16];
-    if (p.residual) {
-        const T *from = static_cast<const T *>(p.residual) + row0 * p.residualPitch + n;
+// What the epilogue of sixteen rows reads from memory, asked for before the rows in front of them are worked on: lane j holds the scale of row j % N.
+template <class T, int N = 16>
+struct RowInputs {
+    float scale;
+    T residual[N];
+    __device__ __forceinline__ void load(const Problem &p, int n, int64_t row0, int count) {
+        const int j = threadIdx.x & (N - 1);
+        scale = j < count ? p.scale[row0 + j] : 0.f;
+        if (p.residual && n < p.outer) {
+            const T *from = static_cast<const T *>(p.residual) + row0 * p.residualPitch + n;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = j < count ? toFloat(from[j * p.residualPitch]) : 0.f;
+            for (int i = 0; i < N; ++i, from += p.residualPitch)
+                if (i < count) residual[i] = *from;
+        }
     }
+};
+// N rows of the accumulator, one channel: epilogue and stores of those below `count`.  All lanes of a warp take part.
+template <class T, int N>
+__device__ __forceinline__ void storeRows(const Problem &p, const Channel &channel, int n, int64_t row0, int count, const RowInputs<T, N> &in, const uint32_t (&acc)[N]) {
+    float y[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) y[j] = channel.value(static_cast<int32_t>(acc[j]), __shfl_sync(0xffffffffu, in.scale, j));
+    activate(y, p.activation);
+    if (p.residual) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) y[j] += toFloat(in.residual[j]);
+    }
+    if (n >= p.outer) return;
     T *to = static_cast<T *>(p.out) + row0 * p.outer + n;
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-        if (j < count) {
-            const float y = channel.value(sums(j), p.scale[row0 + j], p.activation);
-            to[static_cast<int64_t>(j) * p.outer] = fromFloat<T>(p.residual ? y + v[j] : y);
-        }
+    for (int j = 0; j < N; ++j, to += p.outer)
+        if (j < count) *to = fromFloat<T>(y[j]);
 }
 
 // ---- many rows ----------------------------------------------------------------------------------------------------------
 
-constexpr int kPairRows = 256, kPairStages = 6, kPairEpilogueWarps = 8;
+constexpr int kPairRows = 256, kPairStages = 6, kPairEpilogueWarps = 16;
 constexpr int kPairThreads = 32 * (kPairEpilogueWarps + 2);
 constexpr uint32_t kPairStageBytes = 2 * kWeightBytes;   // a CTA's 128 channels and its 128 rows
 constexpr uint32_t kPairShared = 231936;                 // cluster::leastShared(512)
@@ -143,7 +159,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             }
         }
     } else {
-        const int quarter = warp & 3, half = warp >> 2;
+        constexpr int kGroupRows = kPairRows / (kPairEpilogueWarps / 4);   // rows of a tile that a group of four warps takes, kPart at a time
+        constexpr int kPart = 8;
+        const int quarter = warp & 3, group = warp >> 2;
         int item = 0;
         for (int tile = blockIdx.x / 2; tile < tiles; tile += pairs, ++item) {
             int channelTile, rowTile;
@@ -151,21 +169,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             const uint32_t buf = item & 1;
             const int n = channelTile * 2 * kChannels + rank * kChannels + 32 * quarter + lane;
             const Channel channel(p, min(n, p.outer - 1));
+            const int64_t first = static_cast<int64_t>(rowTile) * kPairRows + group * kGroupRows;
+            const int count = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(kGroupRows), p.rows - first)));
+            RowInputs<T, kPart> in;
+            in.load(p, n, first, count);
             wait(&accFull[buf], (item >> 1) & 1);
             fenceAfter();
+            const uint32_t from = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + buf * kPairRows + group * kGroupRows;
 #pragma unroll 1
-            for (int part = 0; part < kPairRows / 32; ++part) {
-                uint32_t acc[16];
-                const int col = half * (kPairRows / 2) + part * 16;
-                loadTmem16(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + buf * kPairRows + col, acc);
+            for (int at = 0; at < kGroupRows; at += kPart) {
+                uint32_t acc[kPart];
+                const RowInputs<T, kPart> now = in;
+                in.load(p, n, first + at + kPart, count - at - kPart);
+                loadTmem8(from + at, acc);
                 loadsDone();
-                if (part + 1 == kPairRows / 32) {
+                if (at + kPart == kGroupRows) {
                     fenceBefore();
                     __syncwarp();
                     if (lane == 0) arriveRemote(cluster::remote(smemAddr(&accFree[buf]), 0));
                 }
-                const int64_t row0 = static_cast<int64_t>(rowTile) * kPairRows + col;
-                if (alive && n < p.outer) storeRows<T>(p, channel, n, row0, static_cast<int>(min(static_cast<int64_t>(16), p.rows - row0)), [&](int j) { return static_cast<int32_t>(acc[j]); });
+                if (alive) storeRows<T>(p, channel, n, first + at, count - at, now, acc);
             }
         }
     }
@@ -183,7 +206,7 @@ constexpr int kSplitThreads = 192;
 template <int NR>
 struct Split {
     static constexpr uint32_t kStageBytes = kWeightBytes + NR * kChunk;
-    static constexpr int kStages = NR <= 32 ? 5 : NR == 64 ? 4 : 3;   // two CTAs an SM
+    static constexpr int kStages = NR <= 32 ? 9 : NR == 64 ? 8 : 6;   // 160 to 192 KB in flight, one CTA an SM
     static constexpr uint32_t kTmemCols = NR < 32 ? 32 : NR;
     static constexpr uint32_t kBytes = kStages * kStageBytes + 1024;   // the parts of the sums, NR x 128 integers, fit the stages
 };
@@ -260,12 +283,16 @@ __global__ void __launch_bounds__(kSplitThreads) codedLinearSplit(const __grid_c
     if (warp >= 2) {
         if (parts == 1) {
             const Channel channel(p, min(n, p.outer - 1));
+            RowInputs<T> in;
+            in.load(p, n, row0, count);
 #pragma unroll 1
-            for (int col = 0; col < NR; col += 16) {
+            for (int col = 0; col < count; col += 16) {
                 uint32_t acc[16];
+                const RowInputs<T> now = in;
+                in.load(p, n, row0 + col + 16, count - col - 16);
                 loadTmem16(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + col, acc);
                 loadsDone();
-                if (alive && n < p.outer && col < count) storeRows<T>(p, channel, n, row0 + col, min(16, count - col), [&](int j) { return static_cast<int32_t>(acc[j]); });
+                if (alive) storeRows<T>(p, channel, n, row0 + col, count - col, now, acc);
             }
         } else {
 #pragma unroll 1
@@ -284,30 +311,23 @@ __global__ void __launch_bounds__(kSplitThreads) codedLinearSplit(const __grid_c
         __syncthreads();
         const bool complete = failed == 0;
         cluster::barrierAll();
-        // the CTA adds up every `parts`th group of four rows of all CTAs
-        if (warp >= 2 && n < p.outer) {
-            const Channel channel(p, n);
-            for (int first = 4 * part; first < count; first += 4 * parts) {
-                int32_t sum[4] = {};
+        // the CTA adds up every `parts`th group of eight rows of all CTAs
+        if (warp >= 2) {
+            const Channel channel(p, min(n, p.outer - 1));
+            for (int first = 8 * part; first < count; first += 8 * parts) {
+                RowInputs<T, 8> in;
+                in.load(p, n, row0 + first, count - first);
+                uint32_t sum[8] = {};
                 for (int from = 0; from < parts; ++from) {
-                    const uint32_t at = cluster::remote(stages, from);
+                    const uint32_t at = cluster::remote(stages, from) + (first * kChannels + 32 * quarter + lane) * 4;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        int32_t v;
-                        asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(at + ((first + j) * kChannels + 32 * quarter + lane) * 4) : "memory");
+                    for (int j = 0; j < 8; ++j) {
+                        uint32_t v;
+                        asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(at + j * kChannels * 4) : "memory");
                         sum[j] += v;
                     }
                 }
-                if (complete) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (first + j < count) {
-                            const int64_t m = row0 + first + j;
-                            float y = channel.value(sum[j], p.scale[m], p.activation);
-                            if (p.residual) y += toFloat(static_cast<const T *>(p.residual)[m * p.residualPitch + n]);
-                            static_cast<T *>(p.out)[m * p.outer + n] = fromFloat<T>(y);
-                        }
-                }
+                if (complete) storeRows<T>(p, channel, n, row0 + first, count - first, in, sum);
             }
         }
         __syncwarp();
@@ -330,12 +350,28 @@ CUtensorMap rowsMap(const int8_t *data, int64_t rows, int inner, int64_t pitch, 
 }
 
 template <int NR>
+size_t splitShared() {
+    return std::max<size_t>(Split<NR>::kBytes, cluster::leastShared(Split<NR>::kTmemCols));
+}
+// CTAs of clusters of `parts` that the device holds at the same time, asked once a process (its GPUs are alike).
+template <int NR>
+int residentParts(int parts) {
+    if (parts == 1) return currentDevice().sms;
+    static std::atomic<int> known[9];
+    if (const int n = known[parts].load(std::memory_order_relaxed)) return n;
+    const void *kernel = reinterpret_cast<const void *>(codedLinearSplit<float, NR>);
+    ensureDynamicSmem(kernel, splitShared<NR>());
+    const int n = std::max(1, residentClusters(kernel, parts, kSplitThreads, splitShared<NR>())) * parts;
+    known[parts].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+template <int NR>
 void launchSplit(const Problem &p, int parts, cudaStream_t st) {
-    using S = Split<NR>;
     const CUtensorMap weights = rowsMap(p.weight, p.outer, p.inner, p.weightPitch, kChannels), codes = rowsMap(p.codes, p.rows, p.inner, p.codesPitch, NR);
     withType(p.outType, [&](auto t) {
         const auto kernel = codedLinearSplit<decltype(t), NR>;
-        const size_t smem = std::max<size_t>(S::kBytes, cluster::leastShared(S::kTmemCols));
+        const size_t smem = splitShared<NR>();
         ensureDynamicSmem(reinterpret_cast<const void *>(kernel), smem);
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(parts, (p.outer + kChannels - 1) / kChannels, static_cast<unsigned>((p.rows + NR - 1) / NR));
@@ -379,14 +415,31 @@ bool takesTensorCores(const Problem &p) {
     return encodeTiled() != nullptr && p.codesPitch % 16 == 0 && p.weightPitch % 16 == 0 && alignedTo(p.codes, 16) && alignedTo(p.weight, 16);
 }
 
+// Which kernel, row tile and number of parts: the least of these estimates, fitted to 700 measured calls of 1 to 2048 rows, K 512 to 4096, 1024 to 8192 channels.  In
+// microseconds: a chunk of K takes a cluster's CTA 0.24 whatever its rows and a pair 0.28; a CTA of few rows begins and ends in 2.8 to 5.8, a sum over parts adds 1.6 to
+// 2.9, and a pair's epilogue takes 3, under the next tile's products if there is one.  K = N = 4096: 16 rows 6.2 in four parts (10.5 in one, pairs 16), 128 rows 9.5
+// (pairs 16), 512 rows 14.9 (64-row tiles 24), 1024 rows 17.9 in pairs (29 in 128-row tiles).
 void launchTensorCores(const Problem &p, cudaStream_t st) {
-    const int sms = currentDevice().sms, chunks = (p.inner + kChunk - 1) / kChunk, channelTiles = (p.outer + kChannels - 1) / kChannels;
-    if (p.rows > 512) return launchPairs(p, st);
-    const int rows = p.rows <= 16 ? 16 : p.rows <= 32 ? 32 : p.rows <= 64 ? 64 : 128;
-    const int64_t tiles = static_cast<int64_t>(channelTiles) * ((p.rows + rows - 1) / rows);
-    int parts = 1;
-    while (parts < 8 && tiles * parts * 2 <= 2 * sms && parts * 2 <= chunks) parts *= 2;
-    if (rows == 16) launchSplit<16>(p, parts, st);
+    const int sms = currentDevice().sms, chunks = (p.inner + kChunk - 1) / kChunk;
+    auto over = [](int64_t a, int64_t b) { return static_cast<double>((a + b - 1) / b); };
+    const double pairTile = 0.28 * chunks, pairEnd = 3.0;
+    double best = 3.0 + over(static_cast<int64_t>(over(p.outer, 2 * kChannels)) * static_cast<int64_t>(over(p.rows, kPairRows)), sms / 2) * std::max(pairTile, pairEnd) +
+                  std::min(pairTile, pairEnd);
+    int rows = 0, parts = 1;
+    for (const int r : {16, 32, 64, 128})
+        for (int q = 1; q <= 8 && q <= chunks; q *= 2) {
+            const int64_t ctas = static_cast<int64_t>(over(p.outer, kChannels)) * static_cast<int64_t>(over(p.rows, r)) * q;
+            const int resident = r == 16 ? residentParts<16>(q) : r == 32 ? residentParts<32>(q) : r == 64 ? residentParts<64>(q) : residentParts<128>(q);
+            const double ends = r == 16 ? 2.8 : r == 32 ? 3.3 : r == 64 ? 4.5 : 5.8;
+            const double time = over(ctas, resident) * (ends + 0.24 * over(chunks, q)) + (q > 1 ? 1.3 + 0.1 * q + 0.8 * r / 128 : 0.0);
+            if (time < best) {
+                best = time;
+                rows = r;
+                parts = q;
+            }
+        }
+    if (rows == 0) launchPairs(p, st);
+    else if (rows == 16) launchSplit<16>(p, parts, st);
     else if (rows == 32) launchSplit<32>(p, parts, st);
     else if (rows == 64) launchSplit<64>(p, parts, st);
     else launchSplit<128>(p, parts, st);

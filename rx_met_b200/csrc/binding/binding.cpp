@@ -572,7 +572,19 @@ struct AttentionArguments {
         const bool step = t.dim() == 3;
         return {dataOf(t), t.stride(0), step ? 0 : t.stride(1), t.stride(step ? 1 : 2), static_cast<int32_t>(t.size(step ? 1 : 2))};
     }
-    static Tensor rowsOf(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+    // Neighbouring elements of a head; sequences of 16-bit elements also start every head, token and row on 16 bytes, as TMA copies them (a copy where
+    // they do not: the kernel without TMA takes several times as long).
+    static Tensor rowsOf(const Tensor &t) {
+        if (t.dim() == 4 && t.scalar_type() != at::kFloat && t.size(1) >= 32) {
+            bool fits = (t.stride(3) == 1 || t.size(3) == 1) && reinterpret_cast<uintptr_t>(dataOf(t)) % 16 == 0;
+            for (int i = 0; i < 3; ++i) fits = fits && (t.size(i) == 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
+            if (fits) return t;
+            const Tensor copy = emptyLike(t, {t.size(0), t.size(1), t.size(2), (t.size(3) + 7) / 8 * 8}, t.scalar_type()).narrow(3, 0, t.size(3));
+            copy.copy_(t);
+            return copy;
+        }
+        return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
+    }
 
     AttentionArguments(const Tensor &queries, const Tensor &keys, const Tensor &values, const Tensor &decays, const MaybeTensor &start,
                        const MaybeTensor &counts, double scale, int64_t dims) {

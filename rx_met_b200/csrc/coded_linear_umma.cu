@@ -420,6 +420,7 @@ bool takesTensorCores(const Problem &p) {
 // 2.9, and a pair's epilogue takes 3, under the next tile's products if there is one.  K = N = 4096: 16 rows 6.2 in four parts (10.5 in one, pairs 16), 128 rows 9.5
 // (pairs 16), 512 rows 14.9 (64-row tiles 24), 1024 rows 17.9 in pairs (29 in 128-row tiles).
 void launchTensorCores(const Problem &p, cudaStream_t st) {
+    bindContext();
     const int sms = currentDevice().sms, chunks = (p.inner + kChunk - 1) / kChunk;
     auto over = [](int64_t a, int64_t b) { return static_cast<double>((a + b - 1) / b); };
     const double pairTile = 0.28 * chunks, pairEnd = 3.0;

@@ -59,6 +59,40 @@ void roles(Pass &p, const rxmet_head_tensor &q, const rxmet_head_tensor &k, cons
 }
 
 
+// Passes of the gradients.
+Pass queryPass(const rxmet_decayed_attention &a, const rxmet_head_tensor &q, const rxmet_head_tensor &k, const rxmet_head_tensor &v, const rxmet_head_tensor &d) {
+    Pass p = passOf(a);
+    roles(p, d, v, k, a.value_dim, a.key_dim, true, a);
+    return p;
+}
+Pass keyPass(const rxmet_decayed_attention &a, const rxmet_head_tensor &q, const rxmet_head_tensor &k, const rxmet_head_tensor &v, const rxmet_head_tensor &d) {
+    Pass p = passOf(a);
+    roles(p, v, d, q, a.value_dim, a.key_dim, true, a);
+    p.reverse = true;
+    p.inScale = 1.f / a.scale;
+    return p;
+}
+Pass valuePass(const rxmet_decayed_attention &a, const rxmet_head_tensor &q, const rxmet_head_tensor &k, const rxmet_head_tensor &v, const rxmet_head_tensor &d) {
+    Pass p = passOf(a);
+    roles(p, k, q, d, a.key_dim, a.value_dim, false, a);
+    p.reverse = true;
+    p.inScale = 1.f / a.scale;
+    p.finalScale = a.scale;
+    return p;
+}
+Pass forwardPass(const rxmet_decayed_attention &a) {
+    Pass p = passOf(a);
+    roles(p, a.q, a.k, a.v, a.key_dim, a.value_dim, false, a);
+    return p;
+}
+
+// Kernels by size and type.  Chunks from 32 tokens on; tensors that TMA cannot copy and 32-bit ones go token by token.
+void launchPass(const Pass &p, int type, float *states, cudaStream_t st) {
+    const ChunkPlan plan = planChunks(p, type);
+    if (plan.taken && chunksCanCopy(p)) launchChunks(p, type, plan, states, st);
+    else launchRecurrent(p, type, st);
+}
+
 }  // namespace
 }  // namespace decayed
 }  // namespace rxmet
@@ -70,7 +104,15 @@ extern "C" {
 
 size_t rxmet_decayed_attention_workspace_bytes(const rxmet_decayed_attention *a, int backward) {
     WorkspaceSizer size;
-    if (!a || !backward) return 0;
+    if (!a || a->batch <= 0 || a->tokens <= 0) return 0;
+    const rxmet_head_tensor none{};
+    size_t states = 0;
+    if (!backward) states = planChunks(forwardPass(*a), a->type).stateFloats(forwardPass(*a));
+    else
+        for (const Pass &p : {queryPass(*a, none, none, none, none), keyPass(*a, none, none, none, none), valuePass(*a, none, none, none, none)})
+            states = std::max(states, planChunks(p, a->type).stateFloats(p));
+    if (states > 0) size.take<float>(states);
+    if (!backward) return size.used();
     const size_t rows = static_cast<size_t>(a->batch) * a->tokens * a->heads;
     if (a->q.heads != a->heads) size.take<float>(rows * a->key_dim);
     if (a->k.heads != a->heads) size.take<float>(rows * a->key_dim);
@@ -81,20 +123,24 @@ size_t rxmet_decayed_attention_workspace_bytes(const rxmet_decayed_attention *a,
 int rxmet_decayed_attention_forward(const rxmet_decayed_attention *problem, const float *state_dev, void *out_dev, float *final_state_dev,
                                     void *workspace_dev, size_t workspace_bytes, void *stream) {
     return guarded([&] {
-        (void)workspace_dev;
-        (void)workspace_bytes;
         RXMET_REQUIRE(problem, "decayed_attention: null problem");
         const rxmet_decayed_attention &a = *problem;
         checkSizes(a);
         if (a.batch == 0) return;
         RXMET_REQUIRE(a.log_decay, "decayed_attention: null log_decay");
-        Pass p = passOf(a);
-        if (a.tokens > 0) roles(p, checked(a.q, a.heads, "q"), checked(a.k, a.heads, "k"), checked(a.v, a.heads, "v"), a.key_dim, a.value_dim, false, a);
-        else roles(p, {nullptr, 0, 0, 0, 1}, {nullptr, 0, 0, 0, 1}, {nullptr, 0, 0, 0, 1}, a.key_dim, a.value_dim, false, a);
+        if (a.tokens > 0) {
+            checked(a.q, a.heads, "q");
+            checked(a.k, a.heads, "k");
+            checked(a.v, a.heads, "v");
+        }
+        Pass p = forwardPass(a);
+        if (a.tokens == 0) p.q = p.k = p.v = {nullptr, 0, 0, 0, 1};
         p.stateIn = state_dev;
         p.stateOut = final_state_dev;
         p.out = out_dev;
-        launchRecurrent(p, a.type, static_cast<cudaStream_t>(stream));
+        Workspace ws(workspace_dev, workspace_bytes);
+        const size_t states = planChunks(p, a.type).stateFloats(p);
+        launchPass(p, a.type, states > 0 ? ws.take<float>(states) : nullptr, static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -116,7 +162,11 @@ int rxmet_decayed_attention_backward(const rxmet_decayed_attention *problem, con
             d = checked(*dout, a.heads, "dout");
             RXMET_REQUIRE(d.heads == a.heads, "decayed_attention: dout has %d heads of %d", d.heads, a.heads);
         }
+        const Pass passes[] = {queryPass(a, q, k, v, d), keyPass(a, q, k, v, d), valuePass(a, q, k, v, d)};
         Workspace ws(workspace_dev, workspace_bytes);
+        size_t stateFloats = 0;
+        for (const Pass &p : passes) stateFloats = std::max(stateFloats, planChunks(p, a.type).stateFloats(p));
+        float *states = stateFloats > 0 ? ws.take<float>(stateFloats) : nullptr;   // the passes follow one another on the stream
         const int64_t rows = static_cast<int64_t>(a.batch) * a.tokens;
         auto run = [&](Pass p, int ownHeads, void *out) {
             p.out = out;
@@ -124,7 +174,7 @@ int rxmet_decayed_attention_backward(const rxmet_decayed_attention *problem, con
                 p.out = ws.take<float>(static_cast<size_t>(rows) * a.heads * p.value);
                 p.outFloat = true;
             }
-            launchRecurrent(p, a.type, st);
+            launchPass(p, a.type, states, st);
             if (!p.outFloat || rows == 0) return;
             withType(a.type, [&](auto t) {
                 using T = decltype(t);
@@ -138,27 +188,19 @@ int rxmet_decayed_attention_backward(const rxmet_decayed_attention *problem, con
             });
         };
         if (dq_dev) {
-            Pass p = passOf(a);
-            roles(p, d, v, k, a.value_dim, a.key_dim, true, a);
+            Pass p = passes[0];
             p.stateIn = state_dev;
             run(p, a.q.heads, dq_dev);
         }
         if (dk_dev) {
-            Pass p = passOf(a);
-            roles(p, v, d, q, a.value_dim, a.key_dim, true, a);
-            p.reverse = true;
+            Pass p = passes[1];
             p.stateIn = dfinal_state_dev;
-            p.inScale = 1.f / a.scale;
             run(p, a.k.heads, dk_dev);
         }
         if (dv_dev || dstate_dev) {
-            Pass p = passOf(a);
-            roles(p, k, q, d, a.key_dim, a.value_dim, false, a);
-            p.reverse = true;
+            Pass p = passes[2];
             p.stateIn = dfinal_state_dev;
             p.stateOut = dstate_dev;
-            p.inScale = 1.f / a.scale;
-            p.finalScale = a.scale;
             run(p, a.v.heads, dv_dev);
         }
     });

@@ -35,5 +35,16 @@ struct Pass {
 
 void launchRecurrent(const Pass &p, int type, cudaStream_t st);
 
+// Chunks of 128 tokens on tensor cores, for 16-bit tensors that TMA can copy.  Few heads are cut into segments along time, whose states need a workspace.
+constexpr int kChunkTokens = 128;
+struct ChunkPlan {
+    bool taken;   // by size and type
+    int segments, segmentChunks;
+    size_t stateFloats(const Pass &p) const { return segments > 1 ? static_cast<size_t>(p.batch) * p.heads * segments * p.key * p.value : 0; }
+};
+ChunkPlan planChunks(const Pass &p, int type);
+bool chunksCanCopy(const Pass &p);
+void launchChunks(const Pass &p, int type, const ChunkPlan &plan, float *states, cudaStream_t st);
+
 }  // namespace decayed
 }  // namespace rxmet

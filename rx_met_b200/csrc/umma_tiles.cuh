@@ -31,6 +31,19 @@ __device__ __forceinline__ void copyTile2Pair(uint32_t to, const CUtensorMap *ma
                  "r"(bar & 0xfeffffffu)
                  : "memory");
 }
+__device__ __forceinline__ void copyTile4(uint32_t to, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w),
+                 "r"(bar)
+                 : "memory");
+}
+// Back to memory, in the issuing thread's bulk group; what lies beyond the array is dropped.
+__device__ __forceinline__ void storeTile4(const CUtensorMap *map, uint32_t from, int x, int y, int z, int w) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map), "r"(from), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void storesRead() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void storesDone() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void fenceAsyncProxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void prefetchMap(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
 template <int CTAS>
@@ -62,6 +75,28 @@ __device__ __forceinline__ void productI8(uint32_t tmem, uint64_t a, uint64_t b,
         asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
                      : "memory");
 }
+// kind::f16, 32-bit sums, 128 rows of A: operand formats (0 half, 1 bfloat16) in [7,10) and [10,13); B MN-major with bit 16.
+__host__ __device__ constexpr uint32_t halves(bool bf16, int n, bool bMnMajor) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (bMnMajor ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kTileM >> 4) << 24);
+}
+__device__ __forceinline__ void product(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+// A in tensor memory: lane = row, a column holds two neighbours along K.
+__device__ __forceinline__ void productTmem(uint32_t tmem, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void storeTmem8(uint32_t at, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+                 "r"(v[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tmemStoresDone() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Barrier of some of a CTA's threads.
+__device__ __forceinline__ void groupBarrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
 // Arrives at the barrier of both CTAs of a pair once the products issued so far are complete.
 __device__ __forceinline__ void commitPair(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
@@ -87,6 +122,9 @@ __device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.ar
 __device__ __forceinline__ void arriveRemote(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 
 }  // namespace ummatiles
+
+// Binds the current device's context to this thread, which encoding a tensor map needs: a thread of the autograd engine may come here without one.
+inline void bindContext() { RXMET_CUDA(cudaSetDevice(currentDevice().device)); }
 
 // A word of the current device that kernels set where a bounded wait gave up; their output is not written then.
 int *waitStatus();

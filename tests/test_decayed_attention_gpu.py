@@ -190,6 +190,22 @@ def test_strides_streams_and_reproducibility():
     assert all(torch.isfinite(g).all() for g in only_state)
 
 
+def test_gradients_in_a_thread_without_a_context():
+    """The autograd engine's thread may not have touched the device before."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = ("import torch; from rx_met_b200.decayed_attention import decayed_attention\n"
+            "q, k, v = (torch.randn(2, 256, 2, 64, device='cuda', dtype=torch.bfloat16, requires_grad=True) for _ in range(3))\n"
+            "decay = -torch.ones(2, device='cuda')\n"
+            "warm = torch.empty(1 << 22, device='cuda'); del warm\n"
+            "out, _ = decayed_attention(q, k, v, decay)\n"
+            "grads = torch.autograd.grad([out], [q, k, v], [torch.ones_like(out)])\n"
+            "assert all(torch.isfinite(g).all() for g in grads)\n")
+    done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
 def test_nothing_to_do():
     from rx_met_b200.decayed_attention import decayed_attention
     q, k, v, decay, state = problem(2, 0, 2, 2, 16, 16, torch.bfloat16, state=True, joint=False)

@@ -4,13 +4,16 @@
 //   O = scale (l^(i+1) Q S + ((Q K') . [i >= j] l^(i-j)) V)          S <- l^n S + K'^T diag(l^(n-1-j)) V
 // Exponents are differences of places in a chunk and never negative, so that no power overflows.  A CTA walks over the chunks of one head and of 64 columns of V, warps by role:
 //   copies     Q, K and V of the next chunks as TMA boxes with a 128-byte swizzle
-//   products   one thread issues P = Q K', KV = (weighted K)' V, O1 = Q S and O2 = P V
-//   scores     eight warps: P from tensor memory, times the decays, back as the A operand of the last product; then O1 and O2 to the output tile, which TMA stores
-//   state      eight warps: weighted K, transposed, into tensor memory as the A operand of KV; the state itself, 32 bits, stays in their registers
+//   products   one thread issues P = Q K', KV = K'^T (weighted V), O1 = Q S and O2 = P V; P has two buffers, so that the scores of a chunk and the outputs of the one before
+//              are worked on at the same time
+//   scores     eight warps: P from tensor memory, times the decays, back as the A operand of the last product
+//   outputs    four warps: O1 and O2 to memory, 32 bytes a thread and store
+//   state      eight warps: weighted V for the products; the state itself, 32 bits, stays in their registers
 //
 // Roundings.  Operands of tensor cores have the type of the inputs: P times the decays and S are rounded to it once, next to the rounding of the output.  The state is never
-// rebuilt from rounded values: the weighted K goes in as the sum of three bfloat16 or two half terms, which leaves 2^-24.  half has a short range: its rows of P and its S are scaled by
-// powers of two to the top of it, and the second term of the weighted K is scaled by 2^11 and summed apart.
+// rebuilt from rounded values: the weighted V goes in as the sum of three bfloat16 or two half terms, which leaves 2^-24.  half has a short range: its rows of P and its S are scaled by
+// powers of two to the top of it, and the second term of the weighted V is scaled by 2^11.  The two larger terms lie side by side as 128 columns of one product, which reads
+// K once for both.
 #include "decayed_attention.h"
 #include "dependent_launch.cuh"
 #include "element_types.cuh"
@@ -24,12 +27,22 @@ using namespace ummatiles;
 
 constexpr int kC = kChunkTokens;
 constexpr int kCols = 64;              // columns of V a CTA takes
-constexpr int kScoreWarps = 8, kStateWarps = 8, kCopyWarp = 16, kProductWarp = 17;
-constexpr int kThreads = 32 * 18;
+constexpr int kScoreWarps = 8, kOutputWarps = 4, kStateWarps = 8;
+constexpr int kFirstOutput = kScoreWarps, kFirstState = kFirstOutput + kOutputWarps, kCopyWarp = kFirstState + kStateWarps, kProductWarp = kCopyWarp + 1;
+constexpr int kThreads = 32 * (kProductWarp + 1);
 constexpr uint32_t kTile = kC * 128;   // 128 rows of 64 elements
-constexpr uint32_t kShared = 229888;   // with up to 2.5 KB of static arrays all of an SM, as the tensor memory
-// columns of tensor memory
-constexpr uint32_t kP = 0, kO1 = 128, kO2 = 192, kKV = 256, kWeightedK = 320, kKVLow = 448;
+constexpr uint32_t kShared = 232448;   // all of an SM, as the tensor memory
+// columns of tensor memory: two buffers of P, then the others
+constexpr uint32_t kP = 0, kO1 = 256, kO2 = 320, kKV = 384;   // KV: the larger term, then the others
+enum Barrier { kStateMeets = 1, kLanesMeet };   // named barriers; the last takes four
+
+// Shared memory in groups of 16 bytes.
+__device__ __forceinline__ void loadShared(uint32_t at, uint32_t (&v)[4]) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void storeShared(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 
 struct Segments {
     int count, chunks;   // segments of time, chunks of a segment
@@ -65,6 +78,11 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
     return r;
 }
 template <class T>
+__device__ __forceinline__ uint32_t pack2(Pair p) {
+    const float2 v = floatsOf(p);
+    return pack2<T>(v.x, v.y);
+}
+template <class T>
 __device__ __forceinline__ float2 unpack2(uint32_t v);
 template <>
 __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) { return make_float2(bf16Lo(v), bf16Hi(v)); }
@@ -79,27 +97,34 @@ __device__ __forceinline__ float toTopOfHalf(float most) {
     return __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
 }
 
-// DK: elements of a key that the tiles hold, 64 or 128.  StateOnly: nothing but the state at the end of the segment.
-template <class T, int DK, bool StateOnly>
+// What a CTA keeps in shared memory beside the tiles.
+struct Small {
+    float powers[kC + 4], scaledPowers[32], columnPowers[32];   // l^n; scale l^n; scale l^(31 - j) or scale l^j of a block's columns
+    float rowPeaks[2][kC], statePeaks[kStateWarps], stateScale[2];
+    uint8_t rowScale[3][kC];                  // exponents of the powers of two that rows of P were scaled by, for three chunks
+    uint64_t full[3], freed[3], pFull[2], pReady[2], vReady, kvFull, sReady, sFree, oFull, oFree, productsDone;
+    uint32_t tmemSlot;
+    int failed;
+};
+
+// DK: elements of a key that the tiles hold, 64 or 128.  StateOnly: nothing but the state at the end of the segment.  Wide: outputs of the type of the inputs whose parts of
+// sixteen start on 32 bytes.
+template <class T, int DK, bool StateOnly, bool Wide>
 __global__ void __launch_bounds__(kThreads, 1)
     decayedChunks(const __grid_constant__ Pass p, const __grid_constant__ CUtensorMap qMap, const __grid_constant__ CUtensorMap kMap, const __grid_constant__ CUtensorMap vMap,
-                  const __grid_constant__ CUtensorMap outMap, const bool storeBoxes, const Segments segments, const int terms, int *status) {
+                  const Segments segments, const int terms, int *status) {
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr int kHalves = DK / 64;
     constexpr uint32_t kStageBytes = (2 * kHalves + 1) * kTile;
     constexpr int kStages = DK == 64 ? 3 : 2;
     constexpr uint32_t kSBytes = DK * 128;
-    extern __shared__ uint8_t raw[];
-    __shared__ __align__(16) float powers[kC + 4], columnPowers[32], weights[kC];   // l^n; l^(31 - j) or l^j of a block's columns; of the tokens in the new state
-    __shared__ float rowPeaks[2][kC], statePeaks[kStateWarps], stateScale[2];
-    __shared__ __align__(8) uint64_t full[kStages], freed[kStages], pFull, pReady, aReady, kvFull, sReady, sFree, oFull, oFree;
-    __shared__ uint32_t tmemSlot;
-    __shared__ int failed;
+    static_assert(kStages * kStageBytes + kSBytes + 3 * kTile + sizeof(Small) <= kShared, "shared memory");
+    extern __shared__ __align__(1024) uint8_t raw[];
+    const uint32_t tiles = smemAddr(raw), sTile = tiles + kStages * kStageBytes, weightedV = sTile + kSBytes;
+    Small &small = *reinterpret_cast<Small *>(raw + kStages * kStageBytes + kSBytes + 3 * kTile);
 
     const int warp = warpIndex(), lane = threadIdx.x & 31, tid = threadIdx.x;
     const int slices = gridDim.x / segments.count, slice = blockIdx.x % slices, segment = blockIdx.x / slices, h = blockIdx.y, b = blockIdx.z;
-    const uint32_t tiles = (smemAddr(raw) + 1023u) & ~1023u;
-    const uint32_t sTile = tiles + kStages * kStageBytes, oTile = sTile + kSBytes;
     const bool reverse = p.reverse;
 
     waitForPredecessor();
@@ -109,25 +134,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto tokensOf = [&](int chunk) { return min(kC, length - chunk * kC); };
 
     if (tid == 0) {
-        failed = 0;
-        for (int i = 0; i < kStages; ++i) { cluster::initBarrier(&full[i], 1); cluster::initBarrier(&freed[i], 1); }
-        for (uint64_t *bar : {&pFull, &kvFull, &sFree, &oFull}) cluster::initBarrier(bar, 1);
-        for (uint64_t *bar : {&pReady, &oFree}) cluster::initBarrier(bar, kScoreWarps);
-        for (uint64_t *bar : {&aReady, &sReady}) cluster::initBarrier(bar, kStateWarps);
+        small.failed = 0;
+        for (int i = 0; i < kStages; ++i)
+            for (uint64_t *bar : {&small.full[i], &small.freed[i]}) cluster::initBarrier(bar, 1);
+        // Those of P are one for each of its buffers: a chunk's scores may be done before the products have asked for those of the chunk before.
+        for (uint64_t *bar : {&small.pFull[0], &small.pFull[1], &small.kvFull, &small.sFree, &small.oFull, &small.productsDone}) cluster::initBarrier(bar, 1);
+        for (uint64_t *bar : {&small.pReady[0], &small.pReady[1]}) cluster::initBarrier(bar, kScoreWarps);
+        cluster::initBarrier(&small.oFree, kOutputWarps);
+        for (uint64_t *bar : {&small.vReady, &small.sReady}) cluster::initBarrier(bar, kStateWarps);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (tid <= kC) {
         const double g = p.logDecay[h];
-        powers[tid] = tid == 0 ? 1.f : static_cast<float>(exp(tid * g));
-    } else if (tid >= 256 && tid < 288) {
-        const int apart = reverse ? tid - 256 : 287 - tid;
-        columnPowers[tid - 256] = apart == 0 ? 1.f : static_cast<float>(exp(apart * static_cast<double>(p.logDecay[h])));
+        small.powers[tid] = tid == 0 ? 1.f : static_cast<float>(exp(tid * g));
+    } else if (tid >= 256 && tid < 320) {
+        const int j = tid & 31, apart = tid < 288 || reverse ? j : 31 - j;
+        (tid < 288 ? small.scaledPowers : small.columnPowers)[j] = p.outScale * (apart == 0 ? 1.f : static_cast<float>(exp(apart * static_cast<double>(p.logDecay[h]))));
     }
-    if (warp == kProductWarp) allocTmem<1>(smemAddr(&tmemSlot), 512);
+    if (warp == kProductWarp) allocTmem<1>(smemAddr(&small.tmemSlot), 512);
     fenceBefore();
     __syncthreads();
     fenceAfter();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, tmemSlot, 0);
+    const uint32_t tmem = __shfl_sync(0xffffffffu, small.tmemSlot, 0);
     letDependentsStart();
 
     bool alive = true;
@@ -142,324 +170,326 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kCopyWarp) {
         Turn turn;
         for (int u = 0; u < count; ++u, turn.step(kStages)) {
-            if (turn.again) wait(freed[turn.at], turn.parity ^ 1u);
+            if (turn.again) wait(small.freed[turn.at], turn.parity ^ 1u);
             if (alive && electOne()) {
-                const uint32_t bar = smemAddr(&full[turn.at]), to = tiles + turn.at * kStageBytes;
+                const uint32_t bar = smemAddr(&small.full[turn.at]), to = tiles + turn.at * kStageBytes;
                 const int t = span.chunkAt(u, reverse) * kC;
                 cluster::arriveExpect(bar, StateOnly ? (kHalves + 1) * kTile : kStageBytes);
+                for (int i = 0; i < kHalves; ++i) copyTile4(to + (kHalves + i) * kTile, &kMap, 64 * i, h / (p.heads / p.k.heads), t, b, bar);
                 if (!StateOnly)
                     for (int i = 0; i < kHalves; ++i) copyTile4(to + i * kTile, &qMap, 64 * i, h / (p.heads / p.q.heads), t, b, bar);
-                for (int i = 0; i < kHalves; ++i) copyTile4(to + (kHalves + i) * kTile, &kMap, 64 * i, h / (p.heads / p.k.heads), t, b, bar);
                 copyTile4(to + 2 * kHalves * kTile, &vMap, slice * kCols, h / (p.heads / p.v.heads), t, b, bar);
             }
             __syncwarp();
         }
-        // nothing is left in flight: the products of the last use of each stage are complete
+        // nothing is left in flight: the last use of each stage is over
         for (int i = 0; i < kStages; ++i, turn.step(kStages))
-            if (turn.again) waitSuspended(smemAddr(&freed[turn.at]), turn.parity ^ 1u);
+            if (turn.again) waitSuspended(smemAddr(&small.freed[turn.at]), turn.parity ^ 1u);
     } else if (warp == kProductWarp) {
-        constexpr uint32_t kScores = halves(!kHalf, kC, false), kOthers = halves(!kHalf, kCols, true);
-        Turn turn;
+        constexpr uint32_t kScores = halves(!kHalf, kC, false, false), kOutputs = halves(!kHalf, kCols, false, true);
+        constexpr uint32_t kBothTerms = halves(!kHalf, 2 * kCols, true, true), kThirdTerm = halves(!kHalf, kCols, true, true);
+        Turn turn, next;   // stages of this chunk and of the one whose scores are next
+        auto scores = [&](int u) {
+            wait(small.full[next.at], next.parity);
+            if (u > 1) wait(small.oFull, u & 1);   // the product that read this buffer of P, of chunk u - 2
+            if (electOne()) {
+                fenceAfter();
+                const uint32_t at = tiles + next.at * kStageBytes;
+                const uint64_t q = swizzledDescriptor(at), k = swizzledDescriptor(at + kHalves * kTile);
+#pragma unroll 2
+                for (int i = 0; i < 4 * kHalves; ++i) {
+                    const uint64_t step = (i / 4) * (kTile >> 4) + (i % 4) * 2;
+                    product(tmem + kP + (u & 1) * kC, q + step, k + step, kScores, i > 0);
+                }
+                commitTo(smemAddr(&small.pFull[u & 1]));
+            }
+            __syncwarp();
+            next.step(kStages);
+        };
+        if (!StateOnly && count > 0) scores(0);
         for (int u = 0; u < count; ++u, turn.step(kStages)) {
             const uint32_t at = tiles + turn.at * kStageBytes, parity = u & 1;
-            const uint64_t q = swizzledDescriptor(at), k = swizzledDescriptor(at + kHalves * kTile), v = swizzledDescriptor(at + 2 * kHalves * kTile), s = swizzledDescriptor(sTile);
-            wait(full[turn.at], turn.parity);
-            if (!StateOnly) {
-                if (u > 0) wait(oFull, parity ^ 1u);   // the last product has read P
-                if (alive && electOne()) {
-                    fenceAfter();
-#pragma unroll
-                    for (int i = 0; i < 4 * kHalves; ++i) {
-                        const uint64_t step = (i / 4) * (kTile >> 4) + (i % 4) * 2;
-                        product(tmem + kP, q + step, k + step, kScores, i > 0);
-                    }
-                    commitTo(smemAddr(&pFull));
-                }
-                __syncwarp();
-            }
-            wait(aReady, parity);
-            if (alive && electOne()) {
+            const uint64_t q = swizzledDescriptor(at), kAcross = swizzledDescriptor(at + kHalves * kTile, kTile), v = swizzledDescriptor(at + 2 * kHalves * kTile),
+                           weighted = swizzledDescriptor(weightedV, kTile), third = swizzledDescriptor(weightedV + 2 * kTile), s = swizzledDescriptor(sTile);
+            if (StateOnly) wait(small.full[turn.at], turn.parity);
+            wait(small.vReady, parity);
+            if (electOne()) {
                 fenceAfter();
-                for (int term = terms - 1; term >= 0; --term) {
-                    const bool low = kHalf && term > 0;
-#pragma unroll
-                    for (int i = 0; i < kC / 16; ++i)
-                        productTmem(tmem + (low ? kKVLow : kKV), tmem + kWeightedK + term * 64 + i * 8, v + i * 128, kOthers, i > 0 || (!kHalf && term < terms - 1));
+#pragma unroll 2
+                for (int i = 0; i < kC / 16; ++i) product(tmem + kKV, kAcross + i * 128, weighted + i * 128, kBothTerms, i > 0);
+                if (terms > 2) {
+#pragma unroll 2
+                    for (int i = 0; i < kC / 16; ++i) product(tmem + kKV + kCols, kAcross + i * 128, third + i * 128, kThirdTerm, 1);
                 }
-                commitTo(smemAddr(&kvFull));
-                if (StateOnly) commitTo(smemAddr(&freed[turn.at]));
+                commitTo(smemAddr(&small.kvFull));
+                if (StateOnly) commitTo(smemAddr(&small.freed[turn.at]));
             }
             __syncwarp();
             if (!StateOnly) {
-                wait(sReady, parity);
-                if (u > 0) wait(oFree, parity ^ 1u);
-                if (alive && electOne()) {
+                wait(small.sReady, parity);
+                if (u > 0) wait(small.oFree, parity ^ 1u);
+                if (electOne()) {
                     fenceAfter();
-#pragma unroll
-                    for (int i = 0; i < DK / 16; ++i) product(tmem + kO1, q + (i / 4) * (kTile >> 4) + (i % 4) * 2, s + i * 128, kOthers, i > 0);
-                    commitTo(smemAddr(&sFree));
+#pragma unroll 2
+                    for (int i = 0; i < DK / 16; ++i) product(tmem + kO1, q + (i / 4) * (kTile >> 4) + (i % 4) * 2, s + i * 128, kOutputs, i > 0);
+                    commitTo(smemAddr(&small.sFree));
                 }
                 __syncwarp();
-                wait(pReady, parity);
-                if (alive && electOne()) {
+                if (u + 1 < count) scores(u + 1);
+                wait(small.pReady[parity], (u >> 1) & 1);
+                if (electOne()) {
                     fenceAfter();
-#pragma unroll
-                    for (int i = 0; i < kC / 16; ++i) productTmem(tmem + kO2, tmem + kP + i * 8, v + i * 128, kOthers, i > 0);
-                    commitTo(smemAddr(&oFull));
-                    commitTo(smemAddr(&freed[turn.at]));
+#pragma unroll 2
+                    for (int i = 0; i < kC / 16; ++i) productTmem(tmem + kO2, tmem + kP + parity * kC + (i / 4) * 64 + (i % 4) * 8, v + i * 128, kOutputs, i > 0);
+                    commitTo(smemAddr(&small.oFull));
+                    commitTo(smemAddr(&small.freed[turn.at]));
                 }
                 __syncwarp();
             }
         }
-    } else if (warp < kScoreWarps) {
+        // products go on after a wait that gave up, on whatever the operands hold; they end before the tensor memory is freed
+        if (electOne()) commitTo(smemAddr(&small.productsDone));
+        __syncwarp();
+        waitSuspended(smemAddr(&small.productsDone), 0);
+    } else if (warp < kFirstOutput) {
         if (!StateOnly) {
-            const int quarter = warp & 3, half = warp >> 2, i = 32 * quarter + lane;   // the thread's token; of each block of 32 columns it takes 16
+            // The thread's token, and the half of the columns that it takes: their scores lie in 64 columns of tensor memory, whose first 32 take what becomes of them.
+            const int quarter = warp & 3, half = warp >> 2, i = 32 * quarter + lane;
+            auto empty = [&](int block) { return reverse ? block < quarter : block > quarter; };
+            for (int u = 0; u < count; ++u) {
+                const int n = tokensOf(span.chunkAt(u, reverse));
+                const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + kP + (u & 1) * kC + half * 64;
+                // f(block, scores times the decays) for the two blocks of 32 columns that are not empty
+                auto eachBlock = [&](auto f) {
+#pragma unroll 1
+                    for (int e = 0; e < 2; ++e) {
+                        const int block = 2 * half + e;
+                        if (empty(block)) continue;
+                        uint32_t r[32];
+                        loadTmem32(lanes + e * 32, r);
+                        loadsDone();
+                        if (block == quarter) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                const int apart = reverse ? j - lane : lane - j;
+                                r[j] = apart >= 0 ? __float_as_uint(__uint_as_float(r[j]) * small.scaledPowers[max(apart, 0)]) : 0u;
+                            }
+                        } else {
+                            const float power = small.powers[reverse ? block * 32 - i : i - block * 32 - 31];
+                            const Pair row = pairOf(power, power);
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4) {
+                                const float4 c = *reinterpret_cast<const float4 *>(&small.columnPowers[j]);
+                                const float2 a = floatsOf(mul2(mul2(pairOf(r[j], r[j + 1]), pairOf(c.x, c.y)), row)), b2 = floatsOf(mul2(mul2(pairOf(r[j + 2], r[j + 3]), pairOf(c.z, c.w)), row));
+                                r[j] = __float_as_uint(a.x);
+                                r[j + 1] = __float_as_uint(a.y);
+                                r[j + 2] = __float_as_uint(b2.x);
+                                r[j + 3] = __float_as_uint(b2.y);
+                            }
+                        }
+                        if (reverse && block * 32 + 32 > n) {   // tokens behind the row's end may hold anything
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (block * 32 + j >= n) r[j] = 0u;
+                        }
+                        f(e, r);
+                    }
+                };
+                wait(small.pFull[u & 1], (u >> 1) & 1);
+                fenceAfter();
+                float up = 1.f;
+                if constexpr (kHalf) {
+                    float most = 0.f;
+                    eachBlock([&](int, const uint32_t(&r)[32]) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(__uint_as_float(r[j])));
+                    });
+                    small.rowPeaks[half][i] = most;
+                    groupBarrier(kLanesMeet + quarter, 64);
+                    up = toTopOfHalf(fmaxf(most, small.rowPeaks[half ^ 1][i]));
+                    if (half == 0) small.rowScale[u % 3][i] = static_cast<uint8_t>(__float_as_uint(up) >> 23);
+                    groupBarrier(kLanesMeet + quarter, 64);
+                }
+                eachBlock([&](int e, const uint32_t(&r)[32]) {
+                    uint32_t words[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) words[j] = kHalf ? pack2<T>(mul2(pairOf(r[2 * j], r[2 * j + 1]), pairOf(up, up))) : pack2<T>(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                    storeTmem16(lanes + e * 16, words);
+                });
+#pragma unroll 1
+                for (int e = 0; e < 2; ++e)   // the scores of these are all read by now
+                    if (empty(2 * half + e)) storeTmem16(lanes + e * 16, {});
+                tmemStoresDone();
+                fenceBefore();
+                arriveWarp(small.pReady[u & 1]);
+            }
+        }
+    } else if (warp < kFirstState) {
+        if (!StateOnly) {
+            const int quarter = warp & 3, i = 32 * quarter + lane;   // the thread's token
             const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
             for (int u = 0; u < count; ++u) {
                 const uint32_t parity = u & 1;
                 const int chunk = span.chunkAt(u, reverse), n = tokensOf(chunk);
-                wait(pFull, parity);
+                wait(small.oFull, parity);
                 fenceAfter();
-                // bfloat16 is packed block by block; half waits for the largest score of the row
-                constexpr int kKept = kHalf ? 4 : 1;
-                float scores[kKept][16];
-                uint32_t words[4][8] = {};
-                float most = 0.f;
-                auto empty = [&](int block) { return reverse ? block < quarter : block > quarter; };
-#pragma unroll
-                for (int block = 0; block < 4; ++block) {
-                    if (empty(block)) continue;
-                    float(&mine)[16] = scores[kHalf ? block : 0];
-                    uint32_t r[16];
-                    loadTmem16(lanes + kP + block * 32 + half * 16, r);
-                    loadsDone();
-                    const int first = block * 32 + half * 16;
-                    if (block == quarter) {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const int apart = reverse ? first + j - i : i - first - j;
-                            const bool in = apart >= 0 && (!reverse || first + j < n);
-                            mine[j] = in ? __uint_as_float(r[j]) * powers[max(apart, 0)] * p.outScale : 0.f;
-                        }
-                    } else {
-                        const float row = p.outScale * powers[reverse ? block * 32 - i : i - block * 32 - 31];
-#pragma unroll
-                        for (int j = 0; j < 16; j += 4) {
-                            const float4 c = *reinterpret_cast<const float4 *>(&columnPowers[half * 16 + j]);
-                            const float cs[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) mine[j + e] = __uint_as_float(r[j + e]) * cs[e] * row;
-                        }
-                        if (reverse && n < kC) {   // tokens behind the row's end may hold anything
-#pragma unroll
-                            for (int j = 0; j < 16; ++j)
-                                if (first + j >= n) mine[j] = 0.f;
-                        }
-                    }
-                    if constexpr (kHalf) {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(mine[j]));
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) words[block][j] = pack2<T>(mine[2 * j], mine[2 * j + 1]);
-                    }
-                }
+                const bool live = i < n, in = chunk * kC + i < p.tokens && alive && p.out;
+                const float inter = live ? p.outScale * small.powers[reverse ? n - 1 - i : i + 1] * (kHalf ? small.stateScale[parity] : 1.f) : 0.f;
                 float back = 1.f;
-                if (kHalf) rowPeaks[half][i] = most;
-                groupBarrier(4 + quarter, 64);   // both warps of these lanes have read P, which is written over
-                if constexpr (kHalf) {
-                    const float up = toTopOfHalf(fmaxf(most, rowPeaks[half ^ 1][i]));
-                    back = 1.f / up;
-#pragma unroll
-                    for (int block = 0; block < 4; ++block)
-                        if (!empty(block))
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) words[block][j] = pack2<T>(scores[block][2 * j] * up, scores[block][2 * j + 1] * up);
-                }
-#pragma unroll
-                for (int block = 0; block < 4; ++block) storeTmem8(lanes + kP + block * 16 + half * 8, words[block]);
-                tmemStoresDone();
-                fenceBefore();
-                arriveWarp(pReady);
-
-                wait(oFull, parity);
-                fenceAfter();
-                const bool live = i < n;
-                const float inter = live ? p.outScale * powers[reverse ? n - 1 - i : i + 1] * (kHalf ? stateScale[parity] : 1.f) : 0.f;
-                float out[32];
-#pragma unroll
-                for (int part = 0; part < 2; ++part) {
+                if constexpr (kHalf) back = __uint_as_float((254u - small.rowScale[u % 3][i]) << 23);
+                const size_t row = ((static_cast<size_t>(b) * p.tokens + chunk * kC + i) * p.heads + h) * p.value;
+                // One round of code for all parts: warps of every role fetch instructions from the same cache, and unrolled they halve one another's speed.
+#pragma unroll 1
+                for (int part = 0; part < 4; ++part) {
                     uint32_t o1[16], o2[16];
-                    loadTmem16(lanes + kO1 + half * 32 + part * 16, o1);
-                    loadTmem16(lanes + kO2 + half * 32 + part * 16, o2);
+                    loadTmem16(lanes + kO1 + part * 16, o1);
+                    loadTmem16(lanes + kO2 + part * 16, o2);
                     loadsDone();
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) out[part * 16 + j] = live ? fmaf(__uint_as_float(o1[j]), inter, __uint_as_float(o2[j]) * back) : 0.f;
-                }
-                fenceBefore();
-                arriveWarp(oFree);
-                if (storeBoxes) {
-                    if (tid == 0) storesRead();   // the tile's last copy
-                    groupBarrier(1, 32 * kScoreWarps);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) w[j] = pack2<T>(out[8 * c + 2 * j], out[8 * c + 2 * j + 1]);
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(oTile + i * 128 + (((half * 4 + c) ^ (i & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                    if (part == 3) {
+                        fenceBefore();
+                        arriveWarp(small.oFree);
                     }
-                    fenceAsyncProxy();
-                    groupBarrier(1, 32 * kScoreWarps);
-                    if (tid == 0 && alive) storeTile4(&outMap, oTile, slice * kCols, h, chunk * kC, b);
-                } else if (p.out && chunk * kC + i < p.tokens && alive) {
-                    const int col = slice * kCols + half * 32;
-                    const size_t at = ((static_cast<size_t>(b) * p.tokens + chunk * kC + i) * p.heads + h) * p.value + col;
-                    if (p.outFloat && p.value % 4 == 0) {
+                    const int col = slice * kCols + part * 16;
+                    if (!in || col >= p.value) continue;
+                    uint32_t w[8];
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4)
-                            if (col + j < p.value) *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at + j) = make_float4(out[j], out[j + 1], out[j + 2], out[j + 3]);
-                    } else {
+                    for (int j = 0; j < 16; j += 2) {
+                        const Pair scaled = kHalf ? mul2(pairOf(o2[j], o2[j + 1]), pairOf(back, back)) : pairOf(o2[j], o2[j + 1]);
+                        float2 v = floatsOf(fma2(pairOf(o1[j], o1[j + 1]), pairOf(inter, inter), scaled));
+                        if (!live) v = make_float2(0.f, 0.f);
+                        if constexpr (Wide) {
+                            w[j / 2] = pack2<T>(v.x, v.y);
+                        } else {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            if (col + j >= p.value) continue;
-                            if (p.outFloat) static_cast<float *>(p.out)[at + j] = out[j];
-                            else static_cast<T *>(p.out)[at + j] = fromFloat<T>(out[j]);
+                            for (int e = 0; e < 2; ++e) {
+                                if (col + j + e >= p.value) continue;
+                                if (p.outFloat) static_cast<float *>(p.out)[row + col + j + e] = e ? v.y : v.x;
+                                else static_cast<T *>(p.out)[row + col + j + e] = fromFloat<T>(e ? v.y : v.x);
+                            }
                         }
                     }
+                    if constexpr (Wide)   // a sector of memory a thread
+                        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(static_cast<T *>(p.out) + row + col), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                                     "r"(w[6]), "r"(w[7])
+                                     : "memory");
                 }
             }
-            if (storeBoxes && tid == 0) storesDone();
         }
     } else {
-        const int quarter = warp & 3, half = (warp - kScoreWarps) >> 2, d = 32 * quarter + lane;   // the thread's row of the state, and which half of its columns and of the tokens
-        const bool rows = 32 * quarter < DK;                                                     // warps beyond the keys have none
+        const int quarter = warp & 3, half = (warp - kFirstState) >> 2, d = 32 * quarter + lane;   // the thread's row of the state, and which half of its columns
+        const bool rows = 32 * quarter < DK;                                                   // warps beyond the keys have none
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
-        const int stid = tid - 32 * kScoreWarps;
+        const int stid = tid - 32 * kFirstState;
         const size_t head = static_cast<size_t>(b) * p.heads + h, stateSize = static_cast<size_t>(p.key) * p.value;
         const int col = slice * kCols + half * 32;
-        float s[32];
+        Pair s[16];   // its 32 columns
         const float *in = segments.count > 1 ? (StateOnly ? nullptr : segments.states + (head * segments.count + segment) * stateSize) : p.stateIn ? p.stateIn + head * stateSize : nullptr;
         const int inRow = segments.count > 1 ? p.value : p.stateRow, inCol = segments.count > 1 ? 1 : p.stateCol;
         const float inScale = segments.count > 1 ? 1.f : p.inScale;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = in && d < p.key && col + j < p.value ? inScale * in[static_cast<size_t>(d) * inRow + static_cast<size_t>(col + j) * inCol] : 0.f;
+        for (int j = 0; j < 16; ++j) {
+            float v[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int c = col + 2 * j + e;
+                v[e] = in && d < p.key && c < p.value ? inScale * in[static_cast<size_t>(d) * inRow + static_cast<size_t>(c) * inCol] : 0.f;
+            }
+            s[j] = pairOf(v[0], v[1]);
+        }
 
         auto publish = [&](int u) {   // the state in front of chunk u, as the B operand of O1
             float up = 1.f;
             if constexpr (kHalf) {
                 float most = 0.f;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(s[j]));
+                for (int j = 0; j < 16; ++j) {
+                    const float2 v = floatsOf(s[j]);
+                    most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y)));
+                }
                 const uint32_t peak = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-                if (lane == 0) statePeaks[stid >> 5] = __uint_as_float(peak);
-                groupBarrier(2, 32 * kStateWarps);
+                if (lane == 0) small.statePeaks[stid >> 5] = __uint_as_float(peak);
+                groupBarrier(kStateMeets, 32 * kStateWarps);
                 most = 0.f;
 #pragma unroll
-                for (int w = 0; w < kStateWarps; ++w) most = fmaxf(most, statePeaks[w]);
+                for (int w = 0; w < kStateWarps; ++w) most = fmaxf(most, small.statePeaks[w]);
                 up = toTopOfHalf(most);
-                if (stid == 0) stateScale[u & 1] = 1.f / up;
-                groupBarrier(2, 32 * kStateWarps);
+                if (stid == 0) small.stateScale[u & 1] = 1.f / up;
+                groupBarrier(kStateMeets, 32 * kStateWarps);
             }
             if (rows) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     uint32_t w[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) w[j] = pack2<T>(s[8 * c + 2 * j] * up, s[8 * c + 2 * j + 1] * up);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sTile + d * 128 + (((half * 4 + c) ^ (d & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                    for (int j = 0; j < 4; ++j) w[j] = kHalf ? pack2<T>(mul2(s[4 * c + j], pairOf(up, up))) : pack2<T>(s[4 * c + j]);
+                    storeShared(sTile + d * 128 + (((half * 4 + c) ^ (d & 7)) << 4), w[0], w[1], w[2], w[3]);
                 }
                 fenceAsyncProxy();
             }
-            arriveWarp(sReady);
+            arriveWarp(small.sReady);
         };
         if (!StateOnly && count > 0) publish(0);
 
-        // byte of element d in each of eight rows of a tile of K
-        const uint32_t element = (d & 63) * 2, kHalfTile = (d >> 6) * kTile;
+        const int token = stid >> 1;   // of whose 64 values this thread weights 32
         Turn turn;
-        int weighted = -1;   // tokens that `weights` is for
         for (int u = 0; u < count; ++u, turn.step(kStages)) {
             const uint32_t parity = u & 1, at = tiles + turn.at * kStageBytes;
             const int chunk = span.chunkAt(u, reverse), n = tokensOf(chunk);
-            if (weighted != n) {
-                groupBarrier(2, 32 * kStateWarps);
-                if (stid < kC) weights[stid] = stid < n ? powers[reverse ? stid + 1 : n - 1 - stid] : 0.f;
-                groupBarrier(2, 32 * kStateWarps);
-                weighted = n;
-            }
-            wait(full[turn.at], turn.parity);
-            if (n < kC && chunk * kC + n < p.tokens) {   // V behind the row's end may hold anything, and zero times that is not zero
-                for (int i = n * 8 + stid; i < kC * 8; i += 32 * kStateWarps)
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + 2 * kHalves * kTile + i * 16), "r"(0u) : "memory");
+            wait(small.full[turn.at], turn.parity);
+            if (n < kC && chunk * kC + n < p.tokens) {   // K and V behind the row's end may hold anything, and zero times that is not zero
+                for (int i = (kHalves * kC + n) * 8 + stid; i < (2 * kHalves + 1) * kC * 8; i += 32 * kStateWarps)
+                    if ((i / 8) % kC >= n) storeShared(at + i * 16, 0u, 0u, 0u, 0u);
                 fenceAsyncProxy();
+                groupBarrier(kStateMeets, 32 * kStateWarps);
             }
-            if (rows) {
-                const uint32_t keys = at + kHalves * kTile + kHalfTile;
+            const float w = token < n ? small.powers[reverse ? token + 1 : n - 1 - token] : 0.f;
 #pragma unroll 1
-                for (int j0 = half * 64; j0 < half * 64 + 64; j0 += 16) {
-                    uint32_t hi[8], mid[8], lo[8];
+            for (int c = 0; c < 4; ++c) {
+                const uint32_t place = token * 128 + ((((stid & 1) * 4 + c) ^ (token & 7)) << 4);
+                uint32_t v[4], hi[4], mid[4], lo[4];
+                loadShared(at + 2 * kHalves * kTile + place, v);
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
-                        const float4 w4 = *reinterpret_cast<const float4 *>(&weights[j0 + j]);
-                        const float w[4] = {w4.x, w4.y, w4.z, w4.w};
-                        float x[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t r = (j + e) & 7;   // the place of token j0 + j + e among eight rows
-                            uint16_t bits;
-                            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(keys + (j0 + j + e) * 128 + (element ^ (r << 4))) : "memory");
-                            const T value = *reinterpret_cast<const T *>(&bits);
-                            x[e] = n == kC || j0 + j + e < n ? toFloat(value) * w[e] : 0.f;
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; e += 2) {
-                            const int word = (j + e) / 2;
-                            hi[word] = pack2<T>(x[e], x[e + 1]);
-                            float2 back = unpack2<T>(hi[word]);
-                            float r0 = x[e] - back.x, r1 = x[e + 1] - back.y;
-                            if constexpr (kHalf) {
-                                mid[word] = pack2<T>(r0 * 2048.f, r1 * 2048.f);
-                                lo[word] = 0u;
-                            } else {
-                                mid[word] = pack2<T>(r0, r1);
-                                back = unpack2<T>(mid[word]);
-                                lo[word] = pack2<T>(r0 - back.x, r1 - back.y);
-                            }
-                        }
-                    }
-                    const uint32_t to = lanes + kWeightedK + j0 / 2;
-                    storeTmem8(to, hi);
-                    storeTmem8(to + 64, mid);
-                    if (!kHalf && terms > 2) storeTmem8(to + 128, lo);
+                for (int j = 0; j < 4; ++j) {
+                    auto less = [&](Pair x, uint32_t term) {   // what a term leaves; exact
+                        const float2 t = unpack2<T>(term);
+                        return fma2(pairOf(t.x, t.y), pairOf(-1.f, -1.f), x);
+                    };
+                    const float2 x = unpack2<T>(v[j]);
+                    const Pair weighted = mul2(pairOf(x.x, x.y), pairOf(w, w));
+                    hi[j] = pack2<T>(weighted);
+                    Pair rest = less(weighted, hi[j]);
+                    if constexpr (kHalf) rest = mul2(rest, pairOf(2048.f, 2048.f));
+                    mid[j] = pack2<T>(rest);
+                    if constexpr (!kHalf) lo[j] = pack2<T>(less(rest, mid[j]));
                 }
-                tmemStoresDone();
+                storeShared(weightedV + place, hi[0], hi[1], hi[2], hi[3]);
+                storeShared(weightedV + kTile + place, mid[0], mid[1], mid[2], mid[3]);
+                if constexpr (!kHalf)
+                    if (terms > 2) storeShared(weightedV + 2 * kTile + place, lo[0], lo[1], lo[2], lo[3]);
             }
-            fenceBefore();
-            arriveWarp(aReady);
+            fenceAsyncProxy();
+            arriveWarp(small.vReady);
 
-            wait(kvFull, parity);
+            wait(small.kvFull, parity);
             fenceAfter();
-            const float keep = powers[n];
+            const float keep = small.powers[n];
             if (rows) {
 #pragma unroll
                 for (int part = 0; part < 2; ++part) {
-                    uint32_t r[16];
+                    uint32_t r[16], low[16];
                     loadTmem16(lanes + kKV + half * 32 + part * 16, r);
-                    if constexpr (kHalf) {
-                        uint32_t low[16];
-                        loadTmem16(lanes + kKVLow + half * 32 + part * 16, low);
-                        loadsDone();
+                    loadTmem16(lanes + kKV + kCols + half * 32 + part * 16, low);
+                    loadsDone();
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(fmaf(__uint_as_float(low[j]), 1.f / 2048, __uint_as_float(r[j])));
-                    } else {
-                        loadsDone();
+                    for (int j = 0; j < 8; ++j) {
+                        const Pair high = pairOf(r[2 * j], r[2 * j + 1]), rest = pairOf(low[2 * j], low[2 * j + 1]);
+                        s[part * 8 + j] = fma2(s[part * 8 + j], pairOf(keep, keep), kHalf ? fma2(rest, pairOf(1.f / 2048, 1.f / 2048), high) : add2(high, rest));
                     }
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) s[part * 16 + j] = fmaf(s[part * 16 + j], keep, __uint_as_float(r[j]));
                 }
             }
+            fenceBefore();
             if (!StateOnly && u + 1 < count) {
-                wait(sFree, parity);
+                wait(small.sFree, parity);
                 publish(u + 1);
             }
         }
@@ -468,11 +498,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int outRow = StateOnly ? p.value : p.stateRow, outCol = StateOnly ? 1 : p.stateCol;
             const float scale = StateOnly ? 1.f : p.finalScale;
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (d < p.key && col + j < p.value) last[static_cast<size_t>(d) * outRow + static_cast<size_t>(col + j) * outCol] = s[j] * scale;
+            for (int j = 0; j < 16; ++j) {
+                const float2 v = floatsOf(s[j]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int c = col + 2 * j + e;
+                    if (d < p.key && c < p.value) last[static_cast<size_t>(d) * outRow + static_cast<size_t>(c) * outCol] = (e ? v.y : v.x) * scale;
+                }
+            }
         }
     }
-    if (!alive && lane == 0) failed = 1;
+    if (!alive && lane == 0) small.failed = 1;
     if (!StateOnly && p.out) {   // tokens behind the last chunk, of those that lie in this segment's stretch of time
         const int from = max(span.total, segment * segments.chunks) * kC, to = min(p.tokens, (segment + 1) * segments.chunks * kC);
         const int width = min(kCols, p.value - slice * kCols);
@@ -485,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     fenceBefore();
     __syncthreads();
     if (warp == kProductWarp) freeTmem<1>(tmem, 512);
-    if (tid == 0 && failed) atomicExch(status, 1);
+    if (tid == 0 && small.failed) atomicExch(status, 1);
 }
 
 // From the ends of the segments on their own to their beginnings: one thread for each element of a state, segment after segment.
@@ -545,12 +581,7 @@ void launchChunks(const Pass &p, int type, const ChunkPlan &plan, float *states,
     bool ok = true;
     bindContext();
     const CUtensorMap q = tokenMap(p.q, p.batch, p.tokens, p.key, bf16, ok), k = tokenMap(p.k, p.batch, p.tokens, p.key, bf16, ok), v = tokenMap(p.v, p.batch, p.tokens, p.value, bf16, ok);
-    const bool storeBoxes = p.out && !p.outFloat && p.value % 8 == 0 && alignedTo(p.out, 16);
-    CUtensorMap out = q;
-    if (storeBoxes) {
-        const int64_t row = static_cast<int64_t>(p.heads) * p.value;
-        out = tokenMap({p.out, row * p.tokens, row, p.value, p.heads}, p.batch, p.tokens, p.value, bf16, ok);
-    }
+    const bool wide = !p.outFloat && p.value % 16 == 0 && alignedTo(p.out, 32);   // parts of a row start on 32 bytes
     if (!ok) fail(RXMET_ERR_CUDA, "cuTensorMapEncodeTiled failed");
     const Segments segments{plan.segments, plan.segmentChunks, states};
     const dim3 grid((p.value + kCols - 1) / kCols * plan.segments, p.heads, p.batch);
@@ -558,7 +589,7 @@ void launchChunks(const Pass &p, int type, const ChunkPlan &plan, float *states,
         ensureDynamicSmem(reinterpret_cast<const void *>(kernel), kShared);
         {
             KernelTimer timer__(name, st);
-            launchDependent(kernel, grid, kThreads, kShared, st, p, q, k, v, out, storeBoxes, segments, terms, waitStatus());
+            launchDependent(kernel, grid, kThreads, kShared, st, p, q, k, v, segments, terms, waitStatus());
         }
         afterLaunch(name);
     };
@@ -568,14 +599,14 @@ void launchChunks(const Pass &p, int type, const ChunkPlan &plan, float *states,
         using T = decltype(t);
         constexpr int DK = decltype(dk)::value;
         if (plan.segments > 1) {
-            run(decayedChunks<T, DK, true>, "decayedChunksState", terms);
+            run(decayedChunks<T, DK, true, true>, "decayedChunksState", terms);
             {
                 KernelTimer timer__("joinSegments", st);
                 launchDependent(joinSegments, dim3((p.key * p.value + 255) / 256, p.heads, p.batch), 256, 0, st, p, segments);
             }
             afterLaunch("joinSegments");
         }
-        if (p.out || plan.segments == 1) run(decayedChunks<T, DK, false>, "decayedChunks", plan.segments > 1 ? 2 : terms);
+        if (p.out || plan.segments == 1) run(wide ? decayedChunks<T, DK, false, true> : decayedChunks<T, DK, false, false>, "decayedChunks", plan.segments > 1 ? 2 : terms);
     };
     auto withKeys = [&](auto t) {
         if (p.key <= 64) both(t, std::integral_constant<int, 64>{});

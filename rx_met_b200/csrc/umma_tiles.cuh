@@ -36,13 +36,6 @@ __device__ __forceinline__ void copyTile4(uint32_t to, const CUtensorMap *map, i
                  "r"(bar)
                  : "memory");
 }
-// Back to memory, in the issuing thread's bulk group; what lies beyond the array is dropped.
-__device__ __forceinline__ void storeTile4(const CUtensorMap *map, uint32_t from, int x, int y, int z, int w) {
-    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map), "r"(from), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-}
-__device__ __forceinline__ void storesRead() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void storesDone() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void fenceAsyncProxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void prefetchMap(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
@@ -75,9 +68,9 @@ __device__ __forceinline__ void productI8(uint32_t tmem, uint64_t a, uint64_t b,
         asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
                      : "memory");
 }
-// kind::f16, 32-bit sums, 128 rows of A: operand formats (0 half, 1 bfloat16) in [7,10) and [10,13); B MN-major with bit 16.
-__host__ __device__ constexpr uint32_t halves(bool bf16, int n, bool bMnMajor) {
-    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (bMnMajor ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kTileM >> 4) << 24);
+// kind::f16, 32-bit sums, 128 rows of A: operand formats (0 half, 1 bfloat16) in [7,10) and [10,13); A MN-major with bit 15, B with bit 16.
+__host__ __device__ constexpr uint32_t halves(bool bf16, int n, bool aMnMajor, bool bMnMajor) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (aMnMajor ? 1u << 15 : 0u) | (bMnMajor ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kTileM >> 4) << 24);
 }
 __device__ __forceinline__ void product(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
@@ -86,11 +79,6 @@ __device__ __forceinline__ void product(uint32_t tmem, uint64_t a, uint64_t b, u
 // A in tensor memory: lane = row, a column holds two neighbours along K.
 __device__ __forceinline__ void productTmem(uint32_t tmem, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-                 : "memory");
-}
-__device__ __forceinline__ void storeTmem8(uint32_t at, const uint32_t (&v)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
-                 "r"(v[7])
                  : "memory");
 }
 __device__ __forceinline__ void tmemStoresDone() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -115,6 +103,23 @@ __device__ __forceinline__ void loadTmem8(uint32_t at, uint32_t (&r)[8]) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(at));
 }
+__device__ __forceinline__ void loadTmem32(uint32_t at, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at));
+}
+__device__ __forceinline__ void storeTmem16(uint32_t at, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+        "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
 __device__ __forceinline__ void loadsDone() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fenceBefore() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fenceAfter() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -125,6 +130,35 @@ __device__ __forceinline__ void arriveRemote(uint32_t bar) { asm volatile("mbarr
 
 // Binds the current device's context to this thread, which encoding a tensor map needs: a thread of the autograd engine may come here without one.
 inline void bindContext() { RXMET_CUDA(cudaSetDevice(currentDevice().device)); }
+
+// Two 32-bit floats in one operation each.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pairOf(float a, float b) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ Pair pairOf(uint32_t a, uint32_t b) { return pairOf(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ float2 floatsOf(Pair p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
 
 // A word of the current device that kernels set where a bounded wait gave up; their output is not written then.
 int *waitStatus();

@@ -102,7 +102,7 @@ struct Small {
     float powers[kC + 4], scaledPowers[32], columnPowers[32];   // l^n; scale l^n; scale l^(31 - j) or scale l^j of a block's columns
     float rowPeaks[2][kC], statePeaks[kStateWarps], stateScale[2];
     uint8_t rowScale[3][kC];                  // exponents of the powers of two that rows of P were scaled by, for three chunks
-    uint64_t full[3], freed[3], pFull[2], pReady[2], vReady, kvFull, sReady, sFree, oFull, oFree, productsDone;
+    uint64_t fullK[3], fullQ[3], fullV[3], freeK[3], freeQ[3], freeV[3], pFull[2], pReady[2], vReady, kvFull, sReady, sFree, oFull, oFree, productsDone;
     uint32_t tmemSlot;
     int failed;
 };
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) {
         small.failed = 0;
         for (int i = 0; i < kStages; ++i)
-            for (uint64_t *bar : {&small.full[i], &small.freed[i]}) cluster::initBarrier(bar, 1);
+            for (uint64_t *bar : {&small.fullK[i], &small.fullQ[i], &small.fullV[i], &small.freeK[i], &small.freeQ[i], &small.freeV[i]}) cluster::initBarrier(bar, 1);
         // Those of P are one for each of its buffers: a chunk's scores may be done before the products have asked for those of the chunk before.
         for (uint64_t *bar : {&small.pFull[0], &small.pFull[1], &small.kvFull, &small.sFree, &small.oFull, &small.productsDone}) cluster::initBarrier(bar, 1);
         for (uint64_t *bar : {&small.pReady[0], &small.pReady[1]}) cluster::initBarrier(bar, kScoreWarps);
@@ -170,27 +170,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kCopyWarp) {
         Turn turn;
         for (int u = 0; u < count; ++u, turn.step(kStages)) {
-            if (turn.again) wait(small.freed[turn.at], turn.parity ^ 1u);
-            if (alive && electOne()) {
-                const uint32_t bar = smemAddr(&small.full[turn.at]), to = tiles + turn.at * kStageBytes;
-                const int t = span.chunkAt(u, reverse) * kC;
-                cluster::arriveExpect(bar, StateOnly ? (kHalves + 1) * kTile : kStageBytes);
-                for (int i = 0; i < kHalves; ++i) copyTile4(to + (kHalves + i) * kTile, &kMap, 64 * i, h / (p.heads / p.k.heads), t, b, bar);
-                if (!StateOnly)
-                    for (int i = 0; i < kHalves; ++i) copyTile4(to + i * kTile, &qMap, 64 * i, h / (p.heads / p.q.heads), t, b, bar);
-                copyTile4(to + 2 * kHalves * kTile, &vMap, slice * kCols, h / (p.heads / p.v.heads), t, b, bar);
-            }
-            __syncwarp();
+            // each as soon as its last use is over, in the order in which that is
+            const uint32_t to = tiles + turn.at * kStageBytes;
+            const int t = span.chunkAt(u, reverse) * kC;
+            auto fetch = [&](uint64_t &full, uint64_t &free, const CUtensorMap &map, uint32_t place, int boxes, int x, int head) {
+                if (turn.again) wait(free, turn.parity ^ 1u);
+                if (alive && electOne()) {
+                    cluster::arriveExpect(smemAddr(&full), boxes * kTile);
+                    for (int i = 0; i < boxes; ++i) copyTile4(to + place + i * kTile, &map, x + 64 * i, head, t, b, smemAddr(&full));
+                }
+                __syncwarp();
+            };
+            fetch(small.fullK[turn.at], small.freeK[turn.at], kMap, kHalves * kTile, kHalves, 0, h / (p.heads / p.k.heads));
+            if (!StateOnly) fetch(small.fullQ[turn.at], small.freeQ[turn.at], qMap, 0, kHalves, 0, h / (p.heads / p.q.heads));
+            fetch(small.fullV[turn.at], small.freeV[turn.at], vMap, 2 * kHalves * kTile, 1, slice * kCols, h / (p.heads / p.v.heads));
         }
         // nothing is left in flight: the last use of each stage is over
         for (int i = 0; i < kStages; ++i, turn.step(kStages))
-            if (turn.again) waitSuspended(smemAddr(&small.freed[turn.at]), turn.parity ^ 1u);
+            if (turn.again) {
+                waitSuspended(smemAddr(&small.freeK[turn.at]), turn.parity ^ 1u);
+                if (!StateOnly) waitSuspended(smemAddr(&small.freeQ[turn.at]), turn.parity ^ 1u);
+                waitSuspended(smemAddr(&small.freeV[turn.at]), turn.parity ^ 1u);
+            }
     } else if (warp == kProductWarp) {
         constexpr uint32_t kScores = halves(!kHalf, kC, false, false), kOutputs = halves(!kHalf, kCols, false, true);
         constexpr uint32_t kBothTerms = halves(!kHalf, 2 * kCols, true, true), kThirdTerm = halves(!kHalf, kCols, true, true);
         Turn turn, next;   // stages of this chunk and of the one whose scores are next
         auto scores = [&](int u) {
-            wait(small.full[next.at], next.parity);
+            wait(small.fullK[next.at], next.parity);
+            wait(small.fullQ[next.at], next.parity);
             if (u > 1) wait(small.oFull, u & 1);   // the product that read this buffer of P, of chunk u - 2
             if (electOne()) {
                 fenceAfter();
@@ -211,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t at = tiles + turn.at * kStageBytes, parity = u & 1;
             const uint64_t q = swizzledDescriptor(at), kAcross = swizzledDescriptor(at + kHalves * kTile, kTile), v = swizzledDescriptor(at + 2 * kHalves * kTile),
                            weighted = swizzledDescriptor(weightedV, kTile), third = swizzledDescriptor(weightedV + 2 * kTile), s = swizzledDescriptor(sTile);
-            if (StateOnly) wait(small.full[turn.at], turn.parity);
+            if (StateOnly) wait(small.fullK[turn.at], turn.parity);
             wait(small.vReady, parity);
             if (electOne()) {
                 fenceAfter();
@@ -222,7 +230,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int i = 0; i < kC / 16; ++i) product(tmem + kKV + kCols, kAcross + i * 128, third + i * 128, kThirdTerm, 1);
                 }
                 commitTo(smemAddr(&small.kvFull));
-                if (StateOnly) commitTo(smemAddr(&small.freed[turn.at]));
+                commitTo(smemAddr(&small.freeK[turn.at]));
+                if (StateOnly) commitTo(smemAddr(&small.freeV[turn.at]));
             }
             __syncwarp();
             if (!StateOnly) {
@@ -233,6 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 2
                     for (int i = 0; i < DK / 16; ++i) product(tmem + kO1, q + (i / 4) * (kTile >> 4) + (i % 4) * 2, s + i * 128, kOutputs, i > 0);
                     commitTo(smemAddr(&small.sFree));
+                    commitTo(smemAddr(&small.freeQ[turn.at]));
                 }
                 __syncwarp();
                 if (u + 1 < count) scores(u + 1);
@@ -242,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 2
                     for (int i = 0; i < kC / 16; ++i) productTmem(tmem + kO2, tmem + kP + parity * kC + (i / 4) * 64 + (i % 4) * 8, v + i * 128, kOutputs, i > 0);
                     commitTo(smemAddr(&small.oFull));
-                    commitTo(smemAddr(&small.freed[turn.at]));
+                    commitTo(smemAddr(&small.freeV[turn.at]));
                 }
                 __syncwarp();
             }
@@ -435,8 +445,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int u = 0; u < count; ++u, turn.step(kStages)) {
             const uint32_t parity = u & 1, at = tiles + turn.at * kStageBytes;
             const int chunk = span.chunkAt(u, reverse), n = tokensOf(chunk);
-            wait(small.full[turn.at], turn.parity);
+            wait(small.fullV[turn.at], turn.parity);
             if (n < kC && chunk * kC + n < p.tokens) {   // K and V behind the row's end may hold anything, and zero times that is not zero
+                wait(small.fullK[turn.at], turn.parity);
                 for (int i = (kHalves * kC + n) * 8 + stid; i < (2 * kHalves + 1) * kC * 8; i += 32 * kStateWarps)
                     if ((i / 8) % kC >= n) storeShared(at + i * 16, 0u, 0u, 0u, 0u);
                 fenceAsyncProxy();

@@ -4,8 +4,8 @@
 //   O = scale (l^(i+1) Q S + ((Q K') . [i >= j] l^(i-j)) V)          S <- l^n S + K'^T diag(l^(n-1-j)) V
 // Exponents are differences of places in a chunk and never negative, so that no power overflows.  A CTA walks over the chunks of one head and of 64 columns of V, warps by role:
 //   copies     Q, K and V of the next chunks as TMA boxes with a 128-byte swizzle
-//   products   one thread issues P = Q K', KV = K'^T (weighted V), O1 = Q S and O2 = P V; P has two buffers, so that the scores of a chunk and the outputs of the one before
-//              are worked on at the same time
+//   products   two threads issue KV = K'^T (weighted V) and O1 = Q S, and P = Q K' and O2 = P V; P has two buffers,
+//              so that the next product may run under a chunk's scores
 //   scores     eight warps: P from tensor memory, times the decays, back as the A operand of the last product
 //   outputs    four warps: O1 and O2 to memory, 32 bytes a thread and store
 //   state      eight warps: weighted V for the products; the state itself, 32 bits, stays in their registers
@@ -28,12 +28,12 @@ using namespace ummatiles;
 constexpr int kC = kChunkTokens;
 constexpr int kCols = 64;              // columns of V a CTA takes
 constexpr int kScoreWarps = 8, kOutputWarps = 4, kStateWarps = 8;
-constexpr int kFirstOutput = kScoreWarps, kFirstState = kFirstOutput + kOutputWarps, kCopyWarp = kFirstState + kStateWarps, kProductWarp = kCopyWarp + 1;
-constexpr int kThreads = 32 * (kProductWarp + 1);
+constexpr int kFirstOutput = kScoreWarps, kFirstState = kFirstOutput + kOutputWarps, kCopyWarp = kFirstState + kStateWarps, kStateProducts = kCopyWarp + 1, kScoreProducts = kStateProducts + 1;
+constexpr int kThreads = 32 * (kScoreProducts + 1);
 constexpr uint32_t kTile = kC * 128;   // 128 rows of 64 elements
 constexpr uint32_t kShared = 232448;   // all of an SM, as the tensor memory
-// columns of tensor memory: two buffers of P, then the others
-constexpr uint32_t kP = 0, kO1 = 256, kO2 = 320, kKV = 384;   // KV: the larger term, then the others
+// columns of tensor memory: two buffers of P, then the others; KV is the larger term and then the others
+constexpr uint32_t kP = 0, kO1 = 256, kO2 = 320, kKV = 384;
 enum Barrier { kStateMeets = 1, kLanesMeet };   // named barriers; the last takes four
 
 // Shared memory in groups of 16 bytes.
@@ -102,7 +102,7 @@ struct Small {
     float powers[kC + 4], scaledPowers[32], columnPowers[32];   // l^n; scale l^n; scale l^(31 - j) or scale l^j of a block's columns
     float rowPeaks[2][kC], statePeaks[kStateWarps], stateScale[2];
     uint8_t rowScale[3][kC];                  // exponents of the powers of two that rows of P were scaled by, for three chunks
-    uint64_t fullK[3], fullQ[3], fullV[3], freeK[3], freeQ[3], freeV[3], pFull[2], pReady[2], vReady, kvFull, sReady, sFree, oFull, oFree, productsDone;
+    uint64_t fullK[3], fullQ[3], fullV[3], freeK[3], freeQ[3], freeV[3], vRead[3], pFull[2], pReady[2], pFree[2], vReady, kvFull, sReady, sFree, oFull, oFree, productsDone[2];
     uint32_t tmemSlot;
     int failed;
 };
@@ -132,14 +132,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Span span(length, segment, segments.chunks);
     const int count = span.chunks;
     auto tokensOf = [&](int chunk) { return min(kC, length - chunk * kC); };
+    // Whether the third term of a chunk's weighted V can reach the state at the row's end: what is left of it there is l^(tokens from here on), and two terms
+    // leave 2^-17.
+    const float third = terms > 2 ? p.logDecay[h] : -INFINITY;
+    auto thirdTerm = [&](int u) {
+        const int chunk = span.chunkAt(u, reverse), rest = reverse ? chunk * kC : max(0, length - (chunk + 1) * kC);
+        return terms > 2 && (rest == 0 || third * rest > -6.9f);   // 2^-10
+    };
 
     if (tid == 0) {
         small.failed = 0;
         for (int i = 0; i < kStages; ++i)
-            for (uint64_t *bar : {&small.fullK[i], &small.fullQ[i], &small.fullV[i], &small.freeK[i], &small.freeQ[i], &small.freeV[i]}) cluster::initBarrier(bar, 1);
-        // Those of P are one for each of its buffers: a chunk's scores may be done before the products have asked for those of the chunk before.
-        for (uint64_t *bar : {&small.pFull[0], &small.pFull[1], &small.kvFull, &small.sFree, &small.oFull, &small.productsDone}) cluster::initBarrier(bar, 1);
+            for (uint64_t *bar : {&small.fullK[i], &small.fullQ[i], &small.fullV[i], &small.freeV[i]}) cluster::initBarrier(bar, 1);
+        constexpr int kUsers = StateOnly ? 1 : 2;   // threads whose products read K and Q, and write O1 and O2
+        for (int i = 0; i < kStages; ++i)
+            for (uint64_t *bar : {&small.freeK[i], &small.freeQ[i]}) cluster::initBarrier(bar, kUsers);
+        cluster::initBarrier(&small.oFull, kUsers);
+        for (uint64_t *bar : {&small.pFull[0], &small.pFull[1], &small.pFree[0], &small.pFree[1], &small.kvFull, &small.sFree, &small.productsDone[0], &small.productsDone[1]}) cluster::initBarrier(bar, 1);
+        // Barriers for each buffer of P: a chunk's scores may be done before the products have asked for those of the chunk before.
         for (uint64_t *bar : {&small.pReady[0], &small.pReady[1]}) cluster::initBarrier(bar, kScoreWarps);
+        // One for each stage: the state may be two chunks ahead of the scores, and a barrier in its phase after next looks like one that is not over.
+        for (int i = 0; i < kStages; ++i) cluster::initBarrier(&small.vRead[i], kStateWarps);
         cluster::initBarrier(&small.oFree, kOutputWarps);
         for (uint64_t *bar : {&small.vReady, &small.sReady}) cluster::initBarrier(bar, kStateWarps);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -151,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int j = tid & 31, apart = tid < 288 || reverse ? j : 31 - j;
         (tid < 288 ? small.scaledPowers : small.columnPowers)[j] = p.outScale * (apart == 0 ? 1.f : static_cast<float>(exp(apart * static_cast<double>(p.logDecay[h]))));
     }
-    if (warp == kProductWarp) allocTmem<1>(smemAddr(&small.tmemSlot), 512);
+    if (warp == kStateProducts) allocTmem<1>(smemAddr(&small.tmemSlot), 512);
     fenceBefore();
     __syncthreads();
     fenceAfter();
@@ -192,75 +205,94 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!StateOnly) waitSuspended(smemAddr(&small.freeQ[turn.at]), turn.parity ^ 1u);
                 waitSuspended(smemAddr(&small.freeV[turn.at]), turn.parity ^ 1u);
             }
-    } else if (warp == kProductWarp) {
+    } else if (warp >= kStateProducts) {
+        // Two threads issue the products, those of the state and those of the scores: one alone came to 4200 cycles a chunk, of which the tensor cores work 1300.  They poll, because a
+        // vote of the warp after each wait costs 150 cycles.
         constexpr uint32_t kScores = halves(!kHalf, kC, false, false), kOutputs = halves(!kHalf, kCols, false, true);
         constexpr uint32_t kBothTerms = halves(!kHalf, 2 * kCols, true, true), kThirdTerm = halves(!kHalf, kCols, true, true);
-        Turn turn, next;   // stages of this chunk and of the one whose scores are next
-        auto scores = [&](int u) {
-            wait(small.fullK[next.at], next.parity);
-            wait(small.fullQ[next.at], next.parity);
-            if (u > 1) wait(small.oFull, u & 1);   // the product that read this buffer of P, of chunk u - 2
-            if (electOne()) {
-                fenceAfter();
-                const uint32_t at = tiles + next.at * kStageBytes;
-                const uint64_t q = swizzledDescriptor(at), k = swizzledDescriptor(at + kHalves * kTile);
-#pragma unroll 2
-                for (int i = 0; i < 4 * kHalves; ++i) {
-                    const uint64_t step = (i / 4) * (kTile >> 4) + (i % 4) * 2;
-                    product(tmem + kP + (u & 1) * kC, q + step, k + step, kScores, i > 0);
-                }
-                commitTo(smemAddr(&small.pFull[u & 1]));
-            }
-            __syncwarp();
-            next.step(kStages);
+        auto poll = [&](uint64_t &bar, uint32_t parity) {
+            if (alive) alive = waitPhase(smemAddr(&bar), parity);
+            fenceAfter();
         };
-        if (!StateOnly && count > 0) scores(0);
-        for (int u = 0; u < count; ++u, turn.step(kStages)) {
-            const uint32_t at = tiles + turn.at * kStageBytes, parity = u & 1;
-            const uint64_t q = swizzledDescriptor(at), kAcross = swizzledDescriptor(at + kHalves * kTile, kTile), v = swizzledDescriptor(at + 2 * kHalves * kTile),
-                           weighted = swizzledDescriptor(weightedV, kTile), third = swizzledDescriptor(weightedV + 2 * kTile), s = swizzledDescriptor(sTile);
-            if (StateOnly) wait(small.fullK[turn.at], turn.parity);
-            wait(small.vReady, parity);
+        if (warp == kStateProducts) {
             if (electOne()) {
-                fenceAfter();
+                Turn turn;
+                const uint64_t weighted = swizzledDescriptor(weightedV, kTile), third = swizzledDescriptor(weightedV + 2 * kTile), s = swizzledDescriptor(sTile);
+                for (int u = 0; u < count; ++u, turn.step(kStages)) {
+                    const uint32_t at = tiles + turn.at * kStageBytes, parity = u & 1, kv = tmem + kKV;
+                    const uint64_t q = swizzledDescriptor(at), k = swizzledDescriptor(at + kHalves * kTile, kTile);
+                    poll(small.fullK[turn.at], turn.parity);
+                    poll(small.vReady, parity);
 #pragma unroll 2
-                for (int i = 0; i < kC / 16; ++i) product(tmem + kKV, kAcross + i * 128, weighted + i * 128, kBothTerms, i > 0);
-                if (terms > 2) {
+                    for (int i = 0; i < kC / 16; ++i) product(kv, k + i * 128, weighted + i * 128, kBothTerms, i > 0);
+                    if (!kHalf && thirdTerm(u)) {
 #pragma unroll 2
-                    for (int i = 0; i < kC / 16; ++i) product(tmem + kKV + kCols, kAcross + i * 128, third + i * 128, kThirdTerm, 1);
-                }
-                commitTo(smemAddr(&small.kvFull));
-                commitTo(smemAddr(&small.freeK[turn.at]));
-                if (StateOnly) commitTo(smemAddr(&small.freeV[turn.at]));
-            }
-            __syncwarp();
-            if (!StateOnly) {
-                wait(small.sReady, parity);
-                if (u > 0) wait(small.oFree, parity ^ 1u);
-                if (electOne()) {
-                    fenceAfter();
+                        for (int i = 0; i < kC / 16; ++i) product(kv + kCols, k + i * 128, third + i * 128, kThirdTerm, 1);
+                    }
+                    commitTo(smemAddr(&small.kvFull));
+                    commitTo(smemAddr(&small.freeK[turn.at]));
+                    if (StateOnly) {
+                        commitTo(smemAddr(&small.freeV[turn.at]));
+                        continue;
+                    }
+                    poll(small.fullQ[turn.at], turn.parity);
+                    poll(small.sReady, parity);
+                    if (u > 0) poll(small.oFree, parity ^ 1u);
 #pragma unroll 2
                     for (int i = 0; i < DK / 16; ++i) product(tmem + kO1, q + (i / 4) * (kTile >> 4) + (i % 4) * 2, s + i * 128, kOutputs, i > 0);
                     commitTo(smemAddr(&small.sFree));
                     commitTo(smemAddr(&small.freeQ[turn.at]));
-                }
-                __syncwarp();
-                if (u + 1 < count) scores(u + 1);
-                wait(small.pReady[parity], (u >> 1) & 1);
-                if (electOne()) {
-                    fenceAfter();
-#pragma unroll 2
-                    for (int i = 0; i < kC / 16; ++i) productTmem(tmem + kO2, tmem + kP + parity * kC + (i / 4) * 64 + (i % 4) * 8, v + i * 128, kOutputs, i > 0);
                     commitTo(smemAddr(&small.oFull));
-                    commitTo(smemAddr(&small.freeV[turn.at]));
                 }
-                __syncwarp();
+            }
+        } else if (!StateOnly && electOne()) {
+            // whichever is ready: neither the scores of the next chunk nor the outputs of this one keep the other waiting
+            Turn scoreTurn, outTurn;
+            uint32_t idle = 0;
+            for (int next = 0, u = 0; u < count && alive;) {
+                bool worked = false;
+                if (next < count && next <= u + 1 && testPhase(smemAddr(&small.fullK[scoreTurn.at]), scoreTurn.parity) && testPhase(smemAddr(&small.fullQ[scoreTurn.at]), scoreTurn.parity) &&
+                    (next < 2 || testPhase(smemAddr(&small.pFree[next & 1]), ((next >> 1) - 1) & 1))) {
+                    fenceAfter();
+                    const uint32_t at = tiles + scoreTurn.at * kStageBytes;
+                    const uint64_t q = swizzledDescriptor(at), k = swizzledDescriptor(at + kHalves * kTile);
+#pragma unroll 2
+                    for (int i = 0; i < 4 * kHalves; ++i) {
+                        const uint64_t step = (i / 4) * (kTile >> 4) + (i % 4) * 2;
+                        product(tmem + kP + (next & 1) * kC, q + step, k + step, kScores, i > 0);
+                    }
+                    commitTo(smemAddr(&small.pFull[next & 1]));
+                    commitTo(smemAddr(&small.freeK[scoreTurn.at]));
+                    commitTo(smemAddr(&small.freeQ[scoreTurn.at]));
+                    ++next;
+                    scoreTurn.step(kStages);
+                    worked = true;
+                }
+                // V is clean behind the row's end, and has been read for its weighted form, once the state says so
+                if (u < next && testPhase(smemAddr(&small.pReady[u & 1]), (u >> 1) & 1) && testPhase(smemAddr(&small.vRead[outTurn.at]), outTurn.parity) &&
+                    (u == 0 || testPhase(smemAddr(&small.oFree), (u - 1) & 1))) {
+                    fenceAfter();
+                    const uint64_t v = swizzledDescriptor(tiles + outTurn.at * kStageBytes + 2 * kHalves * kTile);
+#pragma unroll 2
+                    for (int i = 0; i < kC / 16; ++i) productTmem(tmem + kO2, tmem + kP + (u & 1) * kC + (i / 4) * 64 + (i % 4) * 8, v + i * 128, kOutputs, i > 0);
+                    commitTo(smemAddr(&small.pFree[u & 1]));
+                    commitTo(smemAddr(&small.oFull));
+                    commitTo(smemAddr(&small.freeV[outTurn.at]));
+                    ++u;
+                    outTurn.step(kStages);
+                    worked = true;
+                }
+                idle = worked ? 0 : idle + 1;
+                alive = idle < kSpinLimit;
             }
         }
-        // products go on after a wait that gave up, on whatever the operands hold; they end before the tensor memory is freed
-        if (electOne()) commitTo(smemAddr(&small.productsDone));
         __syncwarp();
-        waitSuspended(smemAddr(&small.productsDone), 0);
+        // products go on after a wait that gave up, on whatever the operands hold; they end before the tensor memory is freed
+        uint64_t &done = small.productsDone[warp - kStateProducts];
+        if (electOne()) commitTo(smemAddr(&done));
+        __syncwarp();
+        waitSuspended(smemAddr(&done), 0);
+        alive = __all_sync(0xffffffffu, alive);
     } else if (warp < kFirstOutput) {
         if (!StateOnly) {
             // The thread's token, and the half of the columns that it takes: their scores lie in 64 columns of tensor memory, whose first 32 take what becomes of them.
@@ -438,13 +470,32 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             arriveWarp(small.sReady);
         };
-        if (!StateOnly && count > 0) publish(0);
 
+        auto advance = [&](int u) {   // the state behind chunk u
+            const float keep = small.powers[tokensOf(span.chunkAt(u, reverse))];
+            if (rows) {
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {
+                    uint32_t r[16], low[16];
+                    const uint32_t from = lanes + kKV + half * 32 + part * 16;
+                    loadTmem16(from, r);
+                    loadTmem16(from + kCols, low);
+                    loadsDone();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const Pair high = pairOf(r[2 * j], r[2 * j + 1]), rest = pairOf(low[2 * j], low[2 * j + 1]);
+                        s[part * 8 + j] = fma2(s[part * 8 + j], pairOf(keep, keep), kHalf ? fma2(rest, pairOf(1.f / 2048, 1.f / 2048), high) : add2(high, rest));
+                    }
+                }
+            }
+            fenceBefore();
+        };
         const int token = stid >> 1;   // of whose 64 values this thread weights 32
         Turn turn;
         for (int u = 0; u < count; ++u, turn.step(kStages)) {
             const uint32_t parity = u & 1, at = tiles + turn.at * kStageBytes;
             const int chunk = span.chunkAt(u, reverse), n = tokensOf(chunk);
+            if (u > 0) advance(u - 1);
             wait(small.fullV[turn.at], turn.parity);
             if (n < kC && chunk * kC + n < p.tokens) {   // K and V behind the row's end may hold anything, and zero times that is not zero
                 wait(small.fullK[turn.at], turn.parity);
@@ -453,8 +504,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 fenceAsyncProxy();
                 groupBarrier(kStateMeets, 32 * kStateWarps);
             }
+            const bool withThird = thirdTerm(u);
             const float w = token < n ? small.powers[reverse ? token + 1 : n - 1 - token] : 0.f;
-#pragma unroll 1
+#pragma unroll 2
             for (int c = 0; c < 4; ++c) {
                 const uint32_t place = token * 128 + ((((stid & 1) * 4 + c) ^ (token & 7)) << 4);
                 uint32_t v[4], hi[4], mid[4], lo[4];
@@ -476,34 +528,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                 storeShared(weightedV + place, hi[0], hi[1], hi[2], hi[3]);
                 storeShared(weightedV + kTile + place, mid[0], mid[1], mid[2], mid[3]);
                 if constexpr (!kHalf)
-                    if (terms > 2) storeShared(weightedV + 2 * kTile + place, lo[0], lo[1], lo[2], lo[3]);
+                    if (withThird) storeShared(weightedV + 2 * kTile + place, lo[0], lo[1], lo[2], lo[3]);
             }
             fenceAsyncProxy();
+            if (!StateOnly) arriveWarp(small.vRead[turn.at]);
             arriveWarp(small.vReady);
 
+            if (!StateOnly) {   // under the product of this chunk: the state in front of it
+                if (u > 0) wait(small.sFree, parity ^ 1u);
+                publish(u);
+            }
             wait(small.kvFull, parity);
             fenceAfter();
-            const float keep = small.powers[n];
-            if (rows) {
-#pragma unroll
-                for (int part = 0; part < 2; ++part) {
-                    uint32_t r[16], low[16];
-                    loadTmem16(lanes + kKV + half * 32 + part * 16, r);
-                    loadTmem16(lanes + kKV + kCols + half * 32 + part * 16, low);
-                    loadsDone();
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const Pair high = pairOf(r[2 * j], r[2 * j + 1]), rest = pairOf(low[2 * j], low[2 * j + 1]);
-                        s[part * 8 + j] = fma2(s[part * 8 + j], pairOf(keep, keep), kHalf ? fma2(rest, pairOf(1.f / 2048, 1.f / 2048), high) : add2(high, rest));
-                    }
-                }
-            }
-            fenceBefore();
-            if (!StateOnly && u + 1 < count) {
-                wait(small.sFree, parity);
-                publish(u + 1);
-            }
         }
+        if (count > 0) advance(count - 1);
         float *last = StateOnly ? segments.states + (head * segments.count + segment) * stateSize : segments.count > 1 || !p.stateOut ? nullptr : p.stateOut + head * stateSize;
         if (last && alive) {
             const int outRow = StateOnly ? p.value : p.stateRow, outCol = StateOnly ? 1 : p.stateCol;
@@ -531,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     fenceBefore();
     __syncthreads();
-    if (warp == kProductWarp) freeTmem<1>(tmem, 512);
+    if (warp == kStateProducts) freeTmem<1>(tmem, 512);
     if (tid == 0 && small.failed) atomicExch(status, 1);
 }
 

@@ -29,12 +29,19 @@ constexpr int kC = kChunkTokens;
 constexpr int kCols = 64;              // columns of V a CTA takes
 constexpr int kScoreWarps = 8, kOutputWarps = 4, kStateWarps = 8;
 constexpr int kFirstOutput = kScoreWarps, kFirstState = kFirstOutput + kOutputWarps, kCopyWarp = kFirstState + kStateWarps, kStateProducts = kCopyWarp + 1, kScoreProducts = kStateProducts + 1;
-constexpr int kThreads = 32 * (kScoreProducts + 1);
+constexpr int kThreads = 32 * 24;   // the last warp has no work: registers are dealt to groups of four warps
 constexpr uint32_t kTile = kC * 128;   // 128 rows of 64 elements
 constexpr uint32_t kShared = 232448;   // all of an SM, as the tensor memory
 // columns of tensor memory: two buffers of P, then the others; KV is the larger term and then the others
 constexpr uint32_t kP = 0, kO1 = 256, kO2 = 320, kKV = 384;
 enum Barrier { kStateMeets = 1, kLanesMeet };   // named barriers; the last takes four
+
+// A block starts with 80 registers a thread, 1920 for the lanes of its 24 warps in the same place.  The scores keep theirs (8 warps, 640); outputs give up 16 (4 warps, 256), copies
+// and products 40 (4 warps, 160), and the state takes 104 (8 warps, 832): 1888.  With 80 the state would be spilled (advance() 420 -> 1700 cycles).
+template <int REGISTERS>
+__device__ __forceinline__ void giveRegisters() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGISTERS)); }
+template <int REGISTERS>
+__device__ __forceinline__ void takeRegisters() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGISTERS)); }
 
 // Shared memory in groups of 16 bytes.
 __device__ __forceinline__ void loadShared(uint32_t at, uint32_t (&v)[4]) {
@@ -137,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float third = terms > 2 ? p.logDecay[h] : -INFINITY;
     auto thirdTerm = [&](int u) {
         const int chunk = span.chunkAt(u, reverse), rest = reverse ? chunk * kC : max(0, length - (chunk + 1) * kC);
-        return terms > 2 && (rest == 0 || third * rest > -6.9f);   // 2^-10
+        return terms > 2 && (rest == 0 || third * rest > -2.77f);   // 2^-4: two terms are 2^-21 of the state there
     };
 
     if (tid == 0) {
@@ -180,6 +187,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) arrive(smemAddr(&bar));
     };
 
+    if (warp >= kCopyWarp) {
+        giveRegisters<40>();
     if (warp == kCopyWarp) {
         Turn turn;
         for (int u = 0; u < count; ++u, turn.step(kStages)) {
@@ -205,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!StateOnly) waitSuspended(smemAddr(&small.freeQ[turn.at]), turn.parity ^ 1u);
                 waitSuspended(smemAddr(&small.freeV[turn.at]), turn.parity ^ 1u);
             }
-    } else if (warp >= kStateProducts) {
+    } else if (warp <= kScoreProducts) {
         // Two threads issue the products, those of the state and those of the scores: one alone came to 4200 cycles a chunk, of which the tensor cores work 1300.  They poll, because a
         // vote of the warp after each wait costs 150 cycles.
         constexpr uint32_t kScores = halves(!kHalf, kC, false, false), kOutputs = halves(!kHalf, kCols, false, true);
@@ -293,6 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         waitSuspended(smemAddr(&done), 0);
         alive = __all_sync(0xffffffffu, alive);
+    }
     } else if (warp < kFirstOutput) {
         if (!StateOnly) {
             // The thread's token, and the half of the columns that it takes: their scores lie in 64 columns of tensor memory, whose first 32 take what becomes of them.
@@ -367,6 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else if (warp < kFirstState) {
+        giveRegisters<64>();
         if (!StateOnly) {
             const int quarter = warp & 3, i = 32 * quarter + lane;   // the thread's token
             const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
@@ -418,6 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else {
+        takeRegisters<104>();
         const int quarter = warp & 3, half = (warp - kFirstState) >> 2, d = 32 * quarter + lane;   // the thread's row of the state, and which half of its columns
         const bool rows = 32 * quarter < DK;                                                   // warps beyond the keys have none
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
@@ -491,11 +503,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             fenceBefore();
         };
         const int token = stid >> 1;   // of whose 64 values this thread weights 32
+        const uint32_t place = token * 128, piece = (stid & 1) * 4;
+        auto pieceAt = [&](int c) { return place + (((piece + c) ^ (token & 7)) << 4); };
+        auto weightOf = [&](int n) { return token < n ? small.powers[reverse ? token + 1 : n - 1 - token] : 0.f; };
+        auto less = [&](Pair x, uint32_t term) {   // what a term leaves; exact
+            const float2 t = unpack2<T>(term);
+            return fma2(pairOf(t.x, t.y), pairOf(-1.f, -1.f), x);
+        };
+        uint32_t hi[4][4], mid[4][4];   // the two larger terms of the next chunk's weighted V
         Turn turn;
-        for (int u = 0; u < count; ++u, turn.step(kStages)) {
-            const uint32_t parity = u & 1, at = tiles + turn.at * kStageBytes;
+        auto weigh = [&](int u) {
+            const uint32_t at = tiles + turn.at * kStageBytes;
             const int chunk = span.chunkAt(u, reverse), n = tokensOf(chunk);
-            if (u > 0) advance(u - 1);
             wait(small.fullV[turn.at], turn.parity);
             if (n < kC && chunk * kC + n < p.tokens) {   // K and V behind the row's end may hold anything, and zero times that is not zero
                 wait(small.fullK[turn.at], turn.parity);
@@ -504,40 +523,55 @@ __global__ void __launch_bounds__(kThreads, 1)
                 fenceAsyncProxy();
                 groupBarrier(kStateMeets, 32 * kStateWarps);
             }
-            const bool withThird = thirdTerm(u);
-            const float w = token < n ? small.powers[reverse ? token + 1 : n - 1 - token] : 0.f;
-#pragma unroll 2
-            for (int c = 0; c < 4; ++c) {
-                const uint32_t place = token * 128 + ((((stid & 1) * 4 + c) ^ (token & 7)) << 4);
-                uint32_t v[4], hi[4], mid[4], lo[4];
-                loadShared(at + 2 * kHalves * kTile + place, v);
+            const float w = weightOf(n);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) loadShared(at + 2 * kHalves * kTile + pieceAt(c), hi[c]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    auto less = [&](Pair x, uint32_t term) {   // what a term leaves; exact
-                        const float2 t = unpack2<T>(term);
-                        return fma2(pairOf(t.x, t.y), pairOf(-1.f, -1.f), x);
-                    };
-                    const float2 x = unpack2<T>(v[j]);
+                    const float2 x = unpack2<T>(hi[c][j]);
                     const Pair weighted = mul2(pairOf(x.x, x.y), pairOf(w, w));
-                    hi[j] = pack2<T>(weighted);
-                    Pair rest = less(weighted, hi[j]);
+                    hi[c][j] = pack2<T>(weighted);
+                    Pair rest = less(weighted, hi[c][j]);
                     if constexpr (kHalf) rest = mul2(rest, pairOf(2048.f, 2048.f));
-                    mid[j] = pack2<T>(rest);
-                    if constexpr (!kHalf) lo[j] = pack2<T>(less(rest, mid[j]));
+                    mid[c][j] = pack2<T>(rest);
                 }
-                storeShared(weightedV + place, hi[0], hi[1], hi[2], hi[3]);
-                storeShared(weightedV + kTile + place, mid[0], mid[1], mid[2], mid[3]);
-                if constexpr (!kHalf)
-                    if (withThird) storeShared(weightedV + 2 * kTile + place, lo[0], lo[1], lo[2], lo[3]);
+        };
+        if (count > 0) weigh(0);
+        for (int u = 0; u < count; ++u) {
+            const uint32_t parity = u & 1;
+            if (u > 0) advance(u - 1);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                storeShared(weightedV + pieceAt(c), hi[c][0], hi[c][1], hi[c][2], hi[c][3]);
+                storeShared(weightedV + kTile + pieceAt(c), mid[c][0], mid[c][1], mid[c][2], mid[c][3]);
+            }
+            if (!kHalf && thirdTerm(u)) {
+                const float w = weightOf(tokensOf(span.chunkAt(u, reverse)));
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t v[4];
+                    loadShared(tiles + turn.at * kStageBytes + 2 * kHalves * kTile + pieceAt(c), v);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 x = unpack2<T>(v[j]);
+                        v[j] = pack2<T>(less(less(mul2(pairOf(x.x, x.y), pairOf(w, w)), hi[c][j]), mid[c][j]));
+                    }
+                    storeShared(weightedV + 2 * kTile + pieceAt(c), v[0], v[1], v[2], v[3]);
+                }
             }
             fenceAsyncProxy();
             if (!StateOnly) arriveWarp(small.vRead[turn.at]);
             arriveWarp(small.vReady);
 
-            if (!StateOnly) {   // under the product of this chunk: the state in front of it
+            // under the product of this chunk: the state in front of it, and the terms of the next one
+            if (!StateOnly) {
                 if (u > 0) wait(small.sFree, parity ^ 1u);
                 publish(u);
             }
+            turn.step(kStages);
+            if (u + 1 < count) weigh(u + 1);
             wait(small.kvFull, parity);
             fenceAfter();
         }

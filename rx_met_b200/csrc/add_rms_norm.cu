@@ -1,8 +1,8 @@
 // Residual addition with a root-mean-square norm (to the input's type, or to 8-bit codes with a scale for each row), and its gradient.
 //
-// One pass over the data: a team of 1 to 32 warps holds a row in registers, so that the sum, the largest magnitude and the output need no
+// One pass over the data: a team of 8 to 512 threads holds a row in registers, so that the sum, the largest magnitude and the output need no
 // second read.  A team walks over rows, which keeps the weights in registers, and asks for its next row before it works on this one.
-// Sums run in 32 bits: a lane's own elements in order, lanes and warps as a fixed tree, so that results do not depend on the launch.
+// Sums run in 32 bits: a thread's own elements in order, lanes as a tree, warps in order, so that results do not depend on the grid.
 //
 // Bound: HBM.
 #include <algorithm>
@@ -15,11 +15,11 @@ namespace rxmet {
 namespace {
 
 constexpr int kMaxWidth = 16384;
-constexpr int kMaxWarps = 32;
+constexpr int kMaxThreads = 512, kMaxWarps = kMaxThreads / 32;
 
 struct NormRows {
     int64_t rows;
-    int width, teamWarps;
+    int width, team;   // team: its threads, a power of two up to 32 or a multiple of it
     const void *x, *residual, *weight;
     int64_t xPitch, residualPitch;
     int weightType;
@@ -31,33 +31,36 @@ struct NormRows {
     float *scale;
 };
 
-__device__ __forceinline__ float warpSum(float v) {
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    return v;
-}
-// Sum over the warps of a team; `slot` alternates between two arrays from row to row, so that one barrier is enough.
-__device__ __forceinline__ float teamSum(float v, int teamWarps, float (*shared)[kMaxWarps], int slot) {
-    v = warpSum(v);
-    if (teamWarps == 1) return v;
-    const int warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) shared[slot][warp] = v;
-    __syncthreads();
-    float sum = 0.f;
-    for (int i = 0; i < teamWarps; ++i) sum += shared[slot][i];
-    return sum;
-}
-// Largest magnitude as bits: patterns of non-negative floats order as integers, with NaN above infinity, so that a NaN is not lost.
-__device__ __forceinline__ uint32_t teamMax(uint32_t v, int teamWarps, uint32_t (*shared)[kMaxWarps], int slot) {
-    v = __reduce_max_sync(0xffffffffu, v);
-    if (teamWarps == 1) return v;
-    const int warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) shared[slot][warp] = v;
-    __syncthreads();
-    uint32_t most = 0;
-    for (int i = 0; i < teamWarps; ++i) most = max(most, shared[slot][i]);
-    return most;
-}
+// The place of a thread in its team.  Teams of a CTA work on rows of their own; those of several warps meet at a barrier of their own.
+struct Team {
+    int size, index, count, rank;
+    __device__ __forceinline__ explicit Team(int threads) : size(threads), index(threadIdx.x / threads), count(blockDim.x / threads), rank(threadIdx.x - index * threads) {}
+    template <class V>
+    __device__ __forceinline__ void meet(V (*shared)[kMaxWarps], int slot, V mine) const {
+        if ((threadIdx.x & 31) == 0) shared[slot][threadIdx.x >> 5] = mine;
+        asm volatile("bar.sync %0, %1;" ::"r"(index + 1), "r"(size) : "memory");
+    }
+    // `slot` alternates between two arrays from row to row, so that one barrier is enough.
+    __device__ __forceinline__ float sum(float v, float (*shared)[kMaxWarps], int slot) const {
+        for (int d = min(size, 32) / 2; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+        if (size <= 32) return v;
+        meet(shared, slot, v);
+        const int first = index * size / 32;
+        v = 0.f;
+        for (int i = 0; i < size / 32; ++i) v += shared[slot][first + i];
+        return v;
+    }
+    // Largest magnitude as bits: patterns of non-negative floats order as integers, with NaN above infinity, so that a NaN is not lost.
+    __device__ __forceinline__ uint32_t most(uint32_t v, uint32_t (*shared)[kMaxWarps], int slot) const {
+        for (int d = min(size, 32) / 2; d > 0; d >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
+        if (size <= 32) return v;
+        meet(shared, slot, v);
+        const int first = index * size / 32;
+        v = 0;
+        for (int i = 0; i < size / 32; ++i) v = max(v, shared[slot][first + i]);
+        return v;
+    }
+};
 
 __device__ __forceinline__ float weightAt(const void *weight, int type, int i) {
     if (type == RXMET_TYPE_F32) return static_cast<const float *>(weight)[i];
@@ -65,106 +68,122 @@ __device__ __forceinline__ float weightAt(const void *weight, int type, int i) {
     return toFloat(static_cast<const __half *>(weight)[i]);
 }
 
-// A thread's share of a row: ITEMS groups of W neighbouring elements, `stride` elements apart.
+// A thread's share of a row: ITEMS groups of W neighbouring elements, `stride` elements apart; what lies beyond the row is zero.
 template <class T, int W, int ITEMS>
 struct Share {
     Pack<T, W> v[ITEMS];
     __device__ __forceinline__ void load(const T *row, int first, int stride, int width) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
+        for (int i = 0; i < ITEMS; ++i) {
+            v[i] = {};
             if (first + i * stride < width) v[i] = *reinterpret_cast<const Pack<T, W> *>(row + first + i * stride);
+        }
     }
+    __device__ __forceinline__ float at(int i, int j) const { return toFloat(v[i].v[j]); }
 };
+template <class T, int W>
+__device__ __forceinline__ void put(T *row, int at, const float (&v)[W]) {
+    Pack<T, W> out;
+#pragma unroll
+    for (int j = 0; j < W; ++j) out.v[j] = fromFloat<T>(v[j]);
+    *reinterpret_cast<Pack<T, W> *>(row + at) = out;
+}
 
-// Teams of a CTA work on rows of their own; only a CTA of one team (more than one warp) has barriers.
-// THREADS: the most that a CTA may have, 512 or 1024.
-template <class T, int W, int ITEMS, bool Codes, int THREADS>
-__global__ void __launch_bounds__(THREADS) addRmsNorm(const __grid_constant__ NormRows p) {
+// Up to 16 elements a thread, the next row is in registers before this one is done and the weights stay there; wider rows have a thread's own loads to cover one another,
+// and read the weights again.
+template <int W, int ITEMS>
+constexpr bool kAhead = W *ITEMS <= 16;
+
+template <class T, int W, int ITEMS, bool Codes>
+__global__ void __launch_bounds__(kMaxThreads) addRmsNorm(const __grid_constant__ NormRows p) {
+    constexpr bool Ahead = kAhead<W, ITEMS>;
     __shared__ float sums[2][kMaxWarps];
     __shared__ uint32_t peaks[2][kMaxWarps];
-    const int teamThreads = p.teamWarps * 32, team = threadIdx.x / teamThreads, teams = blockDim.x / teamThreads;
-    const int first = (threadIdx.x - team * teamThreads) * W, stride = teamThreads * W, width = p.width;
+    const Team team(p.team);
+    const int first = team.rank * W, stride = team.size * W, width = p.width;
     const bool norm = p.weight != nullptr;
     waitForPredecessor();
-    float w[ITEMS][W];
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-        for (int j = 0; j < W; ++j) w[i][j] = norm && first + i * stride < width ? weightAt(p.weight, p.weightType, first + i * stride + j) : 1.f;
-
-    const int64_t step = static_cast<int64_t>(gridDim.x) * teams;
-    int64_t row = static_cast<int64_t>(blockIdx.x) * teams + team;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * team.count;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * team.count + team.index;
     Share<T, W, ITEMS> x, r;
     auto ask = [&](int64_t at) {
-        if (at >= p.rows) return;
+        at = min(at, p.rows - 1);   // past the end: a row that is there, and dropped
         x.load(static_cast<const T *>(p.x) + at * p.xPitch, first, stride, width);
         if (p.residual) r.load(static_cast<const T *>(p.residual) + at * p.residualPitch, first, stride, width);
     };
     ask(row);
+    float w[Ahead ? ITEMS : 1][W];
+    auto weights = [&](float(&to)[W], int i) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) to[j] = norm && first + i * stride < width ? weightAt(p.weight, p.weightType, first + i * stride + j) : 1.f;
+    };
+    if constexpr (Ahead)
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) weights(w[i], i);
     letDependentsStart();
-    for (int slot = 0; row < p.rows; row += step, slot ^= 1) {
+    // all teams of a warp go through the same number of rows, because they shuffle together
+    const int64_t rounds = (p.rows + step - 1) / step;
+    for (int64_t round = 0; round < rounds; ++round, row += step) {
+        const int slot = round & 1;
+        const bool real = row < p.rows;
         float t[ITEMS][W], sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const bool in = first + i * stride < width;
-#pragma unroll
-            for (int j = 0; j < W; ++j) {
-                t[i][j] = in ? toFloat(x.v[i].v[j]) + (p.residual ? toFloat(r.v[i].v[j]) : 0.f) : 0.f;
-                sum = fmaf(t[i][j], t[i][j], sum);
-            }
-        }
-        ask(row + step);
-        if (p.residual) {
-            T *total = static_cast<T *>(p.total) + row * width;
-#pragma unroll
-            for (int i = 0; i < ITEMS; ++i) {
-                Pack<T, W> out;
-#pragma unroll
-                for (int j = 0; j < W; ++j) out.v[j] = fromFloat<T>(t[i][j]);
-                if (first + i * stride < width) *reinterpret_cast<Pack<T, W> *>(total + first + i * stride) = out;
-            }
-        }
-        float rms = 1.f;
-        if (norm) {
-            rms = rsqrtf(teamSum(sum, p.teamWarps, sums, slot) / static_cast<float>(width) + p.eps);
-            if (p.rms && first == 0) p.rms[row] = rms;
-        }
-        uint32_t peak = 0;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                t[i][j] = t[i][j] * rms * w[i][j];
-                if (Codes && first + i * stride < width) peak = max(peak, __float_as_uint(t[i][j]) & 0x7fffffffu);
+                t[i][j] = p.residual ? x.at(i, j) + r.at(i, j) : x.at(i, j);
+                sum = fmaf(t[i][j], t[i][j], sum);
             }
-        if constexpr (Codes) {
-            const float most = __uint_as_float(teamMax(peak, p.teamWarps, peaks, slot));
-            const float inverse = most > 0.f ? 127.f / most : 0.f;
-            if (first == 0) p.scale[row] = most / 127.f;
-            int8_t *codes = p.codes + row * p.codesPitch;
+        if (Ahead && round + 1 < rounds) ask(row + step);
+        if (p.residual && real) {
+            T *total = static_cast<T *>(p.total) + row * width;
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i) {
-                Pack<int8_t, W> out;
+            for (int i = 0; i < ITEMS; ++i)
+                if (first + i * stride < width) put(total, first + i * stride, t[i]);
+        }
+        float rms = 1.f;
+        if (norm) {
+            rms = rsqrtf(team.sum(sum, sums, slot) / static_cast<float>(width) + p.eps);
+            if (p.rms && first == 0 && real) p.rms[row] = rms;
+        }
+        uint32_t peak = 0;
 #pragma unroll
-                for (int j = 0; j < W; ++j) out.v[j] = static_cast<int8_t>(__float2int_rn(fminf(fmaxf(t[i][j] * inverse, -127.f), 127.f)));
-                if (first + i * stride < width) *reinterpret_cast<Pack<int8_t, W> *>(codes + first + i * stride) = out;
-            }
-        } else {
-            T *y = static_cast<T *>(p.y) + row * width;
+        for (int i = 0; i < ITEMS; ++i) {
+            if constexpr (!Ahead) weights(w[0], i);
+            const bool in = first + i * stride < width;
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i) {
-                Pack<T, W> out;
-#pragma unroll
-                for (int j = 0; j < W; ++j) out.v[j] = fromFloat<T>(t[i][j]);
-                if (first + i * stride < width) *reinterpret_cast<Pack<T, W> *>(y + first + i * stride) = out;
+            for (int j = 0; j < W; ++j) {
+                t[i][j] = t[i][j] * rms * w[Ahead ? i : 0][j];
+                if (Codes && in) peak = max(peak, __float_as_uint(t[i][j]) & 0x7fffffffu);
             }
         }
+        if constexpr (Codes) {
+            const float most = __uint_as_float(team.most(peak, peaks, slot));
+            const float inverse = most > 0.f ? 127.f / most : 0.f;
+            if (real) {
+                if (first == 0) p.scale[row] = most / 127.f;
+                int8_t *codes = p.codes + row * p.codesPitch;
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i) {
+                    Pack<int8_t, W> out;
+#pragma unroll
+                    for (int j = 0; j < W; ++j) out.v[j] = static_cast<int8_t>(__float2int_rn(fminf(fmaxf(t[i][j] * inverse, -127.f), 127.f)));
+                    if (first + i * stride < width) *reinterpret_cast<Pack<int8_t, W> *>(codes + first + i * stride) = out;
+                }
+            }
+        } else if (real) {
+            T *y = static_cast<T *>(p.y) + row * width;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (first + i * stride < width) put(y, first + i * stride, t[i]);
+        }
+        if (!Ahead && round + 1 < rounds) ask(row + step);
     }
 }
 
 struct NormGradient {
     int64_t rows;
-    int width, teamWarps;
+    int width, team;
     const void *dy, *dtotal, *x, *residual, *weight;
     int64_t xPitch, residualPitch;
     const float *rms;
@@ -173,75 +192,92 @@ struct NormGradient {
     float *partial;   // [CTAs][width], null where dweight is not wanted
 };
 
-// The sum is taken from x and residual again: from its rounded copy, dweight of a bfloat16 step would be off by 1.6e-3 in place of 1.6e-7.
-template <class T, int W, int ITEMS, int THREADS>
-__global__ void __launch_bounds__(THREADS) addRmsNormGrad(const __grid_constant__ NormGradient p) {
+// The sum is taken from x and residual again: from its rounded copy, dweight of a bfloat16 step would be off by 1.6e-3 in place of 1.6e-7.  Sums of dweight over a team's
+// rows stay in registers, of wide rows in shared memory, where each element has one thread.
+template <class T, int W, int ITEMS>
+__global__ void __launch_bounds__(kMaxThreads) addRmsNormGrad(const __grid_constant__ NormGradient p) {
+    constexpr bool Ahead = kAhead<W, ITEMS>;
     __shared__ float sums[2][kMaxWarps];
-    extern __shared__ float teamPartial[];   // [teams][width] where a CTA has more than one team
-    const int teamThreads = p.teamWarps * 32, team = threadIdx.x / teamThreads, teams = blockDim.x / teamThreads;
-    const int first = (threadIdx.x - team * teamThreads) * W, stride = teamThreads * W, width = p.width;
+    extern __shared__ float teamPartial[];   // [teams][width]
+    const Team team(p.team);
+    const int first = team.rank * W, stride = team.size * W, width = p.width;
     waitForPredecessor();
-    float w[ITEMS][W], dw[ITEMS][W];
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-            w[i][j] = first + i * stride < width ? weightAt(p.weight, p.weightType, first + i * stride + j) : 0.f;
-            dw[i][j] = 0.f;
-        }
-    const int64_t step = static_cast<int64_t>(gridDim.x) * teams;
-    int64_t row = static_cast<int64_t>(blockIdx.x) * teams + team;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * team.count;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * team.count + team.index;
     Share<T, W, ITEMS> dy, dt, x, r;
     float rmsNext = 0.f;
     auto ask = [&](int64_t at) {
-        if (at >= p.rows) return;
-        dy.load(static_cast<const T *>(p.dy) + at * width, first, stride, width);
+        const bool real = at < p.rows;
+        at = min(at, p.rows - 1);
+        dy.load(static_cast<const T *>(p.dy) + at * width, first, stride, real ? width : 0);   // a row past the end adds nothing
         x.load(static_cast<const T *>(p.x) + at * p.xPitch, first, stride, width);
         if (p.residual) r.load(static_cast<const T *>(p.residual) + at * p.residualPitch, first, stride, width);
         if (p.dtotal) dt.load(static_cast<const T *>(p.dtotal) + at * width, first, stride, width);
         rmsNext = p.rms[at];
     };
     ask(row);
+    float *mine = teamPartial + static_cast<size_t>(team.index) * width;
+    float w[Ahead ? ITEMS : 1][W], dw[Ahead ? ITEMS : 1][W];
+    auto weights = [&](float(&to)[W], int i) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) to[j] = first + i * stride < width ? weightAt(p.weight, p.weightType, first + i * stride + j) : 0.f;
+    };
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        if constexpr (Ahead) {
+            weights(w[i], i);
+#pragma unroll
+            for (int j = 0; j < W; ++j) dw[i][j] = 0.f;
+        } else if (p.partial && first + i * stride < width) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) mine[first + i * stride + j] = 0.f;
+        }
+    }
     letDependentsStart();
-    for (int slot = 0; row < p.rows; row += step, slot ^= 1) {
+    const int64_t rounds = (p.rows + step - 1) / step;
+    for (int64_t round = 0; round < rounds; ++round, row += step) {
         const float rms = rmsNext;
-        float u[ITEMS][W], d[ITEMS][W], add[ITEMS][W], sum = 0.f;
+        float u[ITEMS][W], sum = 0.f;
+        const Share<T, W, ITEMS> g = dy, add = dt;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
+            if constexpr (!Ahead) weights(w[0], i);
             const bool in = first + i * stride < width;
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                const float g = in ? toFloat(dy.v[i].v[j]) : 0.f;
-                u[i][j] = in ? (toFloat(x.v[i].v[j]) + (p.residual ? toFloat(r.v[i].v[j]) : 0.f)) * rms : 0.f;
-                add[i][j] = in && p.dtotal ? toFloat(dt.v[i].v[j]) : 0.f;
-                dw[i][j] = fmaf(g, u[i][j], dw[i][j]);
-                d[i][j] = g * w[i][j];
-                sum = fmaf(d[i][j], u[i][j], sum);
+                u[i][j] = (p.residual ? x.at(i, j) + r.at(i, j) : x.at(i, j)) * rms;
+                sum = fmaf(g.at(i, j) * w[Ahead ? i : 0][j], u[i][j], sum);
+                if constexpr (Ahead) dw[i][j] = fmaf(g.at(i, j), u[i][j], dw[i][j]);
+                else if (p.partial && in) mine[first + i * stride + j] = fmaf(g.at(i, j), u[i][j], mine[first + i * stride + j]);
             }
         }
-        ask(row + step);
-        const float mean = teamSum(sum, p.teamWarps, sums, slot) / static_cast<float>(width);
-        T *dx = static_cast<T *>(p.dx) + row * width;
+        if (Ahead && round + 1 < rounds) ask(row + step);
+        const float mean = team.sum(sum, sums, round & 1) / static_cast<float>(width);
+        if (row < p.rows) {
+            T *dx = static_cast<T *>(p.dx) + row * width;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            Pack<T, W> out;
+            for (int i = 0; i < ITEMS; ++i) {
+                if (first + i * stride >= width) continue;
+                if constexpr (!Ahead) weights(w[0], i);
+                float out[W];
 #pragma unroll
-            for (int j = 0; j < W; ++j) out.v[j] = fromFloat<T>(fmaf(rms, fmaf(-u[i][j], mean, d[i][j]), add[i][j]));
-            if (first + i * stride < width) *reinterpret_cast<Pack<T, W> *>(dx + first + i * stride) = out;
+                for (int j = 0; j < W; ++j) out[j] = fmaf(rms, fmaf(-u[i][j], mean, g.at(i, j) * w[Ahead ? i : 0][j]), p.dtotal ? add.at(i, j) : 0.f);
+                put(dx, first + i * stride, out);
+            }
         }
+        if (!Ahead && round + 1 < rounds) ask(row + step);
     }
     if (!p.partial) return;
-    float *mine = teams == 1 ? p.partial + static_cast<size_t>(blockIdx.x) * width : teamPartial + static_cast<size_t>(team) * width;
+    if constexpr (Ahead)
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
+        for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-        for (int j = 0; j < W; ++j)
-            if (first + i * stride < width) mine[first + i * stride + j] = dw[i][j];
-    if (teams == 1) return;
+            for (int j = 0; j < W; ++j)
+                if (first + i * stride < width) mine[first + i * stride + j] = dw[i][j];
     __syncthreads();
     for (int c = threadIdx.x; c < width; c += blockDim.x) {
         float s = 0.f;
-        for (int k = 0; k < teams; ++k) s += teamPartial[static_cast<size_t>(k) * width + c];
+        for (int k = 0; k < team.count; ++k) s += teamPartial[static_cast<size_t>(k) * width + c];
         p.partial[static_cast<size_t>(blockIdx.x) * width + c] = s;
     }
 }
@@ -253,6 +289,7 @@ __global__ void __launch_bounds__(1024) addRmsNormWeightGrad(const float *partia
     waitForPredecessor();
     float s = 0.f;
     if (c < width)
+#pragma unroll 4
         for (int k = warp; k < parts; k += 32) s += partial[static_cast<size_t>(k) * width + c];
     sums[warp][threadIdx.x & 31] = s;
     __syncthreads();
@@ -265,27 +302,35 @@ __global__ void __launch_bounds__(1024) addRmsNormWeightGrad(const float *partia
 }
 
 struct TeamPlan {
-    int warps, threads;
+    int team, threads;
+    int teams() const { return threads / team; }
 };
-// The smallest team (a power of two of warps) that holds a row at ITEMS groups of W elements a thread; narrow rows put four teams of one warp into a CTA.
+// The threads that a row needs at `perThread` elements each; CTAs of about 256.
 TeamPlan teamFor(int width, int perThread) {
-    int warps = 1;
-    while (warps * 32 * perThread < width) warps *= 2;
-    return {warps, warps == 1 ? 128 : warps * 32};
+    const int needed = (width + perThread - 1) / perThread;
+    int team = 8;
+    while (team < needed && team < 32) team *= 2;
+    if (needed > 32) team = (needed + 31) / 32 * 32;
+    return {team, team * std::max(1, 256 / team)};
 }
 
-// f(W, ITEMS) as compile-time constants.  16-byte groups where every array's rows start on 16 bytes and the width is made of them, else single elements.
-// `items`: groups a thread may hold.  Few rows take fewer groups a thread, because then the row's latency counts and not the warps that it takes.
-template <class T, int MaxItems, class F>
-void withGroups(int64_t rows, int width, bool vector, F f) {
+// f(W, ITEMS) as compile-time constants.  16-byte groups where every array's rows start on 16 bytes and the width is made of them, else single elements; the fewest groups a
+// thread with which a team holds the row.
+template <class T, class F>
+void withGroups(int width, bool vector, F f) {
     constexpr int V = 16 / sizeof(T);
-    if (!vector) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
+    auto fits = [&](int perThread) { return width <= kMaxThreads * perThread; };
+    auto run = [&](auto w, auto items) { return f(w, items); };
+    using One = std::integral_constant<int, 1>;
     using VW = std::integral_constant<int, V>;
-    auto fits = [&](int items) { return width <= kMaxWarps * 32 * V * items; };
-    const bool few = rows <= currentDevice().sms;
-    if (fits(1) && (few || width <= 32 * V)) return f(VW{}, std::integral_constant<int, 1>{});
-    if (fits(2) && (few || MaxItems == 2 || width <= 64 * V)) return f(VW{}, std::integral_constant<int, 2>{});
-    return f(VW{}, std::integral_constant<int, 4>{});
+    if (vector) {
+        if (fits(V)) return run(VW{}, One{});
+        if (fits(2 * V)) return run(VW{}, std::integral_constant<int, 2>{});
+        return run(VW{}, std::integral_constant<int, 32 / V>{});
+    }
+    if (fits(4)) return run(One{}, std::integral_constant<int, 4>{});
+    if (fits(16)) return run(One{}, std::integral_constant<int, 16>{});
+    return run(One{}, std::integral_constant<int, 32>{});
 }
 
 int gridFor(const void *kernel, int64_t rows, int teams, int threads, size_t smem) {
@@ -308,13 +353,12 @@ void launchNorm(const char *name, NormRows p, int type, cudaStream_t st) {
         const bool vector = p.width % group == 0 && p.xPitch % group == 0 && alignedTo(p.x, 16) &&
                             (!p.residual || (p.residualPitch % group == 0 && alignedTo(p.residual, 16) && alignedTo(p.total, 16))) &&
                             (Codes ? p.codesPitch % group == 0 && alignedTo(p.codes, group) : alignedTo(p.y, 16));
-        withGroups<T, 4>(p.rows, p.width, vector, [&](auto w, auto items) {
+        withGroups<T>(p.width, vector, [&](auto w, auto items) {
             constexpr int W = decltype(w)::value, ITEMS = decltype(items)::value;
+            const auto kernel = addRmsNorm<T, W, ITEMS, Codes>;
             const TeamPlan plan = teamFor(p.width, W * ITEMS);
-            const auto kernel = plan.threads > 512 ? addRmsNorm<T, W, ITEMS, Codes, 1024> : addRmsNorm<T, W, ITEMS, Codes, 512>;
-            p.teamWarps = plan.warps;
-            const int teams = plan.threads / (plan.warps * 32);
-            const int grid = gridFor(reinterpret_cast<const void *>(kernel), p.rows, teams, plan.threads, 0);
+            p.team = plan.team;
+            const int grid = gridFor(reinterpret_cast<const void *>(kernel), p.rows, plan.teams(), plan.threads, 0);
             {
                 KernelTimer timer__(name, st);
                 launchDependent(kernel, grid, plan.threads, 0, st, p);
@@ -330,13 +374,13 @@ template <class F>
 void withGradKernel(int64_t rows, int width, int type, bool vector, F f) {
     withType(type, [&](auto t) {
         using T = decltype(t);
-        withGroups<T, 2>(rows, width, vector, [&](auto w, auto items) {
+        withGroups<T>(width, vector, [&](auto w, auto items) {
             constexpr int W = decltype(w)::value, ITEMS = decltype(items)::value;
+            const auto kernel = addRmsNormGrad<T, W, ITEMS>;
             const TeamPlan plan = teamFor(width, W * ITEMS);
-            const auto kernel = plan.threads > 512 ? addRmsNormGrad<T, W, ITEMS, 1024> : addRmsNormGrad<T, W, ITEMS, 512>;
-            const int teams = plan.threads / (plan.warps * 32);
-            const size_t smem = teams > 1 ? static_cast<size_t>(teams) * width * sizeof(float) : 0;
-            const int grid = gridFor(reinterpret_cast<const void *>(kernel), (rows + kGradRowsOfTeam - 1) / kGradRowsOfTeam, teams, plan.threads, smem);
+            const size_t smem = static_cast<size_t>(plan.teams()) * width * sizeof(float);
+            ensureDynamicSmem(reinterpret_cast<const void *>(kernel), smem);
+            const int grid = gridFor(reinterpret_cast<const void *>(kernel), (rows + kGradRowsOfTeam - 1) / kGradRowsOfTeam, plan.teams(), plan.threads, smem);
             f(kernel, plan, smem, grid);
         });
     });
@@ -399,9 +443,8 @@ int rxmet_add_rms_norm_backward(int64_t rows, int width, int type, const void *d
         const bool vector = width % group == 0 && x_pitch % group == 0 && residual_pitch % group == 0 && alignedTo(dy_dev, 16) && alignedTo(dtotal_dev, 16) &&
                             alignedTo(x_dev, 16) && alignedTo(residual_dev, 16) && alignedTo(dx_dev, 16);
         withGradKernel(rows, width, type, vector, [&](auto kernel, TeamPlan plan, size_t smem, int grid) {
-            NormGradient p{rows, width, plan.warps, dy_dev, dtotal_dev, x_dev, residual_dev, weight_dev, x_pitch, residual_pitch, rms_dev, weight_type, dx_dev, nullptr};
+            NormGradient p{rows, width, plan.team, dy_dev, dtotal_dev, x_dev, residual_dev, weight_dev, x_pitch, residual_pitch, rms_dev, weight_type, dx_dev, nullptr};
             if (dweight_dev) p.partial = Workspace(workspace_dev, workspace_bytes).take<float>(static_cast<size_t>(grid) * width);
-            if (!dweight_dev) smem = 0;
             {
                 KernelTimer timer__("addRmsNormGrad", st);
                 launchDependent(kernel, grid, plan.threads, smem, st, p);

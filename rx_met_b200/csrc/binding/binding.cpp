@@ -415,6 +415,7 @@ void sameDevice(const Tensor &t, const Tensor &like, const char *name) {
 
 // [rows][width] with neighbouring elements, a view where the strides allow one; the distance of its rows.
 Tensor asRows(const Tensor &t) {
+    if (t.dim() == 2 && t.stride(1) == 1) return t;
     const Tensor flat = t.reshape({t.numel() / t.size(-1), t.size(-1)});
     return flat.stride(1) == 1 || flat.size(1) == 1 ? flat : flat.contiguous();
 }

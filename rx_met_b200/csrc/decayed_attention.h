@@ -35,6 +35,10 @@ struct Pass {
 
 void launchRecurrent(const Pass &p, int type, cudaStream_t st);
 
+// One token forward, states of whole 16-byte groups.
+bool takesStep(const Pass &p);
+void launchStep(const Pass &p, int type, cudaStream_t st);
+
 // Chunks of 128 tokens on tensor cores, for 16-bit tensors that TMA can copy.  Few heads are cut into segments along time, whose states need a workspace.
 constexpr int kChunkTokens = 128;
 struct ChunkPlan {

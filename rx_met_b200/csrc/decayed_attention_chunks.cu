@@ -74,28 +74,6 @@ struct Span {
     }
 };
 
-template <class T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) { return packBf16(a, b); }
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    return r;
-}
-template <class T>
-__device__ __forceinline__ uint32_t pack2(Pair p) {
-    const float2 v = floatsOf(p);
-    return pack2<T>(v.x, v.y);
-}
-template <class T>
-__device__ __forceinline__ float2 unpack2(uint32_t v);
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) { return make_float2(bf16Lo(v), bf16Hi(v)); }
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
-
 // The power of two that brings magnitudes up to `most` below 2^15; 1 where there is nothing to scale.
 __device__ __forceinline__ float toTopOfHalf(float most) {
     if (!(most > 0.f) || isinf(most)) return 1.f;

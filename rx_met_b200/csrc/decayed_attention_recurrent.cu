@@ -40,11 +40,21 @@ __global__ void __launch_bounds__(128) decayedRecurrent(const __grid_constant__ 
     const size_t head = (static_cast<size_t>(b) * p.heads + h) * p.key * p.value;
 
     float s[kGroups][4][4];
+    const bool groups = p.stateCol == 1 && p.value % 4 == 0 && (reinterpret_cast<uintptr_t>(p.stateIn) | reinterpret_cast<uintptr_t>(p.stateOut)) % 16 == 0;   // 16 bytes at a time
 #pragma unroll
     for (int i = 0; i < kGroups; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int row = 16 * i + 4 * rowGroup + r;
+            if (groups) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (p.stateIn && row < p.key && col < p.value) v = *reinterpret_cast<const float4 *>(p.stateIn + head + static_cast<size_t>(row) * p.stateRow + col);
+                s[i][r][0] = v.x * p.inScale;
+                s[i][r][1] = v.y * p.inScale;
+                s[i][r][2] = v.z * p.inScale;
+                s[i][r][3] = v.w * p.inScale;
+                continue;
+            }
 #pragma unroll
             for (int c = 0; c < 4; ++c)
                 s[i][r][c] = p.stateIn && row < p.key && col + c < p.value ? p.inScale * p.stateIn[head + static_cast<size_t>(row) * p.stateRow + static_cast<size_t>(col + c) * p.stateCol] : 0.f;
@@ -106,6 +116,12 @@ __global__ void __launch_bounds__(128) decayedRecurrent(const __grid_constant__ 
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int row = 16 * i + 4 * rowGroup + r;
+            if (groups) {
+                if (row < p.key && col < p.value)
+                    *reinterpret_cast<float4 *>(p.stateOut + head + static_cast<size_t>(row) * p.stateRow + col) =
+                        make_float4(s[i][r][0] * p.finalScale, s[i][r][1] * p.finalScale, s[i][r][2] * p.finalScale, s[i][r][3] * p.finalScale);
+                continue;
+            }
 #pragma unroll
             for (int c = 0; c < 4; ++c)
                 if (row < p.key && col + c < p.value) p.stateOut[head + static_cast<size_t>(row) * p.stateRow + static_cast<size_t>(col + c) * p.stateCol] = s[i][r][c] * p.finalScale;

@@ -131,36 +131,4 @@ __device__ __forceinline__ void arriveRemote(uint32_t bar) { asm volatile("mbarr
 // Binds the current device's context to this thread, which encoding a tensor map needs: a thread of the autograd engine may come here without one.
 inline void bindContext() { RXMET_CUDA(cudaSetDevice(currentDevice().device)); }
 
-// Two 32-bit floats in one operation each.
-using Pair = unsigned long long;
-__device__ __forceinline__ Pair pairOf(float a, float b) {
-    Pair r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ Pair pairOf(uint32_t a, uint32_t b) { return pairOf(__uint_as_float(a), __uint_as_float(b)); }
-__device__ __forceinline__ float2 floatsOf(Pair p) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
-    return r;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-    Pair r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-    Pair r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-    Pair r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
-// A word of the current device that kernels set where a bounded wait gave up; their output is not written then.
-int *waitStatus();
-
 }  // namespace rxmet

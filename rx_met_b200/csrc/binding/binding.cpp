@@ -504,7 +504,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
                                                 dataOf(weight), weightType, mutableOf(dx), mutableOf(out[1]), mutableOf(ws), bytes, streamOf(given)),
                     "add_rms_norm backward");
         out[0] = dx;
-        if (ctx->needs_input_grad(2)) out[2] = dx;
+        if (saved[3].defined() && ctx->needs_input_grad(2)) out[2] = dx;   // an absent residual has no place of its own
         return out;
     }
 };

@@ -93,6 +93,24 @@ def test_gradients(rows, width, dtype, weight_type, with_total):
     ml.within(dweight, wanted_weight, wanted_weight.abs() * ml.UNIT[weight_type] * 1.01 + summed * (rows / 32 + 64) * 2.0 ** -24 + ml.TINY[weight_type])
 
 
+def test_gradients_without_a_residual_or_a_trained_weight():
+    from rx_met_b200 import rms_norm
+    x, weight, residual = tensors(70, 96, torch.float32, seed=4)
+    dy = torch.randn(70, 96, device="cuda")
+    _, total, rms = ml.norm(x, weight, None, 1e-5)
+    want, wanted_weight = ml.norm_gradients(dy, None, total, weight, rms)
+    leaf, trained = x.clone().requires_grad_(), weight.clone().requires_grad_()
+    dx, dweight = torch.autograd.grad(rms_norm.add_rms_norm(leaf, trained, None, 1e-5)[0], [leaf, trained], dy)
+    assert torch.allclose(dx.double(), want, rtol=1e-5, atol=1e-5) and torch.allclose(dweight.double(), wanted_weight, rtol=1e-5, atol=1e-4)
+    alone = torch.autograd.grad(rms_norm.add_rms_norm(leaf, weight, None, 1e-5)[0], leaf, dy)[0]
+    assert torch.equal(alone, dx)
+    both = [x.clone().requires_grad_(), residual.clone().requires_grad_()]
+    grads = torch.autograd.grad(rms_norm.add_rms_norm(both[0], weight, both[1], 1e-5)[0], both, dy)
+    assert torch.equal(grads[0], grads[1])
+    only = torch.autograd.grad(rms_norm.add_rms_norm(x, weight, both[1], 1e-5)[0], both[1], dy)[0]
+    assert torch.equal(only, grads[1])
+
+
 def test_gradient_against_differences():
     from rx_met_b200 import rms_norm
     x, weight, residual = (t.requires_grad_() for t in tensors(4, 33, torch.float32, seed=3))

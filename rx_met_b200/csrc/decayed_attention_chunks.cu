@@ -51,6 +51,7 @@ __device__ __forceinline__ void storeShared(uint32_t at, uint32_t a, uint32_t b,
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+constexpr int kMaxSegments = 160;   // no more than SMs
 struct Segments {
     int count, chunks;   // segments of time, chunks of a segment
     float *states;       // [batch][heads][count][key][value]: ends of the segments on their own, then their beginnings
@@ -92,9 +93,10 @@ struct Small {
     int failed;
 };
 
-// DK: elements of a key that the tiles hold, 64 or 128.  StateOnly: nothing but the state at the end of the segment.  Wide: outputs of the type of the inputs whose parts of
-// sixteen start on 32 bytes.
-template <class T, int DK, bool StateOnly, bool Wide>
+// DK: elements of a key that the tiles hold, 64 or 128.  StateOnly: nothing but the state at the end of the segment.  Stores: how outputs leave, by the alignment of their
+// rows.
+enum class Stores { Elements, Packed, Floats };   // one by one; sixteen of the type of the inputs, or eight in 32 bits, at a time
+template <class T, int DK, bool StateOnly, Stores How>
 __global__ void __launch_bounds__(kThreads, 1)
     decayedChunks(const __grid_constant__ Pass p, const __grid_constant__ CUtensorMap qMap, const __grid_constant__ CUtensorMap kMap, const __grid_constant__ CUtensorMap vMap,
                   const Segments segments, const int terms, int *status) {
@@ -382,27 +384,39 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     const int col = slice * kCols + part * 16;
                     if (!in || col >= p.value) continue;
-                    uint32_t w[8];
+                    float out[16];
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
                         const Pair scaled = kHalf ? mul2(pairOf(o2[j], o2[j + 1]), pairOf(back, back)) : pairOf(o2[j], o2[j + 1]);
-                        float2 v = floatsOf(fma2(pairOf(o1[j], o1[j + 1]), pairOf(inter, inter), scaled));
-                        if (!live) v = make_float2(0.f, 0.f);
-                        if constexpr (Wide) {
-                            w[j / 2] = pack2<T>(v.x, v.y);
-                        } else {
+                        const float2 v = floatsOf(fma2(pairOf(o1[j], o1[j + 1]), pairOf(inter, inter), scaled));
+                        out[j] = live ? v.x : 0.f;
+                        out[j + 1] = live ? v.y : 0.f;
+                    }
+                    auto sector = [](void *to, const uint32_t(&w)[8]) {   // a sector of memory a thread
+                        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                                     : "memory");
+                    };
+                    if constexpr (How == Stores::Packed) {
+                        uint32_t w[8];
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                if (col + j + e >= p.value) continue;
-                                if (p.outFloat) static_cast<float *>(p.out)[row + col + j + e] = e ? v.y : v.x;
-                                else static_cast<T *>(p.out)[row + col + j + e] = fromFloat<T>(e ? v.y : v.x);
-                            }
+                        for (int j = 0; j < 8; ++j) w[j] = pack2<T>(out[2 * j], out[2 * j + 1]);
+                        sector(static_cast<T *>(p.out) + row + col, w);
+                    } else if constexpr (How == Stores::Floats) {
+#pragma unroll
+                        for (int half = 0; half < 16; half += 8) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(out[half + j]);
+                            if (col + half < p.value) sector(static_cast<float *>(p.out) + row + col + half, w);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            if (col + j >= p.value) continue;
+                            if (p.outFloat) static_cast<float *>(p.out)[row + col + j] = out[j];
+                            else static_cast<T *>(p.out)[row + col + j] = fromFloat<T>(out[j]);
                         }
                     }
-                    if constexpr (Wide)   // a sector of memory a thread
-                        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(static_cast<T *>(p.out) + row + col), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
-                                     "r"(w[6]), "r"(w[7])
-                                     : "memory");
                 }
             }
         }
@@ -419,14 +433,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int inRow = segments.count > 1 ? p.value : p.stateRow, inCol = segments.count > 1 ? 1 : p.stateCol;
         const float inScale = segments.count > 1 ? 1.f : p.inScale;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            float v[2];
+        for (int j = 0; j < 16; ++j) s[j] = pairOf(0.f, 0.f);
+        if (in && d < p.key) {
+            const float *from = in + static_cast<size_t>(d) * inRow + static_cast<size_t>(col) * inCol;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int c = col + 2 * j + e;
-                v[e] = in && d < p.key && c < p.value ? inScale * in[static_cast<size_t>(d) * inRow + static_cast<size_t>(c) * inCol] : 0.f;
-            }
-            s[j] = pairOf(v[0], v[1]);
+            for (int j = 0; j < 16; ++j, from += 2 * inCol)
+                s[j] = pairOf(col + 2 * j < p.value ? inScale * from[0] : 0.f, col + 2 * j + 1 < p.value ? inScale * from[inCol] : 0.f);
         }
 
         auto publish = [&](int u) {   // the state in front of chunk u, as the B operand of O1
@@ -585,22 +597,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0 && small.failed) atomicExch(status, 1);
 }
 
-// From the ends of the segments on their own to their beginnings: one thread for each element of a state, segment after segment.
+// From the ends of the segments on their own to their beginnings: one thread for each element of a state, segment after segment, eight of them in flight.  The powers of the decay
+// are made once a CTA: in 64 bits and by every thread, they took 35 us for 16 segments (1 x 16384 tokens of 8 heads of 64) in place of 6.
 __global__ void __launch_bounds__(256) joinSegments(const __grid_constant__ Pass p, const Segments segments) {
+    constexpr int kAtOnce = 8;
+    __shared__ float powers[kMaxSegments];   // of the decay over a segment's tokens; below zero for one without any
     const int h = blockIdx.y, b = blockIdx.z, size = p.key * p.value, e = blockIdx.x * 256 + threadIdx.x;
     waitForPredecessor();
     letDependentsStart();
-    if (e >= size) return;
     const int length = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
-    const double g = p.logDecay[h];
+    for (int i = threadIdx.x; i < segments.count; i += 256) {
+        const int tokens = Span(length, i, segments.chunks).tokens(length, p.reverse);
+        powers[i] = tokens > 0 ? static_cast<float>(exp(tokens * static_cast<double>(p.logDecay[h]))) : -1.f;
+    }
+    __syncthreads();
+    if (e >= size) return;
     const size_t head = static_cast<size_t>(b) * p.heads + h, at = head * size + static_cast<size_t>(e / p.value) * p.stateRow + static_cast<size_t>(e % p.value) * p.stateCol;
     float state = p.stateIn ? p.inScale * p.stateIn[at] : 0.f;
-    for (int segment = 0; segment < segments.count; ++segment) {
-        float *own = segments.states + (head * segments.count + segment) * size + e;
-        const int tokens = Span(length, segment, segments.chunks).tokens(length, p.reverse);
-        const float added = tokens > 0 ? *own : 0.f;
-        *own = state;
-        if (tokens > 0) state = fmaf(state, static_cast<float>(exp(tokens * g)), added);
+    float *own = segments.states + head * segments.count * size + e;
+    for (int first = 0; first < segments.count; first += kAtOnce) {
+        float added[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+            if (first + i < segments.count && powers[first + i] >= 0.f) added[i] = own[static_cast<size_t>(first + i) * size];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (first + i >= segments.count) break;
+            own[static_cast<size_t>(first + i) * size] = state;
+            if (powers[first + i] >= 0.f) state = fmaf(state, powers[first + i], added[i]);
+        }
     }
     if (p.stateOut) p.stateOut[at] = state * p.finalScale;
 }
@@ -624,13 +649,22 @@ bool copies(const rxmet_head_tensor &t, int batch, int tokens) {
 
 }  // namespace
 
+// Segments by these estimates, in microseconds, of measured launches: a launch begins and ends in 8, a chunk takes 2.2, 1.3 where only the state is wanted, joining 4.  Eight chunks of 48
+// heads: 26 in one, 31 in three segments; 128 chunks of 8 heads: 290 in one, 48 in sixteen.
 ChunkPlan planChunks(const Pass &p, int type) {
     ChunkPlan plan{type != RXMET_TYPE_F32 && p.tokens >= 32 && encodeTiled() != nullptr, 1, (p.tokens + kC - 1) / kC};
-    const int64_t ctas = static_cast<int64_t>((p.value + kCols - 1) / kCols) * p.heads * p.batch;
-    const int chunks = plan.segmentChunks, most = static_cast<int>(std::min<int64_t>(chunks / 2, currentDevice().sms / std::max<int64_t>(1, ctas)));
-    if (plan.taken && most >= 2) {
-        plan.segmentChunks = (chunks + most - 1) / most;
-        plan.segments = (chunks + plan.segmentChunks - 1) / plan.segmentChunks;
+    if (!plan.taken) return plan;
+    const int chunks = plan.segmentChunks, sms = currentDevice().sms;
+    const int64_t ctas = std::max<int64_t>(1, static_cast<int64_t>((p.value + kCols - 1) / kCols) * p.heads * p.batch);
+    const auto rounds = [&](int segments) { return static_cast<double>((ctas * segments + sms - 1) / sms); };
+    double best = rounds(1) * (8 + 2.2 * chunks);
+    for (int segments = 2; segments <= chunks / 2 && segments <= kMaxSegments && ctas * segments <= 2 * sms; ++segments) {
+        const int each = (chunks + segments - 1) / segments;
+        const double time = rounds(segments) * (16 + 3.5 * each) + 4;
+        if (time >= best) continue;
+        best = time;
+        plan.segmentChunks = each;
+        plan.segments = (chunks + each - 1) / each;
     }
     return plan;
 }
@@ -642,7 +676,7 @@ void launchChunks(const Pass &p, int type, const ChunkPlan &plan, float *states,
     bool ok = true;
     bindContext();
     const CUtensorMap q = tokenMap(p.q, p.batch, p.tokens, p.key, bf16, ok), k = tokenMap(p.k, p.batch, p.tokens, p.key, bf16, ok), v = tokenMap(p.v, p.batch, p.tokens, p.value, bf16, ok);
-    const bool wide = !p.outFloat && p.value % 16 == 0 && alignedTo(p.out, 32);   // parts of a row start on 32 bytes
+    const bool wide = p.value % (p.outFloat ? 8 : 16) == 0 && alignedTo(p.out, 32);   // parts of a row start on 32 bytes
     if (!ok) fail(RXMET_ERR_CUDA, "cuTensorMapEncodeTiled failed");
     const Segments segments{plan.segments, plan.segmentChunks, states};
     const dim3 grid((p.value + kCols - 1) / kCols * plan.segments, p.heads, p.batch);
@@ -660,14 +694,17 @@ void launchChunks(const Pass &p, int type, const ChunkPlan &plan, float *states,
         using T = decltype(t);
         constexpr int DK = decltype(dk)::value;
         if (plan.segments > 1) {
-            run(decayedChunks<T, DK, true, true>, "decayedChunksState", terms);
+            run(decayedChunks<T, DK, true, Stores::Elements>, "decayedChunksState", terms);
             {
                 KernelTimer timer__("joinSegments", st);
                 launchDependent(joinSegments, dim3((p.key * p.value + 255) / 256, p.heads, p.batch), 256, 0, st, p, segments);
             }
             afterLaunch("joinSegments");
         }
-        if (p.out || plan.segments == 1) run(wide ? decayedChunks<T, DK, false, true> : decayedChunks<T, DK, false, false>, "decayedChunks", plan.segments > 1 ? 2 : terms);
+        if (p.out || plan.segments == 1) run(!wide        ? decayedChunks<T, DK, false, Stores::Elements>
+                                                    : p.outFloat ? decayedChunks<T, DK, false, Stores::Floats>
+                                                                 : decayedChunks<T, DK, false, Stores::Packed>,
+                                                    "decayedChunks", plan.segments > 1 ? 2 : terms);
     };
     auto withKeys = [&](auto t) {
         if (p.key <= 64) both(t, std::integral_constant<int, 64>{});

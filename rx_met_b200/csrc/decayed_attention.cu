@@ -86,7 +86,7 @@ Pass forwardPass(const rxmet_decayed_attention &a) {
     return p;
 }
 
-// Kernels by size and type.  Single tokens have a kernel of their own, chunks are taken from 32 tokens on; tensors that TMA cannot copy and 32-bit ones go token by token.
+// Kernels by size and type.  Single tokens have a kernel of their own, chunks are taken from 16 or 32 tokens on (planChunks); tensors that TMA cannot copy and 32-bit ones go token by token.
 void launchPass(const Pass &p, int type, float *states, cudaStream_t st) {
     const ChunkPlan plan = planChunks(p, type);
     if (takesStep(p)) launchStep(p, type, st);

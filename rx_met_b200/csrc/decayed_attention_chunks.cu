@@ -436,6 +436,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < 16; ++j) s[j] = pairOf(0.f, 0.f);
         if (in && d < p.key) {
             const float *from = in + static_cast<size_t>(d) * inRow + static_cast<size_t>(col) * inCol;
+            if (inCol == 1 && p.value % 4 == 0 && (reinterpret_cast<uintptr_t>(in) & 15) == 0) {
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                    if (col + 2 * j >= p.value) continue;
+                    const float4 v = *reinterpret_cast<const float4 *>(from + 2 * j);
+                    s[j] = pairOf(v.x * inScale, v.y * inScale);
+                    s[j + 1] = pairOf(v.z * inScale, v.w * inScale);
+                }
+            } else
 #pragma unroll
             for (int j = 0; j < 16; ++j, from += 2 * inCol)
                 s[j] = pairOf(col + 2 * j < p.value ? inScale * from[0] : 0.f, col + 2 * j + 1 < p.value ? inScale * from[inCol] : 0.f);
@@ -570,13 +579,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (last && alive) {
             const int outRow = StateOnly ? p.value : p.stateRow, outCol = StateOnly ? 1 : p.stateCol;
             const float scale = StateOnly ? 1.f : p.finalScale;
+            float *to = last + static_cast<size_t>(d) * outRow + static_cast<size_t>(col) * outCol;
+            if (d < p.key) {
+                if (outCol == 1 && p.value % 4 == 0 && (reinterpret_cast<uintptr_t>(last) & 15) == 0) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float2 v = floatsOf(s[j]);
+                    for (int j = 0; j < 16; j += 2)
+                        if (col + 2 * j < p.value)
+                            *reinterpret_cast<float4 *>(to + 2 * j) = make_float4(floatsOf(s[j]).x * scale, floatsOf(s[j]).y * scale, floatsOf(s[j + 1]).x * scale, floatsOf(s[j + 1]).y * scale);
+                } else {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int c = col + 2 * j + e;
-                    if (d < p.key && c < p.value) last[static_cast<size_t>(d) * outRow + static_cast<size_t>(c) * outCol] = (e ? v.y : v.x) * scale;
+                    for (int j = 0; j < 32; ++j)
+                        if (col + j < p.value) to[static_cast<size_t>(j) * outCol] = (j & 1 ? floatsOf(s[j / 2]).y : floatsOf(s[j / 2]).x) * scale;
                 }
             }
         }
@@ -649,13 +662,16 @@ bool copies(const rxmet_head_tensor &t, int batch, int tokens) {
 
 }  // namespace
 
+// From 16 tokens on where all CTAs find an SM, else from 32 on: a launch takes 8 to 14 us a round whatever the number of tokens up to 128, token by token a token takes 0.45 to 0.6 us with few
+// heads (8 of 64: 16 tokens 10.8 for 8.6) and less than its share with many (1024 of 128: 31 tokens 123 us, one chunk 171).
 // Segments by these estimates, in microseconds, of measured launches: a launch begins and ends in 8, a chunk takes 2.2, 1.3 where only the state is wanted, joining 4.  Eight chunks of 48
 // heads: 26 in one, 31 in three segments; 128 chunks of 8 heads: 290 in one, 48 in sixteen.
 ChunkPlan planChunks(const Pass &p, int type) {
-    ChunkPlan plan{type != RXMET_TYPE_F32 && p.tokens >= 32 && encodeTiled() != nullptr, 1, (p.tokens + kC - 1) / kC};
-    if (!plan.taken) return plan;
+    ChunkPlan plan{false, 1, (p.tokens + kC - 1) / kC};
     const int chunks = plan.segmentChunks, sms = currentDevice().sms;
     const int64_t ctas = std::max<int64_t>(1, static_cast<int64_t>((p.value + kCols - 1) / kCols) * p.heads * p.batch);
+    plan.taken = type != RXMET_TYPE_F32 && p.tokens >= (ctas <= sms ? 16 : 32) && encodeTiled() != nullptr;
+    if (!plan.taken) return plan;
     const auto rounds = [&](int segments) { return static_cast<double>((ctas * segments + sms - 1) / sms); };
     double best = rounds(1) * (8 + 2.2 * chunks);
     for (int segments = 2; segments <= chunks / 2 && segments <= kMaxSegments && ctas * segments <= 2 * sms; ++segments) {

@@ -1,10 +1,10 @@
 // Linear attention with a decay for each head, token by token, in 32-bit floats.
 //
-// A warp owns 32 columns of a head's state, a CTA all of them: lane = one of eight groups of four columns x one of four groups of rows, so that a row
-// of the state is read and written 128 bytes at a time and the state stays in registers over all tokens.  Rows are dealt to the row groups four at a time,
-// which keeps the four 16-byte reads of a key apart in shared memory.  Tokens come to shared memory sixteen at a time.
+// A warp owns sixteen columns of a head's state, a CTA all of them: lane = one of four groups of four columns x one of eight groups of rows, and the state stays in
+// registers over all tokens, two elements an operation.  Rows are dealt to the row groups four at a time, which keeps the eight 16-byte reads of a key apart in shared memory.
+// Tokens come to shared memory sixteen at a time.  With 32 columns a warp, single operations and loads one after another a token of 64 heads of 128 took 2.2 us, now 0.6.
 //
-// Bound: the state's bytes for single tokens; the multiply-adds for many (4 operations an element of the state and token).
+// Bound: the state's bytes for few tokens; issue for many (two packed operations an element of the state and token).
 #include "decayed_attention.h"
 #include "dependent_launch.cuh"
 #include "element_types.cuh"
@@ -24,40 +24,44 @@ struct Tokens {
 };
 
 // KEYS: rows of the state that the registers hold (64 or 128), those beyond `key` as zeros.
-template <class T, int KEYS>
-__global__ void __launch_bounds__(128) decayedRecurrent(const __grid_constant__ Pass p) {
-    constexpr int kGroups = KEYS / 16;   // groups of four rows that a lane owns
+template <class T, int KEYS, bool Reverse>
+__global__ void __launch_bounds__(256) decayedRecurrent(const __grid_constant__ Pass p) {
+    constexpr int kGroups = KEYS / 32;   // groups of four rows that a lane owns
     __shared__ __align__(16) float sq[kStage][KEYS], sk[kStage][KEYS], sv[kStage][kMaxDim];
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int col = warp * 32 + (lane & 7) * 4, rowGroup = lane >> 3;
+    const int col = warp * 16 + (lane & 3) * 4, rowGroup = lane >> 2;
     waitForPredecessor();
     const int length = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
     // The decay as a sum of two floats: rounded to one, its error would grow with every token that a state remembers (2e-4 of the state over 4096 tokens
     // at a memory of 512).
     const double exact = exp(static_cast<double>(p.logDecay[h]));
-    const float decay = static_cast<float>(exact), rest = static_cast<float>(exact - decay);
+    const Pair decay = pairOf(static_cast<float>(exact), static_cast<float>(exact));
+    const float left = static_cast<float>(exact - static_cast<float>(exact));
+    const Pair rest = pairOf(left, left);
     const Tokens<T> q(p.q, b, h, p.heads), k(p.k, b, h, p.heads), v(p.v, b, h, p.heads);
     const size_t head = (static_cast<size_t>(b) * p.heads + h) * p.key * p.value;
-
-    float s[kGroups][4][4];
     const bool groups = p.stateCol == 1 && p.value % 4 == 0 && (reinterpret_cast<uintptr_t>(p.stateIn) | reinterpret_cast<uintptr_t>(p.stateOut)) % 16 == 0;   // 16 bytes at a time
+
+    Pair s[kGroups][4][2];
 #pragma unroll
     for (int i = 0; i < kGroups; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = 16 * i + 4 * rowGroup + r;
-            if (groups) {
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (p.stateIn && row < p.key && col < p.value) v = *reinterpret_cast<const float4 *>(p.stateIn + head + static_cast<size_t>(row) * p.stateRow + col);
-                s[i][r][0] = v.x * p.inScale;
-                s[i][r][1] = v.y * p.inScale;
-                s[i][r][2] = v.z * p.inScale;
-                s[i][r][3] = v.w * p.inScale;
-                continue;
+            const int row = 32 * i + 4 * rowGroup + r;
+            const float *from = p.stateIn + head + static_cast<size_t>(row) * p.stateRow + static_cast<size_t>(col) * p.stateCol;
+            float4 in = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (p.stateIn && row < p.key) {
+                if (groups) {
+                    if (col < p.value) in = *reinterpret_cast<const float4 *>(from);
+                } else {
+                    if (col < p.value) in.x = from[0];
+                    if (col + 1 < p.value) in.y = from[p.stateCol];
+                    if (col + 2 < p.value) in.z = from[2 * p.stateCol];
+                    if (col + 3 < p.value) in.w = from[3 * p.stateCol];
+                }
             }
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                s[i][r][c] = p.stateIn && row < p.key && col + c < p.value ? p.inScale * p.stateIn[head + static_cast<size_t>(row) * p.stateRow + static_cast<size_t>(col + c) * p.stateCol] : 0.f;
+            s[i][r][0] = pairOf(in.x * p.inScale, in.y * p.inScale);
+            s[i][r][1] = pairOf(in.z * p.inScale, in.w * p.inScale);
         }
     letDependentsStart();
 
@@ -71,60 +75,79 @@ __global__ void __launch_bounds__(128) decayedRecurrent(const __grid_constant__ 
         const int count = min(kStage, length - done);
         __syncthreads();
         // token i of the stage, in the order of the pass
-        auto tokenOf = [&](int i) { return static_cast<int64_t>(p.reverse ? length - 1 - done - i : done + i); };
-        for (int i = tid; i < count * KEYS; i += blockDim.x) {
-            const int t = i / KEYS, d = i % KEYS;
-            sq[t][d] = d < p.key ? toFloat(q.data[tokenOf(t) * q.strideT + d]) : 0.f;
-            sk[t][d] = d < p.key ? toFloat(k.data[tokenOf(t) * k.strideT + d]) : 0.f;
-        }
-        for (int i = tid; i < count * kMaxDim; i += blockDim.x) {
-            const int t = i / kMaxDim, d = i % kMaxDim;
-            sv[t][d] = d < p.value ? toFloat(v.data[tokenOf(t) * v.strideT + d]) : 0.f;
-        }
+        auto tokenOf = [&](int i) { return static_cast<int64_t>(Reverse ? length - 1 - done - i : done + i); };
+        // eight loads in flight a thread: one after another, they took more time than the tokens
+        auto fill = [&](const Tokens<T> &from, float *to, int dims, int width) {   // rows of `width` floats, zeros from `dims` on
+            for (int i0 = tid; i0 < count * width; i0 += 8 * blockDim.x) {
+                T in[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int i = i0 + e * blockDim.x, t = i / width, d = i - t * width;
+                    in[e] = i < count * width && d < dims ? from.data[tokenOf(t) * from.strideT + d] : fromFloat<T>(0.f);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (i0 + e * static_cast<int>(blockDim.x) < count * width) to[i0 + e * blockDim.x] = toFloat(in[e]);
+            }
+        };
+        fill(q, sq[0], p.key, KEYS);
+        fill(k, sk[0], p.key, KEYS);
+        fill(v, sv[0], p.value, kMaxDim);
         __syncthreads();
+#pragma unroll 1
         for (int t = 0; t < count; ++t) {
             const float4 vv = *reinterpret_cast<const float4 *>(&sv[t][col]);
-            float o[4] = {};
+            const Pair vs[2] = {pairOf(vv.x, vv.y), pairOf(vv.z, vv.w)};
+            Pair o[2] = {pairOf(0.f, 0.f), pairOf(0.f, 0.f)};
 #pragma unroll
             for (int i = 0; i < kGroups; ++i) {
-                const float4 kk = *reinterpret_cast<const float4 *>(&sk[t][16 * i + 4 * rowGroup]), qq = *reinterpret_cast<const float4 *>(&sq[t][16 * i + 4 * rowGroup]);
-                const float ks[4] = {kk.x, kk.y, kk.z, kk.w}, qs[4] = {qq.x, qq.y, qq.z, qq.w}, vs[4] = {vv.x, vv.y, vv.z, vv.w};
+                const float4 kk = *reinterpret_cast<const float4 *>(&sk[t][32 * i + 4 * rowGroup]), qq = *reinterpret_cast<const float4 *>(&sq[t][32 * i + 4 * rowGroup]);
+                const float ks[4] = {kk.x, kk.y, kk.z, kk.w}, qs[4] = {qq.x, qq.y, qq.z, qq.w};
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const float before = s[i][r][c], kv = ks[r] * vs[c];
-                        const float now = p.reverse ? before + kv : fmaf(before, decay, fmaf(before, rest, kv));
-                        o[c] = fmaf(qs[r], now, o[c]);
-                        s[i][r][c] = p.reverse ? fmaf(now, decay, now * rest) : now;
+                    for (int c = 0; c < 2; ++c) {
+                        const Pair kr = pairOf(ks[r], ks[r]), qr = pairOf(qs[r], qs[r]);
+                        Pair &state = s[i][r][c];
+                        if constexpr (Reverse) {
+                            const Pair now = fma2(kr, vs[c], state);
+                            o[c] = fma2(qr, now, o[c]);
+                            state = fma2(now, decay, mul2(now, rest));
+                        } else {
+                            state = fma2(state, decay, fma2(state, rest, mul2(kr, vs[c])));
+                            o[c] = fma2(qr, state, o[c]);
+                        }
                     }
             }
+            float sums[4] = {floatsOf(o[0]).x, floatsOf(o[0]).y, floatsOf(o[1]).x, floatsOf(o[1]).y};
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                o[c] += __shfl_xor_sync(0xffffffffu, o[c], 8);
-                o[c] += __shfl_xor_sync(0xffffffffu, o[c], 16);
-            }
-            // each row group stores one of the four columns
-            const float mine = rowGroup == 0 ? o[0] : rowGroup == 1 ? o[1] : rowGroup == 2 ? o[2] : o[3];
-            store(static_cast<int>(tokenOf(t)), col + rowGroup, mine * p.outScale);
+            for (int d = 4; d < 32; d *= 2)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) sums[c] += __shfl_xor_sync(0xffffffffu, sums[c], d);
+            // four of the row groups store one of the four columns each
+            const float mine = rowGroup == 0 ? sums[0] : rowGroup == 1 ? sums[1] : rowGroup == 2 ? sums[2] : sums[3];
+            if (rowGroup < 4) store(static_cast<int>(tokenOf(t)), col + rowGroup, mine * p.outScale);
         }
     }
-    for (int t = length; t < p.tokens; ++t) store(t, col + rowGroup, 0.f);
+    if (rowGroup < 4)
+        for (int t = length; t < p.tokens; ++t) store(t, col + rowGroup, 0.f);
     if (!p.stateOut) return;
 #pragma unroll
     for (int i = 0; i < kGroups; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = 16 * i + 4 * rowGroup + r;
+            const int row = 32 * i + 4 * rowGroup + r;
+            if (row >= p.key) continue;
+            float *to = p.stateOut + head + static_cast<size_t>(row) * p.stateRow + static_cast<size_t>(col) * p.stateCol;
+            const float2 a = floatsOf(s[i][r][0]), c = floatsOf(s[i][r][1]);
+            const float values[4] = {a.x * p.finalScale, a.y * p.finalScale, c.x * p.finalScale, c.y * p.finalScale};
             if (groups) {
-                if (row < p.key && col < p.value)
-                    *reinterpret_cast<float4 *>(p.stateOut + head + static_cast<size_t>(row) * p.stateRow + col) =
-                        make_float4(s[i][r][0] * p.finalScale, s[i][r][1] * p.finalScale, s[i][r][2] * p.finalScale, s[i][r][3] * p.finalScale);
+                if (col < p.value) *reinterpret_cast<float4 *>(to) = make_float4(values[0], values[1], values[2], values[3]);
                 continue;
             }
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (row < p.key && col + c < p.value) p.stateOut[head + static_cast<size_t>(row) * p.stateRow + static_cast<size_t>(col + c) * p.stateCol] = s[i][r][c] * p.finalScale;
+            for (int e = 0; e < 4; ++e)
+                if (col + e < p.value) to[static_cast<size_t>(e) * p.stateCol] = values[e];
         }
 }
 
@@ -132,14 +155,17 @@ __global__ void __launch_bounds__(128) decayedRecurrent(const __grid_constant__ 
 
 void launchRecurrent(const Pass &p, int type, cudaStream_t st) {
     const dim3 grid(p.heads, p.batch);
-    const int threads = (p.value + 31) / 32 * 32;
+    const int threads = (p.value + 15) / 16 * 32;
     withType(type, [&](auto t) {
         using T = decltype(t);
-        {
+        auto run = [&](auto reverse) {
+            constexpr bool Reverse = decltype(reverse)::value;
             KernelTimer timer__("decayedRecurrent", st);
-            if (p.key <= 64) launchDependent(decayedRecurrent<T, 64>, grid, threads, 0, st, p);
-            else launchDependent(decayedRecurrent<T, 128>, grid, threads, 0, st, p);
-        }
+            if (p.key <= 64) launchDependent(decayedRecurrent<T, 64, Reverse>, grid, threads, 0, st, p);
+            else launchDependent(decayedRecurrent<T, 128, Reverse>, grid, threads, 0, st, p);
+        };
+        if (p.reverse) run(std::true_type{});
+        else run(std::false_type{});
         afterLaunch("decayedRecurrent");
     });
 }

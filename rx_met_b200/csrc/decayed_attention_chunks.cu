@@ -168,121 +168,122 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     if (warp >= kCopyWarp) {
+        // The test stands alone in front of the three roles: only so does the compiler see whose registers these are.
         giveRegisters<40>();
-    if (warp == kCopyWarp) {
-        Turn turn;
-        for (int u = 0; u < count; ++u, turn.step(kStages)) {
-            // each as soon as its last use is over, in the order in which that is
-            const uint32_t to = tiles + turn.at * kStageBytes;
-            const int t = span.chunkAt(u, reverse) * kC;
-            auto fetch = [&](uint64_t &full, uint64_t &free, const CUtensorMap &map, uint32_t place, int boxes, int x, int head) {
-                if (turn.again) wait(free, turn.parity ^ 1u);
-                if (alive && electOne()) {
-                    cluster::arriveExpect(smemAddr(&full), boxes * kTile);
-                    for (int i = 0; i < boxes; ++i) copyTile4(to + place + i * kTile, &map, x + 64 * i, head, t, b, smemAddr(&full));
+        if (warp == kCopyWarp) {
+            Turn turn;
+            for (int u = 0; u < count; ++u, turn.step(kStages)) {
+                // each as soon as its last use is over, in the order in which that is
+                const uint32_t to = tiles + turn.at * kStageBytes;
+                const int t = span.chunkAt(u, reverse) * kC;
+                auto fetch = [&](uint64_t &full, uint64_t &free, const CUtensorMap &map, uint32_t place, int boxes, int x, int head) {
+                    if (turn.again) wait(free, turn.parity ^ 1u);
+                    if (alive && electOne()) {
+                        cluster::arriveExpect(smemAddr(&full), boxes * kTile);
+                        for (int i = 0; i < boxes; ++i) copyTile4(to + place + i * kTile, &map, x + 64 * i, head, t, b, smemAddr(&full));
+                    }
+                    __syncwarp();
+                };
+                fetch(small.fullK[turn.at], small.freeK[turn.at], kMap, kHalves * kTile, kHalves, 0, h / (p.heads / p.k.heads));
+                if (!StateOnly) fetch(small.fullQ[turn.at], small.freeQ[turn.at], qMap, 0, kHalves, 0, h / (p.heads / p.q.heads));
+                fetch(small.fullV[turn.at], small.freeV[turn.at], vMap, 2 * kHalves * kTile, 1, slice * kCols, h / (p.heads / p.v.heads));
+            }
+            // nothing is left in flight: the last use of each stage is over
+            for (int i = 0; i < kStages; ++i, turn.step(kStages))
+                if (turn.again) {
+                    waitSuspended(smemAddr(&small.freeK[turn.at]), turn.parity ^ 1u);
+                    if (!StateOnly) waitSuspended(smemAddr(&small.freeQ[turn.at]), turn.parity ^ 1u);
+                    waitSuspended(smemAddr(&small.freeV[turn.at]), turn.parity ^ 1u);
                 }
-                __syncwarp();
+        } else if (warp <= kScoreProducts) {
+            // Two threads issue the products, those of the state and those of the scores: one alone came to 4200 cycles a chunk, of which the tensor cores work 1300.  They poll, because a
+            // vote of the warp after each wait costs 150 cycles.
+            constexpr uint32_t kScores = halves(!kHalf, kC, false, false), kOutputs = halves(!kHalf, kCols, false, true);
+            constexpr uint32_t kBothTerms = halves(!kHalf, 2 * kCols, true, true), kThirdTerm = halves(!kHalf, kCols, true, true);
+            auto poll = [&](uint64_t &bar, uint32_t parity) {
+                if (alive) alive = waitPhase(smemAddr(&bar), parity);
+                fenceAfter();
             };
-            fetch(small.fullK[turn.at], small.freeK[turn.at], kMap, kHalves * kTile, kHalves, 0, h / (p.heads / p.k.heads));
-            if (!StateOnly) fetch(small.fullQ[turn.at], small.freeQ[turn.at], qMap, 0, kHalves, 0, h / (p.heads / p.q.heads));
-            fetch(small.fullV[turn.at], small.freeV[turn.at], vMap, 2 * kHalves * kTile, 1, slice * kCols, h / (p.heads / p.v.heads));
+            if (warp == kStateProducts) {
+                if (electOne()) {
+                    Turn turn;
+                    const uint64_t weighted = swizzledDescriptor(weightedV, kTile), third = swizzledDescriptor(weightedV + 2 * kTile), s = swizzledDescriptor(sTile);
+                    for (int u = 0; u < count; ++u, turn.step(kStages)) {
+                        const uint32_t at = tiles + turn.at * kStageBytes, parity = u & 1, kv = tmem + kKV;
+                        const uint64_t q = swizzledDescriptor(at), k = swizzledDescriptor(at + kHalves * kTile, kTile);
+                        poll(small.fullK[turn.at], turn.parity);
+                        poll(small.vReady, parity);
+#pragma unroll 2
+                        for (int i = 0; i < kC / 16; ++i) product(kv, k + i * 128, weighted + i * 128, kBothTerms, i > 0);
+                        if (!kHalf && thirdTerm(u)) {
+#pragma unroll 2
+                            for (int i = 0; i < kC / 16; ++i) product(kv + kCols, k + i * 128, third + i * 128, kThirdTerm, 1);
+                        }
+                        commitTo(smemAddr(&small.kvFull));
+                        commitTo(smemAddr(&small.freeK[turn.at]));
+                        if (StateOnly) {
+                            commitTo(smemAddr(&small.freeV[turn.at]));
+                            continue;
+                        }
+                        poll(small.fullQ[turn.at], turn.parity);
+                        poll(small.sReady, parity);
+                        if (u > 0) poll(small.oFree, parity ^ 1u);
+#pragma unroll 2
+                        for (int i = 0; i < DK / 16; ++i) product(tmem + kO1, q + (i / 4) * (kTile >> 4) + (i % 4) * 2, s + i * 128, kOutputs, i > 0);
+                        commitTo(smemAddr(&small.sFree));
+                        commitTo(smemAddr(&small.freeQ[turn.at]));
+                        commitTo(smemAddr(&small.oFull));
+                    }
+                }
+            } else if (!StateOnly && electOne()) {
+                // whichever is ready: neither the scores of the next chunk nor the outputs of this one keep the other waiting
+                Turn scoreTurn, outTurn;
+                uint32_t idle = 0;
+                for (int next = 0, u = 0; u < count && alive;) {
+                    bool worked = false;
+                    if (next < count && next <= u + 1 && testPhase(smemAddr(&small.fullK[scoreTurn.at]), scoreTurn.parity) && testPhase(smemAddr(&small.fullQ[scoreTurn.at]), scoreTurn.parity) &&
+                        (next < 2 || testPhase(smemAddr(&small.pFree[next & 1]), ((next >> 1) - 1) & 1))) {
+                        fenceAfter();
+                        const uint32_t at = tiles + scoreTurn.at * kStageBytes;
+                        const uint64_t q = swizzledDescriptor(at), k = swizzledDescriptor(at + kHalves * kTile);
+#pragma unroll 2
+                        for (int i = 0; i < 4 * kHalves; ++i) {
+                            const uint64_t step = (i / 4) * (kTile >> 4) + (i % 4) * 2;
+                            product(tmem + kP + (next & 1) * kC, q + step, k + step, kScores, i > 0);
+                        }
+                        commitTo(smemAddr(&small.pFull[next & 1]));
+                        commitTo(smemAddr(&small.freeK[scoreTurn.at]));
+                        commitTo(smemAddr(&small.freeQ[scoreTurn.at]));
+                        ++next;
+                        scoreTurn.step(kStages);
+                        worked = true;
+                    }
+                    // V is clean behind the row's end, and has been read for its weighted form, once the state says so
+                    if (u < next && testPhase(smemAddr(&small.pReady[u & 1]), (u >> 1) & 1) && testPhase(smemAddr(&small.vRead[outTurn.at]), outTurn.parity) &&
+                        (u == 0 || testPhase(smemAddr(&small.oFree), (u - 1) & 1))) {
+                        fenceAfter();
+                        const uint64_t v = swizzledDescriptor(tiles + outTurn.at * kStageBytes + 2 * kHalves * kTile);
+#pragma unroll 2
+                        for (int i = 0; i < kC / 16; ++i) productTmem(tmem + kO2, tmem + kP + (u & 1) * kC + (i / 4) * 64 + (i % 4) * 8, v + i * 128, kOutputs, i > 0);
+                        commitTo(smemAddr(&small.pFree[u & 1]));
+                        commitTo(smemAddr(&small.oFull));
+                        commitTo(smemAddr(&small.freeV[outTurn.at]));
+                        ++u;
+                        outTurn.step(kStages);
+                        worked = true;
+                    }
+                    idle = worked ? 0 : idle + 1;
+                    alive = idle < kSpinLimit;
+                }
+            }
+            __syncwarp();
+            // products go on after a wait that gave up, on whatever the operands hold; they end before the tensor memory is freed
+            uint64_t &done = small.productsDone[warp - kStateProducts];
+            if (electOne()) commitTo(smemAddr(&done));
+            __syncwarp();
+            waitSuspended(smemAddr(&done), 0);
+            alive = __all_sync(0xffffffffu, alive);
         }
-        // nothing is left in flight: the last use of each stage is over
-        for (int i = 0; i < kStages; ++i, turn.step(kStages))
-            if (turn.again) {
-                waitSuspended(smemAddr(&small.freeK[turn.at]), turn.parity ^ 1u);
-                if (!StateOnly) waitSuspended(smemAddr(&small.freeQ[turn.at]), turn.parity ^ 1u);
-                waitSuspended(smemAddr(&small.freeV[turn.at]), turn.parity ^ 1u);
-            }
-    } else if (warp <= kScoreProducts) {
-        // Two threads issue the products, those of the state and those of the scores: one alone came to 4200 cycles a chunk, of which the tensor cores work 1300.  They poll, because a
-        // vote of the warp after each wait costs 150 cycles.
-        constexpr uint32_t kScores = halves(!kHalf, kC, false, false), kOutputs = halves(!kHalf, kCols, false, true);
-        constexpr uint32_t kBothTerms = halves(!kHalf, 2 * kCols, true, true), kThirdTerm = halves(!kHalf, kCols, true, true);
-        auto poll = [&](uint64_t &bar, uint32_t parity) {
-            if (alive) alive = waitPhase(smemAddr(&bar), parity);
-            fenceAfter();
-        };
-        if (warp == kStateProducts) {
-            if (electOne()) {
-                Turn turn;
-                const uint64_t weighted = swizzledDescriptor(weightedV, kTile), third = swizzledDescriptor(weightedV + 2 * kTile), s = swizzledDescriptor(sTile);
-                for (int u = 0; u < count; ++u, turn.step(kStages)) {
-                    const uint32_t at = tiles + turn.at * kStageBytes, parity = u & 1, kv = tmem + kKV;
-                    const uint64_t q = swizzledDescriptor(at), k = swizzledDescriptor(at + kHalves * kTile, kTile);
-                    poll(small.fullK[turn.at], turn.parity);
-                    poll(small.vReady, parity);
-#pragma unroll 2
-                    for (int i = 0; i < kC / 16; ++i) product(kv, k + i * 128, weighted + i * 128, kBothTerms, i > 0);
-                    if (!kHalf && thirdTerm(u)) {
-#pragma unroll 2
-                        for (int i = 0; i < kC / 16; ++i) product(kv + kCols, k + i * 128, third + i * 128, kThirdTerm, 1);
-                    }
-                    commitTo(smemAddr(&small.kvFull));
-                    commitTo(smemAddr(&small.freeK[turn.at]));
-                    if (StateOnly) {
-                        commitTo(smemAddr(&small.freeV[turn.at]));
-                        continue;
-                    }
-                    poll(small.fullQ[turn.at], turn.parity);
-                    poll(small.sReady, parity);
-                    if (u > 0) poll(small.oFree, parity ^ 1u);
-#pragma unroll 2
-                    for (int i = 0; i < DK / 16; ++i) product(tmem + kO1, q + (i / 4) * (kTile >> 4) + (i % 4) * 2, s + i * 128, kOutputs, i > 0);
-                    commitTo(smemAddr(&small.sFree));
-                    commitTo(smemAddr(&small.freeQ[turn.at]));
-                    commitTo(smemAddr(&small.oFull));
-                }
-            }
-        } else if (!StateOnly && electOne()) {
-            // whichever is ready: neither the scores of the next chunk nor the outputs of this one keep the other waiting
-            Turn scoreTurn, outTurn;
-            uint32_t idle = 0;
-            for (int next = 0, u = 0; u < count && alive;) {
-                bool worked = false;
-                if (next < count && next <= u + 1 && testPhase(smemAddr(&small.fullK[scoreTurn.at]), scoreTurn.parity) && testPhase(smemAddr(&small.fullQ[scoreTurn.at]), scoreTurn.parity) &&
-                    (next < 2 || testPhase(smemAddr(&small.pFree[next & 1]), ((next >> 1) - 1) & 1))) {
-                    fenceAfter();
-                    const uint32_t at = tiles + scoreTurn.at * kStageBytes;
-                    const uint64_t q = swizzledDescriptor(at), k = swizzledDescriptor(at + kHalves * kTile);
-#pragma unroll 2
-                    for (int i = 0; i < 4 * kHalves; ++i) {
-                        const uint64_t step = (i / 4) * (kTile >> 4) + (i % 4) * 2;
-                        product(tmem + kP + (next & 1) * kC, q + step, k + step, kScores, i > 0);
-                    }
-                    commitTo(smemAddr(&small.pFull[next & 1]));
-                    commitTo(smemAddr(&small.freeK[scoreTurn.at]));
-                    commitTo(smemAddr(&small.freeQ[scoreTurn.at]));
-                    ++next;
-                    scoreTurn.step(kStages);
-                    worked = true;
-                }
-                // V is clean behind the row's end, and has been read for its weighted form, once the state says so
-                if (u < next && testPhase(smemAddr(&small.pReady[u & 1]), (u >> 1) & 1) && testPhase(smemAddr(&small.vRead[outTurn.at]), outTurn.parity) &&
-                    (u == 0 || testPhase(smemAddr(&small.oFree), (u - 1) & 1))) {
-                    fenceAfter();
-                    const uint64_t v = swizzledDescriptor(tiles + outTurn.at * kStageBytes + 2 * kHalves * kTile);
-#pragma unroll 2
-                    for (int i = 0; i < kC / 16; ++i) productTmem(tmem + kO2, tmem + kP + (u & 1) * kC + (i / 4) * 64 + (i % 4) * 8, v + i * 128, kOutputs, i > 0);
-                    commitTo(smemAddr(&small.pFree[u & 1]));
-                    commitTo(smemAddr(&small.oFull));
-                    commitTo(smemAddr(&small.freeV[outTurn.at]));
-                    ++u;
-                    outTurn.step(kStages);
-                    worked = true;
-                }
-                idle = worked ? 0 : idle + 1;
-                alive = idle < kSpinLimit;
-            }
-        }
-        __syncwarp();
-        // products go on after a wait that gave up, on whatever the operands hold; they end before the tensor memory is freed
-        uint64_t &done = small.productsDone[warp - kStateProducts];
-        if (electOne()) commitTo(smemAddr(&done));
-        __syncwarp();
-        waitSuspended(smemAddr(&done), 0);
-        alive = __all_sync(0xffffffffu, alive);
-    }
     } else if (warp < kFirstOutput) {
         if (!StateOnly) {
             // The thread's token, and the half of the columns that it takes: their scores lie in 64 columns of tensor memory, whose first 32 take what becomes of them.

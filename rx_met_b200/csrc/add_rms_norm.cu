@@ -493,10 +493,12 @@ TeamPlan teamFor(int width, int perThread) {
 
 // f(W, ITEMS) as compile-time constants.  16-byte groups where every array's rows start on 16 bytes and the width is made of them, else single elements.  A thread takes
 // sixteen elements, 32 of the widest rows and, in 16-byte groups, in front of codes: sums over a team cost the same for few as for many, and codes need two (8192 x 4096 bfloat16 with
-// codes 8 elements 77 us, 16 60 us, 32 42 us; without 59, 49, 50, and 4096 x 8192 53 with 16 and 50 with 32; gradients 92, 78).  Half of them or a quarter where the rows are few and a row's latency counts (one row of
-// 1024: 2.8 us, with 16 elements 3.8), or where 16 would leave lanes of a warp without any.
+// codes 8 elements 77 us, 16 60 us, 32 42 us; without 59, 49, 50, and 4096 x 8192 61 with 16 and 49 with 32, in 32 bits 84 and 94; gradients 92, 78, 93).  Half of them or a quarter where the rows are few and a row's latency counts (one row of
+// 1024: 2.8 us, with 16 elements 3.8), or where 16 would leave lanes of a warp without any; four or twelve for gradients of single elements, whose registers 16 overflow (5003 x 1001
+// 40 us for 34, 3000 x 5001 91 for 72).
+enum class Output { Rows, Codes, Gradients };
 template <class T, class F>
-void withGroups(int64_t rows, int width, bool vector, bool codes, F f) {
+void withGroups(int64_t rows, int width, bool vector, Output output, F f) {
     constexpr int V = 16 / sizeof(T);
     const bool small = rows <= currentDevice().sms || width < 512;
     auto fits = [&](int perThread) { return width <= kMaxThreads * perThread; };
@@ -504,10 +506,13 @@ void withGroups(int64_t rows, int width, bool vector, bool codes, F f) {
     using VW = std::integral_constant<int, V>;
     if (vector) {
         if (small && fits(V)) return f(VW{}, One{});
-        if (width <= 256 * 16 && !(codes && width >= 512)) return f(VW{}, std::integral_constant<int, 16 / V>{});
+        const bool wide = output == Output::Codes ? width >= 512 : output == Output::Rows && sizeof(T) == 2 && width > 256 * 16;
+        if (fits(16) && !wide) return f(VW{}, std::integral_constant<int, 16 / V>{});
         return f(VW{}, std::integral_constant<int, 32 / V>{});
     }
-    if (small && fits(4)) return f(One{}, std::integral_constant<int, 4>{});
+    const bool gradients = output == Output::Gradients;
+    if ((small || gradients) && fits(4)) return f(One{}, std::integral_constant<int, 4>{});
+    if (gradients && fits(12)) return f(One{}, std::integral_constant<int, 12>{});
     if (fits(16)) return f(One{}, std::integral_constant<int, 16>{});
     return f(One{}, std::integral_constant<int, 32>{});
 }
@@ -547,7 +552,7 @@ void launchNorm(const char *name, NormRows p, int type, cudaStream_t st) {
         const bool vector = p.width % group == 0 && p.xPitch % group == 0 && alignedTo(p.x, 16) &&
                             (!p.residual || (p.residualPitch % group == 0 && alignedTo(p.residual, 16) && alignedTo(p.total, 16))) &&
                             (Codes ? p.codesPitch % group == 0 && alignedTo(p.codes, group) : alignedTo(p.y, 16));
-        withGroups<T>(p.rows, p.width, vector, Codes, [&](auto w, auto items) {
+        withGroups<T>(p.rows, p.width, vector, Codes ? Output::Codes : Output::Rows, [&](auto w, auto items) {
             constexpr int W = decltype(w)::value, ITEMS = decltype(items)::value;
             const TeamPlan plan = teamFor(p.width, W * ITEMS);
             p.team = plan.team;
@@ -572,7 +577,7 @@ template <class F>
 void withGradKernel(int64_t rows, int width, int type, bool vector, F f) {
     withType(type, [&](auto t) {
         using T = decltype(t);
-        withGroups<T>(rows, width, vector, false, [&](auto w, auto items) {
+        withGroups<T>(rows, width, vector, Output::Gradients, [&](auto w, auto items) {
             constexpr int W = decltype(w)::value, ITEMS = decltype(items)::value;
             const TeamPlan plan = teamFor(width, W * ITEMS);
             const size_t partial = static_cast<size_t>(plan.teams()) * width * sizeof(float);

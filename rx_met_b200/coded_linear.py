@@ -35,7 +35,7 @@ def coded_linear(codes: torch.Tensor, scale: torch.Tensor, weight: CodedWeight, 
                  dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """activation((codes @ weight.codes.T) * scale * weight.scale + bias) + residual in `dtype` (float32, bfloat16 or float16).
     codes int8 [..., inner], scale float32 [...], bias float32 [outer], residual of `dtype` [..., outer].  gelu is the erf form.  inner is at most
-    131071, the number of rows at most 4194304.  No gradient."""
+    131071, the numbers of rows and of outer channels at most 4194240 each.  No gradient."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"coded_linear: activation {activation!r}, one of {', '.join(ACTIVATIONS)}")
     if dtype not in _TYPES:

@@ -5,6 +5,7 @@
 // kernels, one GRU inference 92 us against 72), so that the small calls were bound by the interpreter.  The C ABI is
 // not linked: the package loads the library globally first, so that an overridden library path reaches this module too.
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/clamp.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -614,7 +615,9 @@ struct AttentionArguments {
         if (counts) {
             sameDevice(*counts, queries, "lengths");
             TORCH_CHECK(counts->dim() == 1 && counts->size(0) == problem.batch && at::isIntegralType(counts->scalar_type(), true), "lengths must be integers of shape [", problem.batch, "]");
-            lengths = counts->to(at::kInt).contiguous();
+            // of 64 bits, they are cut to the tokens that there are before they are cut to 32
+            const int64_t most = dims == 3 ? 1 : queries.size(1);
+            lengths = (counts->scalar_type() == at::kLong ? at::clamp(*counts, 0, most) : *counts).to(at::kInt).contiguous();
         }
         problem.q = view(q);
         problem.k = view(k);

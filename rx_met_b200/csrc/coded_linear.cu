@@ -4,10 +4,13 @@
 
 namespace rxmet {
 namespace codedlinear {
+
+constexpr int kTile = 64;
+
 namespace {
 
 // A CTA computes 64 rows x 64 channels; 64 codes of K at a time go to shared memory byte by byte, packed in words of four for dp4a.
-constexpr int kTile = 64, kWords = 16, kThreads = 256;
+constexpr int kWords = 16, kThreads = 256;
 
 __device__ __forceinline__ uint32_t wordAt(const int8_t *row, int k, int inner) {
     uint32_t word = 0;
@@ -91,7 +94,9 @@ extern "C" int rxmet_coded_linear(int64_t rows, int inner, int outer, const int8
         RXMET_REQUIRE(rows >= 0 && inner >= 1 && outer >= 1, "coded_linear: %lld rows, inner %d, outer %d", static_cast<long long>(rows), inner, outer);
         // -128 * -128 * inner has to stay below 2^31
         if (inner > 131071) fail(RXMET_ERR_UNSUPPORTED, "coded_linear: inner %d, at most 131071", inner);
-        if (rows > (int64_t{1} << 22)) fail(RXMET_ERR_UNSUPPORTED, "coded_linear: %lld rows, at most 4194304", static_cast<long long>(rows));
+        // tiles of 64 along a grid axis of 65535
+        constexpr int64_t kMost = int64_t{65535} * codedlinear::kTile;
+        if (rows > kMost || outer > kMost) fail(RXMET_ERR_UNSUPPORTED, "coded_linear: %lld rows, outer %d, at most %lld each", static_cast<long long>(rows), outer, static_cast<long long>(kMost));
         RXMET_REQUIRE(activation >= RXMET_ACTIVATION_NONE && activation <= RXMET_ACTIVATION_GELU, "coded_linear: unknown activation %d", activation);
         if (rows == 0) return;
         RXMET_REQUIRE(codes_dev && scale_dev && weight_dev && weight_scale_dev && out_dev, "coded_linear: null tensor");

@@ -429,6 +429,7 @@ void launchTensorCores(const Problem &p, cudaStream_t st) {
     int rows = 0, parts = 1;
     for (const int r : {16, 32, 64, 128})
         for (int q = 1; q <= 8 && q <= chunks; q *= 2) {
+            if (p.rows > int64_t{65535} * r) continue;   // of a grid's axis
             const int64_t ctas = static_cast<int64_t>(over(p.outer, kChannels)) * static_cast<int64_t>(over(p.rows, r)) * q;
             const int resident = r == 16 ? residentParts<16>(q) : r == 32 ? residentParts<32>(q) : r == 64 ? residentParts<64>(q) : residentParts<128>(q);
             const double ends = r == 16 ? 2.8 : r == 32 ? 3.3 : r == 64 ? 4.5 : 5.8;

@@ -106,20 +106,22 @@ extern "C" {
 size_t rxmet_decayed_attention_workspace_bytes(const rxmet_decayed_attention *a, int backward) {
     WorkspaceSizer size;
     if (!a || a->batch <= 0 || a->tokens <= 0) return 0;
-    const rxmet_head_tensor none{};
-    auto states = [&](const Pass &p) {
-        if (const size_t floats = planChunks(p, a->type).stateFloats(p)) size.take<float>(floats);
-    };
-    if (!backward) {
-        states(forwardPass(*a));
-        return size.used();
-    }
-    for (const Pass &p : {queryPass(*a, none, none, none, none), keyPass(*a, none, none, none, none), valuePass(*a, none, none, none, none)}) states(p);
-    const size_t rows = static_cast<size_t>(a->batch) * a->tokens * a->heads;
-    if (a->q.heads != a->heads) size.take<float>(rows * a->key_dim);
-    if (a->k.heads != a->heads) size.take<float>(rows * a->key_dim);
-    if (a->v.heads != a->heads) size.take<float>(rows * a->value_dim);
-    return size.used();
+    const int status = guarded([&] {
+        const rxmet_head_tensor none{};
+        auto states = [&](const Pass &p) {
+            if (const size_t floats = planChunks(p, a->type).stateFloats(p)) size.take<float>(floats);
+        };
+        if (!backward) {
+            states(forwardPass(*a));
+            return;
+        }
+        for (const Pass &p : {queryPass(*a, none, none, none, none), keyPass(*a, none, none, none, none), valuePass(*a, none, none, none, none)}) states(p);
+        const size_t rows = static_cast<size_t>(a->batch) * a->tokens * a->heads;
+        if (a->q.heads != a->heads) size.take<float>(rows * a->key_dim);
+        if (a->k.heads != a->heads) size.take<float>(rows * a->key_dim);
+        if (a->v.heads != a->heads) size.take<float>(rows * a->value_dim);
+    });
+    return status == RXMET_OK ? size.used() : 0;
 }
 
 int rxmet_decayed_attention_forward(const rxmet_decayed_attention *problem, const float *state_dev, void *out_dev, float *final_state_dev,

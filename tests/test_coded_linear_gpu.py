@@ -73,6 +73,19 @@ def test_extreme_codes(rows):
     assert torch.isnan(out[0]).all() and torch.isfinite(out[1:]).all()
 
 
+@pytest.mark.parametrize("aligned", [True, False])
+def test_many_rows(aligned):
+    """More rows than a grid's axis has places for the smallest tiles; a few of them are compared."""
+    from rx_met_b200.coded_linear import CodedWeight, coded_linear
+    rows = 1_100_000 if aligned else 300_000
+    inner = 32 if aligned else 33
+    codes = torch.randint(-127, 128, (rows, inner), device="cuda", dtype=torch.int8)
+    weight = torch.randint(-127, 128, (5, inner), device="cuda", dtype=torch.int8)
+    out = coded_linear(codes, torch.ones(rows, device="cuda"), CodedWeight(weight, torch.ones(5, device="cuda")), dtype=torch.float32)
+    at = torch.cat([torch.arange(300, device="cuda"), torch.arange(rows - 300, rows, device="cuda"), torch.randint(0, rows, (2000,), device="cuda")])
+    assert torch.equal(out[at].double(), codes[at].double() @ weight.double().T)
+
+
 def test_strides_and_leading_dimensions():
     from rx_met_b200.coded_linear import CodedWeight, code_weight, coded_linear
     codes, scale, weight, weight_scale, bias, residual = problem(60, 100, 50, dtype=torch.bfloat16)

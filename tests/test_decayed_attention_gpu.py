@@ -73,6 +73,31 @@ def test_ragged_rows(tokens, index_type, dtype):
     assert torch.equal(last[[0, 4]], state[[0, 4]])
 
 
+def test_lengths_beyond_32_bits():
+    from rx_met_b200.decayed_attention import decayed_attention
+    q, k, v, decay, state = problem(2, 40, 2, 2, 32, 32, torch.bfloat16, seed=3, state=True)
+    want = decayed_attention(q, k, v, decay, state=state, lengths=torch.tensor([40, 0], device="cuda"))
+    got = decayed_attention(q, k, v, decay, state=state, lengths=torch.tensor([2 ** 32 + 1, -2 ** 40], device="cuda"))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("queries,keys,values", [(1.0, 1e-4, 1.0), (1.0, 1.0, 1e-4), (1e-4, 300.0, 300.0)])
+def test_small_and_large_values(queries, keys, values, dtype):
+    """Scores and states near both ends of half's range: the bounds hold relative to the magnitudes."""
+    q, k, v, decay, state = problem(2, 300, 2, 2, 64, 64, dtype, seed=13, state=True)
+    q, k, v, state = ((t.double() * f).to(t.dtype) for t, f in ((q, queries), (k, keys), (v, values), (state, keys * values)))
+    from rx_met_b200.decayed_attention import decayed_attention
+    out, last = decayed_attention(q, k, v, decay, state=state)
+    want, wanted_last = ml.attend(q, k, v, decay, state, None, 0.125)
+    magnitude, magnitude_last = ml.magnitudes(lambda a, b, c, s: ml.attend(a, b, c, decay, s, None, 0.125), (q, k, v, state))
+    assert want.abs().max() < torch.finfo(dtype).max
+    # operands are scaled to the top of half's range, so that what they lose is relative to a row's largest: as much as its unit once more
+    bound = ml.attention_bound(magnitude, dtype, 300, 64, dtype) - (192 * 2.0 ** -25 * 5 if dtype == torch.float16 else 0)
+    ml.within(out, want, bound + magnitude * ml.UNIT[dtype])
+    ml.within(last, wanted_last, ml.attention_bound(magnitude_last, torch.float32, 300, 64, torch.float32))
+
+
 @pytest.mark.parametrize("dtype", ml.TYPES)
 @pytest.mark.parametrize("tokens", [5, 300])
 def test_decays(tokens, dtype):

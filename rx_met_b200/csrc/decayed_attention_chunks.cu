@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint64_t weighted = swizzledDescriptor(weightedV, kTile), third = swizzledDescriptor(weightedV + 2 * kTile), s = swizzledDescriptor(sTile);
                     for (int u = 0; u < count; ++u, turn.step(kStages)) {
                         const uint32_t at = tiles + turn.at * kStageBytes, parity = u & 1, kv = tmem + kKV;
-                        const uint64_t q = swizzledDescriptor(at), k = swizzledDescriptor(at + kHalves * kTile, kTile);
+                        const uint64_t q = swizzledDescriptor(at), k = swizzledDescriptor(at + kHalves * kTile, kHalves == 2 ? kTile : 0);   // 64 keys: a stride of 0 lays them down twice, in rows 0 and 64 of KV
                         poll(small.fullK[turn.at], turn.parity);
                         poll(small.vReady, parity);
 #pragma unroll 2
@@ -423,23 +423,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         takeRegisters<104>();
-        const int quarter = warp & 3, half = (warp - kFirstState) >> 2, d = 32 * quarter + lane;   // the thread's row of the state, and which half of its columns
-        const bool rows = 32 * quarter < DK;                                                   // warps beyond the keys have none
+        // The thread's row of the state and its columns of it: a half with 128 keys; a quarter with 64, whose rows stand twice in KV, so that all eight warps
+        // have work (8 x 4096 tokens, 16 heads of 64: 66.4 -> 63.6 us against halves for four of the warps).
+        constexpr int kMine = DK == 64 ? 16 : 32;
+        const int quarter = warp & 3, d = (32 * quarter + lane) % DK, mine = ((warp - kFirstState) >> 2) * (128 / DK) + 32 * quarter / DK;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
         const int stid = tid - 32 * kFirstState;
         const size_t head = static_cast<size_t>(b) * p.heads + h, stateSize = static_cast<size_t>(p.key) * p.value;
-        const int col = slice * kCols + half * 32;
-        Pair s[16];   // its 32 columns
+        const int col = slice * kCols + mine * kMine;
+        Pair s[kMine / 2];
         const float *in = segments.count > 1 ? (StateOnly ? nullptr : segments.states + (head * segments.count + segment) * stateSize) : p.stateIn ? p.stateIn + head * stateSize : nullptr;
         const int inRow = segments.count > 1 ? p.value : p.stateRow, inCol = segments.count > 1 ? 1 : p.stateCol;
         const float inScale = segments.count > 1 ? 1.f : p.inScale;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[j] = pairOf(0.f, 0.f);
+        for (int j = 0; j < kMine / 2; ++j) s[j] = pairOf(0.f, 0.f);
         if (in && d < p.key) {
             const float *from = in + static_cast<size_t>(d) * inRow + static_cast<size_t>(col) * inCol;
             if (inCol == 1 && p.value % 4 == 0 && (reinterpret_cast<uintptr_t>(in) & 15) == 0) {
 #pragma unroll
-                for (int j = 0; j < 16; j += 2) {
+                for (int j = 0; j < kMine / 2; j += 2) {
                     if (col + 2 * j >= p.value) continue;
                     const float4 v = *reinterpret_cast<const float4 *>(from + 2 * j);
                     s[j] = pairOf(v.x * inScale, v.y * inScale);
@@ -447,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             } else
 #pragma unroll
-            for (int j = 0; j < 16; ++j, from += 2 * inCol)
+            for (int j = 0; j < kMine / 2; ++j, from += 2 * inCol)
                 s[j] = pairOf(col + 2 * j < p.value ? inScale * from[0] : 0.f, col + 2 * j + 1 < p.value ? inScale * from[inCol] : 0.f);
         }
 
@@ -456,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if constexpr (kHalf) {
                 float most = 0.f;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
+                for (int j = 0; j < kMine / 2; ++j) {
                     const float2 v = floatsOf(s[j]);
                     most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y)));
                 }
@@ -470,34 +472,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (stid == 0) small.stateScale[u & 1] = 1.f / up;
                 groupBarrier(kStateMeets, 32 * kStateWarps);
             }
-            if (rows) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t w[4];
+            for (int c = 0; c < kMine / 8; ++c) {
+                uint32_t w[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) w[j] = kHalf ? pack2<T>(mul2(s[4 * c + j], pairOf(up, up))) : pack2<T>(s[4 * c + j]);
-                    storeShared(sTile + d * 128 + (((half * 4 + c) ^ (d & 7)) << 4), w[0], w[1], w[2], w[3]);
-                }
-                fenceAsyncProxy();
+                for (int j = 0; j < 4; ++j) w[j] = kHalf ? pack2<T>(mul2(s[4 * c + j], pairOf(up, up))) : pack2<T>(s[4 * c + j]);
+                storeShared(sTile + d * 128 + (((mine * (kMine / 8) + c) ^ (d & 7)) << 4), w[0], w[1], w[2], w[3]);
             }
+            fenceAsyncProxy();
             arriveWarp(small.sReady);
         };
 
         auto advance = [&](int u) {   // the state behind chunk u
             const float keep = small.powers[tokensOf(span.chunkAt(u, reverse))];
-            if (rows) {
 #pragma unroll
-                for (int part = 0; part < 2; ++part) {
-                    uint32_t r[16], low[16];
-                    const uint32_t from = lanes + kKV + half * 32 + part * 16;
-                    loadTmem16(from, r);
-                    loadTmem16(from + kCols, low);
-                    loadsDone();
+            for (int part = 0; part < kMine / 16; ++part) {
+                uint32_t r[16], low[16];
+                const uint32_t from = lanes + kKV + mine * kMine + part * 16;
+                loadTmem16(from, r);
+                loadTmem16(from + kCols, low);
+                loadsDone();
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const Pair high = pairOf(r[2 * j], r[2 * j + 1]), rest = pairOf(low[2 * j], low[2 * j + 1]);
-                        s[part * 8 + j] = fma2(s[part * 8 + j], pairOf(keep, keep), kHalf ? fma2(rest, pairOf(1.f / 2048, 1.f / 2048), high) : add2(high, rest));
-                    }
+                for (int j = 0; j < 8; ++j) {
+                    const Pair high = pairOf(r[2 * j], r[2 * j + 1]), rest = pairOf(low[2 * j], low[2 * j + 1]);
+                    s[part * 8 + j] = fma2(s[part * 8 + j], pairOf(keep, keep), kHalf ? fma2(rest, pairOf(1.f / 2048, 1.f / 2048), high) : add2(high, rest));
                 }
             }
             fenceBefore();
@@ -584,12 +582,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (d < p.key) {
                 if (outCol == 1 && p.value % 4 == 0 && (reinterpret_cast<uintptr_t>(last) & 15) == 0) {
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2)
+                    for (int j = 0; j < kMine / 2; j += 2)
                         if (col + 2 * j < p.value)
                             *reinterpret_cast<float4 *>(to + 2 * j) = make_float4(floatsOf(s[j]).x * scale, floatsOf(s[j]).y * scale, floatsOf(s[j + 1]).x * scale, floatsOf(s[j + 1]).y * scale);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
+                    for (int j = 0; j < kMine; ++j)
                         if (col + j < p.value) to[static_cast<size_t>(j) * outCol] = (j & 1 ? floatsOf(s[j / 2]).y : floatsOf(s[j / 2]).x) * scale;
                 }
             }

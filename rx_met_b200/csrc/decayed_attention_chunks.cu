@@ -75,18 +75,18 @@ struct Span {
     }
 };
 
-// The power of two that brings magnitudes up to `most` below 2^15; 1 where there is nothing to scale.
-__device__ __forceinline__ float toTopOfHalf(float most) {
-    if (!(most > 0.f) || isinf(most)) return 1.f;
-    const int e = static_cast<int>(__float_as_uint(most) >> 23) - 127;   // floor(log2), -127 below the normal range
-    const int up = min(14 - e, 100);
-    return __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+// The power of two that brings magnitudes up to one with the exponent bits `exponent` below 2^15; 1 where there is nothing to scale.
+__device__ __forceinline__ uint32_t exponentBits(float most) { return __float_as_uint(most) >> 23; }
+__device__ __forceinline__ float toTopOfHalf(uint32_t exponent) {
+    if (exponent == 0 || exponent == 255) return 1.f;   // none that a half could show; infinite
+    return __uint_as_float(static_cast<uint32_t>(127 + min(14 + 127 - static_cast<int>(exponent), 100)) << 23);
 }
 
 // What a CTA keeps in shared memory beside the tiles.
 struct Small {
     float powers[kC + 4], scaledPowers[32], columnPowers[32];   // l^n; scale l^n; scale l^(31 - j) or scale l^j of a block's columns
-    float rowPeaks[2][kC], statePeaks[kStateWarps], stateScale[2];
+    float statePeaks[2][kStateWarps], stateScale[2];   // of two chunks in turn, so that the warps meet once a chunk
+    uint8_t rowPeaks[2][2][kC];               // exponents, of two chunks in turn
     uint8_t rowScale[3][kC];                  // exponents of the powers of two that rows of P were scaled by, for three chunks
     uint64_t fullK[3], fullQ[3], fullV[3], freeK[3], freeQ[3], freeV[3], vRead[3], pFull[2], pReady[2], pFree[2], vReady, kvFull, sReady, sFree, oFull, oFree, productsDone[2];
     uint32_t tmemSlot;
@@ -337,11 +337,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(__uint_as_float(r[j])));
                     });
-                    small.rowPeaks[half][i] = most;
+                    const uint32_t own = exponentBits(most);
+                    small.rowPeaks[u & 1][half][i] = static_cast<uint8_t>(own);
                     groupBarrier(kLanesMeet + quarter, 64);
-                    up = toTopOfHalf(fmaxf(most, small.rowPeaks[half ^ 1][i]));
-                    if (half == 0) small.rowScale[u % 3][i] = static_cast<uint8_t>(__float_as_uint(up) >> 23);
-                    groupBarrier(kLanesMeet + quarter, 64);
+                    up = toTopOfHalf(max(own, static_cast<uint32_t>(small.rowPeaks[u & 1][half ^ 1][i])));
+                    if (half == 0) small.rowScale[u % 3][i] = static_cast<uint8_t>(exponentBits(up));
                 }
                 eachBlock([&](int e, const uint32_t(&r)[32]) {
                     uint32_t words[16];
@@ -463,14 +463,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y)));
                 }
                 const uint32_t peak = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-                if (lane == 0) small.statePeaks[stid >> 5] = __uint_as_float(peak);
+                if (lane == 0) small.statePeaks[u & 1][stid >> 5] = __uint_as_float(peak);
                 groupBarrier(kStateMeets, 32 * kStateWarps);
                 most = 0.f;
 #pragma unroll
-                for (int w = 0; w < kStateWarps; ++w) most = fmaxf(most, small.statePeaks[w]);
-                up = toTopOfHalf(most);
+                for (int w = 0; w < kStateWarps; ++w) most = fmaxf(most, small.statePeaks[u & 1][w]);
+                up = toTopOfHalf(exponentBits(most));
                 if (stid == 0) small.stateScale[u & 1] = 1.f / up;
-                groupBarrier(kStateMeets, 32 * kStateWarps);
             }
 #pragma unroll
             for (int c = 0; c < kMine / 8; ++c) {

@@ -165,11 +165,11 @@ int residentClusters(const void *kernel, int ctas, int block, size_t smem) {
     return n;
 }
 
-OverlapLane &overlapLane() {
+OverlapLane &overlapLane(int which) {
     constexpr int kMaxDevices = 64;
-    static thread_local OverlapLane lanes[kMaxDevices];
+    static thread_local OverlapLane lanes[kMaxDevices][kLanes];
     const int device = currentDevice().device;
-    OverlapLane &lane = lanes[device];
+    OverlapLane &lane = lanes[device][which];
     if (lane.stream == nullptr) {
         RXMET_CUDA(cudaStreamCreateWithFlags(&lane.stream, cudaStreamNonBlocking));
         for (int i = 0; i < kLaneEvents; ++i) {

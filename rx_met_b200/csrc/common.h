@@ -112,13 +112,13 @@ inline int smsPerPass() { return std::max(1, currentDevice().sms / concurrentPas
 // (record fork[i] there, make the lane wait for it) and joins back (record done[i] on the lane, make the caller's
 // stream wait for it) before it returns, so the pattern is legal inside a stream capture and the caller never
 // sees the lane.
-constexpr int kLaneEvents = 8;
+constexpr int kLaneEvents = 8, kLanes = 2;
 struct OverlapLane {
     cudaStream_t stream = nullptr;
     cudaEvent_t fork[kLaneEvents] = {};
     cudaEvent_t done[kLaneEvents] = {};
 };
-OverlapLane &overlapLane();
+OverlapLane &overlapLane(int which = 0);   // below kLanes
 // Time chunks, in processing order, that a forward (ascending time) or a backward (descending time) over T
 // steps is cut into so that the batched GEMM work of one chunk runs under the recurrence of its neighbour;
 // one chunk = no overlap.  RXMET_GRU_FWD_CHUNKS / RXMET_GRU_BWD_CHUNKS = "15,35,50" (per cent of the steps, in the

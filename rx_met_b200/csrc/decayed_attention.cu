@@ -7,17 +7,30 @@ namespace rxmet {
 namespace decayed {
 namespace {
 
-// out[row][g][d] = sum over the `share` heads of group g of part[row][g * share + i][d], in their order.
-template <class T>
+// out[row][g][d] = sum over the `share` heads of group g of part[row][g * share + i][d], in their order; W elements a thread.  Bound: memory, and the latency of a thread's one round
+// (6000 rows, 8 heads to 2: 64 elements a head 7.3 us by elements, 4.9 by fours; 96 elements 9.8 and 6.0).
+template <class T, int W>
 __global__ void __launch_bounds__(256) sumSharedHeads(const float *part, int64_t rows, int groups, int share, int dim, T *out) {
     waitForPredecessor();
     letDependentsStart();
-    const int64_t count = rows * groups * dim;
+    const int pieces = dim / W;
+    const int64_t count = rows * groups * pieces;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < count; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t group = i / dim, d = i - group * dim;
-        float sum = 0.f;
-        for (int k = 0; k < share; ++k) sum += part[(group * share + k) * dim + d];
-        out[i] = fromFloat<T>(sum);
+        const int64_t group = i / pieces;
+        const int d = static_cast<int>(i - group * pieces) * W;
+        const float *from = part + group * share * dim + d;
+        float sum[W] = {};
+#pragma unroll 4
+        for (int k = 0; k < share; ++k, from += dim) {
+            if constexpr (W == 4) {
+                const float4 v = *reinterpret_cast<const float4 *>(from);
+                sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
+            } else sum[0] += *from;
+        }
+        T *to = out + group * dim + d;
+        if constexpr (W == 4 && sizeof(T) == 2) *reinterpret_cast<uint2 *>(to) = make_uint2(pack2<T>(sum[0], sum[1]), pack2<T>(sum[2], sum[3]));
+        else if constexpr (W == 4) *reinterpret_cast<float4 *>(to) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        else *to = fromFloat<T>(sum[0]);
     }
 }
 
@@ -182,10 +195,11 @@ int rxmet_decayed_attention_backward(const rxmet_decayed_attention *problem, con
             if (!p.outFloat || rows == 0) return;
             withType(a.type, [&](auto t) {
                 using T = decltype(t);
-                const int64_t count = rows * ownHeads * p.value;
+                const bool fours = p.value % 4 == 0 && alignedTo(out, 4 * sizeof(T));
+                const int64_t count = rows * ownHeads * p.value / (fours ? 4 : 1);
                 {
                     KernelTimer timer__("sumSharedHeads", st);
-                    launchDependent(sumSharedHeads<T>, static_cast<unsigned>(std::min<int64_t>((count + 255) / 256, 8 * currentDevice().sms)), 256, 0, st,
+                    launchDependent(fours ? sumSharedHeads<T, 4> : sumSharedHeads<T, 1>, static_cast<unsigned>(std::min<int64_t>((count + 255) / 256, 8 * currentDevice().sms)), 256, 0, st,
                                     static_cast<const float *>(p.out), rows, ownHeads, a.heads / ownHeads, p.value, static_cast<T *>(out));
                 }
                 afterLaunch("sumSharedHeads");

@@ -5,7 +5,7 @@
 // ahead.  With loads to registers one row ahead in its place, 8192 x 4096 bfloat16 take 66 us for 60 (forward with codes) and 105 for 78 (gradients), at the same 16 elements a thread.
 // Sums run in 32 bits: a thread's own elements in order, lanes as a tree, warps in order, so that results do not depend on the grid.
 //
-// Bound: HBM for codes (8192 x 4096 bfloat16 42 us, 5.6 TB/s) and the forward (50 us, 5.3 TB/s); issue and the barrier of a team's sum for the gradients (78 us, 4.3 TB/s).
+// Bound: HBM for codes (8192 x 4096 bfloat16 42 us, 5.6 TB/s) and the forward (49.5 us, 5.4 TB/s); issue and the barrier of a team's sum for the gradients (78 us, 4.3 TB/s).
 #include <algorithm>
 
 #include "common.h"
@@ -170,7 +170,7 @@ __device__ __forceinline__ void storeLanes(T *to, const Lanes<W> &l) {
 // One CTA's side of a ring.
 template <class T, int ARRAYS>
 struct RingReader {
-    const Source (&sources)[ARRAYS];
+    const Source *sources;
     const Ring ring;
     int64_t rows;
     int width, teams;
@@ -363,8 +363,13 @@ struct NormGradient {
 };
 
 // The sum is taken from x and residual again: from its rounded copy, dweight of a bfloat16 step would be off by 1.6e-3 in place of 1.6e-7.  A row is read twice, before and after
-// its mean is known, from the ring.  Sums of dweight over a team's rows stay in registers.
-template <class T, int W, int ITEMS, bool Ringed>
+// its mean is known, from the ring.  Sums of dweight over a team's rows stay in registers, or in shared memory
+// for 32 single elements a thread, where sums and weights would fill the registers (2000 x 16383 half 679 us with them there, 237 so; 1500 x 12001 in 32 bits 429 and 157).
+template <int W, int ITEMS>
+constexpr bool sumsInShared = W == 1 && ITEMS > 16;
+// RINGED: arrays that come through the ring, 0, 4, or 3 for wide rows: dtotal is wanted last, so that it stays out of a ring that has no room for two stages of all four (4096 x 8192 in 32 bits 184
+// us without a ring, 153 so; 2000 x 16384 half 151 and 102).
+template <class T, int W, int ITEMS, int RINGED>
 __global__ void __launch_bounds__(kMaxThreads, W * ITEMS <= 8 ? 2 : 1) addRmsNormGrad(const __grid_constant__ NormGradient p, int *status) {
     using Elements = Lanes<W>;
     __shared__ RingSpace space;
@@ -374,16 +379,16 @@ __global__ void __launch_bounds__(kMaxThreads, W * ITEMS <= 8 ? 2 : 1) addRmsNor
     const Team team(p.team);
     const int first = team.rank * W, stride = team.size * W, width = p.width;
     const float perElement = 1.f / static_cast<float>(width);
-    if constexpr (Ringed) space.init(p.ring.depth);
+    if constexpr (RINGED > 0) space.init(p.ring.depth);
     waitForPredecessor();
     const int64_t step = static_cast<int64_t>(gridDim.x) * team.count, row0 = static_cast<int64_t>(blockIdx.x) * team.count;
     const Source sources[4] = {{p.dy, width}, {p.x, p.xPitch}, {p.residual, p.residualPitch}, {p.dtotal, width}};
-    RingReader<T, 4> ring{sources, p.ring, p.rows, width, team.count, space.full, space.freed, stages};
+    RingReader<T, RINGED> ring{sources, p.ring, p.rows, width, team.count, space.full, space.freed, stages};
     const int64_t rounds = row0 < p.rows ? (p.rows - row0 + step - 1) / step : 0;
     auto asks = [&](int64_t round) {   // the copies of a round, by the first warp
         if (threadIdx.x < 32 && round < rounds) ring.ask(row0 + round * step);
     };
-    if constexpr (Ringed)
+    if constexpr (RINGED > 0)
         for (int i = 0; i < p.ring.depth; ++i) asks(i);
     float *mine = teamPartial + static_cast<size_t>(team.index) * width;
     auto weightOf = [&](int i) {
@@ -393,11 +398,18 @@ __global__ void __launch_bounds__(kMaxThreads, W * ITEMS <= 8 ? 2 : 1) addRmsNor
             for (int j = 0; j < W; ++j) w.set(j, weightAt(p.weight, p.weightType, first + i * stride + j));
         return w;
     };
-    Elements kept[ITEMS], dw[ITEMS];
+    constexpr bool kSumsInShared = sumsInShared<W, ITEMS>;
+    static_assert(!kSumsInShared || RINGED == 0, "the sums lie where a ring would");
+    constexpr int kBatch = 8;   // elements whose loads from memory are under way together; none of them passes a store, which might be to the same place
+    Elements kept[kSumsInShared ? 1 : ITEMS], dw[kSumsInShared ? 1 : ITEMS];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        kept[i] = weightOf(i);
-        dw[i] = allOf<W>(0.f);
+        if constexpr (kSumsInShared) {
+            if (first + i * stride < width) mine[first + i * stride] = 0.f;
+        } else {
+            kept[i] = weightOf(i);
+            dw[i] = allOf<W>(0.f);
+        }
     }
     letDependentsStart();
     bool alive = true;
@@ -408,13 +420,13 @@ __global__ void __launch_bounds__(kMaxThreads, W * ITEMS <= 8 ? 2 : 1) addRmsNor
         rmsNext = p.rms[min(row + step, p.rows - 1)];
         const T *dy = static_cast<const T *>(p.dy) + row * width, *dt = static_cast<const T *>(p.dtotal) + row * width;
         const T *x = static_cast<const T *>(p.x) + row * p.xPitch, *r = static_cast<const T *>(p.residual) + row * p.residualPitch;
-        if constexpr (Ringed) {
+        if constexpr (RINGED > 0) {
             if (alive) alive = ring.wait();
             if (round > 0) asks(round - 1 + p.ring.depth);   // into the stage of the round before, which all warps have read or are about to
             dy = ring.template row<(W > 1)>(0, first0, team.index);
             x = ring.template row<(W > 1)>(1, first0, team.index);
             r = ring.template row<(W > 1)>(2, first0, team.index);
-            dt = ring.template row<(W > 1)>(3, first0, team.index);
+            if constexpr (RINGED == 4) dt = ring.template row<(W > 1)>(3, first0, team.index);
         }
         const int here = row < p.rows ? width : 0;   // a row past the end adds nothing
         auto unit = [&](int at) {   // (x + residual) rms
@@ -422,35 +434,87 @@ __global__ void __launch_bounds__(kMaxThreads, W * ITEMS <= 8 ? 2 : 1) addRmsNor
             if (p.residual) t = t + loadLanes<T, W>(r + at);
             return t * rms;
         };
-        Elements dots = allOf<W>(0.f);
+        // dy, (x + residual) rms and the weight of elements that a thread has one behind the other; the loads of an array together, without a branch between them
+        auto batch = [&](int i0, float(&g)[kBatch], float(&u)[kBatch], float(&w)[kBatch]) {
+            int at[kBatch];
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int at = first + i * stride;
-            if (at >= here) continue;
-            const Elements g = loadLanes<T, W>(dy + at), u = unit(at);
-            dots = dots.plus(g * kept[i], u);
-            dw[i] = dw[i].plus(g, u);
+            for (int i = 0; i < kBatch; ++i) at[i] = min(first + (i0 + i) * stride, width - 1);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                g[i] = toFloat(dy[at[i]]);
+                u[i] = toFloat(x[at[i]]);
+            }
+            if (p.residual)
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) u[i] += toFloat(r[at[i]]);
+            auto weights = [&](auto *from) {
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) w[i] = toFloat(from[at[i]]);
+            };
+            if (p.weightType == RXMET_TYPE_F32) weights(static_cast<const float *>(p.weight));
+            else if (p.weightType == RXMET_TYPE_BF16) weights(static_cast<const __nv_bfloat16 *>(p.weight));
+            else weights(static_cast<const __half *>(p.weight));
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) u[i] *= rms;
+        };
+        Elements dots = allOf<W>(0.f);
+        if constexpr (kSumsInShared) {
+#pragma unroll 1
+            for (int i0 = 0; i0 < ITEMS; i0 += kBatch) {
+                float g[kBatch], u[kBatch], w[kBatch];
+                batch(i0, g, u, w);
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const int at = first + (i0 + i) * stride;
+                    if (at >= here) continue;
+                    dots.v = fmaf(g[i] * w[i], u[i], dots.v);
+                    mine[at] = fmaf(g[i], u[i], mine[at]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int at = first + i * stride;
+                if (at >= here) continue;
+                const Elements g = loadLanes<T, W>(dy + at), u = unit(at);
+                dots = dots.plus(g * kept[i], u);
+                dw[i] = dw[i].plus(g, u);
+            }
         }
         const float mean = team.sum(dots.total(), sums, round & 1) * perElement;
         T *dx = static_cast<T *>(p.dx) + row * width;
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int at = first + i * stride;
-            if (at >= here) continue;
+        auto gradient = [&](int at, const Elements &w) {
             Elements out = p.dtotal ? loadLanes<T, W>(dt + at) : allOf<W>(0.f);
-            out = out.plus((loadLanes<T, W>(dy + at) * kept[i]).plus(unit(at), -mean), rms);
-            storeLanes<T, W>(dx + at, out);
+            return out.plus((loadLanes<T, W>(dy + at) * w).plus(unit(at), -mean), rms);
+        };
+        if constexpr (kSumsInShared) {
+#pragma unroll 1
+            for (int i0 = 0; i0 < ITEMS; i0 += kBatch) {
+                float g[kBatch], u[kBatch], w[kBatch], t[kBatch] = {};
+                batch(i0, g, u, w);
+                if (p.dtotal)
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i) t[i] = toFloat(dt[min(first + (i0 + i) * stride, width - 1)]);
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i)
+                    if (first + (i0 + i) * stride < here) dx[first + (i0 + i) * stride] = fromFloat<T>(fmaf(fmaf(g[i], w[i], u[i] * -mean), rms, t[i]));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (first + i * stride < here) storeLanes<T, W>(dx + first + i * stride, gradient(first + i * stride, kept[i]));
         }
-        if constexpr (Ringed) ring.done();
+        if constexpr (RINGED > 0) ring.done();
     }
     if (!alive && (threadIdx.x & 31) == 0) atomicExch(status, 1);
     if (!p.partial) return;
     __syncthreads();   // the ring is read
+    if constexpr (!kSumsInShared)
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
+        for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-        for (int j = 0; j < W; ++j)
-            if (first + i * stride < width) mine[first + i * stride + j] = dw[i].at(j);
+            for (int j = 0; j < W; ++j)
+                if (first + i * stride < width) mine[first + i * stride + j] = dw[i].at(j);
     __syncthreads();
     for (int c = threadIdx.x; c < width; c += blockDim.x) {
         float s = 0.f;
@@ -581,9 +645,27 @@ void withGradKernel(int64_t rows, int width, int type, bool vector, F f) {
             constexpr int W = decltype(w)::value, ITEMS = decltype(items)::value;
             const TeamPlan plan = teamFor(width, W * ITEMS);
             const size_t partial = static_cast<size_t>(plan.teams()) * width * sizeof(float);
-            const Ring ring = ringFor(reinterpret_cast<const void *>(addRmsNormGrad<T, W, ITEMS, true>), width, sizeof(T), 4, plan);
-            const auto kernel = ring.depth > 0 ? addRmsNormGrad<T, W, ITEMS, true> : addRmsNormGrad<T, W, ITEMS, false>;
-            const size_t smem = std::max(partial, static_cast<size_t>(ring.depth) * ring.arrayBytes * 4);
+            // 64 bytes a thread are rows of up to 32 KB, of which a ring holds four or three arrays; longer ones have three, or no ring.
+            constexpr int kBytes = W * ITEMS * static_cast<int>(sizeof(T));
+            constexpr bool kRing = !sumsInShared<W, ITEMS>;
+            Ring ring;
+            void (*kernel)(NormGradient, int *) = nullptr;
+            int arrays = 0;
+            auto through = [&](auto count) {
+                constexpr int ARRAYS = decltype(count)::value;
+                if (kernel) return;
+                if constexpr (ARRAYS > 0) {
+                    ring = ringFor(reinterpret_cast<const void *>(addRmsNormGrad<T, W, ITEMS, ARRAYS>), width, sizeof(T), ARRAYS, plan);
+                    if (ring.depth == 0) return;
+                }
+                kernel = addRmsNormGrad<T, W, ITEMS, ARRAYS>;
+                arrays = ARRAYS;
+            };
+            if constexpr (kRing && kBytes <= 64) through(std::integral_constant<int, 4>{});
+            if constexpr (kRing && kBytes >= 64) through(std::integral_constant<int, 3>{});
+            if constexpr (!kRing || kBytes > 64) through(std::integral_constant<int, 0>{});
+            if (!kernel) fail(RXMET_ERR_CUDA, "add_rms_norm backward: no kernel for rows of %d elements", width);
+            const size_t smem = std::max(partial, static_cast<size_t>(ring.depth) * ring.arrayBytes * arrays);
             ensureDynamicSmem(reinterpret_cast<const void *>(kernel), smem);
             const int grid = gridFor(reinterpret_cast<const void *>(kernel), (rows + kGradRowsOfTeam - 1) / kGradRowsOfTeam, plan.teams(), plan.threads, smem);
             f(kernel, plan, ring, smem, grid);

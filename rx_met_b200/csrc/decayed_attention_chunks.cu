@@ -14,6 +14,10 @@
 // rebuilt from rounded values: the weighted V goes in as the sum of three bfloat16 or two half terms, which leaves 2^-24.  half has a short range: its rows of P and its S are scaled by
 // powers of two to the top of it, and the second term of the weighted V is scaled by 2^11.  The two larger terms lie side by side as 128 columns of one product, which reads
 // K once for both.
+//
+// Bound: the chain of a chunk (terms of V, their product, the state, its rounding, Q S), 3300 cycles with 64 keys and 4000 with 128 of which the tensor cores work a third, the issue slots half; and
+// one CTA an SM.  8 x 4096 tokens of 16 heads: 152 us with 128 elements a head (3.5 TB/s, two rounds of CTAs), 64 with 64 (4.2 TB/s); half, whose scales take a turn more over scores and
+// state, 172 and 86.
 #include "decayed_attention.h"
 #include "dependent_launch.cuh"
 #include "element_types.cuh"

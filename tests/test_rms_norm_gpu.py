@@ -93,6 +93,14 @@ def test_gradients(rows, width, dtype, weight_type, with_total):
     ml.within(dweight, wanted_weight, wanted_weight.abs() * ml.UNIT[weight_type] * 1.01 + summed * (rows / 32 + 64) * 2.0 ** -24 + ml.TINY[weight_type])
 
 
+# rows of which three arrays fit shared memory, or none; all by groups and by elements, with more rows than CTAs take at once
+@pytest.mark.parametrize("rows,width,dtype", [(650, 8192, torch.float32), (650, 7201, torch.float32), (40, 9000, torch.float32), (40, 12001, torch.float32), (650, 15000, torch.float16),
+                                              (650, 8191, torch.bfloat16), (650, 16381, torch.bfloat16)])
+@pytest.mark.parametrize("with_total", [True, False])
+def test_gradients_of_wide_rows(rows, width, dtype, with_total):
+    test_gradients(rows, width, dtype, None, with_total)
+
+
 def test_gradients_without_a_residual_or_a_trained_weight():
     from rx_met_b200 import rms_norm
     x, weight, residual = tensors(70, 96, torch.float32, seed=4)

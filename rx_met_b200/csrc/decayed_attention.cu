@@ -99,6 +99,23 @@ Pass forwardPass(const rxmet_decayed_attention &a) {
     return p;
 }
 
+// Lanes that were forked from a stream, joined to it in the end whether or not a launch in between has failed: the caller frees what they write.
+struct ForkedLanes {
+    cudaStream_t stream;
+    OverlapLane *lanes[3] = {};
+    cudaError_t join() {
+        cudaError_t first = cudaSuccess;
+        for (OverlapLane *&lane : lanes) {
+            if (!lane) continue;
+            for (const cudaError_t error : {cudaEventRecord(lane->done[0], lane->stream), cudaStreamWaitEvent(stream, lane->done[0], 0)})
+                if (first == cudaSuccess) first = error;
+            lane = nullptr;
+        }
+        return first;
+    }
+    ~ForkedLanes() { join(); }
+};
+
 // Kernels by size and type.  Single tokens have a kernel of their own, chunks are taken from 16 or 32 tokens on (planChunks); tensors that TMA cannot copy and 32-bit ones go token by token.
 void launchPass(const Pass &p, int type, float *states, cudaStream_t st) {
     const ChunkPlan plan = planChunks(p, type);
@@ -208,7 +225,8 @@ int rxmet_decayed_attention_backward(const rxmet_decayed_attention *problem, con
         // The passes run side by side, because none fills the GPU with few heads; those that may have heads to sum begin.  Forward and gradients of 2 x 1024 tokens and 16 heads of 64 take 55 us
         // with two passes one after another beside the third, 40 so; of 6 x 1000 tokens, 8 heads and shared keys 104 and 88; of 8 x 2048 tokens and 16 heads, which fill it, 128 both ways.
         const bool wanted[] = {dq_dev != nullptr, dk_dev != nullptr, dv_dev || dstate_dev};
-        OverlapLane *lanes[3] = {};   // the last of the passes has the caller's stream
+        ForkedLanes forked{st};   // the last of the passes has the caller's stream
+        auto &lanes = forked.lanes;
         for (int i = 2, last = wanted[0] ? 0 : wanted[1] ? 1 : 2; i > last; --i)
             if (wanted[i]) lanes[i] = &overlapLane(i - 1);
         for (OverlapLane *lane : lanes)
@@ -232,11 +250,7 @@ int rxmet_decayed_attention_backward(const rxmet_decayed_attention *problem, con
             p.stateIn = state_dev;
             run(p, states[0], a.q.heads, dq_dev, st);
         }
-        for (OverlapLane *lane : lanes)
-            if (lane) {
-                RXMET_CUDA(cudaEventRecord(lane->done[0], lane->stream));
-                RXMET_CUDA(cudaStreamWaitEvent(st, lane->done[0], 0));
-            }
+        RXMET_CUDA(forked.join());
     });
 }
 

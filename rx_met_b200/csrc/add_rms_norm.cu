@@ -242,6 +242,22 @@ struct RingSpace {
     }
 };
 
+// Codes of a row whose 127 / peak is infinite, in place of those that a thread has just written: values and step are brought up by a power of two.  A step below the normal numbers may have
+// been rounded down by so much that the largest values lie more than 127 of it from zero, or to zero itself.  The row is read again: such rows are rare, and with this in the kernel's
+// registers 8192 x 4096 bfloat16 took 46.5 us for 44.
+template <class T, int W>
+__device__ __noinline__ void tinyCodes(const NormRows &p, int64_t row, float rms, float step, int first, int stride) {
+    constexpr float kUp = 0x1p64f;
+    const float inverse = step > 0.f ? 1.f / (step * kUp) : 0.f;
+    for (int group = first; group < p.width; group += stride)
+        for (int i = group; i < group + W; ++i) {
+            float t = toFloat(static_cast<const T *>(p.x)[row * p.xPitch + i]);
+            if (p.residual) t += toFloat(static_cast<const T *>(p.residual)[row * p.residualPitch + i]);
+            t = t * rms * (p.weight ? weightAt(p.weight, p.weightType, i) : 1.f);
+            p.codes[row * p.codesPitch + i] = static_cast<int8_t>(__float2int_rn(fminf(fmaxf(t * kUp * inverse, -127.f), 127.f)));
+        }
+}
+
 // Ringed: rows come through the ring.  Else straight from memory: few rows, which have no next ones to fetch, and those too wide for a ring.
 template <class T, int W, int ITEMS, bool Codes, bool Ringed>
 __global__ void __launch_bounds__(kMaxThreads) __maxnreg__(W * ITEMS <= 8 ? 64 : W * ITEMS <= 16 ? (W > 1 ? 80 : 96) : 128) addRmsNorm(const __grid_constant__ NormRows p, int *status) {
@@ -340,6 +356,7 @@ __global__ void __launch_bounds__(kMaxThreads) __maxnreg__(W * ITEMS <= 8 ? 64 :
                 }
                 if (first + i * stride < here) *reinterpret_cast<Pack<int8_t, W> *>(codes + first + i * stride) = out;
             }
+            if (isinf(inverse) && real) tinyCodes<T, W>(p, row, rms, most / 127.f, first, stride);
         } else {
             T *y = static_cast<T *>(p.y) + row * width;
 #pragma unroll

@@ -1,0 +1,45 @@
+"""Where the token mixer's operators can go wrong beside their ordinary inputs: ends of the number range, what is not finite, sizes, memory orders."""
+import pytest
+import torch
+
+import mixer_lib as ml
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- rows of codes ------------------------------------------------------------------------------------------------------
+
+def tiny_rows(rows, width, dtype):
+    """Rows whose largest magnitudes go down to the smallest number there is, with zeros in them."""
+    g = torch.Generator(device="cuda").manual_seed(width)
+    x = torch.randn(rows, width, device="cuda", generator=g, dtype=torch.float64)
+    tops = torch.tensor([1e-30, 3e-36, 3.8e-37, 3.7e-37, 1e-37, 1e-39, 1e-41, 2.0 ** -149], device="cuda", dtype=torch.float64)
+    x = (x / x.abs().amax(dim=1, keepdim=True) * tops[torch.arange(rows, device="cuda") % 8][:, None]).to(dtype)
+    x[:, ::3] = 0
+    return x
+
+
+def check_tiny(codes, scale, x):
+    most, step, half = x.double().abs().amax(dim=1), scale.double(), 2.0 ** -150   # half: of the smallest number
+    ml.within(scale, most / 127, most * 2.0 ** -24 + half)
+    # half a step, what the quotient is off by at 127 steps, and what a step that was rounded down leaves of the largest values
+    off = (codes.double() * step[:, None] - x.double()).abs()
+    assert bool((off <= (step * (0.5 + 127 * 2.0 ** -22) + 127 * half)[:, None]).all())
+    assert not codes[x == 0].any() and int(codes.min()) >= -127
+    assert bool((codes.abs().amax(dim=1)[most > 1e-38] == 127).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,width", [(8, 64), (8, 50), (3000, 64), (3000, 1000), (2400, 1001), (600, 4096), (8, 16384), (8, 16383)])
+def test_codes_of_tiny_rows(rows, width, dtype):
+    from rx_met_b200 import rms_norm
+    x = tiny_rows(rows, width, dtype)
+    check_tiny(*rms_norm.code_rows(x), x)
+
+
+def test_codes_behind_a_tiny_weight():
+    from rx_met_b200 import rms_norm
+    x, weight = torch.ones(40, 96, device="cuda"), torch.full((96,), 1e-38, device="cuda")
+    weight[::2] = 0
+    codes, scale, _ = rms_norm.add_rms_norm_codes(x, weight, eps=0.0)
+    check_tiny(codes, scale, weight.expand(40, 96))

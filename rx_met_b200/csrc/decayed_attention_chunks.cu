@@ -11,12 +11,14 @@
 //   state      eight warps: weighted V for the products; the state itself, 32 bits, stays in their registers
 //
 // Roundings.  Operands of tensor cores have the type of the inputs: P times the decays and S are rounded to it once, next to the rounding of the output.  The state is never
-// rebuilt from rounded values: the weighted V goes in as the sum of three bfloat16 or two half terms, which leaves 2^-24.  half has a short range: its rows of P and its S are scaled by
+// rebuilt from rounded values: the weighted V goes in as the sum of three bfloat16 terms, which leave 2^-24, or two of half,
+// 2^-22.  half has a short range: its rows of P and its S are scaled by
 // powers of two to the top of it, and the second term of the weighted V is scaled by 2^11.  The two larger terms lie side by side as 128 columns of one product, which reads
-// K once for both.
+// K once for both.  All chunks have the third term: later ones may add little, so that what an early one leaves in the state is all of it (8 x 4096 tokens of 16 heads of 128: 161 us, 152 with
+// the third term of the last chunks alone, whose states were off by 2^-18.6 there).
 //
 // Bound: the chain of a chunk (terms of V, their product, the state, its rounding, Q S), 3300 cycles with 64 keys and 4000 with 128 of which the tensor cores work a third, the issue slots half; and
-// one CTA an SM.  8 x 4096 tokens of 16 heads: 152 us with 128 elements a head (3.5 TB/s, two rounds of CTAs), 64 with 64 (4.2 TB/s); half, whose scales take a turn more over scores and
+// one CTA an SM.  8 x 4096 tokens of 16 heads: 161 us with 128 elements a head (3.3 TB/s, two rounds of CTAs), 64 with 64 (4.2 TB/s); half, whose scales take a turn more over scores and
 // state, 172 and 86.
 #include "decayed_attention.h"
 #include "dependent_launch.cuh"
@@ -40,8 +42,8 @@ constexpr uint32_t kShared = 232448;   // all of an SM, as the tensor memory
 constexpr uint32_t kP = 0, kO1 = 256, kO2 = 320, kKV = 384;
 enum Barrier { kStateMeets = 1, kLanesMeet };   // named barriers; the last takes four
 
-// A block starts with 80 registers a thread, 1920 for the lanes of its 24 warps in the same place.  The scores keep theirs (8 warps, 640); outputs give up 16 (4 warps, 256), copies
-// and products 40 (4 warps, 160), and the state takes 104 (8 warps, 832): 1888.  With 80 the state would be spilled (advance() 420 -> 1700 cycles).
+// A block starts with 80 registers a thread, 1920 for the lanes of its 24 warps in the same place.  Scores give up 8 (8 warps, 576), outputs 32 (4 warps, 192), copies and products 40 (4
+// warps, 160), and the state takes 120 (8 warps, 960): 1888.  With 80 the state would be spilled (advance() 420 -> 1700 cycles), with 104 its third terms.
 template <int REGISTERS>
 __device__ __forceinline__ void giveRegisters() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGISTERS)); }
 template <int REGISTERS>
@@ -97,13 +99,13 @@ struct Small {
     int failed;
 };
 
-// DK: elements of a key that the tiles hold, 64 or 128.  StateOnly: nothing but the state at the end of the segment.  Stores: how outputs leave, by the alignment of their
+// DK: elements of a key that the tiles hold, 64 or 128.  Third: bfloat16 with a third term of the weighted V.  StateOnly: nothing but the state at the end of the segment.  Stores: how outputs leave, by the alignment of their
 // rows.
 enum class Stores { Elements, Packed, Floats };   // one by one; sixteen of the type of the inputs, or eight in 32 bits, at a time
-template <class T, int DK, bool StateOnly, Stores How>
+template <class T, int DK, bool Third, bool StateOnly, Stores How>
 __global__ void __launch_bounds__(kThreads, 1)
     decayedChunks(const __grid_constant__ Pass p, const __grid_constant__ CUtensorMap qMap, const __grid_constant__ CUtensorMap kMap, const __grid_constant__ CUtensorMap vMap,
-                  const Segments segments, const int terms, int *status) {
+                  const Segments segments, int *status) {
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr int kHalves = DK / 64;
     constexpr uint32_t kStageBytes = (2 * kHalves + 1) * kTile;
@@ -123,14 +125,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Span span(length, segment, segments.chunks);
     const int count = span.chunks;
     auto tokensOf = [&](int chunk) { return min(kC, length - chunk * kC); };
-    // Whether the third term of a chunk's weighted V can reach the state at the row's end: what is left of it there is l^(tokens from here on), and two terms
-    // leave 2^-17.
-    const float third = terms > 2 ? p.logDecay[h] : -INFINITY;
-    auto thirdTerm = [&](int u) {
-        const int chunk = span.chunkAt(u, reverse), rest = reverse ? chunk * kC : max(0, length - (chunk + 1) * kC);
-        return terms > 2 && (rest == 0 || third * rest > -2.77f);   // 2^-4: two terms are 2^-21 of the state there
-    };
-
     if (tid == 0) {
         small.failed = 0;
         for (int i = 0; i < kStages; ++i)
@@ -219,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         poll(small.vReady, parity);
 #pragma unroll 2
                         for (int i = 0; i < kC / 16; ++i) product(kv, k + i * 128, weighted + i * 128, kBothTerms, i > 0);
-                        if (!kHalf && thirdTerm(u)) {
+                        if (Third) {
 #pragma unroll 2
                             for (int i = 0; i < kC / 16; ++i) product(kv + kCols, k + i * 128, third + i * 128, kThirdTerm, 1);
                         }
@@ -289,6 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             alive = __all_sync(0xffffffffu, alive);
         }
     } else if (warp < kFirstOutput) {
+        giveRegisters<72>();
         if (!StateOnly) {
             // The thread's token, and the half of the columns that it takes: their scores lie in 64 columns of tensor memory, whose first 32 take what becomes of them.
             const int quarter = warp & 3, half = warp >> 2, i = 32 * quarter + lane;
@@ -362,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else if (warp < kFirstState) {
-        giveRegisters<64>();
+        giveRegisters<48>();
         if (!StateOnly) {
             const int quarter = warp & 3, i = 32 * quarter + lane;   // the thread's token
             const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
@@ -426,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else {
-        takeRegisters<104>();
+        takeRegisters<120>();
         // The thread's row of the state and its columns of it: a half with 128 keys; a quarter with 64, whose rows stand twice in KV, so that all eight warps
         // have work (8 x 4096 tokens, 16 heads of 64: 66.4 -> 63.6 us against halves for four of the warps).
         constexpr int kMine = DK == 64 ? 16 : 32;
@@ -511,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float2 t = unpack2<T>(term);
             return fma2(pairOf(t.x, t.y), pairOf(-1.f, -1.f), x);
         };
-        uint32_t hi[4][4], mid[4][4];   // the two larger terms of the next chunk's weighted V
+        uint32_t hi[4][4], mid[4][4], low[Third ? 4 : 1][4];   // the terms of the next chunk's weighted V
         Turn turn;
         auto weigh = [&](int u) {
             const uint32_t at = tiles + turn.at * kStageBytes;
@@ -537,6 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     Pair rest = less(weighted, hi[c][j]);
                     if constexpr (kHalf) rest = mul2(rest, pairOf(2048.f, 2048.f));
                     mid[c][j] = pack2<T>(rest);
+                    if constexpr (Third) low[c][j] = pack2<T>(less(rest, mid[c][j]));
                 }
         };
         if (count > 0) weigh(0);
@@ -547,20 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 0; c < 4; ++c) {
                 storeShared(weightedV + pieceAt(c), hi[c][0], hi[c][1], hi[c][2], hi[c][3]);
                 storeShared(weightedV + kTile + pieceAt(c), mid[c][0], mid[c][1], mid[c][2], mid[c][3]);
-            }
-            if (!kHalf && thirdTerm(u)) {
-                const float w = weightOf(tokensOf(span.chunkAt(u, reverse)));
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t v[4];
-                    loadShared(tiles + turn.at * kStageBytes + 2 * kHalves * kTile + pieceAt(c), v);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 x = unpack2<T>(v[j]);
-                        v[j] = pack2<T>(less(less(mul2(pairOf(x.x, x.y), pairOf(w, w)), hi[c][j]), mid[c][j]));
-                    }
-                    storeShared(weightedV + 2 * kTile + pieceAt(c), v[0], v[1], v[2], v[3]);
-                }
+                if constexpr (Third) storeShared(weightedV + 2 * kTile + pieceAt(c), low[c][0], low[c][1], low[c][2], low[c][3]);
             }
             fenceAsyncProxy();
             if (!StateOnly) arriveWarp(small.vRead[turn.at]);
@@ -698,31 +681,36 @@ void launchChunks(const Pass &p, int type, const ChunkPlan &plan, float *states,
     if (!ok) fail(RXMET_ERR_CUDA, "cuTensorMapEncodeTiled failed");
     const Segments segments{plan.segments, plan.segmentChunks, states};
     const dim3 grid((p.value + kCols - 1) / kCols * plan.segments, p.heads, p.batch);
-    auto run = [&](auto kernel, const char *name, int terms) {
+    auto run = [&](auto kernel, const char *name) {
         ensureDynamicSmem(reinterpret_cast<const void *>(kernel), kShared);
         {
             KernelTimer timer__(name, st);
-            launchDependent(kernel, grid, kThreads, kShared, st, p, q, k, v, segments, terms, waitStatus());
+            launchDependent(kernel, grid, kThreads, kShared, st, p, q, k, v, segments, waitStatus());
         }
         afterLaunch(name);
     };
-    // Three bfloat16 terms of the weighted K where the state is an output; two, 2^-17, where it only feeds products that round it to 2^-9.
-    const int terms = bf16 && p.stateOut ? 3 : 2;
     auto both = [&](auto t, auto dk) {
         using T = decltype(t);
         constexpr int DK = decltype(dk)::value;
+        constexpr bool kThree = std::is_same<T, __nv_bfloat16>::value;
+        auto outputs = [&](auto third) {
+            constexpr bool Third = decltype(third)::value;
+            run(!wide        ? decayedChunks<T, DK, Third, false, Stores::Elements>
+                : p.outFloat ? decayedChunks<T, DK, Third, false, Stores::Floats>
+                             : decayedChunks<T, DK, Third, false, Stores::Packed>,
+                "decayedChunks");
+        };
+        // Three bfloat16 terms of the weighted V where the state is an output; two, 2^-17, where it only feeds products that round it to 2^-9.
         if (plan.segments > 1) {
-            run(decayedChunks<T, DK, true, Stores::Elements>, "decayedChunksState", terms);
+            run(p.stateOut ? decayedChunks<T, DK, kThree, true, Stores::Elements> : decayedChunks<T, DK, false, true, Stores::Elements>, "decayedChunksState");
             {
                 KernelTimer timer__("joinSegments", st);
                 launchDependent(joinSegments, dim3((p.key * p.value + 255) / 256, p.heads, p.batch), 256, 0, st, p, segments);
             }
             afterLaunch("joinSegments");
-        }
-        if (p.out || plan.segments == 1) run(!wide        ? decayedChunks<T, DK, false, Stores::Elements>
-                                                    : p.outFloat ? decayedChunks<T, DK, false, Stores::Floats>
-                                                                 : decayedChunks<T, DK, false, Stores::Packed>,
-                                                    "decayedChunks", plan.segments > 1 ? 2 : terms);
+            if (p.out) outputs(std::false_type{});
+        } else if (p.stateOut) outputs(std::integral_constant<bool, kThree>{});
+        else outputs(std::false_type{});
     };
     auto withKeys = [&](auto t) {
         if (p.key <= 64) both(t, std::integral_constant<int, 64>{});

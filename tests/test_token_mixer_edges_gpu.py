@@ -43,3 +43,35 @@ def test_codes_behind_a_tiny_weight():
     weight[::2] = 0
     codes, scale, _ = rms_norm.add_rms_norm_codes(x, weight, eps=0.0)
     check_tiny(codes, scale, weight.expand(40, 96))
+
+
+# ---- states to the last bits ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens", [128, 500, 2000])
+@pytest.mark.parametrize("Dk,Dv", [(64, 64), (128, 48), (40, 128)])
+@pytest.mark.parametrize("loud", ["all", "first", "last"])
+@pytest.mark.parametrize("small", [1.0, 1e-6])
+@pytest.mark.parametrize("dtype", [torch.bfloat16])
+def test_bits_of_a_state(tokens, Dk, Dv, loud, small, dtype):
+    """Relative to the state itself, whichever tokens it comes from.  A chunk's products are added up in 24 steps, each off by 2^-24 of a running sum at most, its operand's terms leave 2^-22 or less: 2^-20.5
+    for a sum of independent ones.  Behind it, every chunk multiplies by a power of the decay that is off by 2^-24."""
+    from rx_met_b200.decayed_attention import decayed_attention
+    g = torch.Generator(device="cuda").manual_seed(2)
+    make = lambda d, f: (torch.randn(2, tokens, 4, d, device="cuda", generator=g) * f).to(dtype)  # noqa: E731
+    q, k, v, dout = make(Dk, 1.0), make(Dk, 1.0), make(Dv, small), make(Dv, small)
+    if loud != "all":   # the tokens that the state, and its gradient, are far from or near to
+        quiet = slice(100, None) if loud == "first" else slice(0, max(0, tokens - 100))
+        v[:, quiet] = 0
+        back = dout.flip(1)
+        back[:, quiet] = 0
+        dout = back.flip(1)
+    decay = torch.tensor([0.0, -0.003, -0.01, -0.03], device="cuda")
+    S = torch.zeros(2, 4, Dk, Dv, device="cuda", requires_grad=True)
+    out, last = decayed_attention(q, k, v, decay, state=S)
+    dstate, = torch.autograd.grad(out, S, dout)
+    t = torch.arange(tokens, device="cuda", dtype=torch.float64)
+    left, gone = torch.exp(decay.double()[:, None] * (tokens - 1 - t)), torch.exp(decay.double()[:, None] * (t + 1))
+    wants = (torch.einsum("bthk,ht,bthv->bhkv", k.double(), left, v.double()), torch.einsum("bthk,ht,bthv->bhkv", q.double(), gone, dout.double()) * Dk ** -0.5)
+    for name, got, want in zip(("state", "dstate"), (last.detach(), dstate), wants):
+        off = (got.double() - want).flatten(2).norm(dim=2) / want.flatten(2).norm(dim=2)
+        assert float(off.max()) < 2.0 ** -20.5 + (tokens // 128) * 2.0 ** -24, (name, off)

@@ -12,8 +12,8 @@
 //
 // Roundings.  Operands of tensor cores have the type of the inputs: P times the decays and S are rounded to it once, next to the rounding of the output.  The state is never
 // rebuilt from rounded values: the weighted V goes in as the sum of three bfloat16 terms, which leave 2^-24, or two of half,
-// 2^-22.  half has a short range: its rows of P and its S are scaled by
-// powers of two to the top of it, and the second term of the weighted V is scaled by 2^11.  The two larger terms lie side by side as 128 columns of one product, which reads
+// 2^-22.  half has a short range: its rows of P, its S and the weighted V of a chunk are scaled by
+// powers of two to the top of it, the second term of the weighted V by 2^11 more (unscaled, values of 1e-6 left 2^-16; 1 x 16384 tokens of 8 heads of 64 45 -> 46.5 us).  The two larger terms lie side by side as 128 columns of one product, which reads
 // K once for both.  All chunks have the third term: later ones may add little, so that what an early one leaves in the state is all of it (8 x 4096 tokens of 16 heads of 128: 161 us, 152 with
 // the third term of the last chunks alone, whose states were off by 2^-18.6 there).
 //
@@ -91,7 +91,7 @@ __device__ __forceinline__ float toTopOfHalf(uint32_t exponent) {
 // What a CTA keeps in shared memory beside the tiles.
 struct Small {
     float powers[kC + 4], scaledPowers[32], columnPowers[32];   // l^n; scale l^n; scale l^(31 - j) or scale l^j of a block's columns
-    float statePeaks[2][kStateWarps], stateScale[2];   // of two chunks in turn, so that the warps meet once a chunk
+    float statePeaks[2][kStateWarps], valuePeaks[2][kStateWarps], stateScale[2];   // of two chunks in turn, so that the warps meet once a chunk
     uint8_t rowPeaks[2][2][kC];               // exponents, of two chunks in turn
     uint8_t rowScale[3][kC];                  // exponents of the powers of two that rows of P were scaled by, for three chunks
     uint64_t fullK[3], fullQ[3], fullV[3], freeK[3], freeQ[3], freeV[3], vRead[3], pFull[2], pReady[2], pFree[2], vReady, kvFull, sReady, sFree, oFull, oFree, productsDone[2];
@@ -481,6 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             arriveWarp(small.sReady);
         };
 
+        float down = 1.f, downNext = 1.f;   // one over the scales of the weighted V of half, of this chunk and the next
         auto advance = [&](int u) {   // the state behind chunk u
             const float keep = small.powers[tokensOf(span.chunkAt(u, reverse))];
 #pragma unroll
@@ -493,7 +494,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const Pair high = pairOf(r[2 * j], r[2 * j + 1]), rest = pairOf(low[2 * j], low[2 * j + 1]);
-                    s[part * 8 + j] = fma2(s[part * 8 + j], pairOf(keep, keep), kHalf ? fma2(rest, pairOf(1.f / 2048, 1.f / 2048), high) : add2(high, rest));
+                    // the power of two that V was scaled by taken out again, exactly
+                    s[part * 8 + j] = fma2(s[part * 8 + j], pairOf(keep, keep), kHalf ? fma2(rest, pairOf(down / 2048, down / 2048), mul2(high, pairOf(down, down))) : add2(high, rest));
                 }
             }
             fenceBefore();
@@ -519,9 +521,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                 fenceAsyncProxy();
                 groupBarrier(kStateMeets, 32 * kStateWarps);
             }
-            const float w = weightOf(n);
+            float w = weightOf(n);
 #pragma unroll
             for (int c = 0; c < 4; ++c) loadShared(at + 2 * kHalves * kTile + pieceAt(c), hi[c]);
+            if constexpr (kHalf) {   // to the top of half's range
+                __half2 most = __float2half2_rn(0.f);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) most = __hmax2(most, __habs2(*reinterpret_cast<const __half2 *>(&hi[c][j])));
+                const uint32_t own = __reduce_max_sync(0xffffffffu, __float_as_uint(w * fmaxf(__low2float(most), __high2float(most))));
+                if (lane == 0) small.valuePeaks[u & 1][stid >> 5] = __uint_as_float(own);
+                groupBarrier(kStateMeets, 32 * kStateWarps);
+                float peak = 0.f;
+#pragma unroll
+                for (int i = 0; i < kStateWarps; ++i) peak = fmaxf(peak, small.valuePeaks[u & 1][i]);
+                const float up = toTopOfHalf(exponentBits(peak));
+                downNext = 1.f / up;
+                w *= up;
+            }
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -539,6 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int u = 0; u < count; ++u) {
             const uint32_t parity = u & 1;
             if (u > 0) advance(u - 1);
+            down = downNext;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 storeShared(weightedV + pieceAt(c), hi[c][0], hi[c][1], hi[c][2], hi[c][3]);

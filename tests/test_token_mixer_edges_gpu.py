@@ -75,3 +75,12 @@ def test_bits_of_a_state(tokens, Dk, Dv, loud, small, dtype):
     for name, got, want in zip(("state", "dstate"), (last.detach(), dstate), wants):
         off = (got.double() - want).flatten(2).norm(dim=2) / want.flatten(2).norm(dim=2)
         assert float(off.max()) < 2.0 ** -20.5 + (tokens // 128) * 2.0 ** -24, (name, off)
+
+
+@pytest.mark.parametrize("tokens", [128, 500, 2000])
+@pytest.mark.parametrize("Dk,Dv", [(64, 64), (128, 48), (40, 128)])
+@pytest.mark.parametrize("loud", ["all", "first", "last"])
+@pytest.mark.parametrize("small", [1.0, 1e-6])
+def test_bits_of_a_state_of_half(tokens, Dk, Dv, loud, small):
+    """Values of 1e-6 are a few of half's smallest steps: usual gradients without a loss scale."""
+    test_bits_of_a_state(tokens, Dk, Dv, loud, small, torch.float16)

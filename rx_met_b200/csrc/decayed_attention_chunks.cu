@@ -10,6 +10,9 @@
 //   outputs    four warps: O1 and O2 to memory, 32 bytes a thread and store
 //   state      eight warps: weighted V for the products; the state itself, 32 bits, stays in their registers
 //
+// P is zero in front of a token, and zero times an infinity or a NaN of V is not: such values, which leave a NaN in the weighted V, are taken out of the V of the last product once the
+// weighted V has them, and outputs says NaN for their column from their token on.
+//
 // Roundings.  Operands of tensor cores have the type of the inputs: P times the decays and S are rounded to it once, next to the rounding of the output.  The state is never
 // rebuilt from rounded values: the weighted V goes in as the sum of three bfloat16 terms, which leave 2^-24, or two of half,
 // 2^-22.  half has a short range: its rows of P, its S and the weighted V of a chunk are scaled by
@@ -42,8 +45,8 @@ constexpr uint32_t kShared = 232448;   // all of an SM, as the tensor memory
 constexpr uint32_t kP = 0, kO1 = 256, kO2 = 320, kKV = 384;
 enum Barrier { kStateMeets = 1, kLanesMeet };   // named barriers; the last takes four
 
-// A block starts with 80 registers a thread, 1920 for the lanes of its 24 warps in the same place.  Scores give up 8 (8 warps, 576), outputs 32 (4 warps, 192), copies and products 40 (4
-// warps, 160), and the state takes 120 (8 warps, 960): 1888.  With 80 the state would be spilled (advance() 420 -> 1700 cycles), with 104 its third terms.
+// A block starts with 80 registers a thread, 1920 for the lanes of its 24 warps in the same place.  Scores give up 8 (8 warps, 576), outputs 24 (4 warps, 224), copies and products 40 (4
+// warps, 160), and the state takes 120 (8 warps, 960): 1920.  With 80 the state would be spilled (advance() 420 -> 1700 cycles), with 104 its third terms.
 template <int REGISTERS>
 __device__ __forceinline__ void giveRegisters() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGISTERS)); }
 template <int REGISTERS>
@@ -55,6 +58,33 @@ __device__ __forceinline__ void loadShared(uint32_t at, uint32_t (&v)[4]) {
 }
 __device__ __forceinline__ void storeShared(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// Two neighbours of a 16-bit type: NaN where the value is not finite, else what was there.
+template <class T>
+__device__ __forceinline__ void addZeroTimes(uint32_t &sum, uint32_t value) {
+    if constexpr (std::is_same<T, __half>::value) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(value), "r"(0u));
+    else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(value), "r"(0u));
+}
+// Orders tokens of the chunks of a pass: a later chunk's keys are larger, and of a chunk's tokens that of the first in the order of the pass.
+__device__ __forceinline__ uint32_t badKey(int u, int token, bool reverse) { return static_cast<uint32_t>(u + 1) << 8 | static_cast<uint32_t>(reverse ? token + 1 : 255 - token); }
+// Takes what is not finite out of 32 values of V, those of a token in the four pieces of 16 bytes from `piece` on, and keeps where.
+template <class T>
+__device__ __forceinline__ void clean(uint32_t row, uint32_t swizzle, uint32_t piece, uint32_t *badFrom, uint32_t key) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < 16; ++i) {
+        const uint32_t at = row + (((piece + (i >> 2)) ^ swizzle) << 4) + (i & 3) * 4;
+        uint32_t w, kept;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
+        kept = w;
+#pragma unroll
+        for (uint32_t j = 0; j < 2; ++j)
+            if ((w >> (16 * j) & 0x7fffu) >= (std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u)) {
+                kept &= j ? 0xffffu : 0xffff0000u;
+                atomicMax(&badFrom[(piece + (i >> 2)) * 8 + (i & 3) * 2 + j], key);
+            }
+        if (kept != w) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(kept) : "memory");
+    }
 }
 
 constexpr int kMaxSegments = 160;   // no more than SMs
@@ -94,6 +124,8 @@ struct Small {
     float statePeaks[2][kStateWarps], valuePeaks[2][kStateWarps], stateScale[2];   // of two chunks in turn, so that the warps meet once a chunk
     uint8_t rowPeaks[2][2][kC];               // exponents, of two chunks in turn
     uint8_t rowScale[3][kC];                  // exponents of the powers of two that rows of P were scaled by, for three chunks
+    uint32_t badFrom[3][kCols];               // where outputs of a column stop being finite, of three chunks in turn (badKey)
+    uint32_t lastBad;                         // the last chunk where they do, counted from 1
     uint64_t fullK[3], fullQ[3], fullV[3], freeK[3], freeQ[3], freeV[3], vRead[3], pFull[2], pReady[2], pFree[2], vReady, kvFull, sReady, sFree, oFull, oFree, productsDone[2];
     uint32_t tmemSlot;
     int failed;
@@ -127,6 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto tokensOf = [&](int chunk) { return min(kC, length - chunk * kC); };
     if (tid == 0) {
         small.failed = 0;
+        small.lastBad = 0;
         for (int i = 0; i < kStages; ++i)
             for (uint64_t *bar : {&small.fullK[i], &small.fullQ[i], &small.fullV[i], &small.freeV[i]}) cluster::initBarrier(bar, 1);
         constexpr int kUsers = StateOnly ? 1 : 2;   // threads whose products read K and Q, and write O1 and O2
@@ -145,6 +178,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid <= kC) {
         const double g = p.logDecay[h];
         small.powers[tid] = tid == 0 ? 1.f : static_cast<float>(exp(tid * g));
+    } else if (tid >= 384 && tid < 384 + 3 * kCols) {
+        small.badFrom[0][tid - 384] = 0;
     } else if (tid >= 256 && tid < 320) {
         const int j = tid & 31, apart = tid < 288 || reverse ? j : 31 - j;
         (tid < 288 ? small.scaledPowers : small.columnPowers)[j] = p.outScale * (apart == 0 ? 1.f : static_cast<float>(exp(apart * static_cast<double>(p.logDecay[h]))));
@@ -357,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else if (warp < kFirstState) {
-        giveRegisters<48>();
+        giveRegisters<56>();
         if (!StateOnly) {
             const int quarter = warp & 3, i = 32 * quarter + lane;   // the thread's token
             const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
@@ -366,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int chunk = span.chunkAt(u, reverse), n = tokensOf(chunk);
                 wait(small.oFull, parity);
                 fenceAfter();
-                const bool live = i < n, in = chunk * kC + i < p.tokens && alive && p.out;
+                const bool live = i < n, in = chunk * kC + i < p.tokens && alive && p.out, bad = __any_sync(0xffffffffu, small.lastBad > static_cast<uint32_t>(u));
                 const float inter = live ? p.outScale * small.powers[reverse ? n - 1 - i : i + 1] * (kHalf ? small.stateScale[parity] : 1.f) : 0.f;
                 float back = 1.f;
                 if constexpr (kHalf) back = __uint_as_float((254u - small.rowScale[u % 3][i]) << 23);
@@ -380,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     loadsDone();
                     if (part == 3) {
                         fenceBefore();
-                        arriveWarp(small.oFree);
+                        if (!bad) arriveWarp(small.oFree);
                     }
                     const int col = slice * kCols + part * 16;
                     if (!in || col >= p.value) continue;
@@ -391,6 +426,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const float2 v = floatsOf(fma2(pairOf(o1[j], o1[j + 1]), pairOf(inter, inter), scaled));
                         out[j] = live ? v.x : 0.f;
                         out[j + 1] = live ? v.y : 0.f;
+                    }
+                    if (bad && live) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (small.badFrom[u % 3][part * 16 + j] >= badKey(u, i, reverse)) out[j] = __int_as_float(0x7fffffff);
                     }
                     auto sector = [](void *to, const uint32_t(&w)[8]) {   // a sector of memory a thread
                         asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
@@ -418,6 +458,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
+                // The state writes of chunk u + 3 what it writes of chunk u, once the outputs of chunk u have let go of their products.
+                if (bad) arriveWarp(small.oFree);
             }
         }
     } else {
@@ -565,14 +607,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if constexpr (Third) storeShared(weightedV + 2 * kTile + pieceAt(c), low[c][0], low[c][1], low[c][2], low[c][3]);
             }
             fenceAsyncProxy();
-            if (!StateOnly) arriveWarp(small.vRead[turn.at]);
             arriveWarp(small.vReady);
-
             // under the product of this chunk: the state in front of it, and the terms of the next one
             if (!StateOnly) {
                 if (u > 0) wait(small.sFree, parity ^ 1u);
                 publish(u);
             }
+            if (!StateOnly) {
+                // A vote: with a branch a thread 8 x 4096 tokens of 16 heads of 64 take 68 us, so 64.  Behind the state's publication: in front of it, 128 elements a head take 163 for 161.
+                uint32_t sums[4] = {};
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) addZeroTimes<T>(sums[j], mid[c][j]);
+                if (__any_sync(0xffffffffu, ((sums[0] | sums[1] | sums[2] | sums[3]) & 0x7fff7fffu) != 0u)) {
+                    clean<T>(tiles + turn.at * kStageBytes + 2 * kHalves * kTile + place, token & 7, piece, small.badFrom[u % 3], badKey(u, token, reverse));
+                    small.lastBad = u + 1;
+                    fenceAsyncProxy();
+                }
+                arriveWarp(small.vRead[turn.at]);
+            }
+
             turn.step(kStages);
             if (u + 1 < count) weigh(u + 1);
             wait(small.kvFull, parity);

@@ -84,3 +84,69 @@ def test_bits_of_a_state(tokens, Dk, Dv, loud, small, dtype):
 def test_bits_of_a_state_of_half(tokens, Dk, Dv, loud, small):
     """Values of 1e-6 are a few of half's smallest steps: usual gradients without a loss scale."""
     test_bits_of_a_state(tokens, Dk, Dv, loud, small, torch.float16)
+
+
+# ---- values that are not finite, in front of which nothing may change ------------------------------------------------------------
+
+def attention_problem(tokens, Dk, Dv, dtype, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q, k, v, dout = (torch.randn(2, tokens, h, d, device="cuda", generator=g).to(dtype) for h, d in ((4, Dk), (2, Dk), (2, Dv), (4, Dv)))
+    return q, k, v, dout, torch.tensor([0.0, -0.01, -0.3, -3.0], device="cuda")
+
+
+def apart(got, want, bound, hit):
+    """`hit`: what cannot be finite; everything else within its bound."""
+    assert not torch.isfinite(got[hit]).any()
+    ml.within(got[~hit], want[~hit], bound[~hit])
+
+
+@pytest.mark.parametrize("dtype", ml.TYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("Dk,Dv", [(64, 64), (96, 100)])
+@pytest.mark.parametrize("tokens,at", [(300, 0), (300, 171), (300, 299), (3000, 2000)])
+def test_a_bad_value_reaches_no_earlier_token(tokens, at, Dk, Dv, bad, dtype):
+    from rx_met_b200.decayed_attention import decayed_attention
+    q, k, v, _, decay = attention_problem(tokens, Dk, Dv, dtype, seed=1)
+    scale = Dk ** -0.5
+    want, wanted_last = ml.attend(q, k, v, decay, None, None, scale)
+    size, size_last = ml.magnitudes(lambda a, b, c: ml.attend(a, b, c, decay, None, None, scale), (q, k, v))
+    bound, bound_last = ml.attention_bound(size, dtype, tokens, Dk, dtype), ml.attention_bound(size_last, torch.float32, tokens, Dk, torch.float32)
+    v[0, at, 1, 5] = bad
+    out, last = decayed_attention(q, k, v, decay)
+    hit, hit_last = torch.zeros_like(out, dtype=torch.bool), torch.zeros_like(last, dtype=torch.bool)
+    hit[0, at:, 2:, 5] = True
+    hit_last[0, 2:, :, 5] = True
+    apart(out, want, bound, hit)
+    apart(last, wanted_last, bound_last, hit_last)
+
+
+@pytest.mark.parametrize("dtype", ml.TYPES)
+@pytest.mark.parametrize("of", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("at", [0, 171, 299])
+def test_gradients_of_a_bad_value(at, of, dtype):
+    """Of a key's or a value's, gradients in front of it do not know; of a query's or an output's, those behind it."""
+    from rx_met_b200.decayed_attention import decayed_attention
+    q, k, v, dout, decay = attention_problem(300, 64, 80, dtype, seed=2)
+    zero = torch.zeros(2, 4, 64, 80, device="cuda")
+    wants = ml.attend_gradients(q, k, v, decay, None, None, 0.125, dout, zero)
+    sizes = ml.magnitudes(lambda a, b, c, s, d, e: ml.attend_gradients(a, b, c, decay, s, None, 0.125, d, e), (q, k, v, None, dout, zero))
+    dict(q=q, k=k, v=v, dout=dout)[of][0, at, 1, 7] = float("nan")
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(decayed_attention(*leaves, decay)[0], leaves, dout)
+    dq, dk, dv = (torch.zeros_like(g, dtype=torch.bool) for g in grads)
+    query, key = slice(1, 2), slice(0, 1)   # heads of q and dout that read head 0 of k and v: 0 and 1; of its head 1: 2 and 3
+    if of == "q":
+        dk[0, :at + 1, key, 7] = True
+        dv[0, :at + 1, key] = True
+    if of == "dout":
+        dq[0, at, query] = True
+        dk[0, :at + 1, key] = True
+        dv[0, :at + 1, key, 7] = True
+    if of == "k":
+        dq[0, at:, 2:, 7] = True
+        dv[0, at, 1] = True
+    if of == "v":
+        dq[0, at:, 2:] = True
+        dk[0, at, 1] = True
+    for got, want, size, hit in zip(grads, wants, sizes, (dq, dk, dv)):
+        apart(got, want, ml.attention_bound(size, dtype, 300, 80, dtype), hit)

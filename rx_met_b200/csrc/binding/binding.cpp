@@ -10,6 +10,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <array>
@@ -510,12 +511,17 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
     }
 };
 
+// A trace would record the buffer that an output is written to, and not the kernel that writes it.
+void refuseTrace(const char *what) { TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be traced: the traced function would return memory that nothing writes"); }
+
 std::vector<Tensor> addRmsNorm(const Tensor &x, const Tensor &weight, const MaybeTensor &residual, double eps) {
+    refuseTrace("add_rms_norm");
     return AddRmsNorm::apply(x, weight, residual, eps);
 }
 
 // Codes, scales and (with a residual) total.
 std::vector<Tensor> addRmsNormCodes(const Tensor &x, const MaybeTensor &weight, const MaybeTensor &residual, double eps) {
+    refuseTrace("add_rms_norm_codes");
     const NormArguments a(x, residual, weight, "add_rms_norm_codes");
     const c10::cuda::CUDAGuard guard(x.device());
     std::vector<Tensor> out{emptyCodes(x, x.sizes()), emptyLike(x, x.sizes().slice(0, x.dim() - 1))};
@@ -530,6 +536,7 @@ std::vector<Tensor> addRmsNormCodes(const Tensor &x, const MaybeTensor &weight, 
 
 Tensor codedLinear(const Tensor &codes, const Tensor &scale, const Tensor &weight, const Tensor &weightScale, const MaybeTensor &bias,
                    int activation, const MaybeTensor &residual, int outType) {
+    refuseTrace("coded_linear");
     constexpr at::ScalarType kTypes[] = {at::kFloat, at::kBFloat16, at::kHalf};
     TORCH_CHECK(outType >= 0 && outType <= 2, "coded_linear: unknown output type");
     TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kChar && codes.dim() >= 1, "codes must be a CUDA int8 tensor");
@@ -682,12 +689,14 @@ struct DecayedAttention : torch::autograd::Function<DecayedAttention> {
 
 std::vector<Tensor> decayedAttention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &logDecay, const MaybeTensor &state,
                                      const MaybeTensor &lengths, double scale) {
+    refuseTrace("decayed_attention");
     return DecayedAttention::apply(q, k, v, logDecay, state, lengths, scale);
 }
 
 // One token for each row; the states go to `newState`, which may be `state` itself.
 Tensor decayedAttentionStep(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &logDecay, const Tensor &state, const Tensor &newState,
                             const MaybeTensor &active, double scale) {
+    refuseTrace("decayed_attention_step");
     if (at::GradMode::is_enabled())
         for (const Tensor *t : {&q, &k, &v, &state, &newState})
             TORCH_CHECK(!t->requires_grad(), "decayed_attention_step has no gradient: use decayed_attention, or no_grad");

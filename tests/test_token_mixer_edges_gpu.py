@@ -150,3 +150,20 @@ def test_gradients_of_a_bad_value(at, of, dtype):
         dk[0, at, 1] = True
     for got, want, size, hit in zip(grads, wants, sizes, (dq, dk, dv)):
         apart(got, want, ml.attention_bound(size, dtype, 300, 80, dtype), hit)
+
+
+# ---- what torch does with calls -----------------------------------------------------------------------------------------------
+
+def test_calls_are_not_traced():
+    """A trace would hold the buffers of the outputs and none of the kernels."""
+    from rx_met_b200 import coded_linear, decayed_attention, rms_norm
+    x, w = torch.randn(3, 16, device="cuda"), torch.randn(16, device="cuda")
+    q, decay, state = torch.randn(3, 5, 1, 16, device="cuda"), -torch.ones(1, device="cuda"), torch.zeros(3, 1, 16, 16, device="cuda")
+    codes, scale = rms_norm.code_rows(x)
+    for call, inputs in ((lambda a: rms_norm.add_rms_norm(a, w)[0], x), (lambda a: rms_norm.add_rms_norm_codes(a, w)[1], x), (lambda a: rms_norm.code_rows(a)[1], x),
+                         (lambda a: coded_linear.coded_linear(codes, a, coded_linear.CodedWeight(codes, scale)), scale),
+                         (lambda a: decayed_attention.decayed_attention(a, q, q, decay)[0], q),
+                         (lambda a: decayed_attention.decayed_attention_step(a, q[:, 0], q[:, 0], decay, state), q[:, 0].contiguous())):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, (inputs,), check_trace=False)
+        call(inputs)

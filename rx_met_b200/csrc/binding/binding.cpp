@@ -10,6 +10,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -461,6 +462,24 @@ struct NormArguments {
 const void *dataOf(const Tensor &t) { return t.defined() && t.numel() > 0 ? t.const_data_ptr() : nullptr; }
 void *mutableOf(const Tensor &t) { return t.defined() && t.numel() > 0 ? t.mutable_data_ptr() : nullptr; }
 
+// Gradients that are to be differentiated again (create_graph) fail when they are: as constants they would leave their terms out in silence.  `from`: the tensors that they
+// depend on, to which the failing node is linked, since only nodes on a way to what is asked for run.
+torch::autograd::variable_list differentiatedOnce(torch::autograd::variable_list grads, torch::autograd::variable_list from, const char *what) {
+    torch::autograd::variable_list all;
+    for (const Tensor &g : grads)
+        if (g.defined()) all.push_back(g.detach());
+    const size_t count = all.size();
+    for (Tensor &t : from)
+        if (t.defined() && t.requires_grad()) all.push_back(std::move(t));
+    if (count == 0 || all.size() == count) return grads;
+    const auto node = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has no second derivatives", static_cast<int64_t>(all.size()));
+    const auto linked = (*node)(std::move(all));
+    size_t i = 0;
+    for (Tensor &g : grads)
+        if (g.defined()) g = linked[i++];
+    return grads;
+}
+
 // The outputs are y and, with a residual, total.
 struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &weight,
@@ -481,6 +500,13 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
     }
 
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        if (!at::GradMode::is_enabled()) return gradients(ctx, std::move(grads));
+        auto from = ctx->get_saved_variables();
+        from.insert(from.end(), grads.begin(), grads.end());
+        return differentiatedOnce(gradients(ctx, std::move(grads)), std::move(from), "add_rms_norm");
+    }
+
+    static torch::autograd::variable_list gradients(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         torch::autograd::variable_list out(4);
         const at::NoGradGuard noGrad;
@@ -663,6 +689,13 @@ struct DecayedAttention : torch::autograd::Function<DecayedAttention> {
     }
 
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        if (!at::GradMode::is_enabled()) return gradients(ctx, std::move(grads));
+        auto from = ctx->get_saved_variables();
+        from.insert(from.end(), grads.begin(), grads.end());
+        return differentiatedOnce(gradients(ctx, std::move(grads)), std::move(from), "decayed_attention");
+    }
+
+    static torch::autograd::variable_list gradients(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         torch::autograd::variable_list out(7);
         if (!grads[0].defined() && !grads[1].defined()) return out;

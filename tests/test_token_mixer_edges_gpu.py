@@ -167,3 +167,18 @@ def test_calls_are_not_traced():
         with pytest.raises(RuntimeError, match="traced"):
             torch.jit.trace(call, (inputs,), check_trace=False)
         call(inputs)
+
+
+def test_second_derivatives_fail():
+    """In silence, their terms would be missing from a sum of which others can be differentiated."""
+    from rx_met_b200 import rms_norm
+    from rx_met_b200.decayed_attention import decayed_attention
+    x, r, w = (torch.randn(*s, device="cuda", requires_grad=True) for s in ((3, 16), (3, 16), (16,)))
+    q = torch.randn(1, 5, 1, 16, device="cuda", requires_grad=True)
+    decay = -torch.ones(1, device="cuda")
+    for f, leaves in ((lambda: rms_norm.add_rms_norm(x, w)[0], [x, w]), (lambda: rms_norm.add_rms_norm(x, w, r)[1], [x, r]), (lambda: decayed_attention(q, q, q, decay)[0], [q])):
+        first = torch.autograd.grad((f() ** 2).sum(), leaves)
+        grads = torch.autograd.grad((f() ** 2).sum(), leaves, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(grads, first))
+        with pytest.raises(RuntimeError, match="no second derivatives"):
+            torch.autograd.grad(sum((g ** 2).sum() for g in grads) + sum((t ** 3).sum() for t in leaves), leaves)

@@ -416,6 +416,11 @@ void sameDevice(const Tensor &t, const Tensor &like, const char *name) {
     TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be a CUDA tensor on ", like.device());
 }
 
+// Sizes that the C ABI takes in 32 bits, refused before they are cut and before anything is copied.
+void checkSizes(at::IntArrayRef sizes, const char *what) {
+    for (const int64_t n : sizes) TORCH_CHECK(n <= INT32_MAX, what, ": a size of ", n, ", at most ", INT32_MAX);
+}
+
 // [rows][width] with neighbouring elements, a view where the strides allow one; the distance of its rows.
 Tensor asRows(const Tensor &t) {
     if (t.dim() == 2 && t.stride(1) == 1) return t;
@@ -439,6 +444,7 @@ struct NormArguments {
     int64_t rows, width;
     NormArguments(const Tensor &input, const MaybeTensor &added, const MaybeTensor &weights, const char *what) {
         TORCH_CHECK(input.is_cuda() && input.dim() >= 1 && input.size(-1) > 0, what, ": x must be a CUDA tensor with a last dimension");
+        checkSizes({input.size(-1)}, what);
         type = typeOf(input, "x");
         width = input.size(-1);
         x = asRows(input);
@@ -568,6 +574,7 @@ Tensor codedLinear(const Tensor &codes, const Tensor &scale, const Tensor &weigh
     TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kChar && codes.dim() >= 1, "codes must be a CUDA int8 tensor");
     sameDevice(weight, codes, "weight codes");
     TORCH_CHECK(weight.scalar_type() == at::kChar && weight.dim() == 2, "weight codes must be an int8 tensor of two dimensions");
+    checkSizes(weight.sizes(), "coded_linear");
     const int64_t inner = weight.size(1), outer = weight.size(0);
     TORCH_CHECK(inner > 0 && outer > 0 && codes.size(-1) == inner, "coded_linear: codes of ", codes.size(-1), " elements for a weight of shape ", listText(weight.sizes()));
     sameDevice(scale, codes, "scale");
@@ -625,6 +632,7 @@ struct AttentionArguments {
                        const MaybeTensor &counts, double scale, int64_t dims) {
         TORCH_CHECK(queries.is_cuda() && queries.dim() == dims, "q must be a CUDA tensor of ", dims, " dimensions");
         problem.type = typeOf(queries, "q");
+        for (const Tensor *t : {&queries, &keys, &values, &decays}) checkSizes(t->sizes(), "decayed_attention");
         for (const auto &[t, name] : {std::pair<const Tensor &, const char *>{keys, "k"}, {values, "v"}}) {
             sameDevice(t, queries, name);
             TORCH_CHECK(t.dim() == dims && t.scalar_type() == queries.scalar_type(), name, " must have the dimensions and type of q");

@@ -182,3 +182,29 @@ def test_second_derivatives_fail():
         assert all(torch.equal(a, b) for a, b in zip(grads, first))
         with pytest.raises(RuntimeError, match="no second derivatives"):
             torch.autograd.grad(sum((g ** 2).sum() for g in grads) + sum((t ** 3).sum() for t in leaves), leaves)
+
+
+# ---- sizes ------------------------------------------------------------------------------------------------------------------
+
+def test_sizes_of_33_bits_are_refused():
+    """They were cut to their lower bits.  Views of one element: nothing of that size is held, and nothing may be copied to it."""
+    from rx_met_b200 import rms_norm
+    from rx_met_b200.coded_linear import CodedWeight, coded_linear
+    from rx_met_b200.decayed_attention import decayed_attention
+    more = 2 ** 32
+    view = lambda dtype, *shape: torch.ones(1, device="cuda", dtype=dtype).expand(*shape)  # noqa: E731
+    of = lambda *shape: view(torch.float32, *shape)  # noqa: E731
+    one, small, rows = of(1), of(1, 1, 1, 1), view(torch.int8, 1, more + 64)
+    torch.cuda.synchronize()
+    held = torch.cuda.max_memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    for call in (lambda: rms_norm.add_rms_norm(view(torch.bfloat16, more + 64), view(torch.bfloat16, more + 64)), lambda: rms_norm.code_rows(view(torch.bfloat16, 2, more + 64)),
+                 lambda: rms_norm.add_rms_norm_codes(of(1, more + 64), of(more + 64)), lambda: coded_linear(rows, one, CodedWeight(rows, one)),
+                 lambda: coded_linear(rows[:, :32], one, CodedWeight(view(torch.int8, more + 3, 32), of(more + 3))),
+                 lambda: decayed_attention(*[of(1, more + 2, 1, 1)] * 3, -one), lambda: decayed_attention(*[of(more + 1, 1, 1, 1)] * 3, -one),
+                 lambda: decayed_attention(of(1, 1, 1, more + 1), of(1, 1, 1, more + 1), small, -one), lambda: decayed_attention(of(1, 1, more + 1, 1), small, small, -one),
+                 lambda: decayed_attention(small, small, of(1, 1, 1, more + 1), -one)):
+        with pytest.raises(RuntimeError, match="at most"):
+            call()
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() < held + 2 ** 30

@@ -58,7 +58,8 @@ RXMET_API int rxmet_coded_linear(int64_t rows, int inner, int outer, const int8_
  * S_t = exp(log_decay[h]) S_{t-1} + k_t v_t',  out_t = scale q_t S_t  for t < lengths[b]; out is zero beyond.
  * A tensor of `heads` heads: element (b, t, h, d) at b * stride_b + t * stride_t + h * stride_h + d.  The operator has `heads` heads;
  * q, k and v have a number of heads that divides it, and head h reads head h / (heads / own heads) of them.  log_decay <= 0 (32 bits, -inf: no memory).
- * state [batch][heads][key_dim][value_dim] in 32 bits, null for zeros.  1 <= key_dim, value_dim <= 128. */
+ * state [batch][heads][key_dim][value_dim] in 32 bits, null for zeros.  1 <= key_dim, value_dim <= 128; batch and heads at most
+ * 65535, tokens at most 2^30. */
 typedef struct rxmet_head_tensor {
     const void *data;
     int64_t stride_b, stride_t, stride_h;

@@ -45,6 +45,7 @@ void checkSizes(const rxmet_decayed_attention &a) {
                   "decayed_attention: batch %d, tokens %d, heads %d, key_dim %d, value_dim %d", a.batch, a.tokens, a.heads, a.key_dim, a.value_dim);
     if (a.key_dim > kMaxDim || a.value_dim > kMaxDim)
         fail(RXMET_ERR_UNSUPPORTED, "decayed_attention: heads of %d and %d elements, at most %d", a.key_dim, a.value_dim, kMaxDim);
+    if (a.tokens > kMaxTokens) fail(RXMET_ERR_UNSUPPORTED, "decayed_attention: %d tokens, at most %d", a.tokens, kMaxTokens);
     if (a.batch > 65535 || a.heads > 65535) fail(RXMET_ERR_UNSUPPORTED, "decayed_attention: batch %d, heads %d, at most 65535 each", a.batch, a.heads);
     RXMET_REQUIRE(a.type >= 0 && a.type <= 2, "decayed_attention: unknown element type %d", a.type);
     RXMET_REQUIRE(std::isfinite(a.scale) && a.scale != 0.f, "decayed_attention: scale has to be finite and not zero");

@@ -10,6 +10,7 @@ namespace rxmet {
 namespace decayed {
 
 constexpr int kMaxDim = 128;
+constexpr int kMaxTokens = 1 << 30;   // places of tokens, rounded up to chunks and segments, are counted in 32 bits
 
 // Forward in time:   S = decay S + k v',  o = outScale q S.
 // Reverse in time:   S = S + k v',  o = outScale q S,  S = decay S   (from the last token to the first).

@@ -453,6 +453,7 @@ void launchTensorCores(const Problem &p, cudaStream_t st) {
 extern "C" int rxmet_wait_status(int *gave_up) {
     return rxmet::guarded([&] {
         RXMET_REQUIRE(gave_up, "wait_status: null pointer");
+        RXMET_CUDA(cudaDeviceSynchronize());   // the copy alone waits for the legacy stream, and not for streams apart from it
         RXMET_CUDA(cudaMemcpy(gave_up, rxmet::waitStatus(), sizeof(int), cudaMemcpyDeviceToHost));
     });
 }

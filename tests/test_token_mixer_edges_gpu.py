@@ -208,3 +208,18 @@ def test_sizes_of_33_bits_are_refused():
             call()
     torch.cuda.synchronize()
     assert torch.cuda.max_memory_allocated() < held + 2 ** 30
+
+
+# ---- waits that run out -----------------------------------------------------------------------------------------------------------
+
+def test_wait_status_waits_for_all_streams():
+    import ctypes as C
+
+    from mixer_abi import library
+    side, done, word = torch.cuda.Stream(), torch.cuda.Event(), C.c_int(-1)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):   # a stream apart from the legacy one, at work for a fifth of a second
+        torch.cuda._sleep(400_000_000)
+        done.record()
+    assert library().rxmet_wait_status(C.byref(word)) == 0 and word.value == 0
+    assert done.query()

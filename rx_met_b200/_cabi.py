@@ -207,6 +207,14 @@ def load_binding():
     return _binding
 
 
+def wait_gave_up() -> bool:
+    """Whether a bounded wait inside one of the token mixer's kernels has run out on the current device since the process began: the results of that call are not
+    to be used.  Waits for the device, so that it is asked now and then (a checkpoint, the end of a run), not after every call; not under a capture."""
+    word = C.c_int(0)
+    check(load_library().rxmet_wait_status(C.byref(word)), "wait_gave_up")
+    return word.value != 0
+
+
 def check(status: int, what: str) -> None:
     """Turn a negative ``rxmet_status`` into the exception the reference raises."""
     if status == 0:

@@ -223,3 +223,8 @@ def test_wait_status_waits_for_all_streams():
         done.record()
     assert library().rxmet_wait_status(C.byref(word)) == 0 and word.value == 0
     assert done.query()
+
+
+def test_no_wait_gave_up():
+    import rx_met_b200
+    assert rx_met_b200.wait_gave_up() is False

@@ -77,7 +77,7 @@ RXMET_API size_t rxmet_decayed_attention_workspace_bytes(const rxmet_decayed_att
 RXMET_API int rxmet_decayed_attention_forward(const rxmet_decayed_attention *problem, const float *state_dev, void *out_dev,
                                               float *final_state_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
 /* Gradients of q, k, v (contiguous, with the heads of q, k, v; gradients of shared heads are summed in 32 bits) and of state, each null
- * where it is not wanted.  dout (heads = problem->heads) or dfinal_state may be null: zeros. */
+ * where it is not wanted.  dout (heads = problem->heads; it or its data) or dfinal_state may be null: zeros; without dout the gradients of k and v go token by token. */
 RXMET_API int rxmet_decayed_attention_backward(const rxmet_decayed_attention *problem, const float *state_dev,
                                                const rxmet_head_tensor *dout, const float *dfinal_state_dev, void *dq_dev, void *dk_dev,
                                                void *dv_dev, float *dstate_dev, void *workspace_dev, size_t workspace_bytes, void *stream);

@@ -117,11 +117,12 @@ struct ForkedLanes {
     ~ForkedLanes() { join(); }
 };
 
-// Kernels by size and type.  Single tokens have a kernel of their own, chunks are taken from 16 or 32 tokens on (planChunks); tensors that TMA cannot copy and 32-bit ones go token by token.
+// Kernels by size and type.  Single tokens have a kernel of their own, chunks are taken from 16 or 32 tokens on (planChunks); tensors that TMA cannot copy, 32-bit ones and those without one of the three go token by token.
 void launchPass(const Pass &p, int type, float *states, cudaStream_t st) {
     const ChunkPlan plan = planChunks(p, type);
-    if (takesStep(p)) launchStep(p, type, st);
-    else if (plan.taken && chunksCanCopy(p)) launchChunks(p, type, plan, states, st);
+    const bool complete = p.q.data && p.k.data && p.v.data;   // else one is all zeros
+    if (complete && takesStep(p)) launchStep(p, type, st);
+    else if (complete && plan.taken && chunksCanCopy(p)) launchChunks(p, type, plan, states, st);
     else launchRecurrent(p, type, st);
 }
 
@@ -187,15 +188,21 @@ int rxmet_decayed_attention_backward(const rxmet_decayed_attention *problem, con
         const rxmet_decayed_attention &a = *problem;
         checkSizes(a);
         if (a.batch == 0) return;
-        RXMET_REQUIRE(a.log_decay && dout, "decayed_attention: null tensor");
+        RXMET_REQUIRE(a.log_decay, "decayed_attention: null log_decay");
+        const bool fromOutputs = dout && dout->data && a.tokens > 0;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         rxmet_head_tensor q{nullptr, 0, 0, 0, 1}, k = q, v = q, d = q;
         if (a.tokens > 0) {
             q = checked(a.q, a.heads, "q");
             k = checked(a.k, a.heads, "k");
             v = checked(a.v, a.heads, "v");
-            d = checked(*dout, a.heads, "dout");
-            RXMET_REQUIRE(d.heads == a.heads, "decayed_attention: dout has %d heads of %d", d.heads, a.heads);
+            d.heads = a.heads;
+            if (fromOutputs) {
+                d = checked(*dout, a.heads, "dout");
+                RXMET_REQUIRE(d.heads == a.heads, "decayed_attention: dout has %d heads of %d", d.heads, a.heads);
+            } else if (dq_dev) {   // the gradient of the final state alone does not reach the queries
+                RXMET_CUDA(cudaMemsetAsync(dq_dev, 0, static_cast<size_t>(a.batch) * a.tokens * q.heads * a.key_dim * typeBytes(a.type), st));
+            }
         }
         const Pass passes[] = {queryPass(a, q, k, v, d), keyPass(a, q, k, v, d), valuePass(a, q, k, v, d)};
         Workspace ws(workspace_dev, workspace_bytes);
@@ -225,7 +232,7 @@ int rxmet_decayed_attention_backward(const rxmet_decayed_attention *problem, con
         };
         // The passes run side by side, because none fills the GPU with few heads; those that may have heads to sum begin.  Forward and gradients of 2 x 1024 tokens and 16 heads of 64 take 55 us
         // with two passes one after another beside the third, 40 so; of 6 x 1000 tokens, 8 heads and shared keys 104 and 88; of 8 x 2048 tokens and 16 heads, which fill it, 128 both ways.
-        const bool wanted[] = {dq_dev != nullptr, dk_dev != nullptr, dv_dev || dstate_dev};
+        const bool wanted[] = {dq_dev && (fromOutputs || a.tokens == 0), dk_dev != nullptr, dv_dev || dstate_dev};
         ForkedLanes forked{st};   // the last of the passes has the caller's stream
         auto &lanes = forked.lanes;
         for (int i = 2, last = wanted[0] ? 0 : wanted[1] ? 1 : 2; i > last; --i)

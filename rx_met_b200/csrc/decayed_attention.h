@@ -20,7 +20,7 @@ constexpr int kMaxTokens = 1 << 30;   // places of tokens, rounded up to chunks 
 // where the scale is taken out of G, so that the state's gradient comes in divided by it and goes out multiplied.
 struct Pass {
     int batch, tokens, heads, key, value;   // key: width of q and k, value: width of v and out
-    rxmet_head_tensor q, k, v;
+    rxmet_head_tensor q, k, v;              // without data, and strides of 0: zeros
     const float *logDecay;
     const int32_t *lengths;
     bool reverse;

@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(256) decayedRecurrent(const __grid_constant__ 
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int i = i0 + e * blockDim.x, t = i / width, d = i - t * width;
-                    in[e] = i < count * width && d < dims ? from.data[tokenOf(t) * from.strideT + d] : fromFloat<T>(0.f);
+                    in[e] = i < count * width && d < dims && from.data ? from.data[tokenOf(t) * from.strideT + d] : fromFloat<T>(0.f);
                 }
 #pragma unroll
                 for (int e = 0; e < 8; ++e)

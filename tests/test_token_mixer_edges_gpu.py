@@ -228,3 +228,33 @@ def test_wait_status_waits_for_all_streams():
 def test_no_wait_gave_up():
     import rx_met_b200
     assert rx_met_b200.wait_gave_up() is False
+
+
+# ---- the C ABI ------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ml.TYPES)
+@pytest.mark.parametrize("struct", [False, True])
+@pytest.mark.parametrize("tokens,Dk,Dv", [(1, 8, 1), (5, 64, 64), (200, 64, 40), (200, 128, 128)])
+def test_gradients_of_the_final_state_alone(tokens, Dk, Dv, struct, dtype):
+    """No gradient of the outputs: neither the structure nor, in it, the data."""
+    import ctypes as C
+
+    from mixer_abi import Heads, Problem, library
+    lib = library()
+    q, k, v = (torch.randn(2, tokens, h, d, device="cuda").to(dtype) for h, d in ((4, Dk), (2, Dk), (4, Dv)))
+    decay, dlast = -torch.rand(4, device="cuda"), torch.randn(2, 4, Dk, Dv, device="cuda")
+    problem = Problem(2, tokens, 4, Dk, Dv, ml.TYPES.index(dtype), Heads.of(q), Heads.of(k), Heads.of(v), decay.data_ptr(), None, 0.25)
+    grads = [torch.full_like(t, float("nan")) for t in (q, k, v, dlast)]
+    size = lib.rxmet_decayed_attention_workspace_bytes(C.byref(problem), 1)
+    held = torch.empty(size, dtype=torch.uint8, device="cuda")
+    none = C.byref(Heads(None, 0, 0, 0, 4)) if struct else None
+    at = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+    status = lib.rxmet_decayed_attention_backward(C.byref(problem), None, none, at(dlast), *(at(g) for g in grads), at(held), C.c_size_t(size),
+                                                  C.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert status == 0, lib.rxmet_last_error()
+    zero = torch.zeros(2, tokens, 4, Dv, device="cuda")
+    wants = ml.attend_gradients(q, k, v, decay, None, None, 0.25, zero, dlast)
+    sizes = ml.magnitudes(lambda a, b, c, s, d, e: ml.attend_gradients(a, b, c, decay, s, None, 0.25, d, e), (q, k, v, None, zero, dlast))
+    for got, want, magnitude in zip(grads, wants, sizes):
+        # decays of up to e^-200 lead below the normal numbers, where every token's two products may be off by half of the smallest one
+        ml.within(got, want, ml.attention_bound(magnitude, dtype, tokens, max(Dk, Dv), got.dtype) + tokens * 2.0 ** -149)

@@ -31,7 +31,8 @@ RXMET_API int rxmet_add_rms_norm(int64_t rows, int width, int type, const void *
                                  void *y_dev, float *rms_dev /* optional [rows]: rsqrt(mean + eps), for the backward */, void *stream);
 /* The same with an output in 8 bits: scale = max|y| / 127 of the row, codes = rne(y / scale) in [-127, 127]; a row of zeros has scale 0
  * and codes 0, a row whose largest magnitude is not finite has that value for its scale and codes that mean nothing.  codes rows start codes_pitch
- * bytes apart.  weight null: no norm (y = total), which codes the rows of any array.  A scale below the normal
+ * bytes apart.  weight null: no norm (y = total), which codes the rows of any array, of up to 131071
+ * elements.  A scale below the normal
  * numbers is as exact as those are; the codes are of y over that scale, and zeros where it rounds to zero.  No output may overlap an input. */
 RXMET_API int rxmet_add_rms_norm_codes(int64_t rows, int width, int type, const void *x_dev, int64_t x_pitch, const void *residual_dev,
                                        int64_t residual_pitch, const void *weight_dev, int weight_type, float eps, void *total_dev,

@@ -5,7 +5,7 @@
 // ahead.  With loads to registers one row ahead in its place, 8192 x 4096 bfloat16 take 66 us for 60 (forward with codes) and 105 for 78 (gradients), at the same 16 elements a thread.
 // Sums run in 32 bits: a thread's own elements in order, lanes as a tree, warps in order, so that results do not depend on the grid.
 //
-// Bound: HBM for codes (8192 x 4096 bfloat16 42 us, 5.6 TB/s) and the forward (49.5 us, 5.4 TB/s); issue and the barrier of a team's sum for the gradients (78 us, 4.3 TB/s).
+// Bound: HBM for codes (8192 x 4096 bfloat16 43 us, 5.5 TB/s) and the forward (49.5 us, 5.4 TB/s); issue and the barrier of a team's sum for the gradients (78 us, 4.3 TB/s).
 #include <algorithm>
 
 #include "common.h"
@@ -18,6 +18,7 @@ namespace rxmet {
 namespace {
 
 constexpr int kMaxWidth = 16384;
+constexpr int kMaxCoded = 131071;   // of rows that are only coded: as many as a product of codes takes
 constexpr int kMaxThreads = 512, kMaxWarps = kMaxThreads / 32;
 
 // The rows of a round (one for each team of a CTA) of up to four arrays, in shared memory.  Bulk copies start and end on 16 bytes, so a copy takes the few bytes
@@ -258,6 +259,24 @@ __device__ __noinline__ void tinyCodes(const NormRows &p, int64_t row, float rms
         }
 }
 
+// Codes of values over a step, whose inverse is given.  1.5 * 2^23 added, the low byte of the sum is the nearest integer, ties to even.  The quotient of the largest magnitude rounds to 127, so
+// none lies beyond.
+template <int W>
+__device__ __forceinline__ Pack<int8_t, W> codesOf(const Lanes<W> &t, float inverse) {
+    const Lanes<W> shifted = allOf<W>(12582912.f).plus(t, inverse);
+    Pack<int8_t, W> out;
+    if constexpr (W == 1) {
+        out.v[0] = static_cast<int8_t>(__float_as_uint(shifted.v) & 0xffu);
+    } else {
+        uint32_t *words = reinterpret_cast<uint32_t *>(&out);
+#pragma unroll
+        for (int j = 0; j < W; j += 4)
+            words[j / 4] = __byte_perm(__byte_perm(__float_as_uint(shifted.at(j)), __float_as_uint(shifted.at(j + 1)), 0x0040),
+                                       __byte_perm(__float_as_uint(shifted.at(j + 2)), __float_as_uint(shifted.at(j + 3)), 0x0040), 0x5410);
+    }
+    return out;
+}
+
 // Ringed: rows come through the ring.  Else straight from memory: few rows, which have no next ones to fetch, and those too wide for a ring.
 template <class T, int W, int ITEMS, bool Codes, bool Ringed>
 __global__ void __launch_bounds__(kMaxThreads) __maxnreg__(W * ITEMS <= 8 ? 64 : W * ITEMS <= 16 ? (W > 1 ? 80 : 96) : 128) addRmsNorm(const __grid_constant__ NormRows p, int *status) {
@@ -342,18 +361,7 @@ __global__ void __launch_bounds__(kMaxThreads) __maxnreg__(W * ITEMS <= 8 ? 64 :
             int8_t *codes = p.codes + row * p.codesPitch;
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
-                // 1.5 * 2^23 added, the low byte of the sum is the nearest integer, ties to even.  The quotient of the largest magnitude rounds to 127, so none lies beyond.
-                const Elements shifted = allOf<W>(12582912.f).plus(t[i], inverse);
-                Pack<int8_t, W> out;
-                if constexpr (W == 1) {
-                    out.v[0] = static_cast<int8_t>(__float_as_uint(shifted.v) & 0xffu);
-                } else {
-                    uint32_t *words = reinterpret_cast<uint32_t *>(&out);
-#pragma unroll
-                    for (int j = 0; j < W; j += 4)
-                        words[j / 4] = __byte_perm(__byte_perm(__float_as_uint(shifted.at(j)), __float_as_uint(shifted.at(j + 1)), 0x0040),
-                                                   __byte_perm(__float_as_uint(shifted.at(j + 2)), __float_as_uint(shifted.at(j + 3)), 0x0040), 0x5410);
-                }
+                const Pack<int8_t, W> out = codesOf(t[i], inverse);
                 if (first + i * stride < here) *reinterpret_cast<Pack<int8_t, W> *>(codes + first + i * stride) = out;
             }
             if (isinf(inverse) && real) tinyCodes<T, W>(p, row, rms, most / 127.f, first, stride);
@@ -365,6 +373,46 @@ __global__ void __launch_bounds__(kMaxThreads) __maxnreg__(W * ITEMS <= 8 ? 64 :
         }
     }
     if (!alive && (threadIdx.x & 31) == 0) atomicExch(status, 1);
+}
+
+// Codes of rows that a team's registers do not hold, without a norm: a CTA reads a row twice, the second time from L2, for its largest magnitude and for the codes.  Bound: the two readings
+// (8192 x 28672 bfloat16 224 us, 3.1 TB/s of what a single reading and the codes would move).
+constexpr int kWideThreads = 1024;
+template <class T, int W>
+__global__ void __launch_bounds__(kWideThreads) codeWideRows(const __grid_constant__ NormRows p) {
+    __shared__ float peaks[2][kWideThreads / 32];
+    const int first = threadIdx.x * W, stride = kWideThreads * W, lane = threadIdx.x & 31;
+    waitForPredecessor();
+    letDependentsStart();
+    int slot = 0;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, slot ^= 1) {
+        const T *x = static_cast<const T *>(p.x) + row * p.xPitch, *r = static_cast<const T *>(p.residual) + row * p.residualPitch;
+        auto sum = [&](int i) {
+            const Lanes<W> t = loadLanes<T, W>(x + i);
+            return p.residual ? t + loadLanes<T, W>(r + i) : t;
+        };
+        float peak = 0.f;
+#pragma unroll 4
+        for (int i = first; i < p.width; i += stride) {
+            const Lanes<W> t = sum(i);
+            if (p.residual) storeLanes<T, W>(static_cast<T *>(p.total) + row * p.width + i, t);
+#pragma unroll
+            for (int j = 0; j < W; ++j) peak = larger(peak, fabsf(t.at(j)));
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) peak = larger(peak, __shfl_xor_sync(0xffffffffu, peak, d));
+        if (lane == 0) peaks[slot][threadIdx.x >> 5] = peak;
+        __syncthreads();
+        peak = peaks[slot][lane];
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) peak = larger(peak, __shfl_xor_sync(0xffffffffu, peak, d));
+        const float inverse = peak > 0.f ? 127.f / peak : 0.f;
+        if (threadIdx.x == 0) p.scale[row] = peak / 127.f;
+        int8_t *codes = p.codes + row * p.codesPitch;
+#pragma unroll 4
+        for (int i = first; i < p.width; i += stride) *reinterpret_cast<Pack<int8_t, W> *>(codes + i) = codesOf(sum(i), inverse);
+        if (isinf(inverse)) tinyCodes<T, W>(p, row, 1.f, peak / 127.f, first, stride);
+    }
 }
 
 struct NormGradient {
@@ -618,10 +666,33 @@ int gridFor(const void *kernel, int64_t rows, int teams, int threads, size_t sme
     return static_cast<int>(std::max<int64_t>(1, std::min(most, (rows + teams - 1) / teams)));
 }
 
-void checkRows(int64_t rows, int width, int type, int weightType) {
+void checkRows(int64_t rows, int width, int type, int weightType, int most = kMaxWidth) {
     RXMET_REQUIRE(rows >= 0 && width >= 1, "add_rms_norm: %lld rows of %d", static_cast<long long>(rows), width);
-    if (width > kMaxWidth) fail(RXMET_ERR_UNSUPPORTED, "add_rms_norm: rows of %d elements, at most %d", width, kMaxWidth);
+    if (width > most) fail(RXMET_ERR_UNSUPPORTED, "add_rms_norm: rows of %d elements, at most %d", width, most);
     RXMET_REQUIRE(type >= 0 && type <= 2 && weightType >= 0 && weightType <= 2, "add_rms_norm: unknown element type");
+}
+
+// Whether all rows start on 16 bytes, those of codes on as many as 16 bytes of T have elements, and consist of such groups.
+template <bool Codes>
+bool inGroups(const NormRows &p, int64_t group) {
+    return p.width % group == 0 && p.xPitch % group == 0 && alignedTo(p.x, 16) &&
+           (!p.residual || (p.residualPitch % group == 0 && alignedTo(p.residual, 16) && alignedTo(p.total, 16))) &&
+           (Codes ? p.codesPitch % group == 0 && alignedTo(p.codes, group) : alignedTo(p.y, 16));
+}
+
+void launchWideCodes(const NormRows &p, int type, cudaStream_t st) {
+    if (p.rows == 0) return;
+    withType(type, [&](auto t) {
+        using T = decltype(t);
+        constexpr int V = 16 / sizeof(T);
+        const auto kernel = inGroups<true>(p, V) ? codeWideRows<T, V> : codeWideRows<T, 1>;
+        const int grid = gridFor(reinterpret_cast<const void *>(kernel), p.rows, 1, kWideThreads, 0);
+        {
+            KernelTimer timer__("codeWideRows", st);
+            launchDependent(kernel, grid, kWideThreads, 0, st, p);
+        }
+        afterLaunch("codeWideRows");
+    });
 }
 
 template <bool Codes>
@@ -629,10 +700,7 @@ void launchNorm(const char *name, NormRows p, int type, cudaStream_t st) {
     if (p.rows == 0) return;
     withType(type, [&](auto t) {
         using T = decltype(t);
-        const int64_t group = 16 / sizeof(T);
-        const bool vector = p.width % group == 0 && p.xPitch % group == 0 && alignedTo(p.x, 16) &&
-                            (!p.residual || (p.residualPitch % group == 0 && alignedTo(p.residual, 16) && alignedTo(p.total, 16))) &&
-                            (Codes ? p.codesPitch % group == 0 && alignedTo(p.codes, group) : alignedTo(p.y, 16));
+        const bool vector = inGroups<Codes>(p, 16 / sizeof(T));
         withGroups<T>(p.rows, p.width, vector, Codes ? Output::Codes : Output::Rows, [&](auto w, auto items) {
             constexpr int W = decltype(w)::value, ITEMS = decltype(items)::value;
             const TeamPlan plan = teamFor(p.width, W * ITEMS);
@@ -712,11 +780,12 @@ int rxmet_add_rms_norm_codes(int64_t rows, int width, int type, const void *x_de
                              int64_t residual_pitch, const void *weight_dev, int weight_type, float eps, void *total_dev,
                              int8_t *codes_dev, int64_t codes_pitch, float *scale_dev, void *stream) {
     return guarded([&] {
-        checkRows(rows, width, type, weight_type);
+        checkRows(rows, width, type, weight_type, weight_dev ? kMaxWidth : kMaxCoded);
         RXMET_REQUIRE(rows == 0 || (x_dev && codes_dev && scale_dev && (!residual_dev || total_dev)), "add_rms_norm_codes: null tensor");
         RXMET_REQUIRE(codes_pitch >= width, "add_rms_norm_codes: rows of %d codes %lld bytes apart", width, static_cast<long long>(codes_pitch));
         NormRows p{rows, width, 1, {}, x_dev, residual_dev, weight_dev, x_pitch, residual_pitch, weight_type, eps, total_dev, nullptr, nullptr, codes_dev, codes_pitch, scale_dev};
-        launchNorm<true>("addRmsNormCodes", p, type, static_cast<cudaStream_t>(stream));
+        if (width > kMaxWidth) launchWideCodes(p, type, static_cast<cudaStream_t>(stream));
+        else launchNorm<true>("addRmsNormCodes", p, type, static_cast<cudaStream_t>(stream));
     });
 }
 

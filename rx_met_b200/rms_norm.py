@@ -2,7 +2,7 @@
 
 One CUDA kernel a call reads the two inputs once and writes the sum and the normalized rows; with the codes' form the rows leave as
 8-bit codes with a scale each, as `coded_linear` reads them.  float32, bfloat16 and float16 CUDA tensors with any leading dimensions,
-rows of up to 16384 elements; sums are held in 32 bits.
+rows of up to 16384 elements (131071 where they are only coded); sums are held in 32 bits.
 """
 from __future__ import annotations
 

@@ -258,3 +258,52 @@ def test_gradients_of_the_final_state_alone(tokens, Dk, Dv, struct, dtype):
     for got, want, magnitude in zip(grads, wants, sizes):
         # decays of up to e^-200 lead below the normal numbers, where every token's two products may be off by half of the smallest one
         ml.within(got, want, ml.attention_bound(magnitude, dtype, tokens, max(Dk, Dv), got.dtype) + tokens * 2.0 ** -149)
+
+
+# ---- wide rows of codes -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ml.TYPES)
+@pytest.mark.parametrize("rows,width,extra", [(1, 16385, 0), (3, 20000, 8), (700, 28672, 0), (5, 28672, 3), (2, 131071, 0), (0, 20000, 0)])
+def test_codes_of_wide_rows(rows, width, extra, dtype):
+    """The rows of what goes into a product may be as wide as the product takes them."""
+    from rx_met_b200 import rms_norm
+    x = torch.randn(rows, width + extra, device="cuda").to(dtype)[:, :width]
+    if rows > 1:
+        x[1] = 0
+    codes, scale = rms_norm.code_rows(x)
+    assert codes.shape == (rows, width) and (rows < 2 or (codes.stride(0) % 16 == 0 and scale[1] == 0 and not codes[1].any()))
+    if rows:
+        assert torch.equal(scale, (x.double().abs().amax(dim=1) / 127).float()) and int(codes.abs().max()) == 127
+    step = scale.double()[:, None]
+    assert bool(((codes.double() * step - x.double()).abs() <= step * (0.5 + 127 * 2.0 ** -22)).all())
+
+
+def test_wide_rows_at_the_ends_of_the_range():
+    from rx_met_b200 import rms_norm
+    x = tiny_rows(8, 20000, torch.float32)
+    check_tiny(*rms_norm.code_rows(x), x)
+    x[0, 19999], x[1, 0] = float("nan"), float("-inf")
+    codes, scale = rms_norm.code_rows(x)
+    assert torch.isnan(scale[0]) and torch.isinf(scale[1])
+    check_tiny(codes[2:], scale[2:], x[2:])
+    with pytest.raises(RuntimeError, match="at most 131071"):
+        rms_norm.code_rows(torch.zeros(1, 131072, device="cuda"))
+    with pytest.raises(RuntimeError, match="at most 16384"):
+        rms_norm.add_rms_norm_codes(torch.zeros(1, 16385, device="cuda"), torch.ones(16385, device="cuda"))
+
+
+def test_a_block_of_many_hidden_units():
+    from rx_met_b200.coded_linear import code_weight, coded_linear
+    from rx_met_b200.decay_block import DecayBlock
+    from rx_met_b200.rms_norm import code_rows
+    torch.manual_seed(0)
+    b = DecayBlock(width=64, heads=2, head_dim=32, hidden=20000)
+    x = torch.randn(2, 9, 64, device="cuda").bfloat16()
+    want = b(x)[0].detach()
+    got, _ = b.coded().prefill(x)
+    assert float((got.double() - want.double()).norm() / want.double().norm()) < 0.05
+    y, w = torch.randn(40, 28672, device="cuda"), torch.randn(24, 28672, device="cuda")
+    rows, channels = code_rows(y), code_weight(w)
+    out = coded_linear(*rows, channels, dtype=torch.float32)
+    exact = (rows[0].double() * rows[1].double()[:, None]) @ (channels.codes.double() * channels.scale.double()[:, None]).T
+    assert bool(((out.double() - exact).abs() <= 4 * 2.0 ** -24 * exact.abs() + 1e-30).all())

@@ -641,7 +641,6 @@ struct AttentionArguments {
         TORCH_CHECK(keys.size(-1) == queries.size(-1), "q and k must have heads of one size");
         sameDevice(decays, queries, "log_decay");
         TORCH_CHECK(decays.scalar_type() == at::kFloat && decays.dim() == 1 && decays.size(0) > 0, "log_decay must be a float32 tensor of one dimension, the heads");
-        TORCH_CHECK(!decays.requires_grad(), "log_decay is a constant of the layer: it has no gradient");
         q = rowsOf(queries);
         k = rowsOf(keys);
         v = rowsOf(values);
@@ -728,9 +727,14 @@ struct DecayedAttention : torch::autograd::Function<DecayedAttention> {
     }
 };
 
+void constantDecay(const Tensor &decays) {
+    TORCH_CHECK(!at::GradMode::is_enabled() || !decays.requires_grad(), "log_decay is a constant of the layer: it has no gradient");
+}
+
 std::vector<Tensor> decayedAttention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &logDecay, const MaybeTensor &state,
                                      const MaybeTensor &lengths, double scale) {
     refuseTrace("decayed_attention");
+    constantDecay(logDecay);
     return DecayedAttention::apply(q, k, v, logDecay, state, lengths, scale);
 }
 
@@ -738,6 +742,7 @@ std::vector<Tensor> decayedAttention(const Tensor &q, const Tensor &k, const Ten
 Tensor decayedAttentionStep(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &logDecay, const Tensor &state, const Tensor &newState,
                             const MaybeTensor &active, double scale) {
     refuseTrace("decayed_attention_step");
+    constantDecay(logDecay);
     if (at::GradMode::is_enabled())
         for (const Tensor *t : {&q, &k, &v, &state, &newState})
             TORCH_CHECK(!t->requires_grad(), "decayed_attention_step has no gradient: use decayed_attention, or no_grad");

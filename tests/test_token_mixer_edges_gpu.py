@@ -307,3 +307,18 @@ def test_a_block_of_many_hidden_units():
     out = coded_linear(*rows, channels, dtype=torch.float32)
     exact = (rows[0].double() * rows[1].double()[:, None]) @ (channels.codes.double() * channels.scale.double()[:, None]).T
     assert bool(((out.double() - exact).abs() <= 4 * 2.0 ** -24 * exact.abs() + 1e-30).all())
+
+
+def test_a_decay_that_could_have_a_gradient():
+    """Refused where gradients are recorded, and only there."""
+    from rx_met_b200.decayed_attention import decayed_attention, decayed_attention_step
+    q, decay = torch.randn(2, 40, 2, 32, device="cuda"), -torch.ones(2, device="cuda")
+    leaf, states = decay.clone().requires_grad_(), [torch.zeros(2, 2, 32, 32, device="cuda") for _ in range(2)]
+    for call in (lambda: decayed_attention(q, q, q, leaf), lambda: decayed_attention_step(q[:, 0], q[:, 0], q[:, 0], leaf, states[0])):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+    with torch.no_grad():
+        for a, b in zip(decayed_attention(q, q, q, leaf), decayed_attention(q, q, q, decay)):
+            assert torch.equal(a, b)
+        steps = [decayed_attention_step(q[:, 0], q[:, 0], q[:, 0], d, s) for d, s in zip((leaf, decay), states)]
+    assert torch.equal(*steps) and torch.equal(*states)

@@ -584,7 +584,12 @@ Tensor codedLinear(const Tensor &codes, const Tensor &scale, const Tensor &weigh
     Shape shape = codes.sizes().vec();
     shape.back() = outer;
     const c10::cuda::CUDAGuard guard(codes.device());
-    const Tensor rows = asRows(codes), weights = asRows(weight), scales = scale.contiguous(), weightScales = weightScale.contiguous();
+    // rows that share memory (a view that repeats one) are laid out apart: the C ABI takes none that overlap
+    auto rowsApart = [](const Tensor &t) {
+        const Tensor r = asRows(t);
+        return r.size(0) > 1 && r.stride(0) < r.size(1) ? r.contiguous() : r;
+    };
+    const Tensor rows = rowsApart(codes), weights = rowsApart(weight), scales = scale.contiguous(), weightScales = weightScale.contiguous();
     Tensor added, biases;
     if (bias) {
         sameDevice(*bias, codes, "bias");

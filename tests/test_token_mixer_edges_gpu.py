@@ -322,3 +322,17 @@ def test_a_decay_that_could_have_a_gradient():
             assert torch.equal(a, b)
         steps = [decayed_attention_step(q[:, 0], q[:, 0], q[:, 0], d, s) for d, s in zip((leaf, decay), states)]
     assert torch.equal(*steps) and torch.equal(*states)
+
+
+# ---- memory orders ------------------------------------------------------------------------------------------------------------
+
+def test_codes_whose_rows_share_memory():
+    from rx_met_b200.coded_linear import CodedWeight, coded_linear
+    codes, weight = (torch.randint(-127, 128, (n, 96), device="cuda", dtype=torch.int8) for n in (1, 8))
+    ones = torch.ones(300, device="cuda")
+    windows = torch.randint(-127, 128, (400,), device="cuda", dtype=torch.int8).unfold(0, 96, 1)[:300]
+    for rows, channels in ((codes.expand(300, 96), weight), (windows, weight), (windows, codes.expand(8, 96))):
+        for inner in (96, 50):
+            a, b = rows[:, :inner], channels[:, :inner]
+            got = coded_linear(a, ones, CodedWeight(b, ones[:8]), dtype=torch.float32)
+            assert torch.equal(got.double(), a.double() @ b.double().T)

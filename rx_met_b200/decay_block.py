@@ -48,20 +48,21 @@ class DecayBlock(torch.nn.Module):
 
 
 class CodedDecayBlock:
-    """The block with 8-bit weights and 8-bit codes in front of every product.  No gradients."""
+    """The block with 8-bit weights and 8-bit codes in front of every product, as the block is when this is made: it keeps copies of all its values.  No gradients."""
 
     def __init__(self, block: DecayBlock):
-        self.block = block
+        self.heads, self.head_dim, self.dtype = block.heads, block.head_dim, block.dtype
         self.qkv, self.out, self.up, self.down = (code_weight(w) for w in (block.w_qkv, block.w_out, block.w_up, block.w_down))
+        self.norm1, self.norm2, self.b_up, self.log_decay = (t.detach().clone() for t in (block.norm1, block.norm2, block.b_up, block.log_decay))
 
     def _around(self, x, attend):
-        b = self.block
-        codes, scale, _ = add_rms_norm_codes(x, b.norm1)
-        out = attend(*b._split(coded_linear(codes, scale, self.qkv, dtype=b.dtype)))
-        h = coded_linear(*code_rows(out.flatten(-2)), self.out, residual=x, dtype=b.dtype)
-        codes, scale, _ = add_rms_norm_codes(h, b.norm2)
-        up = coded_linear(codes, scale, self.up, bias=b.b_up, activation="silu", dtype=b.dtype)
-        return coded_linear(*code_rows(up), self.down, residual=h, dtype=b.dtype)
+        codes, scale, _ = add_rms_norm_codes(x, self.norm1)
+        qkv = coded_linear(codes, scale, self.qkv, dtype=self.dtype)
+        out = attend(*(t.unflatten(-1, (self.heads, self.head_dim)) for t in qkv.chunk(3, dim=-1)))
+        h = coded_linear(*code_rows(out.flatten(-2)), self.out, residual=x, dtype=self.dtype)
+        codes, scale, _ = add_rms_norm_codes(h, self.norm2)
+        up = coded_linear(codes, scale, self.up, bias=self.b_up, activation="silu", dtype=self.dtype)
+        return coded_linear(*code_rows(up), self.down, residual=h, dtype=self.dtype)
 
     @torch.no_grad()
     def prefill(self, x: torch.Tensor, state: Optional[torch.Tensor] = None,
@@ -70,7 +71,7 @@ class CodedDecayBlock:
         last = []
 
         def attend(q, k, v):
-            out, final = decayed_attention(q, k, v, self.block.log_decay, state=state, lengths=lengths)
+            out, final = decayed_attention(q, k, v, self.log_decay, state=state, lengths=lengths)
             last.append(final)
             return out
 
@@ -80,4 +81,4 @@ class CodedDecayBlock:
     @torch.no_grad()
     def step(self, x: torch.Tensor, state: torch.Tensor, active: Optional[torch.Tensor] = None) -> torch.Tensor:
         """y of one token for each row, x [batch, width]; `state` is updated in place."""
-        return self._around(x, lambda q, k, v: decayed_attention_step(q, k, v, self.block.log_decay, state, active=active))
+        return self._around(x, lambda q, k, v: decayed_attention_step(q, k, v, self.log_decay, state, active=active))

@@ -336,3 +336,19 @@ def test_codes_whose_rows_share_memory():
             a, b = rows[:, :inner], channels[:, :inner]
             got = coded_linear(a, ones, CodedWeight(b, ones[:8]), dtype=torch.float32)
             assert torch.equal(got.double(), a.double() @ b.double().T)
+
+
+# ---- the block ----------------------------------------------------------------------------------------------------------------
+
+def test_a_coded_block_keeps_its_values():
+    """Whatever becomes of the block that it was made from."""
+    from rx_met_b200.decay_block import DecayBlock
+    torch.manual_seed(0)
+    b = DecayBlock(width=64, heads=2, head_dim=32, hidden=100)
+    c, x = b.coded(), torch.randn(2, 20, 64, device="cuda").bfloat16()
+    want = c.prefill(x)
+    with torch.no_grad():
+        for t in (*b.parameters(), *b.buffers()):
+            t.mul_(1.5)
+    for got, first in zip(c.prefill(x), want):
+        assert torch.equal(got, first)

@@ -23,7 +23,7 @@ class DecayBlock(torch.nn.Module):
 
     def __init__(self, width: int, heads: int, head_dim: int, hidden: int, longest: float = 512.0, device="cuda", dtype=torch.bfloat16):
         super().__init__()
-        self.heads, self.head_dim, self.dtype = heads, head_dim, dtype
+        self.heads, self.head_dim = heads, head_dim
         inner = heads * head_dim
         make = lambda rows, cols: torch.nn.Parameter((torch.randn(rows, cols, device=device) * cols ** -0.5).to(dtype))  # noqa: E731
         self.norm1 = torch.nn.Parameter(torch.ones(width, device=device))
@@ -31,6 +31,17 @@ class DecayBlock(torch.nn.Module):
         self.w_qkv, self.w_out, self.w_up, self.w_down = make(3 * inner, width), make(width, inner), make(hidden, width), make(width, hidden)
         self.b_up = torch.nn.Parameter(torch.zeros(hidden, device=device))
         self.register_buffer("log_decay", torch.log1p(-1 / torch.logspace(0.30103, float(torch.tensor(longest).log10()), heads, device=device)))
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.w_qkv.dtype
+
+    def _apply(self, fn, recurse=True):
+        """to() and its kind: the decays stay in 32 bits, whose exponents the heads with long memories need."""
+        kept = self.log_decay
+        super()._apply(fn, recurse)
+        self.log_decay = kept.to(self.log_decay.device)
+        return self
 
     def _split(self, qkv):
         return (t.unflatten(-1, (self.heads, self.head_dim)) for t in qkv.chunk(3, dim=-1))
@@ -53,7 +64,7 @@ class CodedDecayBlock:
     def __init__(self, block: DecayBlock):
         self.heads, self.head_dim, self.dtype = block.heads, block.head_dim, block.dtype
         self.qkv, self.out, self.up, self.down = (code_weight(w) for w in (block.w_qkv, block.w_out, block.w_up, block.w_down))
-        self.norm1, self.norm2, self.b_up, self.log_decay = (t.detach().clone() for t in (block.norm1, block.norm2, block.b_up, block.log_decay))
+        self.norm1, self.norm2, self.b_up, self.log_decay = (t.detach().clone() for t in (block.norm1, block.norm2, block.b_up.float(), block.log_decay))
 
     def _around(self, x, attend):
         codes, scale, _ = add_rms_norm_codes(x, self.norm1)

@@ -352,3 +352,19 @@ def test_a_coded_block_keeps_its_values():
             t.mul_(1.5)
     for got, first in zip(c.prefill(x), want):
         assert torch.equal(got, first)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_block_moved_to_another_type(dtype):
+    from rx_met_b200.decay_block import DecayBlock
+    torch.manual_seed(0)
+    b = DecayBlock(width=64, heads=2, head_dim=32, hidden=100, dtype=torch.float32)
+    decay, x = b.log_decay.clone(), torch.randn(2, 20, 64, device="cuda")
+    want = b(x)[0].detach().double()
+    b = b.cpu().to(dtype).cuda()
+    assert b.dtype == dtype and b.log_decay.is_cuda and torch.equal(b.log_decay, decay)
+    for got, off in ((b(x.to(dtype))[0], 0.03), (b.coded().prefill(x.to(dtype))[0], 0.05)):
+        assert got.dtype == dtype and float((got.detach().double() - want).norm() / want.norm()) < off
+    other = DecayBlock(width=64, heads=2, head_dim=32, hidden=100, dtype=dtype)
+    other.load_state_dict(b.state_dict())
+    assert torch.equal(other(x.to(dtype))[0], b(x.to(dtype))[0])

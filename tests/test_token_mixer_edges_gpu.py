@@ -368,3 +368,102 @@ def test_a_block_moved_to_another_type(dtype):
     other = DecayBlock(width=64, heads=2, head_dim=32, hidden=100, dtype=dtype)
     other.load_state_dict(b.state_dict())
     assert torch.equal(other(x.to(dtype))[0], b(x.to(dtype))[0])
+
+
+# ---- what the ordinary tests do not reach -----------------------------------------------------------------------------------------
+
+def apart_rows(t, extra, off):
+    """The same rows further apart, `off` elements into memory whose rest is NaN."""
+    held = torch.full((t.shape[0], t.shape[1] + extra), float("nan"), device="cuda", dtype=t.dtype)
+    held[:, off:off + t.shape[1]] = t
+    return held[:, off:off + t.shape[1]]
+
+
+@pytest.mark.parametrize("dtype", ml.TYPES)
+@pytest.mark.parametrize("width,extra,off", [(512, 64, 8), (512, 64, 3), (1000, 24, 0), (257, 3, 1), (4096, 8, 8), (7000, 16, 8)])
+def test_rows_apart_through_the_ring(width, extra, off, dtype):
+    """More rows than the GPU takes at once, with pitches of their own, on 16 bytes and off them; bounds as for rows behind one another."""
+    from rx_met_b200 import rms_norm
+    from test_rms_norm_gpu import ROUNDINGS
+    rows = 3001
+    g = torch.Generator(device="cuda").manual_seed(width)
+    x, residual, dy, dtotal = (torch.randn(rows, width, device="cuda", generator=g).to(dtype) for _ in range(4))
+    weight = 1 + 0.1 * torch.randn(width, device="cuda", generator=g)
+    exact = x.double() + residual.double()
+    want, _, rms = ml.norm(x, weight, residual, 1e-6)
+    want_dx, want_dw = ml.norm_gradients(dy, dtotal, exact, weight, rms)
+    d, u = (dy.double() * weight.double()).abs(), (exact * rms).abs()
+    size = rms * (d + u * (d * u).mean(dim=1, keepdim=True)) + dtotal.double().abs()
+    top = want.abs().amax(dim=1) / 127
+    for a, b in ((apart_rows(x, extra, off), apart_rows(residual, extra + 16, off)), (apart_rows(x, extra, off), residual), (x, apart_rows(residual, extra, off))):
+        codes, scale, total = rms_norm.add_rms_norm_codes(a, weight, b)
+        ml.within(codes.double() * scale.double()[:, None], want, (top * (0.5 + 127 * (3 * ROUNDINGS + 2.0 ** -21)))[:, None].expand_as(want))
+        leaves = [a.detach().requires_grad_(), weight.clone().requires_grad_(), b.detach().requires_grad_()]
+        y, again = rms_norm.add_rms_norm(*leaves)
+        assert torch.equal(again, total)
+        ml.within(total, exact, exact.abs() * (ml.UNIT[dtype] + 2.0 ** -23) * 1.01 + ml.TINY[dtype])
+        ml.within(y, want, want.abs() * (ml.UNIT[dtype] + ROUNDINGS) * 1.01 + ml.TINY[dtype])
+        dx, dweight, dresidual = torch.autograd.grad([y, again], leaves, [dy, dtotal])
+        assert torch.equal(dx, dresidual)
+        ml.within(dx, want_dx, want_dx.abs() * ml.UNIT[dtype] * 1.01 + size * 3 * ROUNDINGS + ml.TINY[dtype])
+        ml.within(dweight, want_dw, (dy.double().abs() * u).sum(dim=0) * (rows / 32 + 64) * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("dtype", ml.TYPES)
+@pytest.mark.parametrize("rows,inner,outer,activation", [(2500, 1040, 2700, "silu"), (4200, 900, 1300, "gelu"), (600, 2000, 9000, "relu"), (5000, 1040, 1100, "none")])
+def test_several_tiles_a_pair(rows, inner, outer, activation, dtype):
+    """More tiles than pairs of CTAs, K beyond their ring, ragged edges, all of the epilogue."""
+    from test_coded_linear_gpu import check, padded, problem
+    codes, scale, weight, weight_scale, bias, residual = problem(rows, inner, outer, seed=rows, dtype=dtype)
+    check(padded(codes), scale, padded(weight), weight_scale, bias, activation, residual, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("with_state", [True, False])
+def test_gradients_of_ragged_rows_in_segments(with_state, dtype):
+    """Reverse passes whose first segments are empty."""
+    from rx_met_b200.decayed_attention import decayed_attention
+    g = torch.Generator(device="cuda").manual_seed(3)
+    make = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    q, k, v, dout = (make(4, 3000, h, 64).to(dtype) for h in (2, 1, 2, 2))
+    decay, lengths = torch.tensor([-0.002, -0.2], device="cuda"), torch.tensor([3000, 0, 1111, 130], device="cuda")
+    S, dlast = (make(4, 2, 64, 64) if with_state else None for _ in range(2))
+    leaves = [t.requires_grad_() for t in (q, k, v, S) if t is not None]
+    out, last = decayed_attention(q, k, v, decay, state=S, lengths=lengths)
+    grads = torch.autograd.grad([out, last] if with_state else [out], leaves, [dout, dlast] if with_state else [dout])
+    parts = [None if t is None else t.detach() for t in (q, k, v, S, dout, dlast)]
+    wants = ml.attend_gradients(*parts[:3], decay, parts[3], lengths, 0.125, *parts[4:])
+    sizes = ml.magnitudes(lambda a, b, c, s, d, e: ml.attend_gradients(a, b, c, decay, s, lengths, 0.125, d, e), parts)
+    for got, want, size in zip(grads, wants, sizes):
+        ml.within(got, want, ml.attention_bound(size, got.dtype if got.dtype == torch.float32 else dtype, 3000, 64, got.dtype))
+
+
+def test_a_captured_training_step():
+    """With the streams that the gradients' passes run on."""
+    from rx_met_b200 import rms_norm
+    from rx_met_b200.decayed_attention import decayed_attention
+    q, k, v = (torch.randn(2, 300, h, 64, device="cuda").bfloat16().requires_grad_() for h in (4, 2, 4))
+    decay, w = torch.full((4,), -0.1, device="cuda"), torch.ones(64, device="cuda", requires_grad=True)
+
+    def step():
+        out, last = decayed_attention(q, k, rms_norm.add_rms_norm(v, w)[0], decay)
+        return [out, last, *torch.autograd.grad([out, last], [q, k, v, w], [torch.ones_like(out), torch.ones_like(last)])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        with torch.no_grad():
+            for t in (q, k, v):
+                t.copy_(torch.randn_like(t))
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+def test_no_wait_gave_up_in_any_of_these():
+    test_no_wait_gave_up()

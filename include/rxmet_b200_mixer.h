@@ -18,7 +18,8 @@ extern "C" {
 /* Element types of activations. */
 enum { RXMET_TYPE_F32 = 0, RXMET_TYPE_BF16 = 1, RXMET_TYPE_F16 = 2 };
 
-/* 1 in *gave_up once a bounded device-side wait of one of these operators' kernels has run out on the current device (its output is incomplete),
+/* 1 in *gave_up once a bounded device-side wait of one of these operators' kernels has run out on the current device (the results of that call are
+ * not to be used: some may be missing, some wrong),
  * else 0.  Synchronises the device.  No wait runs out in a working program. */
 RXMET_API int rxmet_wait_status(int *gave_up);
 
@@ -57,6 +58,8 @@ RXMET_API int rxmet_coded_linear(int64_t rows, int inner, int outer, const int8_
 
 /* ---- linear attention with a decay for each head ------------------------------------------------
  * S_t = exp(log_decay[h]) S_{t-1} + k_t v_t',  out_t = scale q_t S_t  for t < lengths[b]; out is zero beyond.
+ * What is not finite reaches nothing in front of it: from an infinity or a NaN in v on, its column of out and state is not finite (a NaN where the sum
+ * may be an infinity), from one in k on all of a head.
  * A tensor of `heads` heads: element (b, t, h, d) at b * stride_b + t * stride_t + h * stride_h + d.  The operator has `heads` heads;
  * q, k and v have a number of heads that divides it, and head h reads head h / (heads / own heads) of them.  log_decay <= 0 (32 bits, -inf: no memory).
  * state [batch][heads][key_dim][value_dim] in 32 bits, null for zeros.  1 <= key_dim, value_dim <= 128; batch and heads at most

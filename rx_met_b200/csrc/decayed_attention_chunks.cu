@@ -17,12 +17,12 @@
 // rebuilt from rounded values: the weighted V goes in as the sum of three bfloat16 terms, which leave 2^-24, or two of half,
 // 2^-22.  half has a short range: its rows of P, its S and the weighted V of a chunk are scaled by
 // powers of two to the top of it, the second term of the weighted V by 2^11 more (unscaled, values of 1e-6 left 2^-16; 1 x 16384 tokens of 8 heads of 64 45 -> 46.5 us).  The two larger terms lie side by side as 128 columns of one product, which reads
-// K once for both.  All chunks have the third term: later ones may add little, so that what an early one leaves in the state is all of it (8 x 4096 tokens of 16 heads of 128: 161 us, 152 with
+// K once for both.  All chunks have the third term: later ones may add little, so that what an early one leaves in the state is all of it (8 x 4096 tokens of 16 heads of 128: 163 us, 152 with
 // the third term of the last chunks alone, whose states were off by 2^-18.6 there).
 //
-// Bound: the chain of a chunk (terms of V, their product, the state, its rounding, Q S), 3300 cycles with 64 keys and 4000 with 128 of which the tensor cores work a third, the issue slots half; and
-// one CTA an SM.  8 x 4096 tokens of 16 heads: 161 us with 128 elements a head (3.3 TB/s, two rounds of CTAs), 64 with 64 (4.2 TB/s); half, whose scales take a turn more over scores and
-// state, 172 and 86.
+// Bound: the chain of a chunk (terms of V, their product, the state, its rounding, Q S), about 3400 cycles with 64 keys and 4300 with 128 of which the tensor cores work two fifths, the issue slots half; and
+// one CTA an SM.  8 x 4096 tokens of 16 heads: 163 us with 128 elements a head (3.3 TB/s, two rounds of CTAs), 66 with 64 (4.1 TB/s); half, whose scales take a turn more over scores,
+// state and V, 175 and 85.
 #include "decayed_attention.h"
 #include "dependent_launch.cuh"
 #include "element_types.cuh"

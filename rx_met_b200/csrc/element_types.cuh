@@ -85,7 +85,7 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) { return ma
 template <>
 __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
 
-// A word of the current device that kernels set where a bounded wait gave up; their output is not written then.
+// A word of the current device that kernels set where a bounded wait gave up.  The results of that call are not to be used: some may be missing, some made from what was not there yet.
 int *waitStatus();
 
 inline size_t typeBytes(int type) { return type == RXMET_TYPE_F32 ? 4 : 2; }

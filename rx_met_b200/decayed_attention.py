@@ -22,7 +22,8 @@ def decayed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_dec
     value_dim] in it.  log_decay float32 [heads], at most 0 (-inf: no memory), a constant: it has no gradient.  `state` float32 [batch, heads, key_dim,
     value_dim] is where the sequences go on from (zeros without it).  With `lengths` (integers [batch], on the device) row b has
     lengths[b] tokens: what lies behind them is not used, its outputs and gradients are zero, and the final state is the one after the
-    last token.  `scale` is key_dim ** -0.5 unless given.  Differentiable in q, k, v and state."""
+    last token.  `scale` is key_dim ** -0.5 unless given.  A value that is not finite reaches no token in front of its own; from there on what it
+    reaches is not finite.  Differentiable in q, k, v and state, once; not under a trace."""
     return tuple(cabi.load_binding().decayed_attention(q, k, v, log_decay, state, lengths, q.shape[-1] ** -0.5 if scale is None else scale))
 
 

@@ -17,7 +17,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
                  eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
     """(y, total) with total = x + residual (x itself without one) and y = total * rsqrt(mean(total^2) + eps) * weight, row by row over
     the last dimension.  y is taken from the sum before it is rounded to x's type.  `weight` may be of another type than x.  Differentiable
-    in x, residual and weight; the weight's gradient is summed in a fixed order."""
+    in x, residual and weight, once; the weight's gradient is summed in a fixed order.  Not under a trace, like the other calls here."""
     out = cabi.load_binding().add_rms_norm(x, weight, residual, eps)
     return (out[0], out[1]) if residual is not None else (out[0], x)
 

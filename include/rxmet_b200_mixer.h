@@ -59,7 +59,7 @@ RXMET_API int rxmet_coded_linear(int64_t rows, int inner, int outer, const int8_
 /* ---- linear attention with a decay for each head ------------------------------------------------
  * S_t = exp(log_decay[h]) S_{t-1} + k_t v_t',  out_t = scale q_t S_t  for t < lengths[b]; out is zero beyond.
  * What is not finite reaches nothing in front of it: from an infinity or a NaN in v on, its column of out and state is not finite (a NaN where the sum
- * may be an infinity), from one in k on all of a head.
+ * may be an infinity), from one in k on all of a head's out.
  * A tensor of `heads` heads: element (b, t, h, d) at b * stride_b + t * stride_t + h * stride_h + d.  The operator has `heads` heads;
  * q, k and v have a number of heads that divides it, and head h reads head h / (heads / own heads) of them.  log_decay <= 0 (32 bits, -inf: no memory).
  * state [batch][heads][key_dim][value_dim] in 32 bits, null for zeros.  1 <= key_dim, value_dim <= 128; batch and heads at most

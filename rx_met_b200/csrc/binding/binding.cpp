@@ -4,6 +4,7 @@
 // In Python with ctypes these took 60 to 180 us a call (qdq 4096 x 4096 with its gradients 160 us against 67 us of
 // kernels, one GRU inference 92 us against 72), so that the small calls were bound by the interpreter.  The C ABI is
 // not linked: the package loads the library globally first, so that an overridden library path reaches this module too.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/clamp.h>
 #include <ATen/ops/empty.h>
@@ -23,6 +24,7 @@
 
 #include "rxmet_b200.h"
 #include "rxmet_b200_lstm.h"
+#include "rxmet_b200_gated.h"
 #include "rxmet_b200_mixer.h"
 
 namespace {
@@ -761,6 +763,145 @@ Tensor decayedAttentionStep(const Tensor &q, const Tensor &k, const Tensor &v, c
     return out;
 }
 
+// ---- gated recurrent mixer: recurrence with gates of the tokens -------------------------------------------------------------
+
+// The integers of a batch, [batch] on the device, in 32 bits; of 64 bits, they are cut to the tokens that there are before they are cut to 32.
+Tensor countsOf(const Tensor &counts, const Tensor &like, int64_t batch, int64_t most) {
+    sameDevice(counts, like, "lengths");
+    TORCH_CHECK(counts.dim() == 1 && counts.size(0) == batch && at::isIntegralType(counts.scalar_type(), true), "lengths must be integers of shape [", batch, "]");
+    return (counts.scalar_type() == at::kLong ? at::clamp(counts, 0, most) : counts).to(at::kInt).contiguous();
+}
+
+// Arguments of the gated recurrence as the C ABI takes them; tensors of two dimensions are single tokens.
+struct GatedArguments {
+    Tensor forget, value, input, lengths, state;
+    rxmet_gated_recurrence problem{};
+    Shape stateShape;
+
+    static Tensor rowsOf(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+    static rxmet_token_tensor view(const Tensor &t) { return {dataOf(t), t.stride(0), t.dim() == 2 ? 0 : t.stride(1)}; }
+
+    GatedArguments(const Tensor &forgets, const Tensor &values, const MaybeTensor &inputs, bool tanhValue, const MaybeTensor &start, const MaybeTensor &counts, int64_t dims) {
+        TORCH_CHECK(forgets.is_cuda() && forgets.dim() == dims && forgets.size(-1) > 0, "forget must be a CUDA tensor of ", dims, " dimensions, the last of which is not empty");
+        problem.type = typeOf(forgets, "forget");
+        checkSizes(forgets.sizes(), "gated_recurrence");
+        auto like = [&](const Tensor &t, const char *name) {
+            sameDevice(t, forgets, name);
+            TORCH_CHECK(t.sizes() == forgets.sizes() && t.scalar_type() == forgets.scalar_type(), name, " must have the shape and type of forget");
+        };
+        like(values, "value");
+        if (inputs) like(*inputs, "input");
+        forget = rowsOf(forgets);
+        value = rowsOf(values);
+        if (inputs) input = rowsOf(*inputs);
+        problem.batch = static_cast<int32_t>(forgets.size(0));
+        problem.tokens = dims == 2 ? 1 : static_cast<int32_t>(forgets.size(1));
+        problem.width = static_cast<int32_t>(forgets.size(-1));
+        problem.tanh_value = tanhValue;
+        stateShape = {problem.batch, problem.width};
+        if (start) state = checkedState(*start, "state").contiguous();
+        if (counts) lengths = countsOf(*counts, forgets, problem.batch, problem.tokens);
+        problem.forget = view(forget);
+        problem.value = view(value);
+        if (inputs) problem.input = view(input);
+        problem.lengths = lengths.defined() ? lengths.const_data_ptr<int32_t>() : nullptr;
+    }
+    const Tensor &checkedState(const Tensor &t, const char *name) const {
+        sameDevice(t, forget, name);
+        TORCH_CHECK(t.scalar_type() == at::kFloat && t.sizes() == at::IntArrayRef(stateShape), name, " must be float32 of shape ", listText(stateShape));
+        return t;
+    }
+    Tensor workspace(size_t &bytes) const {
+        bytes = rxmet_gated_recurrence_workspace_bytes(&problem);
+        return bytes > 0 ? emptyLike(forget, {static_cast<int64_t>(bytes)}, at::kByte) : Tensor();
+    }
+    void forward(const Tensor &out, const Tensor &last, const Tensor &marks) const {
+        size_t bytes;
+        const Tensor ws = workspace(bytes);
+        checkStatus(rxmet_gated_recurrence_forward(&problem, pointer<float>(state), mutableOf(out), pointer<float>(last), pointer<float>(marks), mutableOf(ws), bytes, streamOf(forget)),
+                    "gated_recurrence");
+    }
+};
+
+struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &forget, const Tensor &value, const MaybeTensor &input, bool tanhValue,
+                                                  const MaybeTensor &state, const MaybeTensor &lengths) {
+        const GatedArguments a(forget, value, input, tanhValue, state, lengths, 3);
+        const c10::cuda::CUDAGuard guard(forget.device());
+        const Tensor out = emptyLike(forget, forget.sizes(), forget.scalar_type()), last = emptyLike(forget, a.stateShape);
+        const Tensor marks = emptyLike(forget, {static_cast<int64_t>(rxmet_gated_recurrence_marks(&a.problem))});
+        a.forward(out, last, marks);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({forget, value, input ? *input : Tensor(), state ? *state : Tensor(), a.lengths, marks});
+        ctx->saved_data["tanh"] = tanhValue;
+        return {out, last};
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        if (!at::GradMode::is_enabled()) return gradients(ctx, std::move(grads));
+        auto from = ctx->get_saved_variables();
+        from.insert(from.end(), grads.begin(), grads.end());
+        return differentiatedOnce(gradients(ctx, std::move(grads)), std::move(from), "gated_recurrence");
+    }
+
+    static torch::autograd::variable_list gradients(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        torch::autograd::variable_list out(6);
+        if (!grads[0].defined() && !grads[1].defined()) return out;
+        const at::NoGradGuard noGrad;
+        auto maybe = [](const Tensor &t) { return t.defined() ? MaybeTensor(t.detach()) : MaybeTensor(); };
+        const GatedArguments a(saved[0].detach(), saved[1].detach(), maybe(saved[2]), ctx->saved_data["tanh"].toBool(), maybe(saved[3]), maybe(saved[4]), 3);
+        const c10::cuda::CUDAGuard guard(a.forget.device());
+        const Tensor dout = grads[0].defined() ? GatedArguments::rowsOf(grads[0]) : Tensor(), dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+        for (int i = 0; i < 3; ++i)
+            if (saved[i].defined() && ctx->needs_input_grad(i)) out[i] = emptyLike(a.forget, saved[i].sizes(), a.forget.scalar_type());
+        if (saved[3].defined() && ctx->needs_input_grad(saved[2].defined() ? 3 : 2)) out[4] = emptyLike(a.forget, a.stateShape);   // an absent input gate has no place of its own
+        size_t bytes;
+        const Tensor ws = a.workspace(bytes);
+        rxmet_token_tensor d{};
+        if (dout.defined()) d = GatedArguments::view(dout);
+        checkStatus(rxmet_gated_recurrence_backward(&a.problem, pointer<float>(a.state), pointer<float>(saved[5]), &d, pointer<float>(dlast), mutableOf(out[0]), mutableOf(out[1]),
+                                                    mutableOf(out[2]), pointer<float>(out[4]), mutableOf(ws), bytes, streamOf(a.forget)),
+                    "gated_recurrence backward");
+        return out;
+    }
+};
+
+bool anyNeedsGradient(std::initializer_list<const Tensor *> tensors) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor *t : tensors)
+        if (t && t->requires_grad()) return true;
+    return false;
+}
+const Tensor *given(const MaybeTensor &t) { return t ? &*t : nullptr; }
+
+std::vector<Tensor> gatedRecurrence(const Tensor &forget, const Tensor &value, const MaybeTensor &input, bool tanhValue, const MaybeTensor &state, const MaybeTensor &lengths) {
+    refuseTrace("gated_recurrence");
+    if (anyNeedsGradient({&forget, &value, given(input), given(state)})) return GatedRecurrence::apply(forget, value, input, tanhValue, state, lengths);
+    const GatedArguments a(forget, value, input, tanhValue, state, lengths, 3);
+    const c10::cuda::CUDAGuard guard(forget.device());
+    const Tensor out = emptyLike(forget, forget.sizes(), forget.scalar_type()), last = emptyLike(forget, a.stateShape);
+    a.forward(out, last, Tensor());
+    return {out, last};
+}
+
+// One token for each row; the states go to `newState`, which may be `state` itself.
+Tensor gatedRecurrenceStep(const Tensor &forget, const Tensor &value, const Tensor &state, const MaybeTensor &input, bool tanhValue, const Tensor &newState, const MaybeTensor &active) {
+    refuseTrace("gated_recurrence_step");
+    TORCH_CHECK(!anyNeedsGradient({&forget, &value, &state, &newState, given(input)}), "gated_recurrence_step has no gradient: use gated_recurrence, or no_grad");
+    const GatedArguments a(forget, value, input, tanhValue, state, active, 2);
+    a.checkedState(newState, "new_state");
+    TORCH_CHECK(newState.is_contiguous(), "new_state must be contiguous");
+    at::assert_no_partial_overlap(newState, state);
+    for (const Tensor *t : {&forget, &value, given(input)})
+        if (t) at::assert_no_overlap(newState, *t);
+    const c10::cuda::CUDAGuard guard(forget.device());
+    const Tensor out = emptyLike(forget, forget.sizes(), forget.scalar_type());
+    a.forward(out, newState, Tensor());
+    newState.unsafeGetTensorImpl()->bump_version();
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_binding, m) {
@@ -774,5 +915,7 @@ PYBIND11_MODULE(_binding, m) {
     m.def("coded_linear", &codedLinear, pybind11::call_guard<pybind11::gil_scoped_release>());
     m.def("decayed_attention", &decayedAttention, pybind11::call_guard<pybind11::gil_scoped_release>());
     m.def("decayed_attention_step", &decayedAttentionStep, pybind11::call_guard<pybind11::gil_scoped_release>());
+    m.def("gated_recurrence", &gatedRecurrence, pybind11::call_guard<pybind11::gil_scoped_release>());
+    m.def("gated_recurrence_step", &gatedRecurrenceStep, pybind11::call_guard<pybind11::gil_scoped_release>());
     m.def("quantize_dequantize", &quantizeDequantize, pybind11::call_guard<pybind11::gil_scoped_release>());
 }

@@ -1,0 +1,45 @@
+"""Linear recurrence whose gates come from the tokens.
+
+    h_t = f h_{t-1} + z c        f = sigmoid(forget),  c = value or tanh(value),  z = 1 - f, or sigmoid(input)
+
+for every channel by itself, the state h in 32 bits: the gates of a GRU (z = 1 - f) or of an LSTM (an input gate of its own) that do not look at the state, so that all
+tokens of a sequence are worked on at the same time.  `gated_recurrence` takes whole sequences (prompts, training) and is differentiable,
+`gated_recurrence_step` a token for each row.  float32, bfloat16 and float16 CUDA tensors of any width and any strides but a last
+dimension of neighbouring elements (others are copied).
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _cabi as cabi
+
+#: what becomes of `value`
+ACTIVATIONS = ("none", "tanh")
+
+
+def _tanh(activation: str, what: str) -> bool:
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"{what}: activation {activation!r}, one of {', '.join(ACTIVATIONS)}")
+    return activation == "tanh"
+
+
+def gated_recurrence(forget: torch.Tensor, value: torch.Tensor, *, input: Optional[torch.Tensor] = None, activation: str = "none",
+                     state: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(out, final state).  forget, value and input [batch, tokens, width] of one type, in front of their activations; out, the state after every token, like them.
+    `state` float32 [batch, width] is where the sequences go on from (zeros without it).  With `lengths` (integers [batch], on the device) row b has
+    lengths[b] tokens: what lies behind them is not used, its outputs and gradients are zero, and the final state is the one after the last
+    token.  A value that is not finite reaches its own channel, from its token on.  Differentiable in forget, value, input and state, once; not
+    under a trace."""
+    return tuple(cabi.load_binding().gated_recurrence(forget, value, input, _tanh(activation, "gated_recurrence"), state, lengths))
+
+
+def gated_recurrence_step(forget: torch.Tensor, value: torch.Tensor, state: torch.Tensor, *, input: Optional[torch.Tensor] = None,
+                          activation: str = "none", new_state: Optional[torch.Tensor] = None,
+                          active: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token for each row: forget, value and input [batch, width], returns out [batch, width].  The state after the token goes to
+    `new_state` (contiguous, `state` itself or apart from it and from the inputs; `state` without it, which is then updated in place).  Rows with active[b] == 0 keep
+    their state and get zeros.  No gradient."""
+    return cabi.load_binding().gated_recurrence_step(forget, value, state, input, _tanh(activation, "gated_recurrence_step"),
+                                                     state if new_state is None else new_state, active)

@@ -1,0 +1,63 @@
+"""Plain forms of the gated recurrence and of kept codes in 64 bits, with bounds on the errors of the 32-bit and 16-bit ones (test infrastructure)."""
+from __future__ import annotations
+
+import torch
+
+#: a gate or its complement, relative: an exponential and a tanh of two units, a reciprocal of one, a sum and a product of half a one, all of 2^-23
+GATE = 6 * 2.0 ** -23
+#: a step of the recurrence: a gate, a product and a sum, twice over, because runs of tokens are joined once inside and once between the tiles
+STEP = 2 * (GATE + 2 * 2.0 ** -24)
+
+
+def gates(forget, value, input, activation):
+    """f, 1 - f, z, 1 - z and c."""
+    forget, value = forget.double(), value.double()
+    f, shut = torch.sigmoid(forget), torch.sigmoid(-forget)
+    z, rest = (shut, f) if input is None else (torch.sigmoid(input.double()), torch.sigmoid(-input.double()))
+    return f, shut, z, rest, torch.tanh(value) if activation == "tanh" else value
+
+
+def recur(forget, value, input=None, activation="none", state=None, lengths=None):
+    """(out, final state, bound of out, bound of the final state, states in front of the tokens and their bounds): token by token.
+    With M the recurrence of the magnitudes, an error E goes through a token as f E + STEP M."""
+    B, T, D = forget.shape
+    f, _, z, _, c = gates(forget, value, input, activation)
+    h = torch.zeros(B, D, dtype=torch.float64, device=forget.device) if state is None else state.double()
+    M, E = h.abs(), torch.zeros_like(h)
+    out, bound, before, off = (torch.zeros(B, T, D, dtype=torch.float64, device=forget.device) for _ in range(4))
+    for t in range(T):
+        live = torch.ones(B, 1, dtype=torch.bool, device=forget.device) if lengths is None else (t < lengths.to(forget.device))[:, None]
+        before[:, t], off[:, t] = h, E
+        keep = lambda new, old: torch.where(live, new, old)  # noqa: E731
+        h = keep(f[:, t] * h + z[:, t] * c[:, t], h)
+        M = keep(f[:, t] * M + z[:, t] * c[:, t].abs(), M)
+        E = keep(f[:, t] * E + STEP * M, E)
+        out[:, t], bound[:, t] = keep(h, torch.zeros_like(h)), keep(E, torch.zeros_like(E))
+    return out, h, bound, E, before, off
+
+
+def recur_gradients(forget, value, input, activation, state, lengths, dout, dfinal):
+    """[(gradient, bound)] of forget, value, input and state, by the recurrence of the state's gradient, from the last token to the first."""
+    B, T, D = forget.shape
+    f, shut, z, rest, c = gates(forget, value, input, activation)
+    _, _, _, _, before, off = recur(forget, value, input, activation, state, lengths)
+    R = torch.zeros(B, D, dtype=torch.float64, device=forget.device) if dfinal is None else dfinal.double()
+    M, E = R.abs(), torch.zeros_like(R)
+    G, GM, GE = (torch.zeros_like(f) for _ in range(3))
+    for t in reversed(range(T)):
+        live = torch.ones(B, 1, dtype=torch.bool, device=forget.device) if lengths is None else (t < lengths.to(forget.device))[:, None]
+        d = torch.zeros_like(R) if dout is None else torch.where(live, dout[:, t].double(), 0.0)
+        zero = torch.zeros_like(R)
+        G[:, t], GM[:, t], GE[:, t] = torch.where(live, R + d, zero), torch.where(live, M + d.abs(), zero), torch.where(live, E + 2.0 ** -24 * (M + d.abs()), zero)
+        R = torch.where(live, f[:, t] * (R + d), R)
+        E = torch.where(live, f[:, t] * E + STEP * (M + d.abs()) * f[:, t], E)
+        M = torch.where(live, f[:, t] * (M + d.abs()), M)
+    c = torch.where(torch.isfinite(c), c, torch.zeros_like(c))
+    slope, loose = (1 - c * c, 4 * 2.0 ** -23) if activation == "tanh" else (torch.ones_like(c), 0.0)
+    held = before if input is not None else before - c
+    size, wrong = (before.abs(), off) if input is not None else (before.abs() + c.abs(), off + 2 * GATE * c.abs())
+    grads = [(G * f * shut * held, f * shut * (GE * (size + wrong) + GM * (wrong + 3 * GATE * size))),
+             (G * z * slope, z * (GE * (slope + loose) + GM * (2 * GATE * slope + loose)))]
+    grads.append(None if input is None else (G * c * z * rest, z * rest * c.abs() * (GE + 4 * GATE * GM)))
+    grads.append((R, E))
+    return grads

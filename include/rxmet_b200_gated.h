@@ -40,6 +40,34 @@ RXMET_API int rxmet_gated_recurrence_backward(const rxmet_gated_recurrence *prob
                                               const rxmet_token_tensor *dout, const float *dfinal_state_dev, void *dforget_dev, void *dvalue_dev,
                                               void *dinput_dev, float *dstate_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
 
+/* ---- activations kept in 8 bits ------------------------------------------------------------------
+ * A group is RXMET_KEPT_GROUP neighbouring elements of a row (fewer at its end) with one exponent e: value = code * 2^e, code in [-127, 127].  e is the least with which the
+ * group's largest magnitude is at most 127 * 2^e, but not below -126 (half: -24, so that every value is a number of half, too); code = rne(x / 2^e).  A group with an infinity or a NaN
+ * has e = 127 and codes 0, and stands for NaN.  Rows of codes start codes_pitch bytes apart, a multiple of 16, on 16 bytes, and what lies between a row's end and the next
+ * multiple of 8 may be written; exponents [rows][groups of a row].  Rows of at most 131071 elements. */
+enum { RXMET_KEPT_GROUP = 32 };
+RXMET_API int rxmet_keep_codes(int64_t rows, int width, int type, const void *x_dev, int64_t x_pitch, int8_t *codes_dev, int64_t codes_pitch,
+                               int8_t *exponents_dev, void *stream);
+/* out [rows][width], contiguous, in `type`. */
+RXMET_API int rxmet_kept_values(int64_t rows, int width, int type, const int8_t *codes_dev, int64_t codes_pitch, const int8_t *exponents_dev, void *out_dev,
+                                void *stream);
+/* y = activation(gate) * up (RXMET_ACTIVATION_*), contiguous, and the codes of gate and of up (all four null: not kept); rows of both start codes_pitch bytes apart. */
+RXMET_API int rxmet_gated_product(int64_t rows, int width, int type, int activation, const void *gate_dev, int64_t gate_pitch, const void *up_dev,
+                                  int64_t up_pitch, void *y_dev, int8_t *gate_codes_dev, int8_t *gate_exponents_dev, int8_t *up_codes_dev,
+                                  int8_t *up_exponents_dev, int64_t codes_pitch, void *stream);
+/* dgate = dy * up * activation'(gate), dup = dy * activation(gate) with the values that the codes stand for; contiguous, null where not wanted. */
+RXMET_API int rxmet_gated_product_backward(int64_t rows, int width, int type, int activation, const void *dy_dev, int64_t dy_pitch,
+                                           const int8_t *gate_codes_dev, const int8_t *gate_exponents_dev, const int8_t *up_codes_dev,
+                                           const int8_t *up_exponents_dev, int64_t codes_pitch, void *dgate_dev, void *dup_dev, void *stream);
+
+/* ---- gradient of a weight from kept codes ---------------------------------------------------------
+ * out[n][k] = sum_m dy[m][n] * codes[m][k] * 2^exponents[m][k / 32], dy of `type` with rows dy_pitch elements apart, the codes those of an activation of that type;
+ * out [outer][inner] contiguous in out_type.  Products are exact, sums in 32 bits.  tokens and outer at most 2^30, inner at most 131071. */
+RXMET_API size_t rxmet_kept_weight_gradient_workspace_bytes(int64_t tokens, int inner, int outer, int type, const void *dy_dev, int64_t dy_pitch);
+RXMET_API int rxmet_kept_weight_gradient(int64_t tokens, int inner, int outer, int type, const void *dy_dev, int64_t dy_pitch, const int8_t *codes_dev,
+                                         int64_t codes_pitch, const int8_t *exponents_dev, int out_type, void *out_dev, void *workspace_dev,
+                                         size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -902,6 +902,162 @@ Tensor gatedRecurrenceStep(const Tensor &forget, const Tensor &value, const Tens
     return out;
 }
 
+// ---- activations kept in 8 bits ---------------------------------------------------------------------------------------------
+
+Tensor emptyExponents(const Tensor &like, at::IntArrayRef shape) {
+    Shape groups = shape.vec();
+    groups.back() = (groups.back() + RXMET_KEPT_GROUP - 1) / RXMET_KEPT_GROUP;
+    return emptyLike(like, groups, at::kChar);
+}
+int64_t codesPitch(int64_t width) { return (width + 15) / 16 * 16; }
+
+// Rows of an activation as the C ABI takes them.
+struct KeptRows {
+    Tensor rows;
+    int type, width;
+    int64_t count;
+    KeptRows(const Tensor &x, const char *name) {
+        TORCH_CHECK(x.is_cuda() && x.dim() >= 1 && x.size(-1) > 0, name, " must be a CUDA tensor with a last dimension");
+        checkSizes({x.size(-1)}, name);
+        type = typeOf(x, name);
+        width = static_cast<int>(x.size(-1));
+        rows = asRows(x);
+        count = rows.size(0);
+    }
+    const void *data() const { return dataOf(rows); }
+    int64_t pitch() const { return pitchOf(rows); }
+};
+// Codes and exponents that a caller hands in, rows of codes on 16 bytes and apart (others are copied).
+struct HeldCodes {
+    Tensor codes, exponents;
+    int width;
+    int64_t count;
+    HeldCodes(const Tensor &given, const Tensor &powers) {
+        TORCH_CHECK(given.is_cuda() && given.scalar_type() == at::kChar && given.dim() >= 1 && given.size(-1) > 0, "codes must be a CUDA int8 tensor with a last dimension");
+        sameDevice(powers, given, "exponents");
+        Shape groups = given.sizes().vec();
+        groups.back() = (groups.back() + RXMET_KEPT_GROUP - 1) / RXMET_KEPT_GROUP;
+        TORCH_CHECK(powers.scalar_type() == at::kChar && powers.sizes() == at::IntArrayRef(groups), "exponents must be int8 of shape ", listText(groups));
+        checkSizes({given.size(-1)}, "codes");
+        width = static_cast<int>(given.size(-1));
+        codes = asRows(given);
+        count = codes.size(0);
+        const bool fits = reinterpret_cast<uintptr_t>(dataOf(codes)) % 16 == 0 && (count <= 1 || (codes.stride(0) % 16 == 0 && codes.stride(0) >= width));
+        if (!fits) {
+            const Tensor copy = emptyCodes(given, codes.sizes());
+            copy.copy_(codes);
+            codes = copy;
+        }
+        exponents = powers.contiguous();
+    }
+    const int8_t *data() const { return static_cast<const int8_t *>(dataOf(codes)); }
+    int64_t pitch() const { return count > 1 ? codes.stride(0) : codesPitch(width); }
+    const int8_t *powers() const { return static_cast<const int8_t *>(dataOf(exponents)); }
+};
+int8_t *bytesOf(const Tensor &t) { return static_cast<int8_t *>(mutableOf(t)); }
+
+std::vector<Tensor> keepCodes(const Tensor &x) {
+    refuseTrace("keep");
+    const KeptRows a(x, "x");
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor codes = emptyCodes(x, x.sizes()), exponents = emptyExponents(x, x.sizes());
+    checkStatus(rxmet_keep_codes(a.count, a.width, a.type, a.data(), a.pitch(), bytesOf(codes), codesPitch(a.width), bytesOf(exponents), streamOf(x)), "keep");
+    return {codes, exponents};
+}
+
+constexpr at::ScalarType kElementTypes[] = {at::kFloat, at::kBFloat16, at::kHalf};
+
+Tensor keptValues(const Tensor &codes, const Tensor &exponents, int type) {
+    refuseTrace("values");
+    TORCH_CHECK(type >= 0 && type <= 2, "values: unknown type");
+    const HeldCodes h(codes, exponents);
+    const c10::cuda::CUDAGuard guard(codes.device());
+    const Tensor out = emptyLike(codes, codes.sizes(), kElementTypes[type]);
+    checkStatus(rxmet_kept_values(h.count, h.width, type, h.data(), h.pitch(), h.powers(), mutableOf(out), streamOf(codes)), "values");
+    return out;
+}
+
+struct ProductArguments {
+    KeptRows gate, up;
+    ProductArguments(const Tensor &gates, const Tensor &ups) : gate(gates, "gate"), up((checkLike(ups, gates), ups), "up") {}
+    static void checkLike(const Tensor &ups, const Tensor &gates) {
+        sameDevice(ups, gates, "up");
+        TORCH_CHECK(ups.sizes() == gates.sizes() && ups.scalar_type() == gates.scalar_type(), "up must have the shape and type of gate");
+    }
+    // `held`: codes and exponents of gate and of up, or nothing
+    void forward(int activation, const Tensor &y, const std::array<Tensor, 4> &held, void *stream) const {
+        checkStatus(rxmet_gated_product(gate.count, gate.width, gate.type, activation, gate.data(), gate.pitch(), up.data(), up.pitch(), mutableOf(y), bytesOf(held[0]), bytesOf(held[1]),
+                                        bytesOf(held[2]), bytesOf(held[3]), codesPitch(gate.width), stream),
+                    "gated_product");
+    }
+};
+
+struct GatedProduct : torch::autograd::Function<GatedProduct> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &gate, const Tensor &up, int64_t activation) {
+        const ProductArguments a(gate, up);
+        const c10::cuda::CUDAGuard guard(gate.device());
+        const Tensor y = emptyLike(gate, gate.sizes(), gate.scalar_type());
+        const std::array<Tensor, 4> held{emptyCodes(gate, gate.sizes()), emptyExponents(gate, gate.sizes()), emptyCodes(gate, gate.sizes()), emptyExponents(gate, gate.sizes())};
+        a.forward(static_cast<int>(activation), y, held, streamOf(gate));
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({held.begin(), held.end()});
+        ctx->saved_data["activation"] = activation;
+        ctx->saved_data["type"] = static_cast<int64_t>(a.gate.type);
+        return {y};
+    }
+
+    // The kept codes hang on no graph, so that a second derivative has to be refused at the gradient of y.
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        if (!at::GradMode::is_enabled() || !grads[0].defined()) return gradients(ctx, grads);
+        const Tensor from = grads[0].requires_grad() ? grads[0] : grads[0].detach().requires_grad_();
+        return differentiatedOnce(gradients(ctx, std::move(grads)), {from}, "gated_product");
+    }
+
+    static torch::autograd::variable_list gradients(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        torch::autograd::variable_list out(3);
+        if (!grads[0].defined()) return out;
+        const auto held = ctx->get_saved_variables();
+        const at::NoGradGuard noGrad;
+        const KeptRows dy(grads[0].detach(), "the gradient");
+        const c10::cuda::CUDAGuard guard(grads[0].device());
+        for (int i = 0; i < 2; ++i)
+            if (ctx->needs_input_grad(i)) out[i] = emptyLike(grads[0], grads[0].sizes(), grads[0].scalar_type());
+        checkStatus(rxmet_gated_product_backward(dy.count, dy.width, dy.type, static_cast<int>(ctx->saved_data["activation"].toInt()), dy.data(), dy.pitch(), bytesOf(held[0]),
+                                                 bytesOf(held[1]), bytesOf(held[2]), bytesOf(held[3]), codesPitch(dy.width), mutableOf(out[0]), mutableOf(out[1]), streamOf(grads[0])),
+                    "gated_product backward");
+        return out;
+    }
+};
+
+Tensor gatedProduct(const Tensor &gate, const Tensor &up, int activation) {
+    refuseTrace("gated_product");
+    if (anyNeedsGradient({&gate, &up})) return GatedProduct::apply(gate, up, activation)[0];
+    const ProductArguments a(gate, up);
+    const c10::cuda::CUDAGuard guard(gate.device());
+    const Tensor y = emptyLike(gate, gate.sizes(), gate.scalar_type());
+    a.forward(activation, y, {}, streamOf(gate));
+    return y;
+}
+
+Tensor keptWeightGradient(const Tensor &dy, const Tensor &codes, const Tensor &exponents, int type, int outType) {
+    refuseTrace("weight_gradient");
+    TORCH_CHECK(outType >= 0 && outType <= 2, "weight_gradient: unknown type");
+    const HeldCodes h(codes, exponents);
+    sameDevice(dy, codes, "dy");
+    TORCH_CHECK(dy.dim() == codes.dim() && dy.sizes().slice(0, dy.dim() - 1) == codes.sizes().slice(0, dy.dim() - 1), "dy must have the leading dimensions of the codes, ",
+                listText(codes.sizes().slice(0, codes.dim() - 1)));
+    const KeptRows d(dy, "dy");
+    TORCH_CHECK(d.type == type, "dy must be of the type of the activation that was kept");
+    const c10::cuda::CUDAGuard guard(codes.device());
+    const Tensor out = emptyLike(codes, {d.width, h.width}, kElementTypes[outType]);
+    const size_t bytes = rxmet_kept_weight_gradient_workspace_bytes(d.count, h.width, d.width, d.type, d.data(), d.pitch());
+    const Tensor ws = bytes > 0 ? emptyLike(codes, {static_cast<int64_t>(bytes)}, at::kByte) : Tensor();
+    checkStatus(rxmet_kept_weight_gradient(d.count, h.width, d.width, d.type, d.data(), d.pitch(), h.data(), h.pitch(), h.powers(), outType, mutableOf(out), mutableOf(ws), bytes,
+                                           streamOf(codes)),
+                "weight_gradient");
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_binding, m) {
@@ -917,5 +1073,9 @@ PYBIND11_MODULE(_binding, m) {
     m.def("decayed_attention_step", &decayedAttentionStep, pybind11::call_guard<pybind11::gil_scoped_release>());
     m.def("gated_recurrence", &gatedRecurrence, pybind11::call_guard<pybind11::gil_scoped_release>());
     m.def("gated_recurrence_step", &gatedRecurrenceStep, pybind11::call_guard<pybind11::gil_scoped_release>());
+    m.def("keep_codes", &keepCodes, pybind11::call_guard<pybind11::gil_scoped_release>());
+    m.def("kept_values", &keptValues, pybind11::call_guard<pybind11::gil_scoped_release>());
+    m.def("gated_product", &gatedProduct, pybind11::call_guard<pybind11::gil_scoped_release>());
+    m.def("kept_weight_gradient", &keptWeightGradient, pybind11::call_guard<pybind11::gil_scoped_release>());
     m.def("quantize_dequantize", &quantizeDequantize, pybind11::call_guard<pybind11::gil_scoped_release>());
 }

@@ -1,0 +1,498 @@
+// Gradient of a weight from the gradient of its products and the kept codes of its input:
+//   out[n][k] = sum over tokens m of dy[m][n] * code[m][k] * 2^e[m][k / 32]
+//
+// On tcgen05 kind::f16 with 32-bit sums in tensor memory.  A code times its power of two is a number of bfloat16 and of half, so that one product a term is exact; dy in 32 bits comes as
+// its three runs of eight bits, each a number of bfloat16.
+// A pair of CTAs computes tiles of 256 output channels x 256 input channels, 64 tokens at a time; each CTA holds half of both operands.  dy arrives by TMA in the order in which
+// the tensor cores read it across its rows.  The codes arrive as bytes, and eight warps turn them into 16-bit values in that order: ten instructions for four codes, 160 of a
+// chunk's 512 cycles.  Four warps store a tile while the next one is summed, two accumulators in turn.
+// Few tiles leave SMs without work, so the tokens are cut into parts, whose sums another kernel adds up in their order.
+#include "kept_codes.cuh"
+
+#include "dependent_launch.cuh"
+#include "umma_tiles.cuh"
+
+namespace rxmet {
+namespace kept {
+namespace {
+
+using namespace ummatiles;
+
+constexpr int kTile = 256, kHalf = kTile / 2, kTokens = 64, kBlock = 64;   // kBlock: 16-bit elements of a swizzled row
+constexpr int kStages = 5, kConvertWarps = 8, kStoreWarps = 4;
+constexpr int kThreads = 32 * (kConvertWarps + kStoreWarps + 2);
+constexpr uint32_t kBlockBytes = kTokens * kBlock * 2, kOperandBytes = kHalf / kBlock * kBlockBytes, kCodeBytes = kTokens * kHalf;
+constexpr uint32_t kStageBytes = 2 * kOperandBytes + kCodeBytes;
+constexpr uint32_t kShared = 231936;   // cluster::leastShared(512): one CTA an SM
+static_assert(kStages * kStageBytes + 1024 <= kShared, "the stages fit");
+
+struct Problem {
+    int64_t tokens;
+    int inner, outer, terms, parts, chunks;   // chunks: of one term
+    const int8_t *exponents;
+    void *out;
+    float *partial;   // [parts][outer][inner] where there are several
+};
+
+// kind::f16, 256 rows of A by a pair of CTAs, 32-bit sums, both operands read across their rows.
+__host__ __device__ constexpr uint32_t pairHalves(bool bf16) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16) | (static_cast<uint32_t>(kTile >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+}
+__device__ __forceinline__ void productPair(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void copyTile3Pair(uint32_t to, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(z),
+                 "r"(bar & 0xfeffffffu)
+                 : "memory");
+}
+// As waitSuspended, for arrivals from both CTAs of the pair.
+__device__ __forceinline__ bool waitPair(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kSuspendLimit; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+            : "=r"(done)
+            : "r"(bar), "r"(parity), "r"(kSuspendNs)
+            : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+
+// Four codes in words of two 16-bit values each, times a power of two in both halves of `step`.
+template <class T>
+struct Convert;
+template <>
+struct Convert<__nv_bfloat16> {
+    using Two = __nv_bfloat162;
+    static __device__ __forceinline__ uint32_t step(int e) { return e == kBad ? 0x7fc07fc0u : static_cast<uint32_t>(max(e + 127, 0)) * 0x00800080u; }
+    // 128 + its low seven bits, less 128 or, for a code below zero, 256: both are bfloat16 numbers whose low byte is that of the code
+    static __device__ __forceinline__ void four(uint32_t codes, uint32_t step, uint32_t &lo, uint32_t &hi) {
+        const uint32_t low = codes & 0x7f7f7f7fu, sign = codes & 0x80808080u;
+        lo = pair(__byte_perm(low, 0x43u, 0x4140), __byte_perm(sign, 0x43u, 0x4140), step);
+        hi = pair(__byte_perm(low, 0x43u, 0x4342), __byte_perm(sign, 0x43u, 0x4342), step);
+    }
+    static __device__ __forceinline__ uint32_t pair(uint32_t a, uint32_t b, uint32_t step) {
+        const Two r = __hmul2(__hsub2(*reinterpret_cast<Two *>(&a), *reinterpret_cast<Two *>(&b)), *reinterpret_cast<Two *>(&step));
+        return *reinterpret_cast<const uint32_t *>(&r);
+    }
+};
+template <>
+struct Convert<__half> {
+    using Two = __half2;
+    // 2^e as a number of half: normal from -14 on, below that one bit
+    static __device__ __forceinline__ uint32_t step(int e) {
+        const uint32_t one = e == kBad ? 0x7e00u : e > 15 ? 0x7c00u : e >= -14 ? static_cast<uint32_t>(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
+        return one * 0x00010001u;
+    }
+    // 1024 + 128 + the code, less 1152
+    static __device__ __forceinline__ void four(uint32_t codes, uint32_t step, uint32_t &lo, uint32_t &hi) {
+        const uint32_t raised = codes ^ 0x80808080u;
+        lo = pair(__byte_perm(raised, 0x64u, 0x4140), step);
+        hi = pair(__byte_perm(raised, 0x64u, 0x4342), step);
+    }
+    static __device__ __forceinline__ uint32_t pair(uint32_t a, uint32_t step) {
+        const uint32_t base = 0x64806480u;
+        const Two r = __hmul2(__hsub2(*reinterpret_cast<Two *>(&a), *reinterpret_cast<const Two *>(&base)), *reinterpret_cast<Two *>(&step));
+        return *reinterpret_cast<const uint32_t *>(&r);
+    }
+};
+
+// T: the products' type; OUT: that of what is stored (parts: floats).
+template <class T, class OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    keptWeightGradient(const __grid_constant__ Problem p, const __grid_constant__ CUtensorMap dyMap, const __grid_constant__ CUtensorMap codeMap, int *status) {
+    extern __shared__ uint8_t raw[];
+    __shared__ __align__(8) uint64_t dyFull[kStages], codesFull[kStages], converted[kStages], freed[kStages], accFull[2], accFree[2];
+    __shared__ uint32_t tmemSlot;
+    const uint32_t stages = (smemAddr(raw) + 1023u) & ~1023u;
+    const int warp = warpIndex(), lane = threadIdx.x & 31;
+    const uint32_t rank = cluster::rank();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            cluster::initBarrier(&dyFull[i], 1);
+            cluster::initBarrier(&codesFull[i], 1);
+            cluster::initBarrier(&converted[i], 2 * kConvertWarps);
+            cluster::initBarrier(&freed[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            cluster::initBarrier(&accFull[i], 1);
+            cluster::initBarrier(&accFree[i], 2 * kStoreWarps);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetchMap(&dyMap);
+        prefetchMap(&codeMap);
+    }
+    if (warp == 0) allocTmem<2>(smemAddr(&tmemSlot), 512);
+    fenceBefore();
+    __syncthreads();
+    cluster::barrierAll();
+    fenceAfter();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmemSlot, 0);
+    waitForPredecessor();
+    letDependentsStart();
+
+    const int outerTiles = (p.outer + kTile - 1) / kTile, innerTiles = (p.inner + kTile - 1) / kTile;
+    const int tiles = outerTiles * innerTiles, pairs = gridDim.x / 2;
+    const int64_t items = static_cast<int64_t>(tiles) * p.parts;
+    // A part's tiles are neighbours, in columns of eight outer tiles, so that the pairs at work at the same time share both operands.
+    struct Place {
+        int part, n0, k0, first, count;   // count: chunks of a term
+    };
+    auto place = [&](int64_t item) {
+        Place at;
+        at.part = static_cast<int>(item / tiles);
+        const int tile = static_cast<int>(item - static_cast<int64_t>(at.part) * tiles);
+        const int group = tile / (8 * innerTiles), row0 = group * 8, rows = min(8, outerTiles - row0), in = tile - group * 8 * innerTiles;
+        at.k0 = in / rows * kTile;
+        at.n0 = (row0 + in % rows) * kTile;
+        at.first = static_cast<int>(static_cast<int64_t>(p.chunks) * at.part / p.parts);
+        at.count = static_cast<int>(static_cast<int64_t>(p.chunks) * (at.part + 1) / p.parts) - at.first;
+        return at;
+    };
+    bool alive = true;
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        if (alive) alive = __all_sync(0xffffffffu, waitSuspended(smemAddr(bar), parity));
+    };
+
+    if (warp == kConvertWarps + kStoreWarps) {   // copies
+        Turn turn;
+        for (int64_t item = blockIdx.x / 2; item < items; item += pairs) {
+            const Place at = place(item);
+            for (int term = 0; term < p.terms; ++term)
+                for (int c = 0; c < at.count; ++c, turn.step(kStages)) {
+                    if (turn.again) wait(&freed[turn.at], turn.parity ^ 1u);
+                    if (alive && electOne()) {
+                        const uint32_t to = stages + turn.at * kStageBytes, m = (at.first + c) * kTokens;
+                        const uint32_t dyBar = smemAddr(&dyFull[turn.at]), codeBar = smemAddr(&codesFull[turn.at]);
+                        if (rank == 0) cluster::arriveExpect(dyBar, 2 * kOperandBytes);
+                        for (int block = 0; block < kHalf / kBlock; ++block)
+                            copyTile3Pair(to + block * kBlockBytes, &dyMap, at.n0 + rank * kHalf + block * kBlock, m, term, dyBar);
+                        cluster::arriveExpect(codeBar, kCodeBytes);
+                        copyTile2(to + 2 * kOperandBytes, &codeMap, at.k0 + rank * kHalf, m, codeBar);
+                    }
+                    __syncwarp();
+                }
+        }
+        // nothing is left in flight: the last use of each stage is read before this CTA ends
+        for (int i = 0; i < kStages; ++i, turn.step(kStages))
+            if (turn.again) waitSuspended(smemAddr(&freed[turn.at]), turn.parity ^ 1u);
+    } else if (warp == kConvertWarps + kStoreWarps + 1) {   // products, issued by the first CTA for both
+        if (rank == 0) {
+            Turn turn;
+            int done = 0;
+            constexpr uint32_t kIdesc = pairHalves(std::is_same_v<T, __nv_bfloat16>);
+            for (int64_t item = blockIdx.x / 2; item < items; item += pairs, ++done) {
+                const Place at = place(item);
+                const uint32_t buf = done & 1;
+                if (done > 1) wait(&accFree[buf], ((done >> 1) - 1) & 1);
+                fenceAfter();
+                const int chunks = p.terms * at.count;
+                for (int c = 0; c < chunks; ++c, turn.step(kStages)) {
+                    wait(&dyFull[turn.at], turn.parity);
+                    if (alive) alive = __all_sync(0xffffffffu, waitPair(smemAddr(&converted[turn.at]), turn.parity));
+                    if (alive && electOne()) {
+                        fenceAfter();
+                        const uint32_t from = stages + turn.at * kStageBytes;
+                        const uint64_t a = swizzledDescriptor(from, kBlockBytes), b = swizzledDescriptor(from + kOperandBytes, kBlockBytes);
+#pragma unroll
+                        for (int k = 0; k < kTokens / 16; ++k) productPair(tmem + buf * kTile, a + k * (2048 >> 4), b + k * (2048 >> 4), kIdesc, c + k > 0 ? 1u : 0u);
+                        commitPair(smemAddr(&freed[turn.at]));
+                        if (c + 1 == chunks) commitPair(smemAddr(&accFull[buf]));
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    } else if (warp < kConvertWarps) {   // codes to values: a thread takes sixteen codes of a token, twice a chunk
+        constexpr int kPieces = kTokens * kHalf / 16 / (32 * kConvertWarps);
+        const int column = threadIdx.x & 7, row = threadIdx.x >> 3;   // of sixteen codes; of tokens, 32 apart from piece to piece
+        const int groups = groupsOf(p.inner);
+        Turn turn;
+        for (int64_t item = blockIdx.x / 2; item < items; item += pairs) {
+            const Place at = place(item);
+            const int k = at.k0 + rank * kHalf + column * 16, chunks = p.terms * at.count;
+            int next[kPieces];
+            auto ask = [&](int c) {   // of a chunk, in front of the one at work
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    const int64_t m = static_cast<int64_t>(at.first + c % at.count) * kTokens + row + i * (kTokens / kPieces);
+                    next[i] = m < p.tokens && k < p.inner ? p.exponents[m * groups + k / kGroup] : 0;
+                }
+            };
+            ask(0);
+            for (int c = 0; c < chunks; ++c, turn.step(kStages)) {
+                int exponent[kPieces];
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) exponent[i] = next[i];
+                if (c + 1 < chunks) ask(c + 1);
+                wait(&codesFull[turn.at], turn.parity);
+                const uint32_t codes = stages + turn.at * kStageBytes + 2 * kOperandBytes, values = stages + turn.at * kStageBytes + kOperandBytes;
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    const int r = row + i * (kTokens / kPieces);
+                    uint32_t w[4];
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(codes + r * kHalf + column * 16) : "memory");
+                    const uint32_t step = Convert<T>::step(exponent[i]);
+                    uint32_t v[8];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) Convert<T>::four(w[j], step, v[2 * j], v[2 * j + 1]);
+                    // two 16-byte pieces of the row; the columns of the second block store theirs the other way round, which keeps a row's eight threads apart in the banks
+                    const int block = column >> 2, piece = (column & 3) * 2;
+                    const uint32_t base = values + block * kBlockBytes + r * 128;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const bool second = (half ^ block) != 0;
+                        const uint32_t to = base + (((piece + (second ? 1 : 0)) ^ (r & 7)) << 4);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(second ? v[4] : v[0]), "r"(second ? v[5] : v[1]), "r"(second ? v[6] : v[2]),
+                                     "r"(second ? v[7] : v[3])
+                                     : "memory");
+                    }
+                }
+                asm volatile("fence.proxy.async;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) arriveRemote(cluster::remote(smemAddr(&converted[turn.at]), 0));
+            }
+        }
+    } else {   // stores
+        const int quarter = warp & 3;
+        int done = 0;
+        for (int64_t item = blockIdx.x / 2; item < items; item += pairs, ++done) {
+            const Place at = place(item);
+            const uint32_t buf = done & 1;
+            const int n = at.n0 + rank * kHalf + 32 * quarter + lane, count = min(kTile, p.inner - at.k0);
+            OUT *to = nullptr;
+            if constexpr (std::is_same_v<OUT, float>) to = p.parts > 1 ? p.partial + static_cast<int64_t>(at.part) * p.outer * p.inner : static_cast<float *>(p.out);
+            else to = static_cast<OUT *>(p.out);
+            to += static_cast<int64_t>(n) * p.inner + at.k0;
+            constexpr int kPer = 16 / sizeof(OUT);
+            const bool wide = p.inner % kPer == 0 && reinterpret_cast<uintptr_t>(to) % 16 == 0;
+            wait(&accFull[buf], (done >> 1) & 1);
+            fenceAfter();
+            const uint32_t from = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + buf * kTile;
+#pragma unroll 1
+            for (int col = 0; col < kTile; col += 32) {
+                uint32_t acc[32];
+                __syncwarp();
+                loadTmem32(from + col, acc);
+                loadsDone();
+                if (col + 32 == kTile) {
+                    fenceBefore();
+                    __syncwarp();
+                    if (lane == 0) arriveRemote(cluster::remote(smemAddr(&accFree[buf]), 0));
+                }
+                if (!alive || n >= p.outer) continue;
+                if (wide) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += kPer) {
+                        if (col + j >= count) break;
+                        Pack<OUT, kPer> pack;
+#pragma unroll
+                        for (int i = 0; i < kPer; ++i) pack.v[i] = fromFloat<OUT>(__uint_as_float(acc[j + i]));
+                        *reinterpret_cast<Pack<OUT, kPer> *>(to + col + j) = pack;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (col + j < count) to[col + j] = fromFloat<OUT>(__uint_as_float(acc[j]));
+                }
+            }
+        }
+    }
+    if (!alive && lane == 0) atomicExch(status, 1);
+    fenceBefore();
+    __syncthreads();
+    cluster::barrierAll();
+    if (warp == 0) freeTmem<2>(tmem, 512);
+}
+
+// dy in rows that TMA can copy, [term][token][pitch]: a copy of 16-bit elements, or the three runs of eight bits of a float, from the top.
+template <class T, int TERMS>
+__global__ void __launch_bounds__(256) layGradient(const T *dy, int64_t dyPitch, int64_t tokens, int outer, uint16_t *to, int pitch) {
+    const int n = (blockIdx.x * 256 + threadIdx.x) * 2;
+    waitForPredecessor();
+    letDependentsStart();
+    if (n >= outer) return;
+    for (int64_t m = blockIdx.y; m < tokens; m += gridDim.y) {
+        uint32_t out[TERMS] = {};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (n + i >= outer) break;
+            if constexpr (TERMS == 1) {
+                out[0] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(dy + m * dyPitch + n + i)) << (16 * i);
+            } else {
+                float left = dy[m * dyPitch + n + i];
+                const bool finite = (__float_as_uint(left) & 0x7f800000u) != 0x7f800000u;
+                if (isnan(left)) left = __int_as_float(0x7fc00000);   // whose upper half is one, too
+#pragma unroll
+                for (int t = 0; t < TERMS; ++t) {
+                    const uint32_t top = __float_as_uint(left) & 0xffff0000u;
+                    out[t] |= (top >> 16) << (16 * i);
+                    left = finite ? left - __uint_as_float(top) : 0.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) *reinterpret_cast<uint32_t *>(to + (static_cast<int64_t>(t) * tokens + m) * pitch + n) = out[t];
+    }
+}
+
+// The parts' sums, in their order.
+template <class OUT, int W>
+__global__ void __launch_bounds__(256) sumParts(const float *partial, int parts, int64_t total, OUT *out) {
+    waitForPredecessor();
+    letDependentsStart();
+    for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * W; i < total; i += static_cast<int64_t>(gridDim.x) * 256 * W) {
+        float sum[W] = {};
+        for (int part = 0; part < parts; ++part) {
+            const Pack<float, W> v = *reinterpret_cast<const Pack<float, W> *>(partial + part * total + i);
+#pragma unroll
+            for (int j = 0; j < W; ++j) sum[j] += v.v[j];
+        }
+        Pack<OUT, W> r;
+#pragma unroll
+        for (int j = 0; j < W; ++j) r.v[j] = fromFloat<OUT>(sum[j]);
+        *reinterpret_cast<Pack<OUT, W> *>(out + i) = r;
+    }
+}
+
+CUtensorMap mapOf(CUtensorMapDataType type, int rank, const void *data, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box, CUtensorMapSwizzle swizzle) {
+    CUtensorMap map;
+    const cuuint32_t steps[3] = {1, 1, 1};
+    const CUresult rc = encodeTiled()(&map, type, rank, const_cast<void *>(data), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) fail(RXMET_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", static_cast<int>(rc));
+    return map;
+}
+
+// How a call is laid out: whether dy is copied, and into how many parts the tokens are cut.
+struct Plan {
+    int terms, pitch, parts, chunks;
+    bool copied;
+};
+// The least of these estimates, in microseconds: 0.3 for a chunk, 3 to begin and end a tile, and for several parts 2.5 and the writing and reading of their sums.
+Plan planOf(int64_t tokens, int inner, int outer, int type, const void *dy, int64_t dyPitch) {
+    Plan plan;
+    plan.terms = type == RXMET_TYPE_F32 ? 3 : 1;
+    plan.copied = plan.terms > 1 || !alignedTo(dy, 16) || (tokens > 1 && (dyPitch % 8 != 0 || dyPitch < outer));
+    plan.pitch = static_cast<int>(alignUp(outer, 8));
+    plan.chunks = static_cast<int>((tokens + kTokens - 1) / kTokens);
+    const int pairs = std::max(1, currentDevice().sms / 2);
+    const int64_t tiles = static_cast<int64_t>((outer + kTile - 1) / kTile) * ((inner + kTile - 1) / kTile);
+    double best = 0;
+    plan.parts = 1;
+    for (int q = 1; q <= std::min(plan.chunks, pairs); ++q) {
+        const double rounds = static_cast<double>((tiles * q + pairs - 1) / pairs), chunks = (plan.chunks + q - 1) / q * plan.terms;
+        const double time = rounds * (0.3 * chunks + 3.0) + (q > 1 ? 2.5 + 8e-6 / 5 * q * outer * inner : 0.0);
+        if (q == 1 || time < best) {
+            best = time;
+            plan.parts = q;
+        }
+    }
+    return plan;
+}
+template <class W>
+void takeBuffers(W &&ws, const Plan &plan, int64_t tokens, int inner, int outer, uint16_t **laid, float **partial) {
+    const size_t terms = plan.copied ? static_cast<size_t>(plan.terms) * tokens * plan.pitch : 0, sums = plan.parts > 1 ? static_cast<size_t>(plan.parts) * outer * inner : 0;
+    if constexpr (std::is_same_v<std::decay_t<W>, WorkspaceSizer>) {
+        if (terms) ws.template take<uint16_t>(terms);
+        if (sums) ws.template take<float>(sums);
+    } else {
+        if (terms) *laid = ws.template take<uint16_t>(terms);
+        if (sums) *partial = ws.template take<float>(sums);
+    }
+}
+
+void requireSizes(int64_t tokens, int inner, int outer, int type) {
+    RXMET_REQUIRE(tokens >= 0 && inner >= 1 && outer >= 1, "kept_weight_gradient: %lld tokens, inner %d, outer %d", static_cast<long long>(tokens), inner, outer);
+    RXMET_REQUIRE(type == RXMET_TYPE_F32 || type == RXMET_TYPE_BF16 || type == RXMET_TYPE_F16, "kept_weight_gradient: unknown element type %d", type);
+    if (tokens > (1 << 30) || outer > (1 << 30) || inner > 131071)
+        fail(RXMET_ERR_UNSUPPORTED, "kept_weight_gradient: %lld tokens, inner %d, outer %d, at most %d, 131071 and %d", static_cast<long long>(tokens), inner, outer, 1 << 30, 1 << 30);
+}
+
+template <class T, class OUT>
+void launchProduct(const Problem &p, const CUtensorMap &dy, const CUtensorMap &codes, cudaStream_t st) {
+    const auto kernel = keptWeightGradient<T, OUT>;
+    ensureDynamicSmem(reinterpret_cast<const void *>(kernel), kShared);
+    const int64_t items = static_cast<int64_t>((p.outer + kTile - 1) / kTile) * ((p.inner + kTile - 1) / kTile) * p.parts;
+    {
+        KernelTimer timer__("keptWeightGradient", st);
+        launchDependent(kernel, 2 * static_cast<unsigned>(std::min<int64_t>(currentDevice().sms / 2, items)), kThreads, kShared, st, p, dy, codes, waitStatus());
+    }
+    afterLaunch("keptWeightGradient");
+}
+
+}  // namespace
+}  // namespace kept
+}  // namespace rxmet
+
+using namespace rxmet;
+
+extern "C" size_t rxmet_kept_weight_gradient_workspace_bytes(int64_t tokens, int inner, int outer, int type, const void *dy, int64_t dy_pitch) {
+    WorkspaceSizer sizer;
+    guarded([&] {
+        kept::requireSizes(tokens, inner, outer, type);
+        kept::takeBuffers(sizer, kept::planOf(tokens, inner, outer, type, dy, dy_pitch), tokens, inner, outer, nullptr, nullptr);
+    });
+    return sizer.used();
+}
+
+extern "C" int rxmet_kept_weight_gradient(int64_t tokens, int inner, int outer, int type, const void *dy, int64_t dy_pitch, const int8_t *codes, int64_t codes_pitch,
+                                          const int8_t *exponents, int out_type, void *out, void *workspace, size_t workspace_bytes, void *stream) {
+    return guarded([&] {
+        kept::requireSizes(tokens, inner, outer, type);
+        RXMET_REQUIRE(out, "kept_weight_gradient: null pointer");
+        const auto st = static_cast<cudaStream_t>(stream);
+        const int64_t total = static_cast<int64_t>(outer) * inner;
+        if (tokens == 0) {
+            RXMET_CUDA(cudaMemsetAsync(out, 0, total * typeBytes(out_type), st));
+            return;
+        }
+        RXMET_REQUIRE(dy && codes && exponents, "kept_weight_gradient: null pointer");
+        RXMET_REQUIRE(alignedTo(codes, 16) && codes_pitch % 16 == 0 && (tokens == 1 || codes_pitch >= inner), "kept_weight_gradient: rows of codes must start on 16 bytes, and apart");
+        if (encodeTiled() == nullptr) fail(RXMET_ERR_CUDA, "kept_weight_gradient: the driver encodes no tensor maps");
+        bindContext();
+        const kept::Plan plan = kept::planOf(tokens, inner, outer, type, dy, dy_pitch);
+        kept::Problem p{tokens, inner, outer, plan.terms, plan.parts, plan.chunks, exponents, out, nullptr};
+        uint16_t *laid = nullptr;
+        kept::takeBuffers(Workspace(workspace, workspace_bytes), plan, tokens, inner, outer, &laid, &p.partial);
+        if (plan.copied) {
+            const dim3 grid((outer + 511) / 512, static_cast<unsigned>(std::min<int64_t>(tokens, std::max(1, 16 * currentDevice().sms / ((outer + 511) / 512)))));
+            {
+                KernelTimer timer__("layGradient", st);
+                if (type == RXMET_TYPE_F32) launchDependent(kept::layGradient<float, 3>, grid, 256, 0, st, static_cast<const float *>(dy), dy_pitch, tokens, outer, laid, plan.pitch);
+                else launchDependent(kept::layGradient<__half, 1>, grid, 256, 0, st, static_cast<const __half *>(dy), dy_pitch, tokens, outer, laid, plan.pitch);
+            }
+            afterLaunch("layGradient");
+        }
+        const void *from = plan.copied ? laid : dy;
+        const cuuint64_t pitch = 2 * static_cast<cuuint64_t>(plan.copied ? plan.pitch : tokens == 1 ? plan.pitch : dy_pitch);
+        const cuuint64_t dyDims[3] = {static_cast<cuuint64_t>(outer), static_cast<cuuint64_t>(tokens), static_cast<cuuint64_t>(plan.terms)}, dyStrides[2] = {pitch, pitch * tokens};
+        const cuuint32_t dyBox[3] = {kept::kBlock, kept::kTokens, 1};
+        const CUtensorMap dyMap = kept::mapOf(type == RXMET_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, from, dyDims, dyStrides, dyBox, CU_TENSOR_MAP_SWIZZLE_128B);
+        const cuuint64_t codeDims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(tokens)}, codeStrides[1] = {static_cast<cuuint64_t>(tokens == 1 ? alignUp(inner, 16) : codes_pitch)};
+        const cuuint32_t codeBox[2] = {kept::kHalf, kept::kTokens};
+        const CUtensorMap codeMap = kept::mapOf(CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, codeDims, codeStrides, codeBox, CU_TENSOR_MAP_SWIZZLE_NONE);
+        withType(out_type, [&](auto o) {
+            using OUT = decltype(o);
+            if (p.parts > 1) {
+                if (type == RXMET_TYPE_F16) kept::launchProduct<__half, float>(p, dyMap, codeMap, st);
+                else kept::launchProduct<__nv_bfloat16, float>(p, dyMap, codeMap, st);
+                const bool wide = total % 4 == 0 && alignedTo(out, 4 * sizeof(OUT));
+                const int64_t blocks = (total / (wide ? 4 : 1) + 255) / 256;
+                {
+                    KernelTimer timer__("sumParts", st);
+                    launchDependent(wide ? kept::sumParts<OUT, 4> : kept::sumParts<OUT, 1>, static_cast<unsigned>(std::min<int64_t>(blocks, 8 * currentDevice().sms)), 256, 0, st,
+                                    static_cast<const float *>(p.partial), p.parts, total, static_cast<OUT *>(out));
+                }
+                afterLaunch("sumParts");
+            } else if (type == RXMET_TYPE_F16) {
+                kept::launchProduct<__half, OUT>(p, dyMap, codeMap, st);
+            } else {
+                kept::launchProduct<__nv_bfloat16, OUT>(p, dyMap, codeMap, st);
+            }
+        });
+    });
+}

@@ -1,0 +1,86 @@
+"""Training with activations kept in 8 bits: what the backward pass needs of an activation is held as codes, at a half or a quarter of its size.
+
+A group is 32 neighbouring elements of a row (fewer at its end) with one power of two: value = code * 2^exponent, code in [-127, 127], by the least exponent that
+reaches the group's largest magnitude.  `keep` makes codes and `values` gives back what they stand for.  `gated_product` and `linear` are layers that keep codes
+between their forward and their backward pass; `weight_gradient` is the gradient of a weight from codes, a product of a layer's own
+kernel.  float32, bfloat16 and float16 CUDA tensors with any leading dimensions, rows of up to 131071 elements.  The gradients are those of the formulas at the values that the codes
+stand for; forward results are of the activations themselves.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+import torch.nn.functional as F
+
+from . import _cabi as cabi
+from .coded_linear import ACTIVATIONS, _TYPES
+
+#: elements of a row that share an exponent
+GROUP = 32
+
+
+class KeptCodes(NamedTuple):
+    """An activation [..., width] as int8 codes (rows that start at multiples of 16 bytes; others are copied where they are used), int8 exponents [..., groups of 32], and its type."""
+    codes: torch.Tensor
+    exponents: torch.Tensor
+    dtype: torch.dtype
+
+
+def _type(dtype: torch.dtype, what: str) -> int:
+    if dtype not in _TYPES:
+        raise RuntimeError(f"{what}: type {dtype}, one of float32, bfloat16, float16")
+    return _TYPES[dtype]
+
+
+def keep(x: torch.Tensor) -> KeptCodes:
+    """Codes of x, nearest, ties to even.  Exponents are at least -126 (float16: -24, so that all values are numbers of float16, too).  A group with an infinity or
+    a NaN has the exponent 127 and stands for NaN.  No gradient."""
+    return KeptCodes(*cabi.load_binding().keep_codes(x.detach()), x.dtype)
+
+
+def values(kept: KeptCodes) -> torch.Tensor:
+    """What the codes stand for, in the type that was kept; exact but where that type's smallest numbers end."""
+    return cabi.load_binding().kept_values(kept.codes, kept.exponents, _type(kept.dtype, "values"))
+
+
+def gated_product(gate: torch.Tensor, up: torch.Tensor, *, activation: str = "silu") -> torch.Tensor:
+    """activation(gate) * up, of one shape and type; activations as of `coded_linear`.  Differentiable in both, once, with gate and up kept as codes in between:
+    dgate = dy * up * activation'(gate), dup = dy * activation(gate) at the values of the codes.  Not under a trace."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"gated_product: activation {activation!r}, one of {', '.join(ACTIVATIONS)}")
+    return cabi.load_binding().gated_product(gate, up, ACTIVATIONS[activation])
+
+
+def weight_gradient(dy: torch.Tensor, kept: KeptCodes, *, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """[outer, inner] = sum over all rows of dy [..., outer] times the values of kept [..., inner], in `dtype` (that of dy unless given).  dy is of the type that was
+    kept.  Products are exact, sums in 32 bits in a fixed order.  No gradient."""
+    return cabi.load_binding().kept_weight_gradient(dy.detach(), kept.codes, kept.exponents, _type(kept.dtype, "weight_gradient"),
+                                                    _type(dtype or dy.dtype, "weight_gradient"))
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        kept = keep(x) if ctx.needs_input_grad[1] else None
+        ctx.dtype, ctx.biased = x.dtype, bias is not None and ctx.needs_input_grad[2]
+        ctx.save_for_backward(weight if ctx.needs_input_grad[0] else None, *(kept[:2] if kept is not None else (None, None)))
+        with torch.autocast("cuda", enabled=False):
+            return F.linear(x, weight, bias)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        weight, codes, exponents = ctx.saved_tensors
+        dx = None if weight is None else dy @ weight
+        dweight = None if codes is None else weight_gradient(dy, KeptCodes(codes, exponents, ctx.dtype))
+        return dx, dweight, dy.flatten(0, -2).sum(dim=0) if ctx.biased else None
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x @ weight.T + bias, of one type, with x kept as codes for the gradient of the weight.  The products with the weight itself are torch's.  Differentiable, once."""
+    if not x.is_cuda:
+        raise RuntimeError("linear: x must be a CUDA tensor")
+    if weight.dim() != 2 or x.dim() < 2 or any(t.dtype != x.dtype for t in (weight, bias) if t is not None):
+        raise RuntimeError("linear takes x of two dimensions or more, a weight [outer, inner] and a bias [outer], all of one type")
+    return _Linear.apply(x, weight, bias)

@@ -61,3 +61,41 @@ def recur_gradients(forget, value, input, activation, state, lengths, dout, dfin
     grads.append(None if input is None else (G * c * z * rest, z * rest * c.abs() * (GE + 4 * GATE * GM)))
     grads.append((R, E))
     return grads
+
+
+GROUP = 32
+LOWEST = {torch.float32: -126, torch.bfloat16: -126, torch.float16: -24}
+
+
+def keep(x):
+    """(codes, exponents) of rows [.., width]; a group that is not finite has the exponent 127 and codes 0."""
+    lowest, x = LOWEST[x.dtype], x.double()
+    width = x.shape[-1]
+    parts = torch.nn.functional.pad(x, (0, -width % GROUP)).unflatten(-1, (-1, GROUP))
+    bad = ~torch.isfinite(parts).all(dim=-1)
+    parts = torch.where(bad[..., None], torch.zeros_like(parts), parts)
+    most = parts.abs().amax(dim=-1)
+    exponents = torch.full_like(most, lowest)
+    for e in range(lowest, 128):   # the least that reaches the largest magnitude
+        exponents = torch.where(most > 127 * 2.0 ** e, torch.full_like(most, e + 1), exponents)
+    codes = torch.round(parts / torch.exp2(exponents)[..., None])
+    return codes.to(torch.int8).flatten(-2)[..., :width], torch.where(bad, torch.full_like(exponents, 127), exponents).to(torch.int8)
+
+
+def values(codes, exponents):
+    power = torch.where(exponents == 127, torch.full_like(exponents, 0, dtype=torch.float64) * float("nan"), torch.exp2(exponents.double()))
+    return codes.double() * power.repeat_interleave(GROUP, dim=-1)[..., :codes.shape[-1]]
+
+
+def curve(x, activation):
+    """(value, slope, bounds of both): of an activation in 64 bits, and what 32 bits leave."""
+    unit = 2.0 ** -23
+    if activation == "relu":
+        return torch.relu(x), (x > 0).double(), 0 * x, 0 * x
+    if activation == "silu":
+        s, rest = torch.sigmoid(x), torch.sigmoid(-x)
+        return x * s, s + x * s * rest, (x * s).abs() * (GATE + unit), (s + (x * s * rest).abs()) * (2 * GATE + 2 * unit)
+    if activation == "gelu":   # five units for the distribution, two for an exponential whose argument is off by a unit of it
+        p, d = 0.5 * torch.special.erfc(-x * 0.5 ** 0.5), torch.exp(-x * x / 2) * (2 * torch.pi) ** -0.5
+        return x * p, p + x * d, (x * p).abs() * 6 * unit, (6 * p + (x * d).abs() * (5 + x * x)) * unit
+    return x, torch.ones_like(x), 0 * x, 0 * x

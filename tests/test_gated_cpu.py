@@ -40,3 +40,44 @@ def test_tensors_off_the_gpu_are_refused():
             call()
     with pytest.raises(ValueError, match="activation"):
         gated_recurrence.gated_recurrence(x, x, activation="relu")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_plain_codes(dtype):
+    """No value is off by more than half a step, no smaller step would do, and values survive being kept again."""
+    g = torch.Generator().manual_seed(1)
+    x = (torch.randn(6, 100, generator=g) * torch.tensor([1.0, 1e-3, 300.0, 1.0, 0.0, 1.0])[:, None]).to(dtype)
+    x[3, 40] = float("inf")
+    codes, exponents = gl.keep(x)
+    step = torch.exp2(exponents.double()).repeat_interleave(32, dim=1)[:, :100]
+    fine = exponents.repeat_interleave(32, dim=1)[:, :100] != 127
+    got = gl.values(codes, exponents)
+    assert bool(((got - x.double()).abs() <= step / 2)[fine].all()) and torch.isnan(got[3, 32:64]).all() and not torch.isnan(got[3, :32]).any()
+    most = codes.abs().int()
+    for row in (0, 1, 2, 5):
+        for group in range(3):
+            assert 64 <= int(most[row, 32 * group:32 * group + 32].max()) <= 127
+    again = gl.keep(got[:3].to(dtype))
+    assert torch.equal(gl.values(*again), got[:3])
+
+
+@pytest.mark.parametrize("activation", ["none", "relu", "silu", "gelu"])
+def test_slopes_of_the_plain_activations(activation):
+    x = torch.linspace(-9, 9, 301, dtype=torch.float64).requires_grad_()
+    value, slope, *_ = gl.curve(x, activation)
+    want, = torch.autograd.grad(value.sum(), x)
+    assert torch.allclose(slope, want, rtol=1e-12, atol=1e-14)
+
+
+def test_kept_codes_refuse_what_needs_no_gpu():
+    from rx_met_b200 import kept_codes
+    x = torch.zeros(4, 32)
+    kept = kept_codes.KeptCodes(x.to(torch.int8), torch.zeros(4, 1, dtype=torch.int8), torch.float32)
+    for call in (lambda: kept_codes.keep(x), lambda: kept_codes.values(kept), lambda: kept_codes.gated_product(x, x), lambda: kept_codes.weight_gradient(x, kept),
+                 lambda: kept_codes.linear(x, x)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+    with pytest.raises(ValueError, match="activation"):
+        kept_codes.gated_product(x, x, activation="tanh")
+    with pytest.raises(RuntimeError, match="type"):
+        kept_codes.values(kept._replace(dtype=torch.float64))

@@ -4,8 +4,7 @@
 // On tcgen05 kind::f16 with 32-bit sums in tensor memory.  A code times its power of two is a number of bfloat16 and of half, so that one product a term is exact; dy in 32 bits comes as
 // its three runs of eight bits, each a number of bfloat16.
 // A pair of CTAs computes tiles of 256 output channels x 256 input channels, 64 tokens at a time; each CTA holds half of both operands.  dy arrives by TMA in the order in which
-// the tensor cores read it across its rows.  The codes arrive as bytes, and eight warps turn them into 16-bit values in that order: ten instructions for four codes, 160 of a
-// chunk's 512 cycles.  Four warps store a tile while the next one is summed, two accumulators in turn.
+// the tensor cores read it across its rows.  Eight warps load the codes, a few chunks ahead, and turn them into 16-bit values in that order: ten instructions for four codes.  Four warps store a tile while the next one is summed, two accumulators in turn.
 // Few tiles leave SMs without work, so the tokens are cut into parts, whose sums another kernel adds up in their order.
 #include "kept_codes.cuh"
 
@@ -19,17 +18,18 @@ namespace {
 using namespace ummatiles;
 
 constexpr int kTile = 256, kHalf = kTile / 2, kTokens = 64, kBlock = 64;   // kBlock: 16-bit elements of a swizzled row
-constexpr int kStages = 5, kConvertWarps = 8, kStoreWarps = 4;
+constexpr int kStages = 7, kConvertWarps = 16, kTeams = 4, kStoreWarps = 4;   // teams of converting warps take chunks in turn
 constexpr int kThreads = 32 * (kConvertWarps + kStoreWarps + 2);
-constexpr uint32_t kBlockBytes = kTokens * kBlock * 2, kOperandBytes = kHalf / kBlock * kBlockBytes, kCodeBytes = kTokens * kHalf;
-constexpr uint32_t kStageBytes = 2 * kOperandBytes + kCodeBytes;
+constexpr uint32_t kBlockBytes = kTokens * kBlock * 2, kOperandBytes = kHalf / kBlock * kBlockBytes;
+constexpr uint32_t kStageBytes = 2 * kOperandBytes;
 constexpr uint32_t kShared = 231936;   // cluster::leastShared(512): one CTA an SM
 static_assert(kStages * kStageBytes + 1024 <= kShared, "the stages fit");
 
 struct Problem {
     int64_t tokens;
     int inner, outer, terms, parts, chunks;   // chunks: of one term
-    const int8_t *exponents;
+    const int8_t *codes, *exponents;
+    int64_t codesPitch;
     void *out;
     float *partial;   // [parts][outer][inner] where there are several
 };
@@ -47,19 +47,9 @@ __device__ __forceinline__ void copyTile3Pair(uint32_t to, const CUtensorMap *ma
                  "r"(bar & 0xfeffffffu)
                  : "memory");
 }
-// As waitSuspended, for arrivals from both CTAs of the pair.
-__device__ __forceinline__ bool waitPair(uint32_t bar, uint32_t parity) {
-    for (uint32_t i = 0; i < kSuspendLimit; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
-            : "=r"(done)
-            : "r"(bar), "r"(parity), "r"(kSuspendNs)
-            : "memory");
-        if (done) return true;
-    }
-    return false;
-}
+// At the pair's first CTA.  What was written is visible to the tensor cores by the fence in front; the arrival itself orders nothing beyond this CTA (released to the cluster it makes every
+// warp wait for all that it has in flight).
+__device__ __forceinline__ void arrivePair(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster::remote(bar, 0)) : "memory"); }
 
 // Four codes in words of two 16-bit values each, times a power of two in both halves of `step`.
 template <class T>
@@ -103,9 +93,9 @@ struct Convert<__half> {
 // T: the products' type; OUT: that of what is stored (parts: floats).
 template <class T, class OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    keptWeightGradient(const __grid_constant__ Problem p, const __grid_constant__ CUtensorMap dyMap, const __grid_constant__ CUtensorMap codeMap, int *status) {
+    keptWeightGradient(const __grid_constant__ Problem p, const __grid_constant__ CUtensorMap dyMap, int *status) {
     extern __shared__ uint8_t raw[];
-    __shared__ __align__(8) uint64_t dyFull[kStages], codesFull[kStages], converted[kStages], freed[kStages], accFull[2], accFree[2];
+    __shared__ __align__(8) uint64_t dyFull[kStages], converted[kStages], freed[kStages], accFull[2], accFree[2];
     __shared__ uint32_t tmemSlot;
     const uint32_t stages = (smemAddr(raw) + 1023u) & ~1023u;
     const int warp = warpIndex(), lane = threadIdx.x & 31;
@@ -113,8 +103,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) {
             cluster::initBarrier(&dyFull[i], 1);
-            cluster::initBarrier(&codesFull[i], 1);
-            cluster::initBarrier(&converted[i], 2 * kConvertWarps);
+            cluster::initBarrier(&converted[i], 2 * kConvertWarps / kTeams);
             cluster::initBarrier(&freed[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -123,7 +112,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         prefetchMap(&dyMap);
-        prefetchMap(&codeMap);
     }
     if (warp == 0) allocTmem<2>(smemAddr(&tmemSlot), 512);
     fenceBefore();
@@ -166,12 +154,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (turn.again) wait(&freed[turn.at], turn.parity ^ 1u);
                     if (alive && electOne()) {
                         const uint32_t to = stages + turn.at * kStageBytes, m = (at.first + c) * kTokens;
-                        const uint32_t dyBar = smemAddr(&dyFull[turn.at]), codeBar = smemAddr(&codesFull[turn.at]);
-                        if (rank == 0) cluster::arriveExpect(dyBar, 2 * kOperandBytes);
-                        for (int block = 0; block < kHalf / kBlock; ++block)
-                            copyTile3Pair(to + block * kBlockBytes, &dyMap, at.n0 + rank * kHalf + block * kBlock, m, term, dyBar);
-                        cluster::arriveExpect(codeBar, kCodeBytes);
-                        copyTile2(to + 2 * kOperandBytes, &codeMap, at.k0 + rank * kHalf, m, codeBar);
+                        const uint32_t bar = smemAddr(&dyFull[turn.at]);
+                        if (rank == 0) cluster::arriveExpect(bar, 2 * kOperandBytes);
+                        for (int block = 0; block < kHalf / kBlock; ++block) copyTile3Pair(to + block * kBlockBytes, &dyMap, at.n0 + rank * kHalf + block * kBlock, m, term, bar);
                     }
                     __syncwarp();
                 }
@@ -192,7 +177,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int chunks = p.terms * at.count;
                 for (int c = 0; c < chunks; ++c, turn.step(kStages)) {
                     wait(&dyFull[turn.at], turn.parity);
-                    if (alive) alive = __all_sync(0xffffffffu, waitPair(smemAddr(&converted[turn.at]), turn.parity));
+                    wait(&converted[turn.at], turn.parity);
                     if (alive && electOne()) {
                         fenceAfter();
                         const uint32_t from = stages + turn.at * kStageBytes;
@@ -206,54 +191,76 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
             }
         }
-    } else if (warp < kConvertWarps) {   // codes to values: a thread takes sixteen codes of a token, twice a chunk
-        constexpr int kPieces = kTokens * kHalf / 16 / (32 * kConvertWarps);
-        const int column = threadIdx.x & 7, row = threadIdx.x >> 3;   // of sixteen codes; of tokens, 32 apart from piece to piece
-        const int groups = groupsOf(p.inner);
+    } else if (warp < kConvertWarps) {   // codes to values: a thread takes sixteen codes of a token at a time; teams take chunks in turn
+        constexpr int kThreadsOfTeam = 32 * kConvertWarps / kTeams, kRows = kThreadsOfTeam / 8, kPieces = kTokens / kRows;
+        // Eight neighbouring lanes store two rows of a block at once: the swizzle keeps an even row and the odd one behind it apart in the banks.
+        const int team = threadIdx.x / kThreadsOfTeam, index = threadIdx.x % kThreadsOfTeam;
+        const int column = index & 3, block = (index >> 3) & 1, row = ((index >> 2) & 1) + 2 * (index >> 4);
+        const int inRow = block * kBlock + column * 16, groups = groupsOf(p.inner);
+        const uint32_t place0 = kOperandBytes + block * kBlockBytes;
+        int64_t seen = 0;   // chunks of the tiles so far
         Turn turn;
+        turn.step(kStages, team);
         for (int64_t item = blockIdx.x / 2; item < items; item += pairs) {
             const Place at = place(item);
-            const int k = at.k0 + rank * kHalf + column * 16, chunks = p.terms * at.count;
-            int next[kPieces];
-            auto ask = [&](int c) {   // of a chunk, in front of the one at work
-#pragma unroll
-                for (int i = 0; i < kPieces; ++i) {
-                    const int64_t m = static_cast<int64_t>(at.first + c % at.count) * kTokens + row + i * (kTokens / kPieces);
-                    next[i] = m < p.tokens && k < p.inner ? p.exponents[m * groups + k / kGroup] : 0;
-                }
+            const int k = at.k0 + rank * kHalf + inRow, real = p.inner - k, chunks = p.terms * at.count;
+            const int begin = static_cast<int>((team + kTeams - seen % kTeams) % kTeams);
+            seen += chunks;
+            if (begin >= chunks) continue;
+            uint4 codes[kPieces];
+            int exponents[kPieces];
+            int chunk = begin % at.count;   // of the tokens, for what is asked for next
+            const int8_t *codesAt, *exponentsAt;
+            int left;                       // of its tokens, those that there are
+            auto turnTo = [&] {
+                const int64_t m = static_cast<int64_t>(at.first + chunk) * kTokens + row;
+                codesAt = p.codes + m * p.codesPitch + k;
+                exponentsAt = p.exponents + m * groups + k / kGroup;
+                left = real > 0 ? static_cast<int>(min(static_cast<int64_t>(kTokens), p.tokens - m)) : 0;
             };
-            ask(0);
-            for (int c = 0; c < chunks; ++c, turn.step(kStages)) {
-                int exponent[kPieces];
+            auto ask = [&](int i) {
+                codes[i] = make_uint4(0, 0, 0, 0);
+                exponents[i] = 0;
+                if (i * kRows < left) {
+                    codes[i] = __ldg(reinterpret_cast<const uint4 *>(codesAt));
+                    exponents[i] = __ldg(exponentsAt);
+                }
+                codesAt += kRows * p.codesPitch;
+                exponentsAt += kRows * groups;
+            };
+            turnTo();
 #pragma unroll
-                for (int i = 0; i < kPieces; ++i) exponent[i] = next[i];
-                if (c + 1 < chunks) ask(c + 1);
-                wait(&codesFull[turn.at], turn.parity);
-                const uint32_t codes = stages + turn.at * kStageBytes + 2 * kOperandBytes, values = stages + turn.at * kStageBytes + kOperandBytes;
+            for (int i = 0; i < kPieces; ++i) ask(i);
+            for (int c = begin; c < chunks; c += kTeams, turn.step(kStages, kTeams)) {
+                if (turn.again) wait(&freed[turn.at], turn.parity ^ 1u);
+                const uint32_t values = stages + turn.at * kStageBytes + place0 + row * 128;
+                for (chunk += kTeams; chunk >= at.count;) chunk -= at.count;
+                turnTo();
+                if (c + kTeams >= chunks) left = 0;
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) {
-                    const int r = row + i * (kTokens / kPieces);
-                    uint32_t w[4];
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(codes + r * kHalf + column * 16) : "memory");
-                    const uint32_t step = Convert<T>::step(exponent[i]);
-                    uint32_t v[8];
+                    const uint32_t step = Convert<T>::step(exponents[i]);
+                    uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w}, v[8];
+                    if (real < 16) {   // what lies between a row's end and the next row may be anything
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int within = min(4, max(0, real - 4 * j));
+                            w[j] = within == 4 ? w[j] : w[j] & ((1u << (8 * within)) - 1);
+                        }
+                    }
+                    ask(i);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) Convert<T>::four(w[j], step, v[2 * j], v[2 * j + 1]);
-                    // two 16-byte pieces of the row; the columns of the second block store theirs the other way round, which keeps a row's eight threads apart in the banks
-                    const int block = column >> 2, piece = (column & 3) * 2;
-                    const uint32_t base = values + block * kBlockBytes + r * 128;
+                    // rows of a thread are kRows apart, a multiple of eight: one swizzle for all
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const bool second = (half ^ block) != 0;
-                        const uint32_t to = base + (((piece + (second ? 1 : 0)) ^ (r & 7)) << 4);
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(second ? v[4] : v[0]), "r"(second ? v[5] : v[1]), "r"(second ? v[6] : v[2]),
-                                     "r"(second ? v[7] : v[3])
+                    for (int half = 0; half < 2; ++half)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(values + i * kRows * 128 + (((2 * column + half) ^ (row & 7)) << 4)), "r"(v[4 * half]),
+                                     "r"(v[4 * half + 1]), "r"(v[4 * half + 2]), "r"(v[4 * half + 3])
                                      : "memory");
-                    }
                 }
-                asm volatile("fence.proxy.async;" ::: "memory");
+                fenceAsyncProxy();
                 __syncwarp();
-                if (lane == 0) arriveRemote(cluster::remote(smemAddr(&converted[turn.at]), 0));
+                if (lane == 0) arrivePair(smemAddr(&converted[turn.at]));
             }
         }
     } else {   // stores
@@ -413,13 +420,13 @@ void requireSizes(int64_t tokens, int inner, int outer, int type) {
 }
 
 template <class T, class OUT>
-void launchProduct(const Problem &p, const CUtensorMap &dy, const CUtensorMap &codes, cudaStream_t st) {
+void launchProduct(const Problem &p, const CUtensorMap &dy, cudaStream_t st) {
     const auto kernel = keptWeightGradient<T, OUT>;
     ensureDynamicSmem(reinterpret_cast<const void *>(kernel), kShared);
     const int64_t items = static_cast<int64_t>((p.outer + kTile - 1) / kTile) * ((p.inner + kTile - 1) / kTile) * p.parts;
     {
         KernelTimer timer__("keptWeightGradient", st);
-        launchDependent(kernel, 2 * static_cast<unsigned>(std::min<int64_t>(currentDevice().sms / 2, items)), kThreads, kShared, st, p, dy, codes, waitStatus());
+        launchDependent(kernel, 2 * static_cast<unsigned>(std::min<int64_t>(currentDevice().sms / 2, items)), kThreads, kShared, st, p, dy, waitStatus());
     }
     afterLaunch("keptWeightGradient");
 }
@@ -455,7 +462,8 @@ extern "C" int rxmet_kept_weight_gradient(int64_t tokens, int inner, int outer, 
         if (encodeTiled() == nullptr) fail(RXMET_ERR_CUDA, "kept_weight_gradient: the driver encodes no tensor maps");
         bindContext();
         const kept::Plan plan = kept::planOf(tokens, inner, outer, type, dy, dy_pitch);
-        kept::Problem p{tokens, inner, outer, plan.terms, plan.parts, plan.chunks, exponents, out, nullptr};
+        if (tokens == 1) codes_pitch = 0;   // the distance of a single row's next one does not matter
+        kept::Problem p{tokens, inner, outer, plan.terms, plan.parts, plan.chunks, codes, exponents, codes_pitch, out, nullptr};
         uint16_t *laid = nullptr;
         kept::takeBuffers(Workspace(workspace, workspace_bytes), plan, tokens, inner, outer, &laid, &p.partial);
         if (plan.copied) {
@@ -472,14 +480,11 @@ extern "C" int rxmet_kept_weight_gradient(int64_t tokens, int inner, int outer, 
         const cuuint64_t dyDims[3] = {static_cast<cuuint64_t>(outer), static_cast<cuuint64_t>(tokens), static_cast<cuuint64_t>(plan.terms)}, dyStrides[2] = {pitch, pitch * tokens};
         const cuuint32_t dyBox[3] = {kept::kBlock, kept::kTokens, 1};
         const CUtensorMap dyMap = kept::mapOf(type == RXMET_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, from, dyDims, dyStrides, dyBox, CU_TENSOR_MAP_SWIZZLE_128B);
-        const cuuint64_t codeDims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(tokens)}, codeStrides[1] = {static_cast<cuuint64_t>(tokens == 1 ? alignUp(inner, 16) : codes_pitch)};
-        const cuuint32_t codeBox[2] = {kept::kHalf, kept::kTokens};
-        const CUtensorMap codeMap = kept::mapOf(CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, codeDims, codeStrides, codeBox, CU_TENSOR_MAP_SWIZZLE_NONE);
         withType(out_type, [&](auto o) {
             using OUT = decltype(o);
             if (p.parts > 1) {
-                if (type == RXMET_TYPE_F16) kept::launchProduct<__half, float>(p, dyMap, codeMap, st);
-                else kept::launchProduct<__nv_bfloat16, float>(p, dyMap, codeMap, st);
+                if (type == RXMET_TYPE_F16) kept::launchProduct<__half, float>(p, dyMap, st);
+                else kept::launchProduct<__nv_bfloat16, float>(p, dyMap, st);
                 const bool wide = total % 4 == 0 && alignedTo(out, 4 * sizeof(OUT));
                 const int64_t blocks = (total / (wide ? 4 : 1) + 255) / 256;
                 {
@@ -489,9 +494,9 @@ extern "C" int rxmet_kept_weight_gradient(int64_t tokens, int inner, int outer, 
                 }
                 afterLaunch("sumParts");
             } else if (type == RXMET_TYPE_F16) {
-                kept::launchProduct<__half, OUT>(p, dyMap, codeMap, st);
+                kept::launchProduct<__half, OUT>(p, dyMap, st);
             } else {
-                kept::launchProduct<__nv_bfloat16, OUT>(p, dyMap, codeMap, st);
+                kept::launchProduct<__nv_bfloat16, OUT>(p, dyMap, st);
             }
         });
     });

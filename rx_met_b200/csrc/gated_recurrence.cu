@@ -8,135 +8,112 @@ namespace rxmet {
 namespace gated {
 namespace {
 
-constexpr int kStages = 2;
-
-template <class T, int PIECE, bool OWN>
-__global__ void __launch_bounds__(kThreads, 2) gatedForward(const __grid_constant__ Pass p) {
-    constexpr int N = kLane<T>, kTensors = OWN ? 3 : 2;
-    extern __shared__ __align__(128) uint8_t stages[];
-    __shared__ float2 window[kWindow][32 * N], parts[kWarps][32 * N];
-    __shared__ int64_t tileOf[kStages];
-    __shared__ int nearest;
+template <class T, int PIECE, bool OWN, bool TANH>
+__global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __grid_constant__ Pass p) {
+    constexpr int S = kSteps<T, OWN>, kRow = kChannels * sizeof(T);
+    extern __shared__ __align__(128) uint8_t raw[];                                                  // the rows of the tile to come
+    ulonglong2(*const held)[kThreads] = reinterpret_cast<ulonglong2(*)[kThreads]>(raw + (OWN ? 3 : 2) * kTensorBytes<OWN>);   // (f, z c) of the one that waits for its state, each thread's own
+    __shared__ Map shared[kWarps][32];   // of the warps' tokens; of the tiles of a group
+    __shared__ Tile tiles[2];
+    __shared__ Pair front[32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     waitForPredecessor();
     letDependentsStart();
     Tickets tickets(p);
-    if (tid == 0)
-        for (int i = 0; i < kStages; ++i) tileOf[i] = tickets.take();
+    if (tid == 0) tiles[0] = tileOf<T, OWN>(p, tickets.take(), false);
     __syncthreads();
-    auto ask = [&](int stage) {
-        const int64_t index = tileOf[stage];
-        if (index < p.tiles) {
-            const Tile<T> tile(p, index, false);
-            const uint32_t to = umma::smemAddr(stages) + stage * kTensors * kTensorBytes<T>;
+    auto ask = [&](const Tile &tile) {
+        if (tile.real) {
+            const uint32_t to = umma::smemAddr(raw);
             askFor<T, PIECE>(to, p.forget, tile, p.width);
-            askFor<T, PIECE>(to + kTensorBytes<T>, p.value, tile, p.width);
-            if (OWN) askFor<T, PIECE>(to + 2 * kTensorBytes<T>, p.input, tile, p.width);
+            askFor<T, PIECE>(to + kTensorBytes<OWN>, p.value, tile, p.width);
+            if (OWN) askFor<T, PIECE>(to + 2 * kTensorBytes<OWN>, p.input, tile, p.width);
         }
         commitCopies();
     };
-    for (int i = 0; i < kStages; ++i) ask(i);
+    ask(tiles[0]);
 
-    for (int stage = 0;; stage = (stage + 1) % kStages) {
-        const int64_t index = tileOf[stage];
-        if (index >= p.tiles) break;
-        const Tile<T> tile(p, index, false);
-        int64_t later = 0;
-        if (tid == 0) later = tickets.take();
-        copiesArrived<kStages - 1>();
-        __syncthreads();
-
-        const uint8_t *from = stages + stage * kTensors * kTensorBytes<T> + (warp * kSteps * 32 + lane) * N * sizeof(T);
-        const int live = tile.live - warp * kSteps;   // of this warp's tokens
-        float a[kSteps][N], b[kSteps][N], A[N], B[N];
+    Tile waiting{};
+    Map ahead, mine;   // of the waiting tile: what lies in front of the warp's tokens, the whole tile
+    for (int turn = 0;; turn ^= 1) {
+        // the next tile's gates and its map, which nobody has to wait for ...
+        const Tile tile = tiles[turn];
+        Pair a[S], b[S];
+        Map nextAhead, nextMine;
+        if (tile.real) {
+            Tile later{};
+            if (tid == 0) later = tileOf<T, OWN>(p, tickets.take(), false);
+            copiesArrived<0>();
+            __syncthreads();
+            const uint8_t *from = raw + warp * S * kRow + lane * 2 * sizeof(T);
 #pragma unroll
-        for (int v = 0; v < N; ++v) {
-            A[v] = 1.f;
-            B[v] = 0.f;
-        }
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            float forget[N], value[N], input[N];
-            const uint8_t *row = from + s * 32 * N * sizeof(T);
-            readRow<T>(row, forget);
-            readRow<T>(row + kTensorBytes<T>, value);
-            if (OWN) readRow<T>(row + 2 * kTensorBytes<T>, input);
-#pragma unroll
-            for (int v = 0; v < N; ++v) {
-                const Gate f(forget[v]);
-                float c = value[v], z = f.shut;
-                if (p.tanhValue) c = tanhf(c);
-                if (OWN) z = Gate(input[v]).open;
-                a[s][v] = s < live ? f.open : 1.f;
-                b[s][v] = s < live ? z * c : 0.f;
-                A[v] *= a[s][v];
-                B[v] = fmaf(a[s][v], B[v], b[s][v]);
+            for (int s = 0; s < S; ++s) {
+                const Gates f(readRow<T>(from + s * kRow));
+                Pair c = readRow<T>(from + s * kRow + kTensorBytes<OWN>), z = f.shut;
+                if (TANH) c = tanhOf(c);
+                if (OWN) z = Gates(readRow<T>(from + s * kRow + 2 * kTensorBytes<OWN>)).open;
+                a[s] = f.open;
+                b[s] = mul2(z, c);
             }
-        }
+            const int live = tile.live - warp * S;   // of this warp's tokens
+            if (live < S) {                          // what lies behind the sequence may be anything
 #pragma unroll
-        for (int v = 0; v < N; ++v) parts[warp][lane * N + v] = make_float2(A[v], B[v]);
-        if (tid == 0) tileOf[stage] = later;
-        __syncthreads();
-        ask(stage);
-
-        const int d = tile.d0 + lane * N, real = p.width - d;
-        const int64_t link = tile.slab * p.chunks + tile.chunk;
-        const bool last = tile.chunk + 1 == p.chunks;
-        // the last warp speaks for the tile
-        if (warp == kWarps - 1 && !last) {
-#pragma unroll
-            for (int v = 0; v < N; ++v) {
-                A[v] = 1.f;
-                B[v] = 0.f;
-                for (int w = 0; w < kWarps; ++w) {
-                    const float2 part = parts[w][lane * N + v];
-                    A[v] *= part.x;
-                    B[v] = fmaf(part.x, B[v], part.y);
+                for (int s = 0; s < S; ++s) {
+                    a[s] = s < live ? a[s] : bothOf(1.f);
+                    b[s] = s < live ? b[s] : bothOf(0.f);
                 }
             }
-            if (tile.chunk > 0) tellPart<N>(p.chain, link, A, B);
-        }
-        float h[N];
-        if (tile.chunk > 0) stateBefore<N>(p.chain, tile.slab, tile.chunk, p.chunks, window, &nearest, h);
-        else {
+            Map own{a[0], b[0]};
 #pragma unroll
-            for (int v = 0; v < N; ++v) h[v] = p.state && v < real ? p.state[static_cast<int64_t>(tile.b) * p.width + d + v] : 0.f;
-        }
-        if (warp == kWarps - 1 && !last) {
-            float behind[N];
-#pragma unroll
-            for (int v = 0; v < N; ++v) behind[v] = fmaf(A[v], h[v], B[v]);
-            tellWhole<N>(p.chain, link, behind);
-        }
-        if (warp == 0 && p.marks && tile.chunk > 0) {
-#pragma unroll
-            for (int v = 0; v < N; ++v)
-                if (v < real) p.marks[(static_cast<int64_t>(tile.b) * (p.chunks - 1) + tile.chunk - 1) * p.width + d + v] = h[v];
-        }
-        for (int w = 0; w < warp; ++w)
-#pragma unroll
-            for (int v = 0; v < N; ++v) {
-                const float2 part = parts[w][lane * N + v];
-                h[v] = fmaf(part.x, h[v], part.y);
+            for (int s = 1; s < S; ++s) own = Map{a[s], b[s]}.behind(own);
+            shared[warp][lane] = own;
+            if (tid == 0) tiles[turn ^ 1] = later;
+            __syncthreads();
+            ask(tiles[turn ^ 1]);
+            nextAhead = mapBefore(shared, warp);
+            if (warp == kWarps - 1 && tile.chunk + 1 < p.chunks) {
+                nextMine = own.behind(nextAhead);
+                tellTile(p, tile, nextMine);
             }
-        const int here = min(p.tokens - tile.first - warp * kSteps, kSteps);   // tokens that have an output
-        T *to = static_cast<T *>(p.out) + (static_cast<int64_t>(tile.b) * p.tokens + tile.first + warp * kSteps) * p.width + d;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            float y[N];
-#pragma unroll
-            for (int v = 0; v < N; ++v) {
-                h[v] = fmaf(a[s][v], h[v], b[s][v]);
-                y[v] = s < live ? h[v] : 0.f;
+        }
+        // ... and the outputs of the one before, whose state has had that long to come
+        if (waiting.real) {
+            const int d = waiting.d0 + 2 * lane, real = p.width - d, live = waiting.live - warp * S;
+            const bool last = waiting.chunk + 1 == p.chunks;
+            const int64_t row = static_cast<int64_t>(waiting.b) * p.width + d;
+            Pair h;
+            if (waiting.place > 0) h = stateBefore<kWarps - 1>(p, waiting, mine, shared, front);
+            else {
+                h = readFloats(p.state ? p.state + row : nullptr, real);
+                if (warp == 0 && !last) tellStart(p, waiting, h);
             }
-            if (p.out && s < here) writeRow<T>(to, y, real, p.paired);
-            to += p.width;
-        }
-        if (last && warp == kWarps - 1 && p.finalState) {
+            if (warp == 0 && p.marks && waiting.chunk > 0) writeFloats(p.marks + (static_cast<int64_t>(waiting.b) * (p.chunks - 1) + waiting.chunk - 1) * p.width + d, h, real);
+            h = ahead(h);
+            const int here = min(p.tokens - waiting.first - warp * S, S);   // tokens that have an output
+            T *to = static_cast<T *>(p.out) + (static_cast<int64_t>(waiting.b) * p.tokens + waiting.first + warp * S) * p.width + d;
+            if (live >= S && p.paired && p.out) {
 #pragma unroll
-            for (int v = 0; v < N; ++v)
-                if (v < real) p.finalState[static_cast<int64_t>(tile.b) * p.width + d + v] = h[v];
+                for (int s = 0; s < S; ++s, to += p.width) {
+                    const ulonglong2 map = held[s][tid];
+                    h = fma2(map.x, h, map.y);
+                    writeRow<T>(to, h, real, true);
+                }
+            } else {
+#pragma unroll 1
+                for (int s = 0; s < S; ++s, to += p.width) {
+                    const ulonglong2 map = held[s][tid];
+                    h = fma2(map.x, h, map.y);
+                    if (p.out && s < here) writeRow<T>(to, s < live ? h : bothOf(0.f), real, p.paired);
+                }
+            }
+            if (last && warp == kWarps - 1 && p.finalState) writeFloats(p.finalState + row, h, real);
         }
+        if (!tile.real) break;
+#pragma unroll
+        for (int s = 0; s < S; ++s) held[s][tid] = make_ulonglong2(a[s], b[s]);
+        waiting = tile;
+        ahead = nextAhead;
+        mine = nextMine;
     }
 }
 
@@ -161,22 +138,23 @@ __global__ void __launch_bounds__(kThreads) gatedStep(const __grid_constant__ Pa
         if (OWN) input[v] = at(p.input, u);
         h[v] = p.state ? p.state[row + u] : 0.f;
     }
+    const Gates forgets(pairOf(forget[0], forget[1]));
+    const float2 f = floatsOf(forgets.open), z = floatsOf(OWN ? Gates(pairOf(input[0], input[1])).open : forgets.shut);
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
         if (v >= count) continue;
-        const Gate f(forget[v]);
-        const float c = p.tanhValue ? tanhf(value[v]) : value[v], z = OWN ? Gate(input[v]).open : f.shut;
-        const float next = live ? fmaf(f.open, h[v], z * c) : h[v];
+        const float c = p.tanhValue ? tanhf(value[v]) : value[v];
+        const float next = live ? fmaf(v ? f.y : f.x, h[v], (v ? z.y : z.x) * c) : h[v];
         if (p.finalState) p.finalState[row + v] = next;
         if (p.out) static_cast<T *>(p.out)[row + v] = fromFloat<T>(live ? next : 0.f);
     }
 }
 
-// Flags and ticket of a chain.
-__global__ void __launch_bounds__(kThreads) gatedClear(int *words, int64_t count) {
+// Words and ticket of a chain.
+__global__ void __launch_bounds__(kThreads) gatedClear(uint4 *words, int64_t count) {
     waitForPredecessor();
     letDependentsStart();
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < count; i += static_cast<int64_t>(gridDim.x) * kThreads) words[i] = 0;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < count; i += static_cast<int64_t>(gridDim.x) * kThreads) words[i] = make_uint4(0, 0, 0, 0);
 }
 
 Pass passOf(const rxmet_gated_recurrence &problem) {
@@ -187,11 +165,12 @@ Pass passOf(const rxmet_gated_recurrence &problem) {
     p.batch = problem.batch;
     p.tokens = problem.tokens;
     p.width = problem.width;
-    const int channels = static_cast<int>(128 / typeBytes(problem.type));
-    p.chunks = std::max(1, (problem.tokens + kChunk - 1) / kChunk);
-    p.slabsOfRow = (problem.width + channels - 1) / channels;
+    const int tokens = tokensOf(problem.type, problem.input.data != nullptr);
+    p.chunks = std::max(1, (problem.tokens + tokens - 1) / tokens);
+    p.groups = (p.chunks + kGroup - 1) / kGroup;
+    p.slabsOfRow = (problem.width + kChannels - 1) / kChannels;
     const int64_t slabs = static_cast<int64_t>(p.batch) * p.slabsOfRow;
-    if (slabs * p.chunks > INT32_MAX) fail(RXMET_ERR_UNSUPPORTED, "gated_recurrence: %lld runs of %d tokens of %d channels, at most %d", static_cast<long long>(slabs * p.chunks), kChunk, channels, INT32_MAX);
+    if (slabs * p.chunks > INT32_MAX) fail(RXMET_ERR_UNSUPPORTED, "gated_recurrence: %lld runs of %d tokens of %d channels, at most %d", static_cast<long long>(slabs * p.chunks), tokens, kChannels, INT32_MAX);
     p.tiles = slabs * p.chunks;
     p.tanhValue = problem.tanh_value != 0;
     p.forget = problem.forget;
@@ -204,32 +183,19 @@ void requireData(const rxmet_gated_recurrence &problem, int64_t tiles) {
     RXMET_REQUIRE(tiles == 0 || problem.tokens == 0 || (problem.forget.data && problem.value.data), "gated_recurrence: null pointer");
 }
 
-// Links of a chain and their words; nothing for sequences of one tile.
-int64_t chainWords(const Pass &p) { return p.chunks > 1 ? p.tiles + 1 : 0; }
-template <class W>
-void takeChain(W &&ws, const Pass &p, Chain *chain) {
-    if (p.chunks == 1) return;
-    if constexpr (std::is_same_v<std::decay_t<W>, WorkspaceSizer>) {
-        ws.template take<int>(chainWords(p));
-        ws.template take<float2>(p.tiles * 64);
-        ws.template take<float>(p.tiles * 64);
-    } else {
-        int *words = ws.template take<int>(chainWords(p));
-        chain->ticket = reinterpret_cast<unsigned *>(words);
-        chain->flags = words + 1;
-        chain->parts = ws.template take<float2>(p.tiles * 64);
-        chain->whole = ws.template take<float>(p.tiles * 64);
-    }
-}
+// In units of 16 bytes: the ticket's, the parts' words, the fronts'; nothing for sequences of one tile.
+int64_t chainUnits(const Pass &p) { return p.chunks > 1 ? 1 + (p.tiles + p.tiles / p.chunks * p.groups) * (kChannels / 2) : 0; }
 void startChain(Pass &p, void *workspace, size_t bytes, cudaStream_t st) {
     p.chain.status = waitStatus();
-    if (p.chunks == 1) return;
-    takeChain(Workspace(workspace, bytes), p, &p.chain);
-    const int64_t words = chainWords(p);
+    const int64_t units = chainUnits(p);
+    if (units == 0) return;
+    uint4 *at = Workspace(workspace, bytes).take<uint4>(units);
+    p.chain.ticket = reinterpret_cast<unsigned *>(at);
+    p.chain.parts = reinterpret_cast<unsigned long long *>(at + 1);
+    p.chain.fronts = p.chain.parts + p.tiles * kChannels;
     {
         KernelTimer timer__("gatedClear", st);
-        launchDependent(gatedClear, static_cast<unsigned>(std::min<int64_t>((words + kThreads - 1) / kThreads, 4 * currentDevice().sms)), kThreads, 0, st,
-                        reinterpret_cast<int *>(p.chain.ticket), words);
+        launchDependent(gatedClear, static_cast<unsigned>(std::min<int64_t>((units + kThreads - 1) / kThreads, 8 * currentDevice().sms)), kThreads, 0, st, at, units);
     }
     afterLaunch("gatedClear");
 }
@@ -242,11 +208,11 @@ void launchForward(const Pass &p, int type, cudaStream_t st) {
     if (p.input.data) piece = std::min(piece, pieceOf(p.input, p.batch, p.tokens, size));
     withType(type, [&](auto t) {
         using T = decltype(t);
-        auto launch = [&](auto own) {
-            constexpr bool kOwn = decltype(own)::value;
+        auto launch = [&](auto own, auto squash) {
+            constexpr bool kOwn = decltype(own)::value, kTanh = decltype(squash)::value;
             withPiece<T>(piece, [&](auto bytes) {
-                const auto kernel = gatedForward<T, decltype(bytes)::value, kOwn>;
-                const size_t smem = kStages * (kOwn ? 3 : 2) * kTensorBytes<T>;
+                const auto kernel = gatedForward<T, decltype(bytes)::value, kOwn, kTanh>;
+                const size_t smem = (kOwn ? 3 : 2) * kTensorBytes<kOwn> + kSteps<T, kOwn> * kThreads * sizeof(ulonglong2);
                 ensureDynamicSmem(reinterpret_cast<const void *>(kernel), smem);
                 const int resident = residentPerSm(reinterpret_cast<const void *>(kernel), kThreads, smem) * currentDevice().sms;
                 {
@@ -256,8 +222,8 @@ void launchForward(const Pass &p, int type, cudaStream_t st) {
                 afterLaunch("gatedForward");
             });
         };
-        if (p.input.data) launch(std::true_type{});
-        else launch(std::false_type{});
+        if (p.input.data) p.tanhValue ? launch(std::true_type{}, std::true_type{}) : launch(std::true_type{}, std::false_type{});
+        else p.tanhValue ? launch(std::false_type{}, std::true_type{}) : launch(std::false_type{}, std::false_type{});
     });
 }
 
@@ -295,7 +261,8 @@ extern "C" size_t rxmet_gated_recurrence_workspace_bytes(const rxmet_gated_recur
     WorkspaceSizer sizer;
     guarded([&] {
         RXMET_REQUIRE(problem, "gated_recurrence: null pointer");
-        gated::takeChain(sizer, gated::passOf(*problem), nullptr);
+        const int64_t units = gated::chainUnits(gated::passOf(*problem));
+        if (units > 0) sizer.take<uint4>(units);
     });
     return sizer.used();
 }
@@ -311,7 +278,7 @@ extern "C" int rxmet_gated_recurrence_forward(const rxmet_gated_recurrence *prob
         p.out = out;
         p.finalState = final_state;
         p.marks = marks;
-        p.paired = p.width % 2 == 0 && alignedTo(out, 4);
+        p.paired = p.width % 2 == 0 && alignedTo(out, 2 * typeBytes(problem->type));
         const auto st = static_cast<cudaStream_t>(stream);
         if (p.tokens == 1) return gated::launchStep(p, problem->type, st);
         gated::startChain(p, workspace, workspace_bytes, st);
@@ -336,7 +303,8 @@ extern "C" int rxmet_gated_recurrence_backward(const rxmet_gated_recurrence *pro
         p.dvalue = dvalue;
         p.dinput = dinput;
         p.dstate = dstate;
-        p.paired = p.width % 2 == 0 && alignedTo(dforget, 4) && alignedTo(dvalue, 4) && alignedTo(dinput, 4);
+        const size_t two = 2 * typeBytes(problem->type);
+        p.paired = p.width % 2 == 0 && alignedTo(dforget, two) && alignedTo(dvalue, two) && alignedTo(dinput, two);
         const auto st = static_cast<cudaStream_t>(stream);
         gated::startChain(p, workspace, workspace_bytes, st);
         gated::launchBackward(p, problem->type, st);

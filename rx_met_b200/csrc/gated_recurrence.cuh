@@ -1,9 +1,9 @@
 // Gated linear recurrence: what its passes share.
 //
-// A tile is the channels of a warp's row (128 bytes of 16-bit types and of floats) times kChunk tokens of a sequence; each of a CTA's eight warps has kSteps neighbouring tokens.  A run of
-// tokens maps the state before it to the one behind it by h -> A h + B, so that the warps' (A, B), joined in order, give the tile's, and the tiles' of a sequence the state in front of each of
-// them: `Chain`.  The CTAs walk over tiles in the order of tickets, the first tiles of all sequences before the second ones, and a stage of shared memory is filled for the tile to come
-// while one is worked on.
+// A tile is 64 channels times kTokens tokens of a sequence; each of a CTA's eight warps has kSteps neighbouring tokens, each lane two
+// neighbouring channels, whose 32-bit operations go two at a time.  A run of tokens maps the state before it to the one behind it by h -> A h + B, so that the warps' (A, B), joined in order, give
+// the tile's, and the tiles' of a sequence the state in front of each of them: `Chain`.  The CTAs walk over tiles in the order of tickets, the first tiles of all sequences before the second
+// ones, and a stage of shared memory is filled for the tile to come while one is worked on.
 #pragma once
 
 #include "cluster_device.cuh"
@@ -14,30 +14,42 @@
 namespace rxmet {
 namespace gated {
 
+using rxmet::pairOf;
+
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kSteps = 16, kChunk = kWarps * kSteps;
-constexpr int kWindow = 32;                    // tiles that a look back spans
+constexpr int kGroup = 8;                      // tiles, at most the warps of a CTA
+constexpr int kChannels = 64;                  // of a tile, two a lane
 constexpr uint32_t kPollLimit = 1u << 18;      // 0.2 s of polling; a legitimate wait lasts microseconds
 
-template <class T>
-constexpr int kChannels = 128 / static_cast<int>(sizeof(T));   // of a tile
-template <class T>
-constexpr uint32_t kTensorBytes = kChunk * kChannels<T> * sizeof(T);   // of a tile
-template <class T>
-constexpr int kLane = kChannels<T> / 32;
+// Bytes of a lane's channel in a tile: 16 tokens of 16-bit elements or 8 of floats, which 128 registers a thread have room for; half of that beside an input gate, whose rows need the shared memory.
+constexpr int stepBytes(bool own) { return own ? 16 : 32; }
+template <class T, bool OWN>
+constexpr int kSteps = stepBytes(OWN) / static_cast<int>(sizeof(T));   // tokens of a warp
+template <class T, bool OWN>
+constexpr int kTokens = kWarps * kSteps<T, OWN>;                       // of a tile
+inline int tokensOf(int type, bool own) { return kWarps * stepBytes(own) / static_cast<int>(typeBytes(type)); }
+template <bool OWN>
+constexpr uint32_t kTensorBytes = kChannels * kWarps * (OWN ? 16 : 32);   // of a tile
 
-// What the tiles of a sequence tell one another.  `parts`: (A, B) of a tile, `whole`: the state behind it; `flags` says which of them is there (1, 2).
-// A state behind a tile is always A times the state in front plus B, whether one tile took that step or a later one did after looking back over several, so that bits do not depend on who was first.
+// What the tiles of a sequence tell one another: words of 64 bits, one a channel, zero at first.  Value and what it is come in one word, so that nobody has to order two stores or two loads: a fence on
+// either side waits for all that the thread has in flight.
+// The tiles come in groups of kGroup.  `parts` holds a tile's (A, B); `fronts` the state in front of a group, or, until that is known, the (A, B) of the whole group in front of it.  A state in front of
+// a tile is always that in front of its group, taken through the group's tiles one by one, and the next group's is always taken through the whole group at once, so that bits do not depend on who was
+// first.  65536 tokens of 512 channels are 512 tiles in a row: one tile at a time they took 486 us, with groups 60.
 struct Chain {
     unsigned *ticket;
-    int *flags;       // [slab][place in the chain]
-    float2 *parts;    // [slab][place][channels]
-    float *whole;
+    unsigned long long *parts;    // [slab][place in the chain][channels]
+    unsigned long long *fronts;   // [slab][group][channels]
     int *status;
 };
-
+// The low half is B or the state.  The high half: A, a product of gates and at most one, so that two bits are free: the uppermost is set in any word, the next one in that of a state.
+__device__ __forceinline__ unsigned long long partWord(float a, float b) {
+    return (static_cast<unsigned long long>(__float_as_uint(a) | 0x80000000u) << 32) | __float_as_uint(b);
+}
+__device__ __forceinline__ unsigned long long wholeWord(float h) { return (0xc0000000ull << 32) | __float_as_uint(h); }
+__device__ __forceinline__ bool isWhole(unsigned long long word) { return (word >> 62) == 3ull; }   // (or A is a NaN, and so is B)
 struct Pass {
-    int batch, tokens, width, chunks, slabsOfRow, tanhValue;
+    int batch, tokens, width, chunks, groups, slabsOfRow, tanhValue;   // chunks: tiles of a sequence
     bool paired;   // two neighbours of a 16-bit output can be written at once
     int64_t tiles;
     rxmet_token_tensor forget, value, input, dout;
@@ -48,25 +60,41 @@ struct Pass {
     Chain chain;
 };
 
-__device__ __forceinline__ int loadFlag(const int *at) {
-    int v;
-    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(at) : "memory");
-    return v;
+// exp(-x) of two values.  The product x log2(e) is rounded to 24 bits, and what that leaves out is put back, so that the result is as exact as the exponential itself (2 units) for
+// every x; beyond 87 either way sigmoid(x) and its complement are 0 and 1 to 2^-125.  A NaN stays one.
+__device__ __forceinline__ Pair exponentials(Pair x) {
+    const float2 v = floatsOf(x);
+    float a, b;
+    asm("max.NaN.f32 %0, %1, 0fC2AE0000;\n\tmin.NaN.f32 %0, %0, 0f42AE0000;" : "=f"(a) : "f"(v.x));
+    asm("max.NaN.f32 %0, %1, 0fC2AE0000;\n\tmin.NaN.f32 %0, %0, 0f42AE0000;" : "=f"(b) : "f"(v.y));
+    const Pair held = pairOf(a, b), log2e = pairOf(-1.4426950408889634f, -1.4426950408889634f), rest = pairOf(-1.925963033500e-8f, -1.925963033500e-8f);
+    const Pair u = mul2(held, log2e);
+    const float2 whole = floatsOf(u);
+    const Pair left = fma2(held, rest, fma2(held, log2e, pairOf(-whole.x, -whole.y)));
+    float c, d;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(c) : "f"(whole.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(whole.y));
+    const Pair e = pairOf(c, d);
+    return fma2(mul2(e, left), pairOf(0.6931471805599453f, 0.6931471805599453f), e);
 }
-__device__ __forceinline__ void storeFlag(int *at, int v) { asm volatile("st.release.gpu.global.s32 [%0], %1;" ::"l"(at), "r"(v) : "memory"); }
-
-// sigmoid(x) = 1 - sigmoid(-x) from the smaller of the two, so that neither loses bits to a subtraction from one.
-struct Gate {
-    float open, shut;
-    __device__ __forceinline__ explicit Gate(float x) {
-        const float e = expf(-fabsf(x));
-        float most;
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(most) : "f"(1.f + e));   // one unit in the last place; the argument is in [1, 2]
-        const float least = e * most;
-        open = x > 0.f ? most : least;
-        shut = x > 0.f ? least : most;
+// sigmoid(x), and 1 - sigmoid(x) without the bits that a subtraction from one would lose, of two values.
+struct Gates {
+    Pair open, shut;
+    __device__ __forceinline__ explicit Gates(Pair x) {
+        const Pair e = exponentials(x);
+        const float2 sum = floatsOf(add2(e, pairOf(1.f, 1.f)));
+        float a, b;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(sum.x));   // one unit in the last place
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(sum.y));
+        open = pairOf(a, b);
+        shut = mul2(e, open);
     }
 };
+__device__ __forceinline__ Pair bothOf(float v) { return pairOf(v, v); }
+__device__ __forceinline__ Pair tanhOf(Pair x) {
+    const float2 v = floatsOf(x);
+    return pairOf(tanhf(v.x), tanhf(v.y));
+}
 
 // Copies of PIECE bytes from a row of channels to shared memory, `bytes` of them real and the rest zeros.
 template <int PIECE>
@@ -78,28 +106,34 @@ __device__ __forceinline__ void commitCopies() { asm volatile("cp.async.commit_g
 template <int LEFT>
 __device__ __forceinline__ void copiesArrived() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
-// Where a tile lies.
-template <class T>
+// Where a tile lies: worked out by one thread, because of the divisions.
 struct Tile {
     int64_t slab;
-    int chunk, b, d0, live, first;   // live: of its tokens, those of the sequence; first: its first token
-    __device__ __forceinline__ Tile(const Pass &p, int64_t index, bool reverse) {
-        const int64_t slabs = static_cast<int64_t>(p.batch) * p.slabsOfRow;
-        const int place = static_cast<int>(index / slabs);
-        slab = index - place * slabs;
-        chunk = reverse ? p.chunks - 1 - place : place;
-        b = static_cast<int>(slab / p.slabsOfRow);
-        d0 = static_cast<int>(slab - static_cast<int64_t>(b) * p.slabsOfRow) * kChannels<T>;
-        first = chunk * kChunk;
-        const int length = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
-        live = min(max(length - first, 0), kChunk);
-    }
+    int place, chunk, b, d0, live, first;   // place: in the chain; live: of its tokens, those of the sequence; first: its first token
+    bool real;
 };
+template <class T, bool OWN>
+__device__ __forceinline__ Tile tileOf(const Pass &p, int64_t index, bool reverse) {
+    Tile t{};
+    t.real = index < p.tiles;
+    if (!t.real) return t;
+    const uint32_t slabs = static_cast<uint32_t>(p.batch) * static_cast<uint32_t>(p.slabsOfRow), at = static_cast<uint32_t>(index);
+    t.place = static_cast<int>(at / slabs);
+    const uint32_t slab = at - t.place * slabs;
+    t.slab = slab;
+    t.chunk = reverse ? p.chunks - 1 - t.place : t.place;
+    t.b = static_cast<int>(slab / static_cast<uint32_t>(p.slabsOfRow));
+    t.d0 = static_cast<int>(slab - t.b * static_cast<uint32_t>(p.slabsOfRow)) * kChannels;
+    t.first = t.chunk * kTokens<T, OWN>;
+    const int length = p.lengths ? min(max(p.lengths[t.b], 0), p.tokens) : p.tokens;
+    t.live = min(max(length - t.first, 0), kTokens<T, OWN>);
+    return t;
+}
 
 // Asks for the live tokens of a tile's rows of one tensor.  A row of shared memory holds the tile's channels of one token.
 template <class T, int PIECE>
-__device__ __forceinline__ void askFor(uint32_t to, const rxmet_token_tensor &t, const Tile<T> &tile, int width) {
-    constexpr int kRow = kChannels<T> * sizeof(T), kPieces = kRow / PIECE, kPer = PIECE / static_cast<int>(sizeof(T));
+__device__ __forceinline__ void askFor(uint32_t to, const rxmet_token_tensor &t, const Tile &tile, int width) {
+    constexpr int kRow = kChannels * sizeof(T), kPieces = kRow / PIECE, kPer = PIECE / static_cast<int>(sizeof(T));
     const int r0 = threadIdx.x / kPieces, piece = threadIdx.x % kPieces;
     const int real = min(kPer, width - tile.d0 - piece * kPer);
     if (real <= 0) return;
@@ -118,85 +152,152 @@ __device__ __forceinline__ void askFor(uint32_t to, const rxmet_token_tensor &t,
 
 // The lane's channels of a row.
 template <class T>
-__device__ __forceinline__ void readRow(const uint8_t *row, float (&v)[kLane<T>]) {
-    if constexpr (sizeof(T) == 4) v[0] = *reinterpret_cast<const float *>(row);
+__device__ __forceinline__ Pair readRow(const uint8_t *row) {
+    if constexpr (sizeof(T) == 4) return *reinterpret_cast<const Pair *>(row);
     else {
         const float2 two = unpack2<T>(*reinterpret_cast<const uint32_t *>(row));
-        v[0] = two.x;
-        v[1] = two.y;
+        return pairOf(two.x, two.y);
     }
 }
+// `real`: of the two channels, those of the row; `paired`: both can be written at once.
 template <class T>
-__device__ __forceinline__ void writeRow(T *to, const float (&v)[kLane<T>], int real, bool paired) {
-    if constexpr (sizeof(T) == 4) {
-        if (real > 0) *to = v[0];
-    } else {
-        if (paired) {
-            if (real > 0) *reinterpret_cast<uint32_t *>(to) = pack2<T>(v[0], v[1]);
-        } else {
-            if (real > 0) to[0] = fromFloat<T>(v[0]);
-            if (real > 1) to[1] = fromFloat<T>(v[1]);
+__device__ __forceinline__ void writeRow(T *to, Pair v, int real, bool paired) {
+    const float2 two = floatsOf(v);
+    if (paired) {
+        if (real > 0) {
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<Pair *>(to) = v;
+            else *reinterpret_cast<uint32_t *>(to) = pack2<T>(v);
         }
+    } else {
+        if (real > 0) to[0] = fromFloat<T>(two.x);
+        if (real > 1) to[1] = fromFloat<T>(two.y);
     }
+}
+__device__ __forceinline__ Pair readFloats(const float *from, int real) { return pairOf(from && real > 0 ? from[0] : 0.f, from && real > 1 ? from[1] : 0.f); }
+__device__ __forceinline__ void writeFloats(float *to, Pair v, int real) {
+    if (real > 0) to[0] = floatsOf(v).x;
+    if (real > 1) to[1] = floatsOf(v).y;
 }
 
-// The state in front of the tile at `place` of its chain, for the lane's channels.  All threads of the CTA; the predecessors hold lower tickets, whose CTAs are at work already, so that the
-// wait ends.  One warp polls the flags of the last kWindow tiles until the nearest state and every (A, B) behind it are there.
-template <int N>
-__device__ __forceinline__ void stateBefore(const Chain &c, int64_t slab, int place, int chunks, float2 (*window)[32 * N], int *nearest, float (&h)[N]) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t base = slab * chunks + place - 1;
-    if (warp == 0) {
-        int found = -1;
-        for (uint32_t poll = 0; poll < kPollLimit && found < 0; ++poll) {
-            const int flag = place - 1 - lane >= 0 ? loadFlag(c.flags + base - lane) : 0;
-            const unsigned whole = __ballot_sync(0xffffffffu, flag == 2), some = __ballot_sync(0xffffffffu, flag != 0);
-            if (whole) {
-                const int at = __ffs(whole) - 1;
-                const unsigned nearer = (1u << at) - 1;
-                if ((some & nearer) == nearer) found = at;
+__device__ __forceinline__ ulonglong2 loadWords(const unsigned long long *at) {
+    ulonglong2 w;
+    asm volatile("ld.relaxed.gpu.global.v2.u64 {%0, %1}, [%2];" : "=l"(w.x), "=l"(w.y) : "l"(at) : "memory");   // each of the two is whole
+    return w;
+}
+__device__ __forceinline__ void storeWords(unsigned long long *to, unsigned long long x, unsigned long long y) {
+    asm volatile("st.relaxed.gpu.global.v2.u64 [%0], {%1, %2};" ::"l"(to), "l"(x), "l"(y) : "memory");
+}
+__device__ __forceinline__ void tellMap(unsigned long long *to, Pair a, Pair b) {
+    const float2 A = floatsOf(a), B = floatsOf(b);
+    storeWords(to, partWord(A.x, B.x), partWord(A.y, B.y));
+}
+__device__ __forceinline__ void tellState(unsigned long long *to, Pair h) {
+    const float2 v = floatsOf(h);
+    storeWords(to, wholeWord(v.x), wholeWord(v.y));
+}
+// A run of tokens: h -> A h + B.
+struct Map {
+    Pair A, B;
+    __device__ __forceinline__ Pair operator()(Pair h) const { return fma2(A, h, B); }
+    __device__ __forceinline__ Map behind(const Map &front) const { return {mul2(A, front.A), fma2(A, front.B, B)}; }
+};
+__device__ __forceinline__ Map mapOf(const ulonglong2 &w) {
+    auto low = [](unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v)); };
+    auto gate = [](unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v >> 32) & 0x3fffffffu); };
+    return {pairOf(gate(w.x), gate(w.y)), pairOf(low(w.x), low(w.y))};
+}
+__device__ __forceinline__ void gaveUp(const Chain &c) {
+    if ((threadIdx.x & 31) == 0) atomicExch(c.status, 1);   // the results are not to be used
+}
+// (A, B) of a tile, by one warp.  Its CTA holds a lower ticket and is at work already, so that the wait ends.
+__device__ __forceinline__ Map awaitPart(const Chain &c, const unsigned long long *at) {
+    for (uint32_t poll = 0; poll < kPollLimit; ++poll) {
+        const ulonglong2 w = loadWords(at);
+        if (__all_sync(0xffffffffu, w.x != 0 && w.y != 0)) return mapOf(w);
+    }
+    gaveUp(c);
+    return {bothOf(1.f), bothOf(0.f)};
+}
+// The state in front of a group, by one warp: from the nearest of the last eight groups' fronts that is known, taken through the groups in between.
+__device__ __forceinline__ Pair awaitFront(const Chain &c, const unsigned long long *fronts, int group) {
+    constexpr int kBack = 8;
+    for (uint32_t poll = 0; poll < kPollLimit; ++poll) {
+        ulonglong2 w[kBack];
+        if ((poll & 1) == 0) {   // most often it is there
+            w[0] = loadWords(fronts);
+            if (__all_sync(0xffffffffu, isWhole(w[0].x) && isWhole(w[0].y))) return mapOf(w[0]).B;
+            continue;
+        }
+        int nearest = kBack;   // in reach, with all behind it there
+#pragma unroll
+        for (int i = 0; i < kBack; ++i) w[i] = i <= group ? loadWords(fronts - i * kChannels) : make_ulonglong2(0, 0);
+#pragma unroll
+        for (int i = kBack - 1; i >= 0; --i) {
+            const bool there = __all_sync(0xffffffffu, w[i].x != 0 && w[i].y != 0), whole = __all_sync(0xffffffffu, isWhole(w[i].x) && isWhole(w[i].y));
+            nearest = whole ? i : there ? nearest : kBack;
+        }
+        if (nearest == kBack) continue;
+        Pair h = bothOf(0.f);
+#pragma unroll
+        for (int i = kBack - 1; i >= 0; --i) {
+            const Map m = mapOf(w[i]);
+            if (i == nearest) h = m.B;
+            if (i < nearest) {
+                // a channel's state may have come where another's has not
+                const float2 known = floatsOf(m.B), taken = floatsOf(m(h));
+                h = pairOf(isWhole(w[i].x) ? known.x : taken.x, isWhole(w[i].y) ? known.y : taken.y);
             }
         }
-        if (lane == 0) {
-            if (found < 0) atomicExch(c.status, 1);
-            *nearest = found;
+        return h;
+    }
+    gaveUp(c);
+    return bothOf(0.f);
+}
+// The state in front of a tile.  All threads of the CTA.  `mine`: the tile's own map, in warp SPEAKER; `front`: a row of shared memory.
+// `window` may have been read in front of the call.
+template <int SPEAKER>
+__device__ __forceinline__ Pair stateBefore(const Pass &p, const Tile &tile, const Map &mine, Map (*window)[32], Pair *front) {
+    const Chain &c = p.chain;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = tile.place / kGroup, k = tile.place % kGroup;
+    const bool speaks = k == kGroup - 1 && group + 1 < p.groups;   // for its group
+    unsigned long long *parts = c.parts + (tile.slab * p.chunks + group * kGroup) * kChannels + 2 * lane;
+    unsigned long long *fronts = c.fronts + (tile.slab * p.groups + group) * kChannels + 2 * lane;
+    __syncthreads();
+    if (warp < k) window[warp][lane] = awaitPart(c, parts + warp * kChannels);
+    Map all;
+    if (speaks) {
+        if (warp == SPEAKER) window[kGroup - 1][lane] = mine;
+        __syncthreads();
+        if (warp == 0) {
+            all = window[0][lane];
+#pragma unroll
+            for (int i = 1; i < kGroup; ++i) all = window[i][lane].behind(all);
+            tellMap(fronts + kChannels, all.A, all.B);
         }
     }
+    if (warp == kWarps - 1) front[lane] = awaitFront(c, fronts, group);
     __syncthreads();
-    const int back = max(*nearest, 0);
-    for (int i = warp; i < back; i += kWarps)
+    Pair h = front[lane];
+    if (speaks && warp == 0) tellState(fronts + kChannels, all(h));
 #pragma unroll
-        for (int v = 0; v < N; ++v) window[i][lane * N + v] = __ldcg(c.parts + (base - i) * (32 * N) + lane * N + v);
-#pragma unroll
-    for (int v = 0; v < N; ++v) h[v] = __ldcg(c.whole + (base - back) * (32 * N) + lane * N + v);
-    if (back == 0) return;
-    __syncthreads();
-    for (int i = back - 1; i >= 0; --i)
-#pragma unroll
-        for (int v = 0; v < N; ++v) {
-            const float2 part = window[i][lane * N + v];
-            h[v] = fmaf(part.x, h[v], part.y);
-        }
+    for (int i = 0; i < kGroup - 1; ++i)
+        if (i < k) h = window[i][lane](h);
+    return h;
 }
-// By one warp: the tile's (A, B), or the state behind it.
-template <int N>
-__device__ __forceinline__ void tellPart(const Chain &c, int64_t at, const float (&a)[N], const float (&b)[N]) {
-    const int lane = threadIdx.x & 31;
+// What lies between the tile's front and a warp's first token.
+__device__ __forceinline__ Map mapBefore(const Map (*parts)[32], int warp) {
+    Map m{bothOf(1.f), bothOf(0.f)};
 #pragma unroll
-    for (int v = 0; v < N; ++v) __stcg(c.parts + at * (32 * N) + lane * N + v, make_float2(a[v], b[v]));
-    __threadfence();
-    __syncwarp();
-    if (lane == 0) storeFlag(c.flags + at, 1);
+    for (int w = 0; w < kWarps - 1; ++w)
+        if (w < warp) m = parts[w][threadIdx.x & 31].behind(m);
+    return m;
 }
-template <int N>
-__device__ __forceinline__ void tellWhole(const Chain &c, int64_t at, const float (&h)[N]) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int v = 0; v < N; ++v) __stcg(c.whole + at * (32 * N) + lane * N + v, h[v]);
-    __threadfence();
-    __syncwarp();
-    if (lane == 0) storeFlag(c.flags + at, 2);
+// By one warp, as soon as the tile's map is known.
+__device__ __forceinline__ void tellTile(const Pass &p, const Tile &tile, const Map &mine) {
+    if (tile.place % kGroup != kGroup - 1) tellMap(p.chain.parts + (tile.slab * p.chunks + tile.place) * kChannels + 2 * (threadIdx.x & 31), mine.A, mine.B);
 }
+// By one warp of a chain's first tile.
+__device__ __forceinline__ void tellStart(const Pass &p, const Tile &tile, Pair h) { tellState(p.chain.fronts + tile.slab * p.groups * kChannels + 2 * (threadIdx.x & 31), h); }
 
 // The tiles of a CTA: by tickets where tiles wait for one another, else every gridDim.x'th.  `take` is called by one thread, once for each tile.
 struct Tickets {

@@ -14,185 +14,136 @@ namespace {
 
 constexpr int kStages = 2;
 
-// f and 1 - f from the smaller of them, whose sign says which it is.
-__device__ __forceinline__ float packGate(const Gate &g) { return g.open > g.shut ? g.shut : -g.open; }
+// The sum of the two gates is one: the pair is kept as the smaller one, whose sign says which it is.
+__device__ __forceinline__ float packGate(float open, float shut) { return open > shut ? shut : -open; }
 __device__ __forceinline__ float openOf(float packed) { return signbit(packed) ? -packed : 1.f - packed; }
 __device__ __forceinline__ float shutOf(float packed) { return signbit(packed) ? 1.f + packed : packed; }
 
-template <class T, int PIECE, bool OWN>
-__global__ void __launch_bounds__(kThreads, 2) gatedBackward(const __grid_constant__ Pass p) {
-    constexpr int N = kLane<T>, kTensors = OWN ? 4 : 3;
+template <class T, int PIECE, bool OWN, bool TANH>
+__global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __grid_constant__ Pass p) {
+    constexpr int S = kSteps<T, OWN>, kTensors = OWN ? 4 : 3;
     extern __shared__ __align__(128) uint8_t stages[];
-    __shared__ float2 window[kWindow][32 * N], parts[kWarps][32 * N];
-    __shared__ float gradients[kWarps][32 * N];
-    __shared__ int64_t tileOf[kStages];
-    __shared__ int nearest;
+    __shared__ Map window[kGroup][32], parts[kWarps][32];   // of the tiles of a group, of the warps' tokens
+    __shared__ Pair gradients[kWarps][32];     // C
+    __shared__ Tile tiles[kStages];
+    __shared__ Pair front[32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     waitForPredecessor();
     letDependentsStart();
     Tickets tickets(p);
     if (tid == 0)
-        for (int i = 0; i < kStages; ++i) tileOf[i] = tickets.take();
+        for (int i = 0; i < kStages; ++i) tiles[i] = tileOf<T, OWN>(p, tickets.take(), true);
     __syncthreads();
     auto ask = [&](int stage) {
-        const int64_t index = tileOf[stage];
-        if (index < p.tiles) {
-            const Tile<T> tile(p, index, true);
-            const uint32_t to = umma::smemAddr(stages) + stage * kTensors * kTensorBytes<T>;
+        const Tile tile = tiles[stage];
+        if (tile.real) {
+            const uint32_t to = umma::smemAddr(stages) + stage * kTensors * kTensorBytes<OWN>;
             askFor<T, PIECE>(to, p.forget, tile, p.width);
-            askFor<T, PIECE>(to + kTensorBytes<T>, p.value, tile, p.width);
-            if (p.dout.data) askFor<T, PIECE>(to + 2 * kTensorBytes<T>, p.dout, tile, p.width);
-            if (OWN) askFor<T, PIECE>(to + 3 * kTensorBytes<T>, p.input, tile, p.width);
+            askFor<T, PIECE>(to + kTensorBytes<OWN>, p.value, tile, p.width);
+            if (p.dout.data) askFor<T, PIECE>(to + 2 * kTensorBytes<OWN>, p.dout, tile, p.width);
+            if (OWN) askFor<T, PIECE>(to + 3 * kTensorBytes<OWN>, p.input, tile, p.width);
         }
         commitCopies();
     };
     ask(0);
 
     for (int stage = 0;; stage ^= 1) {
-        const int64_t index = tileOf[stage];
-        if (index >= p.tiles) break;
-        const Tile<T> tile(p, index, true);
+        const Tile tile = tiles[stage];
+        if (!tile.real) break;
         copiesArrived<0>();
         __syncthreads();
         ask(stage ^ 1);   // what it held was read in front of the barrier
-        int64_t later = 0;
-        if (tid == 0) later = tickets.take();
+        Tile later{};
+        if (tid == 0) later = tileOf<T, OWN>(p, tickets.take(), true);
 
-        const int d = tile.d0 + lane * N, real = p.width - d;
-        float h[N];   // in front of the tile
-#pragma unroll
-        for (int v = 0; v < N; ++v) {
-            const float *from = tile.chunk > 0 ? p.marks + (static_cast<int64_t>(tile.b) * (p.chunks - 1) + tile.chunk - 1) * p.width : p.state ? p.state + static_cast<int64_t>(tile.b) * p.width : nullptr;
-            h[v] = from && v < real ? from[d + v] : 0.f;
-        }
-        const uint8_t *from = stages + stage * kTensors * kTensorBytes<T> + (warp * kSteps * 32 + lane) * N * sizeof(T);
-        const int live = tile.live - warp * kSteps;
-        auto values = [&](int s, float (&value)[N], float (&dout)[N]) {
-            const uint8_t *row = from + s * 32 * N * sizeof(T);
-            readRow<T>(row + kTensorBytes<T>, value);
-            if (p.dout.data) readRow<T>(row + 2 * kTensorBytes<T>, dout);
-            else
-#pragma unroll
-                for (int v = 0; v < N; ++v) dout[v] = 0.f;
-            if (p.tanhValue)
-#pragma unroll
-                for (int v = 0; v < N; ++v) value[v] = tanhf(value[v]);
+        const int d = tile.d0 + 2 * lane, real = p.width - d;
+        const int64_t row = static_cast<int64_t>(tile.b) * p.width + d;
+        // in front of the tile
+        Pair h = readFloats(tile.chunk > 0 ? p.marks + (static_cast<int64_t>(tile.b) * (p.chunks - 1) + tile.chunk - 1) * p.width + d : p.state ? p.state + row : nullptr, real);
+        constexpr int kRow = kChannels * sizeof(T);
+        const uint8_t *from = stages + stage * kTensors * kTensorBytes<OWN> + warp * S * kRow + lane * 2 * sizeof(T);
+        const int live = tile.live - warp * S;
+        auto valueAt = [&](int s) {
+            const Pair c = readRow<T>(from + s * kRow + kTensorBytes<OWN>);
+            return TANH ? tanhOf(c) : c;
         };
-        auto inputGates = [&](int s, float (&input)[N]) { readRow<T>(from + s * 32 * N * sizeof(T) + 3 * kTensorBytes<T>, input); };
+        auto doutAt = [&](int s) { return p.dout.data ? readRow<T>(from + s * kRow + 2 * kTensorBytes<OWN>) : bothOf(0.f); };
+        auto inputAt = [&](int s) { return Gates(readRow<T>(from + s * kRow + 3 * kTensorBytes<OWN>)); };
 
         // the tile's maps of a state forwards, (A, B), and of a gradient backwards, (A, C)
-        float gate[kSteps][N], before[kSteps][N], A[N], B[N], C[N];
+        float gate[S][2];
+        Pair before[S], A = bothOf(1.f), B = bothOf(0.f), C = bothOf(0.f);
 #pragma unroll
-        for (int v = 0; v < N; ++v) {
-            A[v] = 1.f;
-            B[v] = C[v] = 0.f;
-        }
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            float forget[N], value[N], dout[N], input[N];
-            readRow<T>(from + s * 32 * N * sizeof(T), forget);
-            values(s, value, dout);
-            if (OWN) inputGates(s, input);
-#pragma unroll
-            for (int v = 0; v < N; ++v) {
-                const Gate f(forget[v]);
-                gate[s][v] = packGate(f);
-                const float z = OWN ? Gate(input[v]).open : f.shut;
-                before[s][v] = z * value[v];   // what the token adds, until the state in front of it is known
-                if (s < live) {
-                    A[v] *= f.open;
-                    B[v] = fmaf(f.open, B[v], before[s][v]);
-                    C[v] = fmaf(A[v], dout[v], C[v]);
-                }
+        for (int s = 0; s < S; ++s) {
+            const Gates f(readRow<T>(from + s * kRow));
+            const float2 open = floatsOf(f.open), shut = floatsOf(f.shut);
+            gate[s][0] = packGate(open.x, shut.x);
+            gate[s][1] = packGate(open.y, shut.y);
+            before[s] = mul2(OWN ? inputAt(s).open : f.shut, valueAt(s));   // what the token adds, until the state in front of it is known
+            if (s < live) {
+                A = mul2(A, f.open);
+                B = fma2(f.open, B, before[s]);
+                C = fma2(A, doutAt(s), C);
             }
         }
-#pragma unroll
-        for (int v = 0; v < N; ++v) {
-            parts[warp][lane * N + v] = make_float2(A[v], B[v]);
-            gradients[warp][lane * N + v] = C[v];
-        }
-        if (tid == 0) tileOf[stage] = later;
+        parts[warp][lane] = {A, B};
+        gradients[warp][lane] = C;
+        if (tid == 0) tiles[stage] = later;
         __syncthreads();
 
-        const int place = p.chunks - 1 - tile.chunk;
-        const int64_t link = tile.slab * p.chunks + place;
         const bool last = tile.chunk == 0;   // of the chain
-        if (warp == kWarps - 1 && !last) {
+        h = mapBefore(parts, warp)(h);
+        Map after{bothOf(1.f), bothOf(0.f)};   // of the gradient, from the tile's end to this warp's
 #pragma unroll
-            for (int v = 0; v < N; ++v) {
-                A[v] = 1.f;
-                C[v] = 0.f;
-                for (int w = kWarps - 1; w >= 0; --w) {
-                    const float a = parts[w][lane * N + v].x;
-                    A[v] *= a;
-                    C[v] = fmaf(a, C[v], gradients[w][lane * N + v]);
-                }
-            }
-            if (place > 0) tellPart<N>(p.chain, link, A, C);
+        for (int w = kWarps - 1; w > 0; --w)
+            if (w > warp) after = Map{parts[w][lane].A, gradients[w][lane]}.behind(after);
+        Map mine;
+        if (warp == 0 && !last) {   // speaks for the tile
+            mine = Map{A, C}.behind(after);
+            tellTile(p, tile, mine);
         }
-        float R[N];
-        if (place > 0) stateBefore<N>(p.chain, tile.slab, place, p.chunks, window, &nearest, R);
+        Pair R;
+        if (tile.place > 0) R = stateBefore<0>(p, tile, mine, window, front);
         else {
-#pragma unroll
-            for (int v = 0; v < N; ++v) R[v] = p.dfinal && v < real ? p.dfinal[static_cast<int64_t>(tile.b) * p.width + d + v] : 0.f;
+            R = readFloats(p.dfinal ? p.dfinal + row : nullptr, real);
+            if (warp == 0 && !last) tellStart(p, tile, R);
         }
-        if (warp == kWarps - 1 && !last) {
-            float behind[N];
+        R = after(R);
 #pragma unroll
-            for (int v = 0; v < N; ++v) behind[v] = fmaf(A[v], R[v], C[v]);
-            tellWhole<N>(p.chain, link, behind);
+        for (int s = 0; s < S; ++s) {
+            const Pair next = fma2(pairOf(openOf(gate[s][0]), openOf(gate[s][1])), h, before[s]);
+            before[s] = h;
+            h = next;   // behind the sequence's end nobody reads it
         }
-        for (int w = 0; w < warp; ++w)
+        const int here = min(p.tokens - tile.first - warp * S, S);
+        const int64_t to = (static_cast<int64_t>(tile.b) * p.tokens + tile.first + warp * S) * p.width + d;
+        const Pair minus = bothOf(-1.f);
 #pragma unroll
-            for (int v = 0; v < N; ++v) {
-                const float2 part = parts[w][lane * N + v];
-                h[v] = fmaf(part.x, h[v], part.y);
-            }
-        for (int w = kWarps - 1; w > warp; --w)
-#pragma unroll
-            for (int v = 0; v < N; ++v) R[v] = fmaf(parts[w][lane * N + v].x, R[v], gradients[w][lane * N + v]);
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int v = 0; v < N; ++v) {
-                const float next = fmaf(openOf(gate[s][v]), h[v], before[s][v]);
-                before[s][v] = h[v];
-                h[v] = next;   // behind the sequence's end nobody reads it
-            }
-        const int here = min(p.tokens - tile.first - warp * kSteps, kSteps);
-        const int64_t to = (static_cast<int64_t>(tile.b) * p.tokens + tile.first + warp * kSteps) * p.width + d;
-#pragma unroll
-        for (int s = kSteps - 1; s >= 0; --s) {
-            float value[N], dout[N], input[N], dforget[N], dvalue[N], dinput[N];
-            values(s, value, dout);
-            if (OWN) inputGates(s, input);
-#pragma unroll
-            for (int v = 0; v < N; ++v) {
-                const float f = openOf(gate[s][v]), shut = shutOf(gate[s][v]), G = s < live ? dout[v] + R[v] : 0.f;
-                float z = shut, held = before[s][v] - value[v];
+        for (int s = S - 1; s >= 0; --s) {
+            if (s >= here) continue;
+            Pair dforget = bothOf(0.f), dvalue = bothOf(0.f), dinput = bothOf(0.f);
+            if (s < live) {
+                const Pair c = valueAt(s), G = add2(doutAt(s), R);
+                const Pair open = pairOf(openOf(gate[s][0]), openOf(gate[s][1])), shut = pairOf(shutOf(gate[s][0]), shutOf(gate[s][1]));
+                Pair z = shut, held = before[s];
                 if (OWN) {
-                    const Gate i(input[v]);
+                    const Gates i = inputAt(s);
                     z = i.open;
-                    held = before[s][v];
-                    dinput[v] = s < live ? G * value[v] * (i.open * i.shut) : 0.f;
+                    dinput = mul2(mul2(G, c), mul2(i.open, i.shut));
+                } else {
+                    held = fma2(c, minus, held);
                 }
-                dforget[v] = s < live ? G * held * (f * shut) : 0.f;
-                const float slope = p.tanhValue ? fmaf(-value[v], value[v], 1.f) : 1.f;
-                dvalue[v] = s < live ? G * z * slope : 0.f;
-                if (s < live) R[v] = f * G;
+                R = mul2(open, G);
+                dforget = mul2(R, mul2(held, shut));
+                dvalue = mul2(G, z);
+                if (TANH) dvalue = mul2(dvalue, fma2(mul2(c, minus), c, bothOf(1.f)));
             }
-            if (s < here) {
-                const int64_t at = to + static_cast<int64_t>(s) * p.width;
-                if (p.dforget) writeRow<T>(static_cast<T *>(p.dforget) + at, dforget, real, p.paired);
-                if (p.dvalue) writeRow<T>(static_cast<T *>(p.dvalue) + at, dvalue, real, p.paired);
-                if (OWN && p.dinput) writeRow<T>(static_cast<T *>(p.dinput) + at, dinput, real, p.paired);
-            }
+            const int64_t at = to + static_cast<int64_t>(s) * p.width;
+            if (p.dforget) writeRow<T>(static_cast<T *>(p.dforget) + at, dforget, real, p.paired);
+            if (p.dvalue) writeRow<T>(static_cast<T *>(p.dvalue) + at, dvalue, real, p.paired);
+            if (OWN && p.dinput) writeRow<T>(static_cast<T *>(p.dinput) + at, dinput, real, p.paired);
         }
-        if (last && warp == 0 && p.dstate) {
-#pragma unroll
-            for (int v = 0; v < N; ++v)
-                if (v < real) p.dstate[static_cast<int64_t>(tile.b) * p.width + d + v] = R[v];
-        }
+        if (last && warp == 0 && p.dstate) writeFloats(p.dstate + row, R, real);
     }
 }
 
@@ -205,11 +156,11 @@ void launchBackward(const Pass &p, int type, cudaStream_t st) {
     if (p.input.data) piece = std::min(piece, pieceOf(p.input, p.batch, p.tokens, size));
     withType(type, [&](auto t) {
         using T = decltype(t);
-        auto launch = [&](auto own) {
-            constexpr bool kOwn = decltype(own)::value;
-            auto with = [&](auto bytes) {
-                const auto kernel = gatedBackward<T, decltype(bytes)::value, kOwn>;
-                const size_t smem = kStages * (kOwn ? 4 : 3) * kTensorBytes<T>;
+        auto launch = [&](auto own, auto squash) {
+            constexpr bool kOwn = decltype(own)::value, kTanh = decltype(squash)::value;
+            withPiece<T>(piece, [&](auto bytes) {
+                const auto kernel = gatedBackward<T, decltype(bytes)::value, kOwn, kTanh>;
+                const size_t smem = kStages * (kOwn ? 4 : 3) * kTensorBytes<kOwn>;
                 ensureDynamicSmem(reinterpret_cast<const void *>(kernel), smem);
                 const int resident = residentPerSm(reinterpret_cast<const void *>(kernel), kThreads, smem) * currentDevice().sms;
                 {
@@ -217,11 +168,10 @@ void launchBackward(const Pass &p, int type, cudaStream_t st) {
                     launchDependent(kernel, static_cast<unsigned>(std::min<int64_t>(p.tiles, resident)), kThreads, smem, st, p);
                 }
                 afterLaunch("gatedBackward");
-            };
-            withPiece<T>(piece, with);
+            });
         };
-        if (p.input.data) launch(std::true_type{});
-        else launch(std::false_type{});
+        if (p.input.data) p.tanhValue ? launch(std::true_type{}, std::true_type{}) : launch(std::true_type{}, std::false_type{});
+        else p.tanhValue ? launch(std::false_type{}, std::true_type{}) : launch(std::false_type{}, std::false_type{});
     });
 }
 

@@ -8,112 +8,110 @@ namespace rxmet {
 namespace gated {
 namespace {
 
-template <class T, int PIECE, bool OWN, bool TANH>
+template <class T, Copy COPY, bool OWN, bool TANH>
 __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __grid_constant__ Pass p) {
     constexpr int S = kSteps<T, OWN>, kRow = kChannels * sizeof(T);
-    extern __shared__ __align__(128) uint8_t raw[];                                                  // the rows of the tile to come
-    ulonglong2(*const held)[kThreads] = reinterpret_cast<ulonglong2(*)[kThreads]>(raw + (OWN ? 3 : 2) * kTensorBytes<OWN>);   // (f, z c) of the one that waits for its state, each thread's own
-    __shared__ Map shared[kWarps][32];   // of the warps' tokens; of the tiles of a group
-    __shared__ Tile tiles[2];
+    constexpr uint32_t kStageBytes = (OWN ? 3 : 2) * kTensorBytes<OWN>;
+    extern __shared__ __align__(128) uint8_t stages[];
+    __shared__ Map window[kGroup][32], parts[kWarps][32];   // of the tiles of a group, of the tokens of the warps
+    __shared__ Tile tiles[kStages];
     __shared__ Pair front[32];
+    __shared__ __align__(8) uint64_t full[kStages];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0 && COPY == Copy::Boxes) {
+        for (int i = 0; i < kStages; ++i) cluster::initBarrier(&full[i], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     waitForPredecessor();
     letDependentsStart();
     Tickets tickets(p);
-    if (tid == 0) tiles[0] = tileOf<T, OWN>(p, tickets.take(), false);
-    __syncthreads();
-    auto ask = [&](const Tile &tile) {
-        if (tile.real) {
-            const uint32_t to = umma::smemAddr(raw);
-            askFor<T, PIECE>(to, p.forget, tile, p.width);
-            askFor<T, PIECE>(to + kTensorBytes<OWN>, p.value, tile, p.width);
-            if (OWN) askFor<T, PIECE>(to + 2 * kTensorBytes<OWN>, p.input, tile, p.width);
+    if (tid == 0)
+        for (int i = 0; i < kStages; ++i) {
+            tiles[i] = tileOf<T, OWN>(p, tickets.take(), false);
+            tickets.ask();
         }
-        commitCopies();
-    };
-    ask(tiles[0]);
+    __syncthreads();
+    auto rows = [&](int stage) { return Rows<T, OWN, COPY>{umma::smemAddr(stages) + stage * kStageBytes, &full[stage]}; };
+    constexpr unsigned kUsed = OWN ? 7 : 3;
+    for (int i = 0; i < kStages; ++i) rows(i).ask(p, tiles[i], kUsed);
 
-    Tile waiting{};
-    Map ahead, mine;   // of the waiting tile: what lies in front of the warp's tokens, the whole tile
-    for (int turn = 0;; turn ^= 1) {
-        // the next tile's gates and its map, which nobody has to wait for ...
-        const Tile tile = tiles[turn];
+    uint32_t parities = 0;   // of the stages
+    for (int stage = 0;; stage ^= 1) {
+        const Tile tile = tiles[stage];
+        if (!tile.real) break;
+        Tile later{};
+        if (tid == 0) {
+            later = tileOf<T, OWN>(p, tickets.take(), false);
+            tickets.ask();
+        }
+        if (!rows(stage).arrived(tile, parities >> stage & 1)) gaveUp(p.chain);
+        if (tile.live > 0) parities ^= 1u << stage;
+        if (COPY != Copy::Boxes) __syncthreads();
+
+        const uint8_t *from = stages + stage * kStageBytes + warp * S * kRow + lane * 2 * sizeof(T);
         Pair a[S], b[S];
-        Map nextAhead, nextMine;
-        if (tile.real) {
-            Tile later{};
-            if (tid == 0) later = tileOf<T, OWN>(p, tickets.take(), false);
-            copiesArrived<0>();
-            __syncthreads();
-            const uint8_t *from = raw + warp * S * kRow + lane * 2 * sizeof(T);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const Gates f(readRow<T>(from + s * kRow));
+            Pair c = readRow<T>(from + s * kRow + kTensorBytes<OWN>), z = f.shut;
+            if (TANH) c = tanhOf(c);
+            if (OWN) z = Gates(readRow<T>(from + s * kRow + 2 * kTensorBytes<OWN>)).open;
+            a[s] = f.open;
+            b[s] = mul2(z, c);
+        }
+        const int live = tile.live - warp * S;   // of this warp's tokens
+        if (live < S) {                          // what lies behind the sequence may be anything
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                const Gates f(readRow<T>(from + s * kRow));
-                Pair c = readRow<T>(from + s * kRow + kTensorBytes<OWN>), z = f.shut;
-                if (TANH) c = tanhOf(c);
-                if (OWN) z = Gates(readRow<T>(from + s * kRow + 2 * kTensorBytes<OWN>)).open;
-                a[s] = f.open;
-                b[s] = mul2(z, c);
-            }
-            const int live = tile.live - warp * S;   // of this warp's tokens
-            if (live < S) {                          // what lies behind the sequence may be anything
-#pragma unroll
-                for (int s = 0; s < S; ++s) {
-                    a[s] = s < live ? a[s] : bothOf(1.f);
-                    b[s] = s < live ? b[s] : bothOf(0.f);
-                }
-            }
-            Map own{a[0], b[0]};
-#pragma unroll
-            for (int s = 1; s < S; ++s) own = Map{a[s], b[s]}.behind(own);
-            shared[warp][lane] = own;
-            if (tid == 0) tiles[turn ^ 1] = later;
-            __syncthreads();
-            ask(tiles[turn ^ 1]);
-            nextAhead = mapBefore(shared, warp);
-            if (warp == kWarps - 1 && tile.chunk + 1 < p.chunks) {
-                nextMine = own.behind(nextAhead);
-                tellTile(p, tile, nextMine);
+                a[s] = s < live ? a[s] : bothOf(1.f);
+                b[s] = s < live ? b[s] : bothOf(0.f);
             }
         }
-        // ... and the outputs of the one before, whose state has had that long to come
-        if (waiting.real) {
-            const int d = waiting.d0 + 2 * lane, real = p.width - d, live = waiting.live - warp * S;
-            const bool last = waiting.chunk + 1 == p.chunks;
-            const int64_t row = static_cast<int64_t>(waiting.b) * p.width + d;
-            Pair h;
-            if (waiting.place > 0) h = stateBefore<kWarps - 1>(p, waiting, mine, shared, front);
-            else {
-                h = readFloats(p.state ? p.state + row : nullptr, real);
-                if (warp == 0 && !last) tellStart(p, waiting, h);
-            }
-            if (warp == 0 && p.marks && waiting.chunk > 0) writeFloats(p.marks + (static_cast<int64_t>(waiting.b) * (p.chunks - 1) + waiting.chunk - 1) * p.width + d, h, real);
-            h = ahead(h);
-            const int here = min(p.tokens - waiting.first - warp * S, S);   // tokens that have an output
-            T *to = static_cast<T *>(p.out) + (static_cast<int64_t>(waiting.b) * p.tokens + waiting.first + warp * S) * p.width + d;
-            if (live >= S && p.paired && p.out) {
+        Map own{a[0], b[0]};
 #pragma unroll
-                for (int s = 0; s < S; ++s, to += p.width) {
-                    const ulonglong2 map = held[s][tid];
-                    h = fma2(map.x, h, map.y);
-                    writeRow<T>(to, h, real, true);
-                }
-            } else {
-#pragma unroll 1
-                for (int s = 0; s < S; ++s, to += p.width) {
-                    const ulonglong2 map = held[s][tid];
-                    h = fma2(map.x, h, map.y);
-                    if (p.out && s < here) writeRow<T>(to, s < live ? h : bothOf(0.f), real, p.paired);
-                }
-            }
-            if (last && warp == kWarps - 1 && p.finalState) writeFloats(p.finalState + row, h, real);
+        for (int s = 1; s < S; ++s) own = Map{a[s], b[s]}.behind(own);
+        parts[warp][lane] = own;
+        // Boxes are asked for by one thread, which leaves the tile's place behind the barrier: others may read the one at work as late as in front of it.
+        if (tid == 0 && COPY != Copy::Boxes) tiles[stage] = later;
+        __syncthreads();
+        if (tid == 0 && COPY == Copy::Boxes) tiles[stage] = later;
+        rows(stage).ask(p, COPY == Copy::Boxes ? later : tiles[stage], kUsed);
+
+        const int d = tile.d0 + 2 * lane, real = p.width - d;
+        const bool last = tile.chunk + 1 == p.chunks;
+        const Map ahead = mapBefore(parts, warp);
+        Map mine;
+        if (warp == kWarps - 1 && !last) {   // speaks for the tile
+            mine = own.behind(ahead);
+            tellTile(p, tile, mine);
         }
-        if (!tile.real) break;
+        const int64_t row = static_cast<int64_t>(tile.b) * p.width + d;
+        Pair h;
+        if (tile.place > 0) h = stateBefore<kWarps - 1>(p, tile, mine, window, front);
+        else {
+            h = readFloats(p.state ? p.state + row : nullptr, real);
+            if (warp == 0 && !last) tellStart(p, tile, h);
+        }
+        if (warp == 0 && p.marks && tile.chunk > 0) writeFloats(p.marks + (static_cast<int64_t>(tile.b) * (p.chunks - 1) + tile.chunk - 1) * p.width + d, h, real);
+        h = ahead(h);
+        const int here = min(p.tokens - tile.first - warp * S, S);   // tokens that have an output
+        T *to = static_cast<T *>(p.out) + (static_cast<int64_t>(tile.b) * p.tokens + tile.first + warp * S) * p.width + d;
+        if (live >= S && p.paired && p.out) {
 #pragma unroll
-        for (int s = 0; s < S; ++s) held[s][tid] = make_ulonglong2(a[s], b[s]);
-        waiting = tile;
-        ahead = nextAhead;
-        mine = nextMine;
+            for (int s = 0; s < S; ++s, to += p.width) {
+                h = fma2(a[s], h, b[s]);
+                writeRow<T>(to, h, real, true);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < S; ++s, to += p.width) {
+                h = fma2(a[s], h, b[s]);
+                if (p.out && s < here) writeRow<T>(to, s < live ? h : bothOf(0.f), real, p.paired);
+            }
+        }
+        if (last && warp == kWarps - 1 && p.finalState) writeFloats(p.finalState + row, h, real);
+        // `parts` is written again behind the next barrier of stateBefore's readers
+        if (tile.place == 0) __syncthreads();
     }
 }
 
@@ -202,17 +200,14 @@ void startChain(Pass &p, void *workspace, size_t bytes, cudaStream_t st) {
 
 }  // namespace
 
-void launchForward(const Pass &p, int type, cudaStream_t st) {
-    const size_t size = typeBytes(type);
-    int piece = std::min(pieceOf(p.forget, p.batch, p.tokens, size), pieceOf(p.value, p.batch, p.tokens, size));
-    if (p.input.data) piece = std::min(piece, pieceOf(p.input, p.batch, p.tokens, size));
+void launchForward(Pass &p, int type, cudaStream_t st) {
     withType(type, [&](auto t) {
         using T = decltype(t);
         auto launch = [&](auto own, auto squash) {
             constexpr bool kOwn = decltype(own)::value, kTanh = decltype(squash)::value;
-            withPiece<T>(piece, [&](auto bytes) {
-                const auto kernel = gatedForward<T, decltype(bytes)::value, kOwn, kTanh>;
-                const size_t smem = (kOwn ? 3 : 2) * kTensorBytes<kOwn> + kSteps<T, kOwn> * kThreads * sizeof(ulonglong2);
+            withCopy<T>(p, type, kOwn, [&](auto copy) {
+                const auto kernel = gatedForward<T, decltype(copy)::value, kOwn, kTanh>;
+                const size_t smem = kStages * (kOwn ? 3 : 2) * kTensorBytes<kOwn>;
                 ensureDynamicSmem(reinterpret_cast<const void *>(kernel), smem);
                 const int resident = residentPerSm(reinterpret_cast<const void *>(kernel), kThreads, smem) * currentDevice().sms;
                 {

@@ -10,6 +10,8 @@
 #include "dependent_launch.cuh"
 #include "element_types.cuh"
 #include "rxmet_b200_gated.h"
+#include "tensor_map.cuh"
+#include "umma_tiles.cuh"
 
 namespace rxmet {
 namespace gated {
@@ -18,6 +20,7 @@ using rxmet::pairOf;
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kGroup = 8;                      // tiles, at most the warps of a CTA
+constexpr int kStages = 2;
 constexpr int kChannels = 64;                  // of a tile, two a lane
 constexpr uint32_t kPollLimit = 1u << 18;      // 0.2 s of polling; a legitimate wait lasts microseconds
 
@@ -53,6 +56,7 @@ struct Pass {
     bool paired;   // two neighbours of a 16-bit output can be written at once
     int64_t tiles;
     rxmet_token_tensor forget, value, input, dout;
+    CUtensorMap maps[4];   // of these, in this order, where rows can be copied by TMA
     const int32_t *lengths;
     const float *state, *dfinal;
     void *out, *dforget, *dvalue, *dinput;
@@ -96,12 +100,8 @@ __device__ __forceinline__ Pair tanhOf(Pair x) {
     return pairOf(tanhf(v.x), tanhf(v.y));
 }
 
-// Copies of PIECE bytes from a row of channels to shared memory, `bytes` of them real and the rest zeros.
-template <int PIECE>
-__device__ __forceinline__ void copyPiece(uint32_t to, const void *from, int bytes) {
-    if constexpr (PIECE == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(PIECE), "r"(bytes) : "memory");
-}
+// A copy of four bytes to shared memory, `bytes` of them real and the rest zeros.
+__device__ __forceinline__ void copyWord(uint32_t to, const void *from, int bytes) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory"); }
 __device__ __forceinline__ void commitCopies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT>
 __device__ __forceinline__ void copiesArrived() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
@@ -130,25 +130,64 @@ __device__ __forceinline__ Tile tileOf(const Pass &p, int64_t index, bool revers
     return t;
 }
 
-// Asks for the live tokens of a tile's rows of one tensor.  A row of shared memory holds the tile's channels of one token.
-template <class T, int PIECE>
-__device__ __forceinline__ void askFor(uint32_t to, const rxmet_token_tensor &t, const Tile &tile, int width) {
-    constexpr int kRow = kChannels * sizeof(T), kPieces = kRow / PIECE, kPer = PIECE / static_cast<int>(sizeof(T));
-    const int r0 = threadIdx.x / kPieces, piece = threadIdx.x % kPieces;
-    const int real = min(kPer, width - tile.d0 - piece * kPer);
-    if (real <= 0) return;
-    constexpr int kRows = kThreads / kPieces;
-    const T *from = static_cast<const T *>(t.data) + tile.b * t.stride_b + (static_cast<int64_t>(tile.first) + r0) * t.stride_t + tile.d0 + piece * kPer;
-    const int64_t step = kRows * t.stride_t;
-    uint32_t at = to + r0 * kRow + piece * PIECE;
-    for (int r = r0; r < tile.live; r += kRows, from += step, at += kRows * kRow) {
-        if constexpr (PIECE >= 4) copyPiece<PIECE>(at, from, real * static_cast<int>(sizeof(T)));
-        else {
-            const uint16_t v = *reinterpret_cast<const uint16_t *>(from);   // rows that no asynchronous copy can take
-            asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(v) : "memory");
+__device__ __forceinline__ void gaveUp(const Chain &c) {
+    if ((threadIdx.x & 31) == 0) atomicExch(c.status, 1);   // the results are not to be used
+}
+// The rows of a stage, up to four tensors of a tile: a row of shared memory holds the tile's channels of one token.  TMA copies them as boxes, one instruction a tensor (its threads' own copies
+// took 1200 of 9500 cycles a tile), where rows start on 16 bytes; else threads do, in pieces of four bytes or of one element.
+enum class Copy { Boxes, Words, Elements };
+template <class T, bool OWN, Copy COPY>
+struct Rows {
+    uint32_t to;
+    uint64_t *bar;
+    // Of the tensors forget, value, input and dout; without an input gate dout moves up.
+    static __device__ __forceinline__ int slot(int tensor) { return tensor == 3 && !OWN ? 2 : tensor; }
+    // Copies by threads: the live tokens of one tensor.
+    __device__ __forceinline__ void copy(int place, const rxmet_token_tensor &t, const Tile &tile, int width) const {
+        constexpr int kPer = COPY == Copy::Words ? 4 / static_cast<int>(sizeof(T)) : 1, kPieces = kChannels / kPer, kRow = kChannels * sizeof(T), kRows = kThreads / kPieces;
+        const int r0 = threadIdx.x / kPieces, piece = threadIdx.x % kPieces;
+        const int real = min(kPer, width - tile.d0 - piece * kPer);
+        if (real <= 0) return;
+        const T *from = static_cast<const T *>(t.data) + tile.b * t.stride_b + (static_cast<int64_t>(tile.first) + r0) * t.stride_t + tile.d0 + piece * kPer;
+        const int64_t step = kRows * t.stride_t;
+        uint32_t at = to + place * kTensorBytes<OWN> + r0 * kRow + piece * kPer * static_cast<int>(sizeof(T));
+        for (int r = r0; r < tile.live; r += kRows, from += step, at += kRows * kRow) {
+            if constexpr (COPY == Copy::Words) copyWord(at, from, real * static_cast<int>(sizeof(T)));
+            else {
+                const uint16_t v = *reinterpret_cast<const uint16_t *>(from);   // no asynchronous copy takes two bytes
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(v) : "memory");
+            }
         }
     }
-}
+    // All threads: `used` has bit i set where tensor i is wanted.
+    __device__ __forceinline__ void ask(const Pass &p, const Tile &tile, unsigned used) const {
+        if constexpr (COPY == Copy::Boxes) {
+            if (threadIdx.x == 0 && tile.real && tile.live > 0) {
+                const uint32_t b = umma::smemAddr(bar);
+                cluster::arriveExpect(b, __popc(used) * kTensorBytes<OWN>);
+                for (int i = 0; i < 4; ++i)
+                    if (used >> i & 1)
+                        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to + slot(i) * kTensorBytes<OWN>),
+                                     "l"(&p.maps[i]), "r"(tile.d0), "r"(tile.first), "r"(tile.b), "r"(b)
+                                     : "memory");
+            }
+        } else {
+            if (tile.real) {
+                const rxmet_token_tensor *tensors[4] = {&p.forget, &p.value, &p.input, &p.dout};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (used >> i & 1) copy(slot(i), *tensors[i], tile, p.width);
+            }
+            commitCopies();
+        }
+    }
+    // The stage asked for first has arrived, before a barrier of all threads; `parity` changes with every tile that had live tokens.
+    __device__ __forceinline__ bool arrived(const Tile &tile, uint32_t parity) const {
+        if constexpr (COPY == Copy::Boxes) return tile.live == 0 || umma::waitPhase(umma::smemAddr(bar), parity);
+        else copiesArrived<1>();
+        return true;
+    }
+};
 
 // The lane's channels of a row.
 template <class T>
@@ -206,9 +245,6 @@ __device__ __forceinline__ Map mapOf(const ulonglong2 &w) {
     auto gate = [](unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v >> 32) & 0x3fffffffu); };
     return {pairOf(gate(w.x), gate(w.y)), pairOf(low(w.x), low(w.y))};
 }
-__device__ __forceinline__ void gaveUp(const Chain &c) {
-    if ((threadIdx.x & 31) == 0) atomicExch(c.status, 1);   // the results are not to be used
-}
 // (A, B) of a tile, by one warp.  Its CTA holds a lower ticket and is at work already, so that the wait ends.
 __device__ __forceinline__ Map awaitPart(const Chain &c, const unsigned long long *at) {
     for (uint32_t poll = 0; poll < kPollLimit; ++poll) {
@@ -254,7 +290,6 @@ __device__ __forceinline__ Pair awaitFront(const Chain &c, const unsigned long l
     return bothOf(0.f);
 }
 // The state in front of a tile.  All threads of the CTA.  `mine`: the tile's own map, in warp SPEAKER; `front`: a row of shared memory.
-// `window` may have been read in front of the call.
 template <int SPEAKER>
 __device__ __forceinline__ Pair stateBefore(const Pass &p, const Tile &tile, const Map &mine, Map (*window)[32], Pair *front) {
     const Chain &c = p.chain;
@@ -262,7 +297,6 @@ __device__ __forceinline__ Pair stateBefore(const Pass &p, const Tile &tile, con
     const bool speaks = k == kGroup - 1 && group + 1 < p.groups;   // for its group
     unsigned long long *parts = c.parts + (tile.slab * p.chunks + group * kGroup) * kChannels + 2 * lane;
     unsigned long long *fronts = c.fronts + (tile.slab * p.groups + group) * kChannels + 2 * lane;
-    __syncthreads();
     if (warp < k) window[warp][lane] = awaitPart(c, parts + warp * kChannels);
     Map all;
     if (speaks) {
@@ -299,37 +333,64 @@ __device__ __forceinline__ void tellTile(const Pass &p, const Tile &tile, const 
 // By one warp of a chain's first tile.
 __device__ __forceinline__ void tellStart(const Pass &p, const Tile &tile, Pair h) { tellState(p.chain.fronts + tile.slab * p.groups * kChannels + 2 * (threadIdx.x & 31), h); }
 
-// The tiles of a CTA: by tickets where tiles wait for one another, else every gridDim.x'th.  `take` is called by one thread, once for each tile.
+// The tiles of a CTA: by tickets where tiles wait for one another, else every gridDim.x'th.  One thread asks for a ticket a while before it needs it.
 struct Tickets {
     const Pass &p;
     int64_t next;
-    __device__ __forceinline__ explicit Tickets(const Pass &pass) : p(pass), next(blockIdx.x) {}
+    __device__ __forceinline__ explicit Tickets(const Pass &pass) : p(pass), next(blockIdx.x) {
+        if (threadIdx.x == 0) ask();
+    }
+    __device__ __forceinline__ void ask() {
+        if (p.chunks > 1) next = atomicAdd(p.chain.ticket, 1u);
+    }
     __device__ __forceinline__ int64_t take() {
-        if (p.chunks > 1) return atomicAdd(p.chain.ticket, 1u);
         const int64_t now = next;
-        next += gridDim.x;
+        if (p.chunks == 1) next += gridDim.x;
         return now;
     }
 };
 
-// Bytes that copies of a tensor's rows can take at once: 16, 4 or one element.
-inline int pieceOf(const rxmet_token_tensor &t, int batch, int tokens, size_t size) {
+// How the rows of a call's tensors can be copied.
+inline Copy copyOf(const rxmet_token_tensor &t, int batch, int tokens, size_t size) {
     auto fits = [&](int bytes) {
         return alignedTo(t.data, bytes) && (batch == 1 || t.stride_b * static_cast<int64_t>(size) % bytes == 0) && (tokens == 1 || t.stride_t * static_cast<int64_t>(size) % bytes == 0);
     };
-    return fits(16) ? 16 : fits(4) ? 4 : 2;
+    const bool apart = (batch == 1 || t.stride_b > 0) && (tokens == 1 || t.stride_t > 0);   // a box has no strides of zero
+    return apart && fits(16) && encodeTiled() ? Copy::Boxes : fits(4) ? Copy::Words : Copy::Elements;
 }
-// f(size of a copy) for the rows' alignment.
+inline CUtensorMap boxesOf(const rxmet_token_tensor &t, const Pass &p, int type, int boxTokens) {
+    CUtensorMap map;
+    const cuuint64_t size = typeBytes(type), width = alignUp(p.width * size, 16);
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(p.width), static_cast<cuuint64_t>(p.tokens), static_cast<cuuint64_t>(p.batch)};
+    // the distance of a single token's next one, or a single row's, does not matter
+    const cuuint64_t strides[2] = {p.tokens == 1 ? width : t.stride_t * size, p.batch == 1 ? width : t.stride_b * size};
+    const cuuint32_t box[3] = {kChannels, static_cast<cuuint32_t>(boxTokens), 1}, steps[3] = {1, 1, 1};
+    const CUtensorMapDataType kinds[] = {CU_TENSOR_MAP_DATA_TYPE_FLOAT32, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_DATA_TYPE_FLOAT16};
+    const CUresult rc = encodeTiled()(&map, kinds[type], 3, const_cast<void *>(t.data), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) fail(RXMET_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", static_cast<int>(rc));
+    return map;
+}
+// f(how to copy), and the maps in p where it is by boxes.
 template <class T, class F>
-void withPiece(int piece, F f) {
-    if (piece == 16) f(std::integral_constant<int, 16>{});
-    else if (piece == 4 || sizeof(T) == 4) f(std::integral_constant<int, 4>{});
-    else f(std::integral_constant<int, sizeof(T) == 4 ? 4 : 2>{});
+void withCopy(Pass &p, int type, bool own, F f) {
+    const rxmet_token_tensor *tensors[4] = {&p.forget, &p.value, &p.input, &p.dout};
+    Copy copy = Copy::Boxes;
+    for (const auto *t : tensors)
+        if (t->data) copy = std::max(copy, copyOf(*t, p.batch, p.tokens, typeBytes(type)));
+    if (copy == Copy::Boxes && p.tokens > 0) {
+        bindContext();
+        for (int i = 0; i < 4; ++i)
+            if (tensors[i]->data) p.maps[i] = boxesOf(*tensors[i], p, type, tokensOf(type, own));
+    }
+    if (copy == Copy::Boxes) f(std::integral_constant<Copy, Copy::Boxes>{});
+    else if (copy == Copy::Words || sizeof(T) == 4) f(std::integral_constant<Copy, Copy::Words>{});
+    else f(std::integral_constant<Copy, sizeof(T) == 4 ? Copy::Words : Copy::Elements>{});
 }
 
 // Launches of gated_recurrence.cu and gated_recurrence_backward.cu.
-void launchForward(const Pass &p, int type, cudaStream_t st);
-void launchBackward(const Pass &p, int type, cudaStream_t st);
+void launchForward(Pass &p, int type, cudaStream_t st);
+void launchBackward(Pass &p, int type, cudaStream_t st);
 
 }  // namespace gated
 }  // namespace rxmet

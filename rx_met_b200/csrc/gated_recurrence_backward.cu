@@ -12,63 +12,69 @@ namespace rxmet {
 namespace gated {
 namespace {
 
-constexpr int kStages = 2;
-
 // The sum of the two gates is one: the pair is kept as the smaller one, whose sign says which it is.
 __device__ __forceinline__ float packGate(float open, float shut) { return open > shut ? shut : -open; }
 __device__ __forceinline__ float openOf(float packed) { return signbit(packed) ? -packed : 1.f - packed; }
 __device__ __forceinline__ float shutOf(float packed) { return signbit(packed) ? 1.f + packed : packed; }
 
-template <class T, int PIECE, bool OWN, bool TANH>
+template <class T, Copy COPY, bool OWN, bool TANH>
 __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __grid_constant__ Pass p) {
     constexpr int S = kSteps<T, OWN>, kTensors = OWN ? 4 : 3;
+    constexpr uint32_t kStageBytes = kTensors * kTensorBytes<OWN>;
     extern __shared__ __align__(128) uint8_t stages[];
-    __shared__ Map window[kGroup][32], parts[kWarps][32];   // of the tiles of a group, of the warps' tokens
-    __shared__ Pair gradients[kWarps][32];     // C
+    __shared__ Map window[kGroup][32], parts[kWarps][32];   // of the tiles of a group, of the tokens of the warps
+    __shared__ Pair gradients[kWarps][32];                  // C
     __shared__ Tile tiles[kStages];
     __shared__ Pair front[32];
+    __shared__ __align__(8) uint64_t full[kStages];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0 && COPY == Copy::Boxes) {
+        for (int i = 0; i < kStages; ++i) cluster::initBarrier(&full[i], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     waitForPredecessor();
     letDependentsStart();
     Tickets tickets(p);
     if (tid == 0)
-        for (int i = 0; i < kStages; ++i) tiles[i] = tileOf<T, OWN>(p, tickets.take(), true);
-    __syncthreads();
-    auto ask = [&](int stage) {
-        const Tile tile = tiles[stage];
-        if (tile.real) {
-            const uint32_t to = umma::smemAddr(stages) + stage * kTensors * kTensorBytes<OWN>;
-            askFor<T, PIECE>(to, p.forget, tile, p.width);
-            askFor<T, PIECE>(to + kTensorBytes<OWN>, p.value, tile, p.width);
-            if (p.dout.data) askFor<T, PIECE>(to + 2 * kTensorBytes<OWN>, p.dout, tile, p.width);
-            if (OWN) askFor<T, PIECE>(to + 3 * kTensorBytes<OWN>, p.input, tile, p.width);
+        for (int i = 0; i < kStages; ++i) {
+            tiles[i] = tileOf<T, OWN>(p, tickets.take(), true);
+            tickets.ask();
         }
-        commitCopies();
-    };
-    ask(0);
+    __syncthreads();
+    auto rows = [&](int stage) { return Rows<T, OWN, COPY>{umma::smemAddr(stages) + stage * kStageBytes, &full[stage]}; };
+    constexpr int kDout = OWN ? 3 : 2;   // its place in a stage
+    const unsigned used = 3u | (OWN ? 4u : 0u) | (p.dout.data ? 8u : 0u);
+    rows(0).ask(p, tiles[0], used);
+    if (COPY != Copy::Boxes) commitCopies();
 
+    uint32_t parities = 0;   // of the stages
     for (int stage = 0;; stage ^= 1) {
         const Tile tile = tiles[stage];
         if (!tile.real) break;
-        copiesArrived<0>();
+        if (!rows(stage).arrived(tile, parities >> stage & 1)) gaveUp(p.chain);
+        if (tile.live > 0) parities ^= 1u << stage;
         __syncthreads();
-        ask(stage ^ 1);   // what it held was read in front of the barrier
+        rows(stage ^ 1).ask(p, tiles[stage ^ 1], used);   // what it held was read in front of the barrier
+        if (COPY != Copy::Boxes) commitCopies();
         Tile later{};
-        if (tid == 0) later = tileOf<T, OWN>(p, tickets.take(), true);
+        if (tid == 0) {
+            later = tileOf<T, OWN>(p, tickets.take(), true);
+            tickets.ask();
+        }
 
         const int d = tile.d0 + 2 * lane, real = p.width - d;
         const int64_t row = static_cast<int64_t>(tile.b) * p.width + d;
         // in front of the tile
         Pair h = readFloats(tile.chunk > 0 ? p.marks + (static_cast<int64_t>(tile.b) * (p.chunks - 1) + tile.chunk - 1) * p.width + d : p.state ? p.state + row : nullptr, real);
         constexpr int kRow = kChannels * sizeof(T);
-        const uint8_t *from = stages + stage * kTensors * kTensorBytes<OWN> + warp * S * kRow + lane * 2 * sizeof(T);
+        const uint8_t *from = stages + stage * kStageBytes + warp * S * kRow + lane * 2 * sizeof(T);
         const int live = tile.live - warp * S;
         auto valueAt = [&](int s) {
             const Pair c = readRow<T>(from + s * kRow + kTensorBytes<OWN>);
             return TANH ? tanhOf(c) : c;
         };
-        auto doutAt = [&](int s) { return p.dout.data ? readRow<T>(from + s * kRow + 2 * kTensorBytes<OWN>) : bothOf(0.f); };
-        auto inputAt = [&](int s) { return Gates(readRow<T>(from + s * kRow + 3 * kTensorBytes<OWN>)); };
+        auto doutAt = [&](int s) { return p.dout.data ? readRow<T>(from + s * kRow + kDout * kTensorBytes<OWN>) : bothOf(0.f); };
+        auto inputAt = [&](int s) { return Gates(readRow<T>(from + s * kRow + 2 * kTensorBytes<OWN>)); };
 
         // the tile's maps of a state forwards, (A, B), and of a gradient backwards, (A, C)
         float gate[S][2];
@@ -149,17 +155,13 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
 
 }  // namespace
 
-void launchBackward(const Pass &p, int type, cudaStream_t st) {
-    const size_t size = typeBytes(type);
-    int piece = std::min(pieceOf(p.forget, p.batch, p.tokens, size), pieceOf(p.value, p.batch, p.tokens, size));
-    if (p.dout.data) piece = std::min(piece, pieceOf(p.dout, p.batch, p.tokens, size));
-    if (p.input.data) piece = std::min(piece, pieceOf(p.input, p.batch, p.tokens, size));
+void launchBackward(Pass &p, int type, cudaStream_t st) {
     withType(type, [&](auto t) {
         using T = decltype(t);
         auto launch = [&](auto own, auto squash) {
             constexpr bool kOwn = decltype(own)::value, kTanh = decltype(squash)::value;
-            withPiece<T>(piece, [&](auto bytes) {
-                const auto kernel = gatedBackward<T, decltype(bytes)::value, kOwn, kTanh>;
+            withCopy<T>(p, type, kOwn, [&](auto copy) {
+                const auto kernel = gatedBackward<T, decltype(copy)::value, kOwn, kTanh>;
                 const size_t smem = kStages * (kOwn ? 4 : 3) * kTensorBytes<kOwn>;
                 ensureDynamicSmem(reinterpret_cast<const void *>(kernel), smem);
                 const int resident = residentPerSm(reinterpret_cast<const void *>(kernel), kThreads, smem) * currentDevice().sms;

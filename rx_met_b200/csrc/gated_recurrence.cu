@@ -13,6 +13,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
     constexpr int S = kSteps<T, OWN>, kRow = kChannels * sizeof(T);
     constexpr uint32_t kStageBytes = (OWN ? 3 : 2) * kTensorBytes<OWN>;
     extern __shared__ __align__(128) uint8_t stages[];
+    uint8_t *const outputs = stages + kStages * kStageBytes;
     __shared__ Map window[kGroup][32], parts[kWarps][32];   // of the tiles of a group, of the tokens of the warps
     __shared__ Tile tiles[kStages];
     __shared__ Pair front[32];
@@ -52,10 +53,10 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
         Pair a[S], b[S];
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const Gates f(readRow<T>(from + s * kRow));
+            const Gates<T> f(from + s * kRow);
             Pair c = readRow<T>(from + s * kRow + kTensorBytes<OWN>), z = f.shut;
             if (TANH) c = tanhOf(c);
-            if (OWN) z = Gates(readRow<T>(from + s * kRow + 2 * kTensorBytes<OWN>)).open;
+            if (OWN) z = Gates<T>(from + s * kRow + 2 * kTensorBytes<OWN>).open;
             a[s] = f.open;
             b[s] = mul2(z, c);
         }
@@ -73,6 +74,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
         parts[warp][lane] = own;
         // Boxes are asked for by one thread, which leaves the tile's place behind the barrier: others may read the one at work as late as in front of it.
         if (tid == 0 && COPY != Copy::Boxes) tiles[stage] = later;
+        if (tid == 0) storesRead();
         __syncthreads();
         if (tid == 0 && COPY == Copy::Boxes) tiles[stage] = later;
         rows(stage).ask(p, COPY == Copy::Boxes ? later : tiles[stage], kUsed);
@@ -94,25 +96,34 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
         }
         if (warp == 0 && p.marks && tile.chunk > 0) writeFloats(p.marks + (static_cast<int64_t>(tile.b) * (p.chunks - 1) + tile.chunk - 1) * p.width + d, h, real);
         h = ahead(h);
-        const int here = min(p.tokens - tile.first - warp * S, S);   // tokens that have an output
-        T *to = static_cast<T *>(p.out) + (static_cast<int64_t>(tile.b) * p.tokens + tile.first + warp * S) * p.width + d;
-        if (live >= S && p.paired && p.out) {
+        if (p.outBoxes) {
+            uint8_t *to = outputs + warp * S * kRow + lane * 2 * sizeof(T);
 #pragma unroll
-            for (int s = 0; s < S; ++s, to += p.width) {
+            for (int s = 0; s < S; ++s) {
                 h = fma2(a[s], h, b[s]);
-                writeRow<T>(to, h, real, true);
+                keepRow<T>(to + s * kRow, h);
+            }
+            if (live < S)
+                for (int s = max(live, 0); s < S; ++s) keepRow<T>(to + s * kRow, bothOf(0.f));
+            ummatiles::fenceAsyncProxy();
+            __syncthreads();
+            if (tid == 0) {
+                storeBox(&p.outMaps[0], umma::smemAddr(outputs), tile);
+                commitStores();
             }
         } else {
+            const int here = min(p.tokens - tile.first - warp * S, S);   // tokens that have an output
+            T *to = static_cast<T *>(p.out) + (static_cast<int64_t>(tile.b) * p.tokens + tile.first + warp * S) * p.width + d;
 #pragma unroll
             for (int s = 0; s < S; ++s, to += p.width) {
                 h = fma2(a[s], h, b[s]);
                 if (p.out && s < here) writeRow<T>(to, s < live ? h : bothOf(0.f), real, p.paired);
             }
+            __syncthreads();   // `parts` is written again
         }
         if (last && warp == kWarps - 1 && p.finalState) writeFloats(p.finalState + row, h, real);
-        // `parts` is written again behind the next barrier of stateBefore's readers
-        if (tile.place == 0) __syncthreads();
     }
+    if (tid == 0) storesRead();
 }
 
 // Single tokens: a thread for two neighbouring channels of a row.
@@ -124,20 +135,21 @@ __global__ void __launch_bounds__(kThreads) gatedStep(const __grid_constant__ Pa
     letDependentsStart();
     if (b >= p.batch) return;
     const bool live = !p.lengths || p.lengths[b] > 0;
-    auto at = [&](const rxmet_token_tensor &t, int v) { return toFloat(static_cast<const T *>(t.data)[b * t.stride_b + d + v]); };
+    auto at = [&](const rxmet_token_tensor &t, int v) { return static_cast<const T *>(t.data)[b * t.stride_b + d + v]; };
     const int64_t row = static_cast<int64_t>(b) * p.width + d;
     const int count = min(2, p.width - d);
-    float forget[2], value[2], input[2], h[2];
+    alignas(8) T forget[2], input[2];
+    float value[2], h[2];
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
         const int u = min(v, count - 1);
         forget[v] = at(p.forget, u);
-        value[v] = at(p.value, u);
+        value[v] = toFloat(at(p.value, u));
         if (OWN) input[v] = at(p.input, u);
         h[v] = p.state ? p.state[row + u] : 0.f;
     }
-    const Gates forgets(pairOf(forget[0], forget[1]));
-    const float2 f = floatsOf(forgets.open), z = floatsOf(OWN ? Gates(pairOf(input[0], input[1])).open : forgets.shut);
+    const Gates<T> forgets(reinterpret_cast<const uint8_t *>(forget));
+    const float2 f = floatsOf(forgets.open), z = floatsOf(OWN ? Gates<T>(reinterpret_cast<const uint8_t *>(input)).open : forgets.shut);
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
         if (v >= count) continue;
@@ -201,13 +213,14 @@ void startChain(Pass &p, void *workspace, size_t bytes, cudaStream_t st) {
 }  // namespace
 
 void launchForward(Pass &p, int type, cudaStream_t st) {
+    if (p.out) mapOutputs(p, type, p.input.data != nullptr, {p.out});
     withType(type, [&](auto t) {
         using T = decltype(t);
         auto launch = [&](auto own, auto squash) {
             constexpr bool kOwn = decltype(own)::value, kTanh = decltype(squash)::value;
             withCopy<T>(p, type, kOwn, [&](auto copy) {
                 const auto kernel = gatedForward<T, decltype(copy)::value, kOwn, kTanh>;
-                const size_t smem = kStages * (kOwn ? 3 : 2) * kTensorBytes<kOwn>;
+                const size_t smem = (kStages * (kOwn ? 3 : 2) + 1) * kTensorBytes<kOwn>;
                 ensureDynamicSmem(reinterpret_cast<const void *>(kernel), smem);
                 const int resident = residentPerSm(reinterpret_cast<const void *>(kernel), kThreads, smem) * currentDevice().sms;
                 {

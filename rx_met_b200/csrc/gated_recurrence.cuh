@@ -57,6 +57,8 @@ struct Pass {
     int64_t tiles;
     rxmet_token_tensor forget, value, input, dout;
     CUtensorMap maps[4];   // of these, in this order, where rows can be copied by TMA
+    CUtensorMap outMaps[3];   // of out, or of dforget, dvalue and dinput, likewise
+    bool outBoxes;
     const int32_t *lengths;
     const float *state, *dfinal;
     void *out, *dforget, *dvalue, *dinput;
@@ -64,28 +66,47 @@ struct Pass {
     Chain chain;
 };
 
-// exp(-x) of two values.  The product x log2(e) is rounded to 24 bits, and what that leaves out is put back, so that the result is as exact as the exponential itself (2 units) for
-// every x; beyond 87 either way sigmoid(x) and its complement are 0 and 1 to 2^-125.  A NaN stays one.
-__device__ __forceinline__ Pair exponentials(Pair x) {
-    const float2 v = floatsOf(x);
-    float a, b;
-    asm("max.NaN.f32 %0, %1, 0fC2AE0000;\n\tmin.NaN.f32 %0, %0, 0f42AE0000;" : "=f"(a) : "f"(v.x));
-    asm("max.NaN.f32 %0, %1, 0fC2AE0000;\n\tmin.NaN.f32 %0, %0, 0f42AE0000;" : "=f"(b) : "f"(v.y));
-    const Pair held = pairOf(a, b), log2e = pairOf(-1.4426950408889634f, -1.4426950408889634f), rest = pairOf(-1.925963033500e-8f, -1.925963033500e-8f);
-    const Pair u = mul2(held, log2e);
-    const float2 whole = floatsOf(u);
-    const Pair left = fma2(held, rest, fma2(held, log2e, pairOf(-whole.x, -whole.y)));
-    float c, d;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(c) : "f"(whole.x));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(whole.y));
-    const Pair e = pairOf(c, d);
-    return fma2(mul2(e, left), pairOf(0.6931471805599453f, 0.6931471805599453f), e);
+// x of two channels between -87 and 87, beyond which sigmoid(x) and its complement are 0 and 1 to 2^-125; a NaN stays one.
+template <class T>
+__device__ __forceinline__ Pair clampRow(const uint8_t *row) {
+    if constexpr (sizeof(T) == 4) {
+        const float2 v = *reinterpret_cast<const float2 *>(row);
+        float a, b;
+        asm("max.NaN.f32 %0, %1, 0fC2AE0000;\n\tmin.NaN.f32 %0, %0, 0f42AE0000;" : "=f"(a) : "f"(v.x));
+        asm("max.NaN.f32 %0, %1, 0fC2AE0000;\n\tmin.NaN.f32 %0, %0, 0f42AE0000;" : "=f"(b) : "f"(v.y));
+        return pairOf(a, b);
+    } else {
+        uint32_t w = *reinterpret_cast<const uint32_t *>(row);
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) asm("max.NaN.bf16x2 %0, %0, %1;\n\tmin.NaN.bf16x2 %0, %0, %2;" : "+r"(w) : "r"(0xc2aec2aeu), "r"(0x42ae42aeu));
+        else asm("max.NaN.f16x2 %0, %0, %1;\n\tmin.NaN.f16x2 %0, %0, %2;" : "+r"(w) : "r"(0xd570d570u), "r"(0x55705570u));
+        const float2 v = unpack2<T>(w);
+        return pairOf(v.x, v.y);
+    }
 }
-// sigmoid(x), and 1 - sigmoid(x) without the bits that a subtraction from one would lose, of two values.
+// exp(-x) of two such values: 2^u with u = -x log2(e) to 24 bits, times 1 + what u leaves out.  Of 16-bit types, x of 8 or 11 bits times the upper 16 or 13 bits of log2(e) is exact, and x times the
+// rest is left out; of floats, the rounding of u as well.  As exact as the exponential itself, 2 units (of half, beyond 16: 2^-17 at 87).
+template <class T>
+__device__ __forceinline__ Pair exponentials(Pair x) {
+    constexpr bool kShort = sizeof(T) == 2, kBf16 = std::is_same_v<T, __nv_bfloat16>;
+    constexpr float kUpper = kBf16 ? 1.44268798828125f : kShort ? 1.442626953125f : 1.4426950408889634f;
+    constexpr float kRest = kBf16 ? 7.0526077e-6f : kShort ? 6.8087764e-5f : 1.925963033500e-8f, kLn2 = 0.6931471805599453f;
+    const Pair u = mul2(x, pairOf(-kUpper, -kUpper));
+    const float2 v = floatsOf(u);
+    Pair left;
+    if constexpr (kShort) left = mul2(x, pairOf(-kRest * kLn2, -kRest * kLn2));
+    else left = mul2(fma2(x, pairOf(-kRest, -kRest), fma2(x, pairOf(-kUpper, -kUpper), pairOf(-v.x, -v.y))), pairOf(kLn2, kLn2));
+    float c, d;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(c) : "f"(v.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(v.y));
+    const Pair e = pairOf(c, d);
+    return fma2(e, left, e);
+}
+// sigmoid(x), and 1 - sigmoid(x) without the bits that a subtraction from one would lose, of the two channels of a row.
+template <class T>
 struct Gates {
     Pair open, shut;
-    __device__ __forceinline__ explicit Gates(Pair x) {
-        const Pair e = exponentials(x);
+    __device__ __forceinline__ explicit Gates(Pair clamped) {
+        const Pair e = exponentials<T>(clamped);
         const float2 sum = floatsOf(add2(e, pairOf(1.f, 1.f)));
         float a, b;
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(sum.x));   // one unit in the last place
@@ -93,6 +114,7 @@ struct Gates {
         open = pairOf(a, b);
         shut = mul2(e, open);
     }
+    __device__ __forceinline__ explicit Gates(const uint8_t *row) : Gates(clampRow<T>(row)) {}
 };
 __device__ __forceinline__ Pair bothOf(float v) { return pairOf(v, v); }
 __device__ __forceinline__ Pair tanhOf(Pair x) {
@@ -189,7 +211,19 @@ struct Rows {
     }
 };
 
+// A tile of an output from shared memory, by one thread; what lies beyond the array is left out.  Those that it began have been read once `stored` returns.
+__device__ __forceinline__ void storeBox(const CUtensorMap *map, uint32_t from, const Tile &tile) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(tile.d0), "r"(tile.first), "r"(tile.b), "r"(from) : "memory");
+}
+__device__ __forceinline__ void commitStores() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void storesRead() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
 // The lane's channels of a row.
+template <class T>
+__device__ __forceinline__ void keepRow(uint8_t *row, Pair v) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<Pair *>(row) = v;
+    else *reinterpret_cast<uint32_t *>(row) = pack2<T>(v);
+}
 template <class T>
 __device__ __forceinline__ Pair readRow(const uint8_t *row) {
     if constexpr (sizeof(T) == 4) return *reinterpret_cast<const Pair *>(row);
@@ -370,6 +404,19 @@ inline CUtensorMap boxesOf(const rxmet_token_tensor &t, const Pass &p, int type,
                                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (rc != CUDA_SUCCESS) fail(RXMET_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", static_cast<int>(rc));
     return map;
+}
+// The maps of the outputs, where all rows of all of them start on 16 bytes.
+inline void mapOutputs(Pass &p, int type, bool own, std::initializer_list<void *> outputs) {
+    const int64_t pitch = static_cast<int64_t>(p.width) * static_cast<int64_t>(typeBytes(type));
+    p.outBoxes = encodeTiled() && pitch % 16 == 0 && p.tokens > 0;
+    for (void *out : outputs) p.outBoxes = p.outBoxes && alignedTo(out, 16);
+    if (!p.outBoxes) return;
+    bindContext();
+    int i = 0;
+    for (void *out : outputs) {
+        if (out) p.outMaps[i] = boxesOf({out, static_cast<int64_t>(p.tokens) * p.width, p.width}, p, type, tokensOf(type, own));
+        ++i;
+    }
 }
 // f(how to copy), and the maps in p where it is by boxes.
 template <class T, class F>

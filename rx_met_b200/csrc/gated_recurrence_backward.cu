@@ -54,7 +54,8 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
         if (!rows(stage).arrived(tile, parities >> stage & 1)) gaveUp(p.chain);
         if (tile.live > 0) parities ^= 1u << stage;
         __syncthreads();
-        rows(stage ^ 1).ask(p, tiles[stage ^ 1], used);   // what it held was read in front of the barrier
+        if (tid == 0) storesRead();
+        rows(stage ^ 1).ask(p, tiles[stage ^ 1], used);   // what it held was read in front of the barrier, or left by a store
         if (COPY != Copy::Boxes) commitCopies();
         Tile later{};
         if (tid == 0) {
@@ -67,21 +68,21 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
         // in front of the tile
         Pair h = readFloats(tile.chunk > 0 ? p.marks + (static_cast<int64_t>(tile.b) * (p.chunks - 1) + tile.chunk - 1) * p.width + d : p.state ? p.state + row : nullptr, real);
         constexpr int kRow = kChannels * sizeof(T);
-        const uint8_t *from = stages + stage * kStageBytes + warp * S * kRow + lane * 2 * sizeof(T);
+        uint8_t *from = stages + stage * kStageBytes + warp * S * kRow + lane * 2 * sizeof(T);
         const int live = tile.live - warp * S;
         auto valueAt = [&](int s) {
             const Pair c = readRow<T>(from + s * kRow + kTensorBytes<OWN>);
             return TANH ? tanhOf(c) : c;
         };
         auto doutAt = [&](int s) { return p.dout.data ? readRow<T>(from + s * kRow + kDout * kTensorBytes<OWN>) : bothOf(0.f); };
-        auto inputAt = [&](int s) { return Gates(readRow<T>(from + s * kRow + 2 * kTensorBytes<OWN>)); };
+        auto inputAt = [&](int s) { return Gates<T>(from + s * kRow + 2 * kTensorBytes<OWN>); };
 
         // the tile's maps of a state forwards, (A, B), and of a gradient backwards, (A, C)
         float gate[S][2];
         Pair before[S], A = bothOf(1.f), B = bothOf(0.f), C = bothOf(0.f);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const Gates f(readRow<T>(from + s * kRow));
+            const Gates<T> f(from + s * kRow);
             const float2 open = floatsOf(f.open), shut = floatsOf(f.shut);
             gate[s][0] = packGate(open.x, shut.x);
             gate[s][1] = packGate(open.y, shut.y);
@@ -124,16 +125,16 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
         const int here = min(p.tokens - tile.first - warp * S, S);
         const int64_t to = (static_cast<int64_t>(tile.b) * p.tokens + tile.first + warp * S) * p.width + d;
         const Pair minus = bothOf(-1.f);
+        // gradients of a token take the place of what they come from, if a box of them can be stored
 #pragma unroll
         for (int s = S - 1; s >= 0; --s) {
-            if (s >= here) continue;
             Pair dforget = bothOf(0.f), dvalue = bothOf(0.f), dinput = bothOf(0.f);
             if (s < live) {
                 const Pair c = valueAt(s), G = add2(doutAt(s), R);
                 const Pair open = pairOf(openOf(gate[s][0]), openOf(gate[s][1])), shut = pairOf(shutOf(gate[s][0]), shutOf(gate[s][1]));
                 Pair z = shut, held = before[s];
                 if (OWN) {
-                    const Gates i = inputAt(s);
+                    const Gates<T> i = inputAt(s);
                     z = i.open;
                     dinput = mul2(mul2(G, c), mul2(i.open, i.shut));
                 } else {
@@ -144,18 +145,38 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
                 dvalue = mul2(G, z);
                 if (TANH) dvalue = mul2(dvalue, fma2(mul2(c, minus), c, bothOf(1.f)));
             }
-            const int64_t at = to + static_cast<int64_t>(s) * p.width;
-            if (p.dforget) writeRow<T>(static_cast<T *>(p.dforget) + at, dforget, real, p.paired);
-            if (p.dvalue) writeRow<T>(static_cast<T *>(p.dvalue) + at, dvalue, real, p.paired);
-            if (OWN && p.dinput) writeRow<T>(static_cast<T *>(p.dinput) + at, dinput, real, p.paired);
+            if (p.outBoxes) {
+                uint8_t *row = from + s * kRow;
+                keepRow<T>(row, dforget);
+                keepRow<T>(row + kTensorBytes<OWN>, dvalue);
+                if (OWN) keepRow<T>(row + 2 * kTensorBytes<OWN>, dinput);
+            } else if (s < here) {
+                const int64_t at = to + static_cast<int64_t>(s) * p.width;
+                if (p.dforget) writeRow<T>(static_cast<T *>(p.dforget) + at, dforget, real, p.paired);
+                if (p.dvalue) writeRow<T>(static_cast<T *>(p.dvalue) + at, dvalue, real, p.paired);
+                if (OWN && p.dinput) writeRow<T>(static_cast<T *>(p.dinput) + at, dinput, real, p.paired);
+            }
+        }
+        if (p.outBoxes) {
+            ummatiles::fenceAsyncProxy();
+            __syncthreads();
+            if (tid == 0) {
+                const uint32_t at = umma::smemAddr(stages) + stage * kStageBytes;
+                if (p.dforget) storeBox(&p.outMaps[0], at, tile);
+                if (p.dvalue) storeBox(&p.outMaps[1], at + kTensorBytes<OWN>, tile);
+                if (OWN && p.dinput) storeBox(&p.outMaps[2], at + 2 * kTensorBytes<OWN>, tile);
+                commitStores();
+            }
         }
         if (last && warp == 0 && p.dstate) writeFloats(p.dstate + row, R, real);
     }
+    if (tid == 0) storesRead();
 }
 
 }  // namespace
 
 void launchBackward(Pass &p, int type, cudaStream_t st) {
+    mapOutputs(p, type, p.input.data != nullptr, {p.dforget, p.dvalue, p.dinput});
     withType(type, [&](auto t) {
         using T = decltype(t);
         auto launch = [&](auto own, auto squash) {

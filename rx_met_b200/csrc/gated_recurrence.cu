@@ -51,8 +51,10 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
 
         const uint8_t *from = stages + stage * kStageBytes + warp * S * kRow + lane * 2 * sizeof(T);
         Pair a[S], b[S];
+        Before before(p, tile);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
+            if (s == S * 3 / 4) before.look();
             const Gates<T> f(from + s * kRow);
             Pair c = readRow<T>(from + s * kRow + kTensorBytes<OWN>), z = f.shut;
             if (TANH) c = tanhOf(c);
@@ -89,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
         }
         const int64_t row = static_cast<int64_t>(tile.b) * p.width + d;
         Pair h;
-        if (tile.place > 0) h = stateBefore<kWarps - 1>(p, tile, mine, window, front);
+        if (tile.place > 0) h = stateBefore<kWarps - 1>(p, tile, before, mine, window, front);
         else {
             h = readFloats(p.state ? p.state + row : nullptr, real);
             if (warp == 0 && !last) tellStart(p, tile, h);

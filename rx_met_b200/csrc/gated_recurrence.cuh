@@ -19,7 +19,7 @@ namespace gated {
 using rxmet::pairOf;
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kGroup = 8;                      // tiles, at most the warps of a CTA
+constexpr int kGroup = 8;                      // tiles; as many as a CTA has warps: all but the last wait for a tile each, the last for the front
 constexpr int kStages = 2;
 constexpr int kChannels = 64;                  // of a tile, two a lane
 constexpr uint32_t kPollLimit = 1u << 18;      // 0.2 s of polling; a legitimate wait lasts microseconds
@@ -279,25 +279,21 @@ __device__ __forceinline__ Map mapOf(const ulonglong2 &w) {
     auto gate = [](unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v >> 32) & 0x3fffffffu); };
     return {pairOf(gate(w.x), gate(w.y)), pairOf(low(w.x), low(w.y))};
 }
-// (A, B) of a tile, by one warp.  Its CTA holds a lower ticket and is at work already, so that the wait ends.
-__device__ __forceinline__ Map awaitPart(const Chain &c, const unsigned long long *at) {
+// (A, B) of a tile, by one warp, which has looked once already.  Its CTA holds a lower ticket and is at work, so that the wait ends.
+__device__ __forceinline__ Map awaitPart(const Chain &c, const unsigned long long *at, ulonglong2 w) {
     for (uint32_t poll = 0; poll < kPollLimit; ++poll) {
-        const ulonglong2 w = loadWords(at);
         if (__all_sync(0xffffffffu, w.x != 0 && w.y != 0)) return mapOf(w);
+        w = loadWords(at);
     }
     gaveUp(c);
     return {bothOf(1.f), bothOf(0.f)};
 }
-// The state in front of a group, by one warp: from the nearest of the last eight groups' fronts that is known, taken through the groups in between.
-__device__ __forceinline__ Pair awaitFront(const Chain &c, const unsigned long long *fronts, int group) {
+// The state in front of a group, by one warp, likewise: from the nearest of the last eight groups' fronts that is known, taken through the groups in between.
+__device__ __forceinline__ Pair awaitFront(const Chain &c, const unsigned long long *fronts, int group, const ulonglong2 &first) {
     constexpr int kBack = 8;
+    if (__all_sync(0xffffffffu, isWhole(first.x) && isWhole(first.y))) return mapOf(first).B;   // most often it is there
     for (uint32_t poll = 0; poll < kPollLimit; ++poll) {
         ulonglong2 w[kBack];
-        if ((poll & 1) == 0) {   // most often it is there
-            w[0] = loadWords(fronts);
-            if (__all_sync(0xffffffffu, isWhole(w[0].x) && isWhole(w[0].y))) return mapOf(w[0]).B;
-            continue;
-        }
         int nearest = kBack;   // in reach, with all behind it there
 #pragma unroll
         for (int i = 0; i < kBack; ++i) w[i] = i <= group ? loadWords(fronts - i * kChannels) : make_ulonglong2(0, 0);
@@ -323,15 +319,30 @@ __device__ __forceinline__ Pair awaitFront(const Chain &c, const unsigned long l
     gaveUp(c);
     return bothOf(0.f);
 }
+// What a warp waits for in front of a tile: the map of another tile of the group, or, the last warp, the group's front.  It looks for it while the gates are worked out, and most often finds it.
+struct Before {
+    const unsigned long long *at;
+    ulonglong2 words;
+    bool waits;
+    __device__ __forceinline__ Before(const Pass &p, const Tile &tile) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = tile.place / kGroup;
+        const bool part = warp < tile.place % kGroup;
+        waits = tile.place > 0 && (part || warp == kWarps - 1);
+        at = part ? p.chain.parts + (tile.slab * p.chunks + group * kGroup + warp) * kChannels + 2 * lane : p.chain.fronts + (tile.slab * p.groups + group) * kChannels + 2 * lane;
+        words = make_ulonglong2(0, 0);
+    }
+    __device__ __forceinline__ void look() {
+        if (waits) words = loadWords(at);
+    }
+};
 // The state in front of a tile.  All threads of the CTA.  `mine`: the tile's own map, in warp SPEAKER; `front`: a row of shared memory.
 template <int SPEAKER>
-__device__ __forceinline__ Pair stateBefore(const Pass &p, const Tile &tile, const Map &mine, Map (*window)[32], Pair *front) {
+__device__ __forceinline__ Pair stateBefore(const Pass &p, const Tile &tile, const Before &before, const Map &mine, Map (*window)[32], Pair *front) {
     const Chain &c = p.chain;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = tile.place / kGroup, k = tile.place % kGroup;
     const bool speaks = k == kGroup - 1 && group + 1 < p.groups;   // for its group
-    unsigned long long *parts = c.parts + (tile.slab * p.chunks + group * kGroup) * kChannels + 2 * lane;
-    unsigned long long *fronts = c.fronts + (tile.slab * p.groups + group) * kChannels + 2 * lane;
-    if (warp < k) window[warp][lane] = awaitPart(c, parts + warp * kChannels);
+    unsigned long long *next = c.fronts + (tile.slab * p.groups + group + 1) * kChannels + 2 * lane;
+    if (warp < k) window[warp][lane] = awaitPart(c, before.at, before.words);
     Map all;
     if (speaks) {
         if (warp == SPEAKER) window[kGroup - 1][lane] = mine;
@@ -340,13 +351,13 @@ __device__ __forceinline__ Pair stateBefore(const Pass &p, const Tile &tile, con
             all = window[0][lane];
 #pragma unroll
             for (int i = 1; i < kGroup; ++i) all = window[i][lane].behind(all);
-            tellMap(fronts + kChannels, all.A, all.B);
+            tellMap(next, all.A, all.B);
         }
     }
-    if (warp == kWarps - 1) front[lane] = awaitFront(c, fronts, group);
+    if (warp == kWarps - 1) front[lane] = awaitFront(c, before.at, group, before.words);
     __syncthreads();
     Pair h = front[lane];
-    if (speaks && warp == 0) tellState(fronts + kChannels, all(h));
+    if (speaks && warp == 0) tellState(next, all(h));
 #pragma unroll
     for (int i = 0; i < kGroup - 1; ++i)
         if (i < k) h = window[i][lane](h);

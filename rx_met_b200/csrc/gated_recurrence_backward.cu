@@ -80,8 +80,10 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
         // the tile's maps of a state forwards, (A, B), and of a gradient backwards, (A, C)
         float gate[S][2];
         Pair before[S], A = bothOf(1.f), B = bothOf(0.f), C = bothOf(0.f);
+        Before earlier(p, tile);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
+            if (s == S * 3 / 4) earlier.look();
             const Gates<T> f(from + s * kRow);
             const float2 open = floatsOf(f.open), shut = floatsOf(f.shut);
             gate[s][0] = packGate(open.x, shut.x);
@@ -110,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
             tellTile(p, tile, mine);
         }
         Pair R;
-        if (tile.place > 0) R = stateBefore<0>(p, tile, mine, window, front);
+        if (tile.place > 0) R = stateBefore<0>(p, tile, earlier, mine, window, front);
         else {
             R = readFloats(p.dfinal ? p.dfinal + row : nullptr, real);
             if (warp == 0 && !last) tellStart(p, tile, R);

@@ -44,6 +44,11 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
     auto rows = [&](int stage) { return Rows<T, OWN, COPY>{umma::smemAddr(stages) + stage * kStageBytes, &full[stage]}; };
     constexpr int kDout = OWN ? 3 : 2;   // its place in a stage
     const unsigned used = 3u | (OWN ? 4u : 0u) | (p.dout.data ? 8u : 0u);
+    if (!p.dout.data)   // zeros, which nothing writes over
+        for (int i = tid; i < kStages * static_cast<int>(kTensorBytes<OWN> / 16); i += kThreads) {
+            constexpr int kOf = kTensorBytes<OWN> / 16;
+            reinterpret_cast<uint4 *>(stages + i / kOf * kStageBytes + kDout * kTensorBytes<OWN>)[i % kOf] = make_uint4(0, 0, 0, 0);
+        }
     rows(0).ask(p, tiles[0], used);
     if (COPY != Copy::Boxes) commitCopies();
 
@@ -74,27 +79,31 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
             const Pair c = readRow<T>(from + s * kRow + kTensorBytes<OWN>);
             return TANH ? tanhOf(c) : c;
         };
-        auto doutAt = [&](int s) { return p.dout.data ? readRow<T>(from + s * kRow + kDout * kTensorBytes<OWN>) : bothOf(0.f); };
+        auto doutAt = [&](int s) { return readRow<T>(from + s * kRow + kDout * kTensorBytes<OWN>); };
         auto inputAt = [&](int s) { return Gates<T>(from + s * kRow + 2 * kTensorBytes<OWN>); };
 
-        // the tile's maps of a state forwards, (A, B), and of a gradient backwards, (A, C)
+        // the tile's maps of a state forwards, (A, B), and of a gradient backwards, (A, C); a warp whose tokens are all of the sequence has nothing to test
         float gate[S][2];
         Pair before[S], A = bothOf(1.f), B = bothOf(0.f), C = bothOf(0.f);
         Before earlier(p, tile);
+        auto mapTokens = [&](auto all) {
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            if (s == S * 3 / 4) earlier.look();
-            const Gates<T> f(from + s * kRow);
-            const float2 open = floatsOf(f.open), shut = floatsOf(f.shut);
-            gate[s][0] = packGate(open.x, shut.x);
-            gate[s][1] = packGate(open.y, shut.y);
-            before[s] = mul2(OWN ? inputAt(s).open : f.shut, valueAt(s));   // what the token adds, until the state in front of it is known
-            if (s < live) {
-                A = mul2(A, f.open);
-                B = fma2(f.open, B, before[s]);
-                C = fma2(A, doutAt(s), C);
+            for (int s = 0; s < S; ++s) {
+                if (s == S * 3 / 4) earlier.look();
+                const Gates<T> f(from + s * kRow);
+                const float2 open = floatsOf(f.open), shut = floatsOf(f.shut);
+                gate[s][0] = packGate(open.x, shut.x);
+                gate[s][1] = packGate(open.y, shut.y);
+                before[s] = mul2(OWN ? inputAt(s).open : f.shut, valueAt(s));   // what the token adds, until the state in front of it is known
+                if (decltype(all)::value || s < live) {
+                    A = mul2(A, f.open);
+                    B = fma2(f.open, B, before[s]);
+                    C = fma2(A, doutAt(s), C);
+                }
             }
-        }
+        };
+        if (live >= S) mapTokens(std::true_type{});
+        else mapTokens(std::false_type{});
         parts[warp][lane] = {A, B};
         gradients[warp][lane] = C;
         if (tid == 0) tiles[stage] = later;
@@ -128,37 +137,41 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
         const int64_t to = (static_cast<int64_t>(tile.b) * p.tokens + tile.first + warp * S) * p.width + d;
         const Pair minus = bothOf(-1.f);
         // gradients of a token take the place of what they come from, if a box of them can be stored
+        auto giveTokens = [&](auto all) {
 #pragma unroll
-        for (int s = S - 1; s >= 0; --s) {
-            Pair dforget = bothOf(0.f), dvalue = bothOf(0.f), dinput = bothOf(0.f);
-            if (s < live) {
-                const Pair c = valueAt(s), G = add2(doutAt(s), R);
-                const Pair open = pairOf(openOf(gate[s][0]), openOf(gate[s][1])), shut = pairOf(shutOf(gate[s][0]), shutOf(gate[s][1]));
-                Pair z = shut, held = before[s];
-                if (OWN) {
-                    const Gates<T> i = inputAt(s);
-                    z = i.open;
-                    dinput = mul2(mul2(G, c), mul2(i.open, i.shut));
-                } else {
-                    held = fma2(c, minus, held);
+            for (int s = S - 1; s >= 0; --s) {
+                Pair dforget = bothOf(0.f), dvalue = bothOf(0.f), dinput = bothOf(0.f);
+                if (decltype(all)::value || s < live) {
+                    const Pair c = valueAt(s), G = add2(doutAt(s), R);
+                    const Pair open = pairOf(openOf(gate[s][0]), openOf(gate[s][1])), shut = pairOf(shutOf(gate[s][0]), shutOf(gate[s][1]));
+                    Pair z = shut, held = before[s];
+                    if (OWN) {
+                        const Gates<T> i = inputAt(s);
+                        z = i.open;
+                        dinput = mul2(mul2(G, c), mul2(i.open, i.shut));
+                    } else {
+                        held = fma2(c, minus, held);
+                    }
+                    R = mul2(open, G);
+                    dforget = mul2(R, mul2(held, shut));
+                    dvalue = mul2(G, z);
+                    if (TANH) dvalue = mul2(dvalue, fma2(mul2(c, minus), c, bothOf(1.f)));
                 }
-                R = mul2(open, G);
-                dforget = mul2(R, mul2(held, shut));
-                dvalue = mul2(G, z);
-                if (TANH) dvalue = mul2(dvalue, fma2(mul2(c, minus), c, bothOf(1.f)));
+                if (decltype(all)::value || p.outBoxes) {
+                    uint8_t *row = from + s * kRow;
+                    keepRow<T>(row, dforget);
+                    keepRow<T>(row + kTensorBytes<OWN>, dvalue);
+                    if (OWN) keepRow<T>(row + 2 * kTensorBytes<OWN>, dinput);
+                } else if (s < here) {
+                    const int64_t at = to + static_cast<int64_t>(s) * p.width;
+                    if (p.dforget) writeRow<T>(static_cast<T *>(p.dforget) + at, dforget, real, p.paired);
+                    if (p.dvalue) writeRow<T>(static_cast<T *>(p.dvalue) + at, dvalue, real, p.paired);
+                    if (OWN && p.dinput) writeRow<T>(static_cast<T *>(p.dinput) + at, dinput, real, p.paired);
+                }
             }
-            if (p.outBoxes) {
-                uint8_t *row = from + s * kRow;
-                keepRow<T>(row, dforget);
-                keepRow<T>(row + kTensorBytes<OWN>, dvalue);
-                if (OWN) keepRow<T>(row + 2 * kTensorBytes<OWN>, dinput);
-            } else if (s < here) {
-                const int64_t at = to + static_cast<int64_t>(s) * p.width;
-                if (p.dforget) writeRow<T>(static_cast<T *>(p.dforget) + at, dforget, real, p.paired);
-                if (p.dvalue) writeRow<T>(static_cast<T *>(p.dvalue) + at, dvalue, real, p.paired);
-                if (OWN && p.dinput) writeRow<T>(static_cast<T *>(p.dinput) + at, dinput, real, p.paired);
-            }
-        }
+        };
+        if (live >= S && p.outBoxes) giveTokens(std::true_type{});
+        else giveTokens(std::false_type{});
         if (p.outBoxes) {
             ummatiles::fenceAsyncProxy();
             __syncthreads();

@@ -15,7 +15,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
     extern __shared__ __align__(128) uint8_t stages[];
     uint8_t *const outputs = stages + kStages * kStageBytes;
     __shared__ Map window[kGroup][32], parts[kWarps][32];   // of the tiles of a group, of the tokens of the warps
-    __shared__ Tile tiles[kStages];
+    __shared__ Tile tiles[kPlaces];
     __shared__ Pair front[32];
     __shared__ __align__(8) uint64_t full[kStages];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -37,8 +37,8 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
     for (int i = 0; i < kStages; ++i) rows(i).ask(p, tiles[i], kUsed);
 
     uint32_t parities = 0;   // of the stages
-    for (int stage = 0;; stage ^= 1) {
-        const Tile tile = tiles[stage];
+    for (int stage = 0, at = 0, behind = 2;; stage ^= 1, at = at == 2 ? 0 : at + 1, behind = behind == 2 ? 0 : behind + 1) {
+        const Tile &tile = tiles[at];
         if (!tile.real) break;
         Tile later{};
         if (tid == 0) {
@@ -74,14 +74,14 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
 #pragma unroll
         for (int s = 1; s < S; ++s) own = Map{a[s], b[s]}.behind(own);
         parts[warp][lane] = own;
-        // Boxes are asked for by one thread, which leaves the tile's place behind the barrier: others may read the one at work as late as in front of it.
-        if (tid == 0 && COPY != Copy::Boxes) tiles[stage] = later;
+        // Boxes are asked for by one thread, which leaves the tile's place behind the barrier: in front of it others may still be at the tile before, whose place it takes.
+        if (tid == 0 && COPY != Copy::Boxes) tiles[behind] = later;
         if (tid == 0) storesRead();
         __syncthreads();
-        if (tid == 0 && COPY == Copy::Boxes) tiles[stage] = later;
-        rows(stage).ask(p, COPY == Copy::Boxes ? later : tiles[stage], kUsed);
+        if (tid == 0 && COPY == Copy::Boxes) tiles[behind] = later;
+        rows(stage).ask(p, COPY == Copy::Boxes ? later : tiles[behind], kUsed);
 
-        const int d = tile.d0 + 2 * lane, real = p.width - d;
+        const int real = p.width - tile.d0 - 2 * lane;
         const bool last = tile.chunk + 1 == p.chunks;
         const Map ahead = mapBefore(parts, warp);
         Map mine;
@@ -89,14 +89,14 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
             mine = own.behind(ahead);
             tellTile(p, tile, mine);
         }
-        const int64_t row = static_cast<int64_t>(tile.b) * p.width + d;
+        const int64_t row = tile.row + 2 * lane;
         Pair h;
         if (tile.place > 0) h = stateBefore<kWarps - 1>(p, tile, before, mine, window, front);
         else {
             h = readFloats(p.state ? p.state + row : nullptr, real);
             if (warp == 0 && !last) tellStart(p, tile, h);
         }
-        if (warp == 0 && p.marks && tile.chunk > 0) writeFloats(p.marks + (static_cast<int64_t>(tile.b) * (p.chunks - 1) + tile.chunk - 1) * p.width + d, h, real);
+        if (warp == 0 && p.marks && tile.chunk > 0) writeFloats(p.marks + tile.mark + 2 * lane, h, real);
         h = ahead(h);
         if (p.outBoxes) {
             uint8_t *to = outputs + warp * S * kRow + lane * 2 * sizeof(T);
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
             }
         } else {
             const int here = min(p.tokens - tile.first - warp * S, S);   // tokens that have an output
-            T *to = static_cast<T *>(p.out) + (static_cast<int64_t>(tile.b) * p.tokens + tile.first + warp * S) * p.width + d;
+            T *to = static_cast<T *>(p.out) + tile.out + static_cast<int64_t>(warp * S) * p.width + 2 * lane;
 #pragma unroll
             for (int s = 0; s < S; ++s, to += p.width) {
                 h = fma2(a[s], h, b[s]);

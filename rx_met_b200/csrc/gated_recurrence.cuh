@@ -20,7 +20,7 @@ using rxmet::pairOf;
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kGroup = 8;                      // tiles; as many as a CTA has warps: all but the last wait for a tile each, the last for the front
-constexpr int kStages = 2;
+constexpr int kStages = 2, kPlaces = 3;        // of tiles' rows, of tiles' places: the one at work, the next one, the one behind that
 constexpr int kChannels = 64;                  // of a tile, two a lane
 constexpr uint32_t kPollLimit = 1u << 18;      // 0.2 s of polling; a legitimate wait lasts microseconds
 
@@ -105,8 +105,8 @@ __device__ __forceinline__ Pair exponentials(Pair x) {
 template <class T>
 struct Gates {
     Pair open, shut;
-    __device__ __forceinline__ explicit Gates(Pair clamped) {
-        const Pair e = exponentials<T>(clamped);
+    // from exp(-x)
+    __device__ __forceinline__ explicit Gates(Pair e) {
         const float2 sum = floatsOf(add2(e, pairOf(1.f, 1.f)));
         float a, b;
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(sum.x));   // one unit in the last place
@@ -114,7 +114,7 @@ struct Gates {
         open = pairOf(a, b);
         shut = mul2(e, open);
     }
-    __device__ __forceinline__ explicit Gates(const uint8_t *row) : Gates(clampRow<T>(row)) {}
+    __device__ __forceinline__ explicit Gates(const uint8_t *row) : Gates(exponentials<T>(clampRow<T>(row))) {}
 };
 __device__ __forceinline__ Pair bothOf(float v) { return pairOf(v, v); }
 __device__ __forceinline__ Pair tanhOf(Pair x) {
@@ -130,8 +130,8 @@ __device__ __forceinline__ void copiesArrived() { asm volatile("cp.async.wait_gr
 
 // Where a tile lies: worked out by one thread, because of the divisions.
 struct Tile {
-    int64_t slab;
-    int place, chunk, b, d0, live, first;   // place: in the chain; live: of its tokens, those of the sequence; first: its first token
+    int64_t parts, fronts, row, mark, out;   // elements in front of: its group's maps, its group's front, its channels of a state, of a mark, of an output
+    int place, chunk, b, d0, live, first;    // place: in the chain; live: of its tokens, those of the sequence; first: its first token
     bool real;
 };
 template <class T, bool OWN>
@@ -142,11 +142,16 @@ __device__ __forceinline__ Tile tileOf(const Pass &p, int64_t index, bool revers
     const uint32_t slabs = static_cast<uint32_t>(p.batch) * static_cast<uint32_t>(p.slabsOfRow), at = static_cast<uint32_t>(index);
     t.place = static_cast<int>(at / slabs);
     const uint32_t slab = at - t.place * slabs;
-    t.slab = slab;
     t.chunk = reverse ? p.chunks - 1 - t.place : t.place;
     t.b = static_cast<int>(slab / static_cast<uint32_t>(p.slabsOfRow));
     t.d0 = static_cast<int>(slab - t.b * static_cast<uint32_t>(p.slabsOfRow)) * kChannels;
     t.first = t.chunk * kTokens<T, OWN>;
+    const int group = t.place / kGroup;
+    t.parts = (static_cast<int64_t>(slab) * p.chunks + group * kGroup) * kChannels;
+    t.fronts = (static_cast<int64_t>(slab) * p.groups + group) * kChannels;
+    t.row = static_cast<int64_t>(t.b) * p.width + t.d0;
+    t.mark = (static_cast<int64_t>(t.b) * (p.chunks - 1) + t.chunk - 1) * p.width + t.d0;
+    t.out = (static_cast<int64_t>(t.b) * p.tokens + t.first) * p.width + t.d0;
     const int length = p.lengths ? min(max(p.lengths[t.b], 0), p.tokens) : p.tokens;
     t.live = min(max(length - t.first, 0), kTokens<T, OWN>);
     return t;
@@ -331,10 +336,10 @@ struct Before {
     ulonglong2 words;
     bool waits;
     __device__ __forceinline__ Before(const Pass &p, const Tile &tile) {
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = tile.place / kGroup;
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
         const bool part = warp < tile.place % kGroup;
         waits = tile.place > 0 && (part || warp == kWarps - 1);
-        at = part ? p.chain.parts + (tile.slab * p.chunks + group * kGroup + warp) * kChannels + 2 * lane : p.chain.fronts + (tile.slab * p.groups + group) * kChannels + 2 * lane;
+        at = (part ? p.chain.parts + tile.parts + warp * kChannels : p.chain.fronts + tile.fronts) + 2 * lane;
         words = make_ulonglong2(0, 0);
     }
     __device__ __forceinline__ void look() {
@@ -347,7 +352,7 @@ __device__ __forceinline__ Pair stateBefore(const Pass &p, const Tile &tile, con
     const Chain &c = p.chain;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = tile.place / kGroup, k = tile.place % kGroup;
     const bool speaks = k == kGroup - 1 && group + 1 < p.groups;   // for its group
-    unsigned long long *next = c.fronts + (tile.slab * p.groups + group + 1) * kChannels + 2 * lane;
+    unsigned long long *next = c.fronts + tile.fronts + kChannels + 2 * lane;
     if (warp < k) window[warp][lane] = awaitPart(c, before.at, before.words);
     Map all;
     if (speaks) {
@@ -379,10 +384,10 @@ __device__ __forceinline__ Map mapBefore(const Map (*parts)[32], int warp) {
 }
 // By one warp, as soon as the tile's map is known.
 __device__ __forceinline__ void tellTile(const Pass &p, const Tile &tile, const Map &mine) {
-    if (tile.place % kGroup != kGroup - 1) tellMap(p.chain.parts + (tile.slab * p.chunks + tile.place) * kChannels + 2 * (threadIdx.x & 31), mine.A, mine.B);
+    if (tile.place % kGroup != kGroup - 1) tellMap(p.chain.parts + tile.parts + tile.place % kGroup * kChannels + 2 * (threadIdx.x & 31), mine.A, mine.B);
 }
 // By one warp of a chain's first tile.
-__device__ __forceinline__ void tellStart(const Pass &p, const Tile &tile, Pair h) { tellState(p.chain.fronts + tile.slab * p.groups * kChannels + 2 * (threadIdx.x & 31), h); }
+__device__ __forceinline__ void tellStart(const Pass &p, const Tile &tile, Pair h) { tellState(p.chain.fronts + tile.fronts + 2 * (threadIdx.x & 31), h); }
 
 // The tiles of a CTA: by tickets where tiles wait for one another, else every gridDim.x'th.  One thread asks for a ticket a while before it needs it.
 struct Tickets {

@@ -4,18 +4,13 @@
 //   dvalue = G z c',  dforget = G (h_{t-1} - c) f (1 - f)  (G h_{t-1} f (1 - f) beside an input gate),  dinput = G c z (1 - z)
 //
 // A tile reads its gates and values again and takes the state in front of it from what the forward pass marked, so that no state of a token is kept between the passes; the gradient R that
-// reaches its end comes from the chain, whose first tile is a sequence's last.  In registers: a gate (the smaller of f and 1 - f, signed) and h_{t-1} of sixteen tokens a thread;
+// reaches its end comes from the chain, whose first tile is a sequence's last.  In registers: exp(-forget), from which both gates are one reciprocal away, and h_{t-1} of sixteen tokens a thread;
 // values and gradients are read a second time from shared memory.
 #include "gated_recurrence.cuh"
 
 namespace rxmet {
 namespace gated {
 namespace {
-
-// The sum of the two gates is one: the pair is kept as the smaller one, whose sign says which it is.
-__device__ __forceinline__ float packGate(float open, float shut) { return open > shut ? shut : -open; }
-__device__ __forceinline__ float openOf(float packed) { return signbit(packed) ? -packed : 1.f - packed; }
-__device__ __forceinline__ float shutOf(float packed) { return signbit(packed) ? 1.f + packed : packed; }
 
 template <class T, Copy COPY, bool OWN, bool TANH>
 __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __grid_constant__ Pass p) {
@@ -24,7 +19,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
     extern __shared__ __align__(128) uint8_t stages[];
     __shared__ Map window[kGroup][32], parts[kWarps][32];   // of the tiles of a group, of the tokens of the warps
     __shared__ Pair gradients[kWarps][32];                  // C
-    __shared__ Tile tiles[kStages];
+    __shared__ Tile tiles[kPlaces];
     __shared__ Pair front[32];
     __shared__ __align__(8) uint64_t full[kStages];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -53,25 +48,27 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
     if (COPY != Copy::Boxes) commitCopies();
 
     uint32_t parities = 0;   // of the stages
-    for (int stage = 0;; stage ^= 1) {
-        const Tile tile = tiles[stage];
+    for (int stage = 0, at = 0, behind = 2;; stage ^= 1, at = at == 2 ? 0 : at + 1, behind = behind == 2 ? 0 : behind + 1) {
+        const Tile &tile = tiles[at], &next = tiles[at == 2 ? 0 : at + 1];
         if (!tile.real) break;
         if (!rows(stage).arrived(tile, parities >> stage & 1)) gaveUp(p.chain);
         if (tile.live > 0) parities ^= 1u << stage;
         __syncthreads();
         if (tid == 0) storesRead();
-        rows(stage ^ 1).ask(p, tiles[stage ^ 1], used);   // what it held was read in front of the barrier, or left by a store
+        rows(stage ^ 1).ask(p, next, used);   // what it held was read in front of the barrier, or left by a store
         if (COPY != Copy::Boxes) commitCopies();
+        // the next tile's marks lie far away
+        if (warp == 1 && lane < 2 && next.real && next.chunk > 0 && next.d0 + 32 * lane < p.width) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.marks + next.mark + 32 * lane));
         Tile later{};
         if (tid == 0) {
             later = tileOf<T, OWN>(p, tickets.take(), true);
             tickets.ask();
         }
 
-        const int d = tile.d0 + 2 * lane, real = p.width - d;
-        const int64_t row = static_cast<int64_t>(tile.b) * p.width + d;
+        const int real = p.width - tile.d0 - 2 * lane;
+        const int64_t row = tile.row + 2 * lane;
         // in front of the tile
-        Pair h = readFloats(tile.chunk > 0 ? p.marks + (static_cast<int64_t>(tile.b) * (p.chunks - 1) + tile.chunk - 1) * p.width + d : p.state ? p.state + row : nullptr, real);
+        Pair h = readFloats(tile.chunk > 0 ? p.marks + tile.mark + 2 * lane : p.state ? p.state + row : nullptr, real);
         constexpr int kRow = kChannels * sizeof(T);
         uint8_t *from = stages + stage * kStageBytes + warp * S * kRow + lane * 2 * sizeof(T);
         const int live = tile.live - warp * S;
@@ -83,17 +80,14 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
         auto inputAt = [&](int s) { return Gates<T>(from + s * kRow + 2 * kTensorBytes<OWN>); };
 
         // the tile's maps of a state forwards, (A, B), and of a gradient backwards, (A, C); a warp whose tokens are all of the sequence has nothing to test
-        float gate[S][2];
-        Pair before[S], A = bothOf(1.f), B = bothOf(0.f), C = bothOf(0.f);
+        Pair gate[S], before[S], A = bothOf(1.f), B = bothOf(0.f), C = bothOf(0.f);
         Before earlier(p, tile);
         auto mapTokens = [&](auto all) {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
                 if (s == S * 3 / 4) earlier.look();
-                const Gates<T> f(from + s * kRow);
-                const float2 open = floatsOf(f.open), shut = floatsOf(f.shut);
-                gate[s][0] = packGate(open.x, shut.x);
-                gate[s][1] = packGate(open.y, shut.y);
+                gate[s] = exponentials<T>(clampRow<T>(from + s * kRow));
+                const Gates<T> f(gate[s]);
                 before[s] = mul2(OWN ? inputAt(s).open : f.shut, valueAt(s));   // what the token adds, until the state in front of it is known
                 if (decltype(all)::value || s < live) {
                     A = mul2(A, f.open);
@@ -106,7 +100,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
         else mapTokens(std::false_type{});
         parts[warp][lane] = {A, B};
         gradients[warp][lane] = C;
-        if (tid == 0) tiles[stage] = later;
+        if (tid == 0) tiles[behind] = later;
         __syncthreads();
 
         const bool last = tile.chunk == 0;   // of the chain
@@ -129,12 +123,12 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
         R = after(R);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const Pair next = fma2(pairOf(openOf(gate[s][0]), openOf(gate[s][1])), h, before[s]);
+            const Pair next = fma2(Gates<T>(gate[s]).open, h, before[s]);
             before[s] = h;
             h = next;   // behind the sequence's end nobody reads it
         }
         const int here = min(p.tokens - tile.first - warp * S, S);
-        const int64_t to = (static_cast<int64_t>(tile.b) * p.tokens + tile.first + warp * S) * p.width + d;
+        const int64_t to = tile.out + static_cast<int64_t>(warp * S) * p.width + 2 * lane;
         const Pair minus = bothOf(-1.f);
         // gradients of a token take the place of what they come from, if a box of them can be stored
         auto giveTokens = [&](auto all) {
@@ -143,8 +137,8 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
                 Pair dforget = bothOf(0.f), dvalue = bothOf(0.f), dinput = bothOf(0.f);
                 if (decltype(all)::value || s < live) {
                     const Pair c = valueAt(s), G = add2(doutAt(s), R);
-                    const Pair open = pairOf(openOf(gate[s][0]), openOf(gate[s][1])), shut = pairOf(shutOf(gate[s][0]), shutOf(gate[s][1]));
-                    Pair z = shut, held = before[s];
+                    const Gates<T> f(gate[s]);
+                    Pair z = f.shut, held = before[s];
                     if (OWN) {
                         const Gates<T> i = inputAt(s);
                         z = i.open;
@@ -152,8 +146,8 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
                     } else {
                         held = fma2(c, minus, held);
                     }
-                    R = mul2(open, G);
-                    dforget = mul2(R, mul2(held, shut));
+                    R = mul2(f.open, G);
+                    dforget = mul2(R, mul2(held, f.shut));
                     dvalue = mul2(G, z);
                     if (TANH) dvalue = mul2(dvalue, fma2(mul2(c, minus), c, bothOf(1.f)));
                 }

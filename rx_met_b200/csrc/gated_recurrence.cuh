@@ -251,13 +251,7 @@ __device__ __forceinline__ void writeRow(T *to, Pair v, int real, bool paired) {
         if (real > 1) to[1] = fromFloat<T>(two.y);
     }
 }
-// (volatile, or the loads end up where their values are used)
-__device__ __forceinline__ Pair readFloats(const float *from, int real) {
-    float a = 0.f, b = 0.f;
-    if (from && real > 0) asm volatile("ld.global.f32 %0, [%1];" : "=f"(a) : "l"(from) : "memory");
-    if (from && real > 1) asm volatile("ld.global.f32 %0, [%1];" : "=f"(b) : "l"(from + 1) : "memory");
-    return pairOf(a, b);
-}
+__device__ __forceinline__ Pair readFloats(const float *from, int real) { return pairOf(from && real > 0 ? from[0] : 0.f, from && real > 1 ? from[1] : 0.f); }
 __device__ __forceinline__ void writeFloats(float *to, Pair v, int real) {
     if (real > 0) to[0] = floatsOf(v).x;
     if (real > 1) to[1] = floatsOf(v).y;

@@ -21,6 +21,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
     __shared__ Pair gradients[kWarps][32];                  // C
     __shared__ Tile tiles[kPlaces];
     __shared__ Pair front[32];
+    __shared__ __align__(16) float starts[kStages][kChannels];
     __shared__ __align__(8) uint64_t full[kStages];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0 && COPY == Copy::Boxes) {
@@ -44,6 +45,17 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
             constexpr int kOf = kTensorBytes<OWN> / 16;
             reinterpret_cast<uint4 *>(stages + i / kOf * kStageBytes + kDout * kTensorBytes<OWN>)[i % kOf] = make_uint4(0, 0, 0, 0);
         }
+    // The state in front of a tile, by two warps, in front of the tile's rows: behind them it would come when they have.
+    auto askState = [&](int stage, const Tile &tile) {
+        const int channel = tid - 64;
+        if (channel >= 0 && channel < kChannels && tile.real) {
+            const float *from = tile.chunk > 0 ? p.marks + tile.mark : p.state ? p.state + tile.row : nullptr;
+            const bool there = from && channel < p.width - tile.d0;
+            copyWord(umma::smemAddr(&starts[stage][channel]), there ? from + channel : reinterpret_cast<const float *>(p.chain.status), there ? 4 : 0);
+        }
+        if (COPY == Copy::Boxes) commitCopies();
+    };
+    askState(0, tiles[0]);
     rows(0).ask(p, tiles[0], used);
     if (COPY != Copy::Boxes) commitCopies();
 
@@ -53,12 +65,12 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
         if (!tile.real) break;
         if (!rows(stage).arrived(tile, parities >> stage & 1)) gaveUp(p.chain);
         if (tile.live > 0) parities ^= 1u << stage;
+        if (COPY == Copy::Boxes) copiesArrived<0>();
         __syncthreads();
+        askState(stage ^ 1, next);
         if (tid == 0) storesRead();
         rows(stage ^ 1).ask(p, next, used);   // what it held was read in front of the barrier, or left by a store
         if (COPY != Copy::Boxes) commitCopies();
-        // the next tile's marks lie far away
-        if (warp == 1 && lane < 2 && next.real && next.chunk > 0 && next.d0 + 32 * lane < p.width) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.marks + next.mark + 32 * lane));
         Tile later{};
         if (tid == 0) {
             later = tileOf<T, OWN>(p, tickets.take(), true);
@@ -67,8 +79,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
 
         const int real = p.width - tile.d0 - 2 * lane;
         const int64_t row = tile.row + 2 * lane;
-        // in front of the tile
-        Pair h = readFloats(tile.chunk > 0 ? p.marks + tile.mark + 2 * lane : p.state ? p.state + row : nullptr, real);
+        Pair h = *reinterpret_cast<const Pair *>(&starts[stage][2 * lane]);   // in front of the tile
         constexpr int kRow = kChannels * sizeof(T);
         uint8_t *from = stages + stage * kStageBytes + warp * S * kRow + lane * 2 * sizeof(T);
         const int live = tile.live - warp * S;

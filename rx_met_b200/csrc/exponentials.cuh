@@ -1,0 +1,64 @@
+// exp(-x) and the sigmoid of two values at a time, shared by the gated recurrence and the products of activated gates.
+#pragma once
+
+#include <type_traits>
+
+#include "element_types.cuh"
+
+namespace rxmet {
+
+__device__ __forceinline__ Pair bothOf(float v) { return pairOf(v, v); }
+
+// Bits of a type's significand.
+template <class T>
+constexpr int kSignificant = std::is_same_v<T, __nv_bfloat16> ? 8 : std::is_same_v<T, __half> ? 11 : 24;
+
+// A NaN stays one.
+__device__ __forceinline__ float atLeast(float v, float least) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(least));
+    return r;
+}
+__device__ __forceinline__ float atMost(float v, float most) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(most));
+    return r;
+}
+// Between -87 and 87, beyond which sigmoid(x) and its complement are 0 and 1 to 2^-125.
+constexpr float kFarGate = 87.f;
+__device__ __forceinline__ Pair clampPair(Pair x) {
+    const float2 v = floatsOf(x);
+    return pairOf(atMost(atLeast(v.x, -kFarGate), kFarGate), atMost(atLeast(v.y, -kFarGate), kFarGate));
+}
+
+// exp(-x) of x in [-87, 87]: 2^u with u = -x log2(e) to 24 bits, times 1 + what u leaves out.  For x of 8 or 11 significant bits the product with the upper 16 or 13 bits of log2(e) is exact, and x times
+// the rest is left out; for floats, the rounding of u as well.  As exact as the exponential itself, 2 units (11 bits, beyond 16: 2^-17 at 87).
+template <int BITS>
+__device__ __forceinline__ Pair exponentials(Pair x) {
+    constexpr float kUpper = BITS <= 8 ? 1.44268798828125f : BITS <= 11 ? 1.442626953125f : 1.4426950408889634f;
+    constexpr float kRest = BITS <= 8 ? 7.0526077e-6f : BITS <= 11 ? 6.8087764e-5f : 1.925963033500e-8f, kLn2 = 0.6931471805599453f;
+    const Pair u = mul2(x, bothOf(-kUpper));
+    const float2 v = floatsOf(u);
+    Pair left;
+    if constexpr (BITS <= 11) left = mul2(x, bothOf(-kRest * kLn2));
+    else left = mul2(fma2(x, bothOf(-kRest), fma2(x, bothOf(-kUpper), pairOf(-v.x, -v.y))), bothOf(kLn2));
+    float c, d;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(c) : "f"(v.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(v.y));
+    const Pair e = pairOf(c, d);
+    return fma2(e, left, e);
+}
+// sigmoid(x), and 1 - sigmoid(x) without the bits that a subtraction from one would lose, from exp(-x).
+struct Sigmoids {
+    Pair open, shut;
+    __device__ __forceinline__ explicit Sigmoids(Pair e) {
+        const float2 sum = floatsOf(add2(e, bothOf(1.f)));
+        float a, b;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(sum.x));   // one unit in the last place
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(sum.y));
+        open = pairOf(a, b);
+        shut = mul2(e, open);
+    }
+};
+
+}  // namespace rxmet

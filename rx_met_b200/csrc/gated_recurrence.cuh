@@ -9,14 +9,13 @@
 #include "cluster_device.cuh"
 #include "dependent_launch.cuh"
 #include "element_types.cuh"
+#include "exponentials.cuh"
 #include "rxmet_b200_gated.h"
 #include "tensor_map.cuh"
 #include "umma_tiles.cuh"
 
 namespace rxmet {
 namespace gated {
-
-using rxmet::pairOf;
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kGroup = 8;                      // tiles; as many as a CTA has warps: all but the last wait for a tile each, the last for the front
@@ -66,57 +65,24 @@ struct Pass {
     Chain chain;
 };
 
-// x of two channels between -87 and 87, beyond which sigmoid(x) and its complement are 0 and 1 to 2^-125; a NaN stays one.
+// Two channels of a row, clamped.
 template <class T>
 __device__ __forceinline__ Pair clampRow(const uint8_t *row) {
-    if constexpr (sizeof(T) == 4) {
-        const float2 v = *reinterpret_cast<const float2 *>(row);
-        float a, b;
-        asm("max.NaN.f32 %0, %1, 0fC2AE0000;\n\tmin.NaN.f32 %0, %0, 0f42AE0000;" : "=f"(a) : "f"(v.x));
-        asm("max.NaN.f32 %0, %1, 0fC2AE0000;\n\tmin.NaN.f32 %0, %0, 0f42AE0000;" : "=f"(b) : "f"(v.y));
-        return pairOf(a, b);
-    } else {
-        uint32_t w = *reinterpret_cast<const uint32_t *>(row);
+    if constexpr (sizeof(T) == 4) return clampPair(*reinterpret_cast<const Pair *>(row));
+    else {
+        uint32_t w = *reinterpret_cast<const uint32_t *>(row);   // both at once: 87 is a number of either type
         if constexpr (std::is_same_v<T, __nv_bfloat16>) asm("max.NaN.bf16x2 %0, %0, %1;\n\tmin.NaN.bf16x2 %0, %0, %2;" : "+r"(w) : "r"(0xc2aec2aeu), "r"(0x42ae42aeu));
         else asm("max.NaN.f16x2 %0, %0, %1;\n\tmin.NaN.f16x2 %0, %0, %2;" : "+r"(w) : "r"(0xd570d570u), "r"(0x55705570u));
         const float2 v = unpack2<T>(w);
         return pairOf(v.x, v.y);
     }
 }
-// exp(-x) of two such values: 2^u with u = -x log2(e) to 24 bits, times 1 + what u leaves out.  Of 16-bit types, x of 8 or 11 bits times the upper 16 or 13 bits of log2(e) is exact, and x times the
-// rest is left out; of floats, the rounding of u as well.  As exact as the exponential itself, 2 units (of half, beyond 16: 2^-17 at 87).
+// Both gates of two channels, from exp(-x) or from a row.
 template <class T>
-__device__ __forceinline__ Pair exponentials(Pair x) {
-    constexpr bool kShort = sizeof(T) == 2, kBf16 = std::is_same_v<T, __nv_bfloat16>;
-    constexpr float kUpper = kBf16 ? 1.44268798828125f : kShort ? 1.442626953125f : 1.4426950408889634f;
-    constexpr float kRest = kBf16 ? 7.0526077e-6f : kShort ? 6.8087764e-5f : 1.925963033500e-8f, kLn2 = 0.6931471805599453f;
-    const Pair u = mul2(x, pairOf(-kUpper, -kUpper));
-    const float2 v = floatsOf(u);
-    Pair left;
-    if constexpr (kShort) left = mul2(x, pairOf(-kRest * kLn2, -kRest * kLn2));
-    else left = mul2(fma2(x, pairOf(-kRest, -kRest), fma2(x, pairOf(-kUpper, -kUpper), pairOf(-v.x, -v.y))), pairOf(kLn2, kLn2));
-    float c, d;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(c) : "f"(v.x));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(v.y));
-    const Pair e = pairOf(c, d);
-    return fma2(e, left, e);
-}
-// sigmoid(x), and 1 - sigmoid(x) without the bits that a subtraction from one would lose, of the two channels of a row.
-template <class T>
-struct Gates {
-    Pair open, shut;
-    // from exp(-x)
-    __device__ __forceinline__ explicit Gates(Pair e) {
-        const float2 sum = floatsOf(add2(e, pairOf(1.f, 1.f)));
-        float a, b;
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(sum.x));   // one unit in the last place
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(sum.y));
-        open = pairOf(a, b);
-        shut = mul2(e, open);
-    }
-    __device__ __forceinline__ explicit Gates(const uint8_t *row) : Gates(exponentials<T>(clampRow<T>(row))) {}
+struct Gates : Sigmoids {
+    using Sigmoids::Sigmoids;
+    __device__ __forceinline__ explicit Gates(const uint8_t *row) : Sigmoids(exponentials<kSignificant<T>>(clampRow<T>(row))) {}
 };
-__device__ __forceinline__ Pair bothOf(float v) { return pairOf(v, v); }
 __device__ __forceinline__ Pair tanhOf(Pair x) {
     const float2 v = floatsOf(x);
     return pairOf(tanhf(v.x), tanhf(v.y));

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
 #pragma unroll
             for (int s = 0; s < S; ++s) {
                 if (s == S * 3 / 4) earlier.look();
-                gate[s] = exponentials<T>(clampRow<T>(from + s * kRow));
+                gate[s] = exponentials<kSignificant<T>>(clampRow<T>(from + s * kRow));
                 const Gates<T> f(gate[s]);
                 before[s] = mul2(OWN ? inputAt(s).open : f.shut, valueAt(s));   // what the token adds, until the state in front of it is known
                 if (decltype(all)::value || s < live) {

@@ -5,6 +5,7 @@
 #include "kept_codes.cuh"
 
 #include "dependent_launch.cuh"
+#include "exponentials.cuh"
 #include "row_words.cuh"
 
 namespace rxmet {
@@ -19,53 +20,97 @@ struct Codes {
 };
 struct Pass {
     int64_t rows;
-    int width, words, lowest, activation;   // words: of eight elements in a row, a multiple of four
+    int width, words, lowest;   // words: of eight elements in a row, a multiple of four
     const void *a, *b;
     int64_t aPitch, bPitch, codesPitch;
     Codes first, second;
     void *y, *z;
 };
 
-template <class T, bool WIDE>
-__device__ __forceinline__ void loadEight(const void *data, int64_t pitch, const RowWord &at, int count, float (&v)[kPer]) {
-    const T *from = static_cast<const T *>(data) + static_cast<int64_t>(at.row) * pitch + at.word * kPer;
-    if (WIDE && count > 0) {
-        constexpr int W = 16 / sizeof(T);
+constexpr int kPairs = kPer / 2;   // of elements in 32 bits, two to a register pair
+// Eight neighbouring elements as they lie in memory; those that there are not are zeros.
+template <class T>
+struct alignas(16) Raw {
+    uint32_t w[kPer * sizeof(T) / 4];
+    __device__ __forceinline__ void unpack(Pair (&v)[kPairs]) const {
 #pragma unroll
-        for (int i = 0; i < kPer / W; ++i) {
-            const Pack<T, W> p = *reinterpret_cast<const Pack<T, W> *>(from + i * W);
-#pragma unroll
-            for (int j = 0; j < W; ++j) v[i * W + j] = toFloat(p.v[j]);
+        for (int i = 0; i < kPairs; ++i) {
+            if constexpr (sizeof(T) == 4) v[i] = pairOf(w[2 * i], w[2 * i + 1]);
+            else {
+                const float2 two = unpack2<T>(w[i]);
+                v[i] = pairOf(two.x, two.y);
+            }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) v[i] = !WIDE && i < count ? toFloat(from[i]) : 0.f;
     }
+    // Bits of the largest magnitude, as of a float; an infinity or a NaN counts as more than any number.
+    __device__ __forceinline__ uint32_t most() const {
+        if constexpr (sizeof(T) == 4) {
+            uint32_t r = 0;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) r = max(r, w[i] & 0x7fffffffu);
+            return r;
+        } else {
+            uint32_t r = w[0] & 0x7fff7fffu;
+#pragma unroll
+            for (int i = 1; i < kPairs; ++i) {
+                const uint32_t next = w[i] & 0x7fff7fffu;
+                if constexpr (std::is_same_v<T, __nv_bfloat16>) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(r) : "r"(next));
+                else asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(r) : "r"(next));
+            }
+            const float2 two = unpack2<T>(r);
+            return max(__float_as_uint(two.x) & 0x7fffffffu, __float_as_uint(two.y) & 0x7fffffffu);
+        }
+    }
+};
+template <class T, bool WIDE>
+__device__ __forceinline__ Raw<T> loadEight(const void *data, int64_t pitch, const RowWord &at, int count) {
+    const T *from = static_cast<const T *>(data) + static_cast<int64_t>(at.row) * pitch + at.word * kPer;
+    Raw<T> r{};
+    if (WIDE && count > 0) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4 *>(r.w)[i] = reinterpret_cast<const uint4 *>(from)[i];
+    }
+    if (!WIDE) {
+        T one[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) one[i] = i < count ? from[i] : fromFloat<T>(0.f);
+#pragma unroll
+        for (int i = 0; i < kPer * static_cast<int>(sizeof(T)) / 4; ++i) {
+            if constexpr (sizeof(T) == 4) r.w[i] = __float_as_uint(one[i]);
+            else r.w[i] = static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(one)[2 * i]) | static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(one)[2 * i + 1]) << 16;
+        }
+    }
+    return r;
 }
 template <class T, bool WIDE>
-__device__ __forceinline__ void storeEight(void *data, int width, const RowWord &at, int count, const float (&v)[kPer]) {
+__device__ __forceinline__ void storeEight(void *data, int width, const RowWord &at, int count, const Pair (&v)[kPairs]) {
     T *to = static_cast<T *>(data) + static_cast<int64_t>(at.row) * width + at.word * kPer;
     if (WIDE && count > 0) {
-        constexpr int W = 16 / sizeof(T);
+        Raw<T> r;
 #pragma unroll
-        for (int i = 0; i < kPer / W; ++i) {
-            Pack<T, W> p;
-#pragma unroll
-            for (int j = 0; j < W; ++j) p.v[j] = fromFloat<T>(v[i * W + j]);
-            *reinterpret_cast<Pack<T, W> *>(to + i * W) = p;
+        for (int i = 0; i < kPairs; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                const float2 two = floatsOf(v[i]);
+                r.w[2 * i] = __float_as_uint(two.x);
+                r.w[2 * i + 1] = __float_as_uint(two.y);
+            } else {
+                r.w[i] = pack2<T>(v[i]);
+            }
         }
-    } else {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4 *>(to)[i] = reinterpret_cast<const uint4 *>(r.w)[i];
+    }
+    if (!WIDE) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-            if (!WIDE && i < count) to[i] = fromFloat<T>(v[i]);
+            if (i < count) to[i] = fromFloat<T>(i & 1 ? floatsOf(v[i / 2]).y : floatsOf(v[i / 2]).x);
     }
 }
 
 // By the four threads of a group.
-__device__ __forceinline__ void keepEight(const Pass &p, const Codes &to, const RowWord &at, int count, const float (&v)[kPer]) {
-    uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
+template <class T>
+__device__ __forceinline__ void keepEight(const Pass &p, const Codes &to, const RowWord &at, int count, const Raw<T> &raw, const Pair (&v)[kPairs]) {
+    uint32_t most = raw.most();
     const unsigned group = 0xfu << (threadIdx.x & 28);
     most = max(most, __shfl_xor_sync(group, most, 1));
     most = max(most, __shfl_xor_sync(group, most, 2));
@@ -74,7 +119,7 @@ __device__ __forceinline__ void keepEight(const Pass &p, const Codes &to, const 
         uint2 codes = make_uint2(0, 0);
         if (e != kBad) {
             const float inverse = powerOf(-e);
-            codes = make_uint2(codesOf(v, inverse), codesOf(v + 4, inverse));
+            codes = make_uint2(codesOf(v[0], v[1], inverse), codesOf(v[2], v[3], inverse));
         }
         *reinterpret_cast<uint2 *>(to.codes + static_cast<int64_t>(at.row) * p.codesPitch + at.word * kPer) = codes;
     }
@@ -92,44 +137,35 @@ __device__ __forceinline__ Held heldEight(const Pass &p, const Codes &from, cons
     }
     return h;
 }
-__device__ __forceinline__ void valuesOfEight(const Held &h, float (&v)[kPer]) {
+__device__ __forceinline__ void valuesOfEight(const Held &h, Pair (&v)[kPairs]) {
     const float step = stepOf(h.exponent);
-    valuesOf(h.codes.x, step, v);
-    valuesOf(h.codes.y, step, v + 4);
+    valuesOf(h.codes.x, step, v[0], v[1]);
+    valuesOf(h.codes.y, step, v[2], v[3]);
 }
 __device__ __forceinline__ int countOf(const Pass &p, const RowWord &at) { return at.real ? min(kPer, max(0, p.width - at.word * kPer)) : 0; }
 
-// The activation's values, and its slopes where they are wanted; one test for all elements.  Normal distribution for gelu: Phi(x) keeps its bits for x far below zero, where 1 + erf does not.
-template <bool SLOPES>
-__device__ __forceinline__ void activate(int activation, const float (&x)[kPer], float (&y)[kPer], float (&slope)[kPer]) {
-    if (activation == RXMET_ACTIVATION_RELU) {
+// The activation's values, and its slopes where they are wanted.  Normal distribution for gelu: Phi(x) keeps its bits for x far below zero, where 1 + erf does not.  BITS: significant ones of x.
+template <int ACTIVATION, bool SLOPES, int BITS>
+__device__ __forceinline__ void activate(const Pair (&x)[kPairs], Pair (&y)[kPairs], Pair (&slope)[kPairs]) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            y[i] = x[i] < 0.f ? 0.f : x[i];   // keeps a NaN
-            if (SLOPES) slope[i] = x[i] > 0.f ? 1.f : x[i] <= 0.f ? 0.f : x[i];
-        }
-    } else if (activation == RXMET_ACTIVATION_SILU) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const float e = expf(-fabsf(x[i]));
-            float most;
-            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(most) : "f"(1.f + e));
-            const float least = e * most, open = x[i] > 0.f ? most : least, shut = x[i] > 0.f ? least : most;
-            y[i] = x[i] * open;
-            if (SLOPES) slope[i] = fmaf(y[i], shut, open);
-        }
-    } else if (activation == RXMET_ACTIVATION_GELU) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const float p = normcdff(x[i]);
-            y[i] = x[i] * p;
-            if (SLOPES) slope[i] = fmaf(x[i], 0.3989422804014327f * expf(-0.5f * x[i] * x[i]), p);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
+    for (int i = 0; i < kPairs; ++i) {
+        const float2 v = floatsOf(x[i]);
+        if constexpr (ACTIVATION == RXMET_ACTIVATION_RELU) {
+            y[i] = pairOf(v.x < 0.f ? 0.f : v.x, v.y < 0.f ? 0.f : v.y);   // keeps a NaN
+            auto step = [](float f) { return f > 0.f ? 1.f : f <= 0.f ? 0.f : f; };
+            if (SLOPES) slope[i] = pairOf(step(v.x), step(v.y));
+        } else if constexpr (ACTIVATION == RXMET_ACTIVATION_SILU) {
+            const Sigmoids s(exponentials<BITS>(clampPair(x[i])));
+            y[i] = mul2(x[i], s.open);
+            if (SLOPES) slope[i] = fma2(y[i], s.shut, s.open);
+        } else if constexpr (ACTIVATION == RXMET_ACTIVATION_GELU) {
+            const Pair p = pairOf(normcdff(v.x), normcdff(v.y));
+            y[i] = mul2(x[i], p);
+            auto density = [](float f) { return 0.3989422804014327f * expf(-0.5f * f * f); };
+            if (SLOPES) slope[i] = fma2(x[i], pairOf(density(v.x), density(v.y)), p);
+        } else {
             y[i] = x[i];
-            if (SLOPES) slope[i] = 1.f;
+            if (SLOPES) slope[i] = bothOf(1.f);
         }
     }
 }
@@ -139,12 +175,16 @@ __global__ void __launch_bounds__(kThreads) keepCodes(const __grid_constant__ Pa
     waitForPredecessor();
     letDependentsStart();
     eachRowWord<kAtOnce>(p.rows, p.words, blockIdx.x, gridDim.x, [&](const RowWord(&at)[kAtOnce]) {
-        float v[kAtOnce][kPer];
+        Raw<T> raw[kAtOnce];
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) loadEight<T, WIDE>(p.a, p.aPitch, at[n], countOf(p, at[n]), v[n]);
+        for (int n = 0; n < kAtOnce; ++n) raw[n] = loadEight<T, WIDE>(p.a, p.aPitch, at[n], countOf(p, at[n]));
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n)
-            if (at[n].real) keepEight(p, p.first, at[n], countOf(p, at[n]), v[n]);
+        for (int n = 0; n < kAtOnce; ++n) {
+            if (!at[n].real) continue;
+            Pair v[kPairs];
+            raw[n].unpack(v);
+            keepEight<T>(p, p.first, at[n], countOf(p, at[n]), raw[n], v);
+        }
     });
 }
 
@@ -158,7 +198,7 @@ __global__ void __launch_bounds__(kThreads) keptValues(const __grid_constant__ P
         for (int n = 0; n < kAtOnce; ++n) held[n] = heldEight(p, p.first, at[n], countOf(p, at[n]));
 #pragma unroll
         for (int n = 0; n < kAtOnce; ++n) {
-            float v[kPer];
+            Pair v[kPairs];
             valuesOfEight(held[n], v);
             storeEight<T, WIDE>(p.y, p.width, at[n], countOf(p, at[n]), v);
         }
@@ -166,60 +206,63 @@ __global__ void __launch_bounds__(kThreads) keptValues(const __grid_constant__ P
 }
 
 // a: gate, b: up.
-template <class T, bool WIDE>
-__global__ void __launch_bounds__(kThreads) gatedProduct(const __grid_constant__ Pass p) {
+template <class T, bool WIDE, int ACTIVATION>
+__global__ void __launch_bounds__(kThreads, 4) gatedProduct(const __grid_constant__ Pass p) {
     waitForPredecessor();
     letDependentsStart();
     eachRowWord<kAtOnce>(p.rows, p.words, blockIdx.x, gridDim.x, [&](const RowWord(&at)[kAtOnce]) {
-        float gate[kAtOnce][kPer], up[kAtOnce][kPer];
+        Raw<T> gates[kAtOnce], ups[kAtOnce];
 #pragma unroll
         for (int n = 0; n < kAtOnce; ++n) {
-            loadEight<T, WIDE>(p.a, p.aPitch, at[n], countOf(p, at[n]), gate[n]);
-            loadEight<T, WIDE>(p.b, p.bPitch, at[n], countOf(p, at[n]), up[n]);
+            gates[n] = loadEight<T, WIDE>(p.a, p.aPitch, at[n], countOf(p, at[n]));
+            ups[n] = loadEight<T, WIDE>(p.b, p.bPitch, at[n], countOf(p, at[n]));
         }
 #pragma unroll
         for (int n = 0; n < kAtOnce; ++n) {
             if (!at[n].real) continue;
             const int count = countOf(p, at[n]);
+            Pair gate[kPairs], up[kPairs], y[kPairs], slope[kPairs];
+            gates[n].unpack(gate);
+            ups[n].unpack(up);
             if (p.first.codes) {
-                keepEight(p, p.first, at[n], count, gate[n]);
-                keepEight(p, p.second, at[n], count, up[n]);
+                keepEight<T>(p, p.first, at[n], count, gates[n], gate);
+                keepEight<T>(p, p.second, at[n], count, ups[n], up);
             }
-            float y[kPer], slope[kPer];
-            activate<false>(p.activation, gate[n], y, slope);
+            activate<ACTIVATION, false, kSignificant<T>>(gate, y, slope);
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) y[i] *= up[n][i];
+            for (int i = 0; i < kPairs; ++i) y[i] = mul2(y[i], up[i]);
             storeEight<T, WIDE>(p.y, p.width, at[n], count, y);
         }
     });
 }
 
 // a: dy, y: dgate, z: dup.
-template <class T, bool WIDE>
-__global__ void __launch_bounds__(kThreads) gatedProductBackward(const __grid_constant__ Pass p) {
+template <class T, bool WIDE, int ACTIVATION>
+__global__ void __launch_bounds__(kThreads, 4) gatedProductBackward(const __grid_constant__ Pass p) {
     waitForPredecessor();
     letDependentsStart();
     eachRowWord<kAtOnce>(p.rows, p.words, blockIdx.x, gridDim.x, [&](const RowWord(&at)[kAtOnce]) {
-        float dy[kAtOnce][kPer];
+        Raw<T> dys[kAtOnce];
         Held gates[kAtOnce], ups[kAtOnce];
 #pragma unroll
         for (int n = 0; n < kAtOnce; ++n) {
             const int count = countOf(p, at[n]);
-            loadEight<T, WIDE>(p.a, p.aPitch, at[n], count, dy[n]);
+            dys[n] = loadEight<T, WIDE>(p.a, p.aPitch, at[n], count);
             gates[n] = heldEight(p, p.first, at[n], count);
             ups[n] = heldEight(p, p.second, at[n], count);
         }
 #pragma unroll
         for (int n = 0; n < kAtOnce; ++n) {
             const int count = countOf(p, at[n]);
-            float gate[kPer], up[kPer], y[kPer], slope[kPer];
+            Pair dy[kPairs], gate[kPairs], up[kPairs], y[kPairs], slope[kPairs];
+            dys[n].unpack(dy);
             valuesOfEight(gates[n], gate);
             valuesOfEight(ups[n], up);
-            activate<true>(p.activation, gate, y, slope);
+            activate<ACTIVATION, true, 8>(gate, y, slope);   // a code has eight bits, times a power of two
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                y[i] *= dy[n][i];
-                slope[i] *= up[i] * dy[n][i];
+            for (int i = 0; i < kPairs; ++i) {
+                y[i] = mul2(y[i], dy[i]);
+                slope[i] = mul2(slope[i], mul2(up[i], dy[i]));
             }
             if (p.z) storeEight<T, WIDE>(p.z, p.width, at[n], count, y);
             if (p.y) storeEight<T, WIDE>(p.y, p.width, at[n], count, slope);
@@ -243,6 +286,15 @@ Pass passOf(int64_t rows, int width, int type, const char *what) {
 void requireCodes(const Pass &p, const void *codes, const void *exponents, const char *what) {
     RXMET_REQUIRE(codes && exponents, "%s: null pointer", what);
     RXMET_REQUIRE(alignedTo(codes, 16) && p.codesPitch % 16 == 0 && (p.rows == 1 || p.codesPitch >= p.width), "%s: rows of codes must start on 16 bytes, and apart", what);
+}
+
+// f(the activation as a constant).
+template <class F>
+void withActivation(int activation, F f) {
+    if (activation == RXMET_ACTIVATION_RELU) f(std::integral_constant<int, RXMET_ACTIVATION_RELU>{});
+    else if (activation == RXMET_ACTIVATION_SILU) f(std::integral_constant<int, RXMET_ACTIVATION_SILU>{});
+    else if (activation == RXMET_ACTIVATION_GELU) f(std::integral_constant<int, RXMET_ACTIVATION_GELU>{});
+    else f(std::integral_constant<int, RXMET_ACTIVATION_NONE>{});
 }
 
 template <class F>
@@ -302,7 +354,6 @@ extern "C" int rxmet_gated_product(int64_t rows, int width, int type, int activa
         kept::Pass p = kept::passOf(rows, width, type, "gated_product");
         RXMET_REQUIRE(activation >= RXMET_ACTIVATION_NONE && activation <= RXMET_ACTIVATION_GELU, "gated_product: unknown activation %d", activation);
         if (rows == 0) return;
-        p.activation = activation;
         p.codesPitch = codes_pitch;
         RXMET_REQUIRE(gate && up && y, "gated_product: null pointer");
         if (gate_codes || gate_exponents || up_codes || up_exponents) {
@@ -320,7 +371,10 @@ extern "C" int rxmet_gated_product(int64_t rows, int width, int type, int activa
         const bool wide = width % 8 == 0 && kept::wideRows(gate, rows, gate_pitch, size) && kept::wideRows(up, rows, up_pitch, size) && alignedTo(y, 16);
         withType(type, [&](auto t) {
             using T = decltype(t);
-            kept::launch(wide ? kept::gatedProduct<T, true> : kept::gatedProduct<T, false>, "gatedProduct", p, static_cast<cudaStream_t>(stream));
+            kept::withActivation(activation, [&](auto a) {
+                constexpr int kActivation = decltype(a)::value;
+                kept::launch(wide ? kept::gatedProduct<T, true, kActivation> : kept::gatedProduct<T, false, kActivation>, "gatedProduct", p, static_cast<cudaStream_t>(stream));
+            });
         });
     });
 }
@@ -331,7 +385,6 @@ extern "C" int rxmet_gated_product_backward(int64_t rows, int width, int type, i
         kept::Pass p = kept::passOf(rows, width, type, "gated_product backward");
         RXMET_REQUIRE(activation >= RXMET_ACTIVATION_NONE && activation <= RXMET_ACTIVATION_GELU, "gated_product backward: unknown activation %d", activation);
         if (rows == 0 || (!dgate && !dup)) return;
-        p.activation = activation;
         p.codesPitch = codes_pitch;
         RXMET_REQUIRE(dy, "gated_product backward: null pointer");
         kept::requireCodes(p, gate_codes, gate_exponents, "gated_product backward");
@@ -345,7 +398,10 @@ extern "C" int rxmet_gated_product_backward(int64_t rows, int width, int type, i
         const bool wide = width % 8 == 0 && kept::wideRows(dy, rows, dy_pitch, typeBytes(type)) && alignedTo(dgate, 16) && alignedTo(dup, 16);
         withType(type, [&](auto t) {
             using T = decltype(t);
-            kept::launch(wide ? kept::gatedProductBackward<T, true> : kept::gatedProductBackward<T, false>, "gatedProductBackward", p, static_cast<cudaStream_t>(stream));
+            kept::withActivation(activation, [&](auto a) {
+                constexpr int kActivation = decltype(a)::value;
+                kept::launch(wide ? kept::gatedProductBackward<T, true, kActivation> : kept::gatedProductBackward<T, false, kActivation>, "gatedProductBackward", p, static_cast<cudaStream_t>(stream));
+            });
         });
     });
 }

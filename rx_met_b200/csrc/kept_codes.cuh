@@ -23,17 +23,18 @@ __device__ __forceinline__ float powerOf(int e) { return __int_as_float((e + 127
 __device__ __forceinline__ float stepOf(int exponent) { return exponent == kBad ? __int_as_float(0x7fc00000) : powerOf(max(exponent, -126)); }
 
 // Four codes of values times `inverse` = 2^-e: the sum with 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the low bits.
-__device__ __forceinline__ uint32_t codesOf(const float *v, float inverse) {
-    uint32_t r[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(fmaf(v[i], inverse, 12582912.f));
-    return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+__device__ __forceinline__ uint32_t codesOf(Pair a, Pair b, float inverse) {
+    const Pair by = pairOf(inverse, inverse), half = pairOf(12582912.f, 12582912.f);
+    const float2 lo = floatsOf(fma2(a, by, half)), hi = floatsOf(fma2(b, by, half));
+    return __byte_perm(__byte_perm(__float_as_uint(lo.x), __float_as_uint(lo.y), 0x0040), __byte_perm(__float_as_uint(hi.x), __float_as_uint(hi.y), 0x0040), 0x5410);
 }
 // What four codes stand for, by bytes of 2^23 + 128 + code.
-__device__ __forceinline__ void valuesOf(uint32_t codes, float step, float *v) {
+__device__ __forceinline__ void valuesOf(uint32_t codes, float step, Pair &a, Pair &b) {
     const uint32_t raised = codes ^ 0x80808080u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (__uint_as_float(__byte_perm(raised, 0x4b000000u, 0x7440 + i)) - 8388736.f) * step;
+    const Pair base = pairOf(-8388736.f, -8388736.f), by = pairOf(step, step);
+    auto two = [&](int i) { return pairOf(__byte_perm(raised, 0x4b000000u, 0x7440 + i), __byte_perm(raised, 0x4b000000u, 0x7441 + i)); };
+    a = mul2(add2(two(0), base), by);
+    b = mul2(add2(two(2), base), by);
 }
 
 }  // namespace kept

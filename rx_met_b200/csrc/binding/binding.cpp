@@ -922,6 +922,7 @@ struct KeptRows {
         type = typeOf(x, name);
         width = static_cast<int>(x.size(-1));
         rows = asRows(x);
+        if (pitchOf(rows) * static_cast<int64_t>(x.element_size()) > INT32_MAX) rows = rows.contiguous();   // further apart than the C ABI takes them
         count = rows.size(0);
     }
     const void *data() const { return dataOf(rows); }

@@ -6,26 +6,58 @@
 
 #include "dependent_launch.cuh"
 #include "exponentials.cuh"
-#include "row_words.cuh"
 
 namespace rxmet {
 namespace kept {
 namespace {
 
-constexpr int kThreads = 256, kAtOnce = 2, kPer = 8;
+constexpr int kThreads = 256, kPer = 8;
 constexpr int kMaxWidth = 131071;   // as of codes of rows
 
+// Rows of an array, and the same from a row on.
+struct Rows {
+    uint8_t *at;
+    uint32_t pitch;   // bytes
+    __device__ __forceinline__ Rows from(int64_t row) const { return {at + row * pitch, pitch}; }
+    __device__ __forceinline__ uint8_t *place(uint32_t row, uint32_t byte) const { return at + static_cast<uint64_t>(row) * pitch + byte; }
+};
 struct Codes {
-    int8_t *codes, *exponents;
+    Rows codes, exponents;
+    __device__ __forceinline__ Codes from(int64_t row) const { return {codes.from(row), exponents.from(row)}; }
 };
 struct Pass {
     int64_t rows;
     int width, words, lowest;   // words: of eight elements in a row, a multiple of four
-    const void *a, *b;
-    int64_t aPitch, bPitch, codesPitch;
+    Rows a, b, y, z;
     Codes first, second;
-    void *y, *z;
 };
+
+// Eight elements of a row of a chunk.
+struct Spot {
+    uint32_t row, word;
+    bool real;
+};
+// The walk of the CTAs over all words: COUNT a thread at a time, so that it can ask for all operands before it uses the first; f(first row of the chunk, spots).  Rows and words of a chunk are 32-bit numbers,
+// and 64-bit addresses are worked out once a chunk.
+template <int COUNT, class F>
+__device__ __forceinline__ void eachSpot(const Pass &p, F f) {
+    const uint32_t words = p.words, per = COUNT * kThreads, rowsOf = max(1u, per / words), wordsOf = rowsOf * words;   // of a chunk
+    const uint32_t magic = 0xffffffffu / words + 1;   // i / words = high word of i * magic for i < 2^32 / words; at most 16384 words here
+    const int64_t chunks = (p.rows + rowsOf - 1) / rowsOf;
+    for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+        const int64_t first = chunk * rowsOf;
+        const uint32_t end = static_cast<uint32_t>(min(static_cast<int64_t>(rowsOf), p.rows - first)) * words;
+        for (uint32_t base = threadIdx.x; base < wordsOf; base += per) {
+            Spot at[COUNT];
+#pragma unroll
+            for (int n = 0; n < COUNT; ++n) {
+                const uint32_t i = base + n * kThreads, r = __umulhi(i, magic);
+                at[n] = {r, i - r * words, i < end};
+            }
+            f(first, at);
+        }
+    }
+}
 
 constexpr int kPairs = kPer / 2;   // of elements in 32 bits, two to a register pair
 // Eight neighbouring elements as they lie in memory; those that there are not are zeros.
@@ -63,8 +95,8 @@ struct alignas(16) Raw {
     }
 };
 template <class T, bool WIDE>
-__device__ __forceinline__ Raw<T> loadEight(const void *data, int64_t pitch, const RowWord &at, int count) {
-    const T *from = static_cast<const T *>(data) + static_cast<int64_t>(at.row) * pitch + at.word * kPer;
+__device__ __forceinline__ Raw<T> loadEight(const Rows &rows, const Spot &at, int count) {
+    const T *from = reinterpret_cast<const T *>(rows.place(at.row, at.word * (kPer * sizeof(T))));
     Raw<T> r{};
     if (WIDE && count > 0) {
 #pragma unroll
@@ -83,8 +115,8 @@ __device__ __forceinline__ Raw<T> loadEight(const void *data, int64_t pitch, con
     return r;
 }
 template <class T, bool WIDE>
-__device__ __forceinline__ void storeEight(void *data, int width, const RowWord &at, int count, const Pair (&v)[kPairs]) {
-    T *to = static_cast<T *>(data) + static_cast<int64_t>(at.row) * width + at.word * kPer;
+__device__ __forceinline__ void storeEight(const Rows &rows, const Spot &at, int count, const Pair (&v)[kPairs]) {
+    T *to = reinterpret_cast<T *>(rows.place(at.row, at.word * (kPer * sizeof(T))));
     if (WIDE && count > 0) {
         Raw<T> r;
 #pragma unroll
@@ -109,7 +141,7 @@ __device__ __forceinline__ void storeEight(void *data, int width, const RowWord 
 
 // By the four threads of a group.
 template <class T>
-__device__ __forceinline__ void keepEight(const Pass &p, const Codes &to, const RowWord &at, int count, const Raw<T> &raw, const Pair (&v)[kPairs]) {
+__device__ __forceinline__ void keepEight(const Pass &p, const Codes &to, const Spot &at, int count, const Raw<T> &raw, const Pair (&v)[kPairs]) {
     uint32_t most = raw.most();
     const unsigned group = 0xfu << (threadIdx.x & 28);
     most = max(most, __shfl_xor_sync(group, most, 1));
@@ -121,19 +153,19 @@ __device__ __forceinline__ void keepEight(const Pass &p, const Codes &to, const 
             const float inverse = powerOf(-e);
             codes = make_uint2(codesOf(v[0], v[1], inverse), codesOf(v[2], v[3], inverse));
         }
-        *reinterpret_cast<uint2 *>(to.codes + static_cast<int64_t>(at.row) * p.codesPitch + at.word * kPer) = codes;
+        *reinterpret_cast<uint2 *>(to.codes.place(at.row, at.word * kPer)) = codes;
     }
-    if ((threadIdx.x & 3) == 0) to.exponents[static_cast<int64_t>(at.row) * (p.words / 4) + at.word / 4] = static_cast<int8_t>(e);
+    if ((threadIdx.x & 3) == 0) *to.exponents.place(at.row, at.word / 4) = static_cast<uint8_t>(e);
 }
 struct Held {
     uint2 codes;
     int exponent;
 };
-__device__ __forceinline__ Held heldEight(const Pass &p, const Codes &from, const RowWord &at, int count) {
+__device__ __forceinline__ Held heldEight(const Codes &from, const Spot &at, int count) {
     Held h{make_uint2(0, 0), 0};
     if (count > 0) {
-        h.codes = *reinterpret_cast<const uint2 *>(from.codes + static_cast<int64_t>(at.row) * p.codesPitch + at.word * kPer);
-        h.exponent = from.exponents[static_cast<int64_t>(at.row) * (p.words / 4) + at.word / 4];
+        h.codes = *reinterpret_cast<const uint2 *>(from.codes.place(at.row, at.word * kPer));
+        h.exponent = static_cast<int8_t>(*from.exponents.place(at.row, at.word / 4));
     }
     return h;
 }
@@ -142,7 +174,13 @@ __device__ __forceinline__ void valuesOfEight(const Held &h, Pair (&v)[kPairs]) 
     valuesOf(h.codes.x, step, v[0], v[1]);
     valuesOf(h.codes.y, step, v[2], v[3]);
 }
-__device__ __forceinline__ int countOf(const Pass &p, const RowWord &at) { return at.real ? min(kPer, max(0, p.width - at.word * kPer)) : 0; }
+// Elements of a spot that there are; all or none where the width is a multiple of eight.
+template <bool WIDE>
+__device__ __forceinline__ int countOf(const Pass &p, const Spot &at) {
+    const int left = p.width - static_cast<int>(at.word * kPer);
+    if (WIDE) return at.real && left > 0 ? kPer : 0;
+    return at.real ? min(kPer, max(0, left)) : 0;
+}
 
 // The activation's values, and its slopes where they are wanted.  Normal distribution for gelu: Phi(x) keeps its bits for x far below zero, where 1 + erf does not.  BITS: significant ones of x.
 template <int ACTIVATION, bool SLOPES, int BITS>
@@ -170,20 +208,24 @@ __device__ __forceinline__ void activate(const Pair (&x)[kPairs], Pair (&y)[kPai
     }
 }
 
+constexpr int kCodesAtOnce = 2, kValuesAtOnce = 4, kProductsAtOnce = 2, kGradientsAtOnce = 2;
+
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(kThreads) keepCodes(const __grid_constant__ Pass p) {
     waitForPredecessor();
     letDependentsStart();
-    eachRowWord<kAtOnce>(p.rows, p.words, blockIdx.x, gridDim.x, [&](const RowWord(&at)[kAtOnce]) {
-        Raw<T> raw[kAtOnce];
+    eachSpot<kCodesAtOnce>(p, [&](int64_t first, const Spot(&at)[kCodesAtOnce]) {
+        const Rows x = p.a.from(first);
+        const Codes to = p.first.from(first);
+        Raw<T> raw[kCodesAtOnce];
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) raw[n] = loadEight<T, WIDE>(p.a, p.aPitch, at[n], countOf(p, at[n]));
+        for (int n = 0; n < kCodesAtOnce; ++n) raw[n] = loadEight<T, WIDE>(x, at[n], countOf<WIDE>(p, at[n]));
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) {
+        for (int n = 0; n < kCodesAtOnce; ++n) {
             if (!at[n].real) continue;
             Pair v[kPairs];
             raw[n].unpack(v);
-            keepEight<T>(p, p.first, at[n], countOf(p, at[n]), raw[n], v);
+            keepEight<T>(p, to, at[n], countOf<WIDE>(p, at[n]), raw[n], v);
         }
     });
 }
@@ -192,15 +234,17 @@ template <class T, bool WIDE>
 __global__ void __launch_bounds__(kThreads) keptValues(const __grid_constant__ Pass p) {
     waitForPredecessor();
     letDependentsStart();
-    eachRowWord<kAtOnce>(p.rows, p.words, blockIdx.x, gridDim.x, [&](const RowWord(&at)[kAtOnce]) {
-        Held held[kAtOnce];
+    eachSpot<kValuesAtOnce>(p, [&](int64_t first, const Spot(&at)[kValuesAtOnce]) {
+        const Codes from = p.first.from(first);
+        const Rows out = p.y.from(first);
+        Held held[kValuesAtOnce];
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) held[n] = heldEight(p, p.first, at[n], countOf(p, at[n]));
+        for (int n = 0; n < kValuesAtOnce; ++n) held[n] = heldEight(from, at[n], countOf<WIDE>(p, at[n]));
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) {
+        for (int n = 0; n < kValuesAtOnce; ++n) {
             Pair v[kPairs];
             valuesOfEight(held[n], v);
-            storeEight<T, WIDE>(p.y, p.width, at[n], countOf(p, at[n]), v);
+            storeEight<T, WIDE>(out, at[n], countOf<WIDE>(p, at[n]), v);
         }
     });
 }
@@ -210,28 +254,30 @@ template <class T, bool WIDE, int ACTIVATION>
 __global__ void __launch_bounds__(kThreads, 4) gatedProduct(const __grid_constant__ Pass p) {
     waitForPredecessor();
     letDependentsStart();
-    eachRowWord<kAtOnce>(p.rows, p.words, blockIdx.x, gridDim.x, [&](const RowWord(&at)[kAtOnce]) {
-        Raw<T> gates[kAtOnce], ups[kAtOnce];
+    eachSpot<kProductsAtOnce>(p, [&](int64_t first, const Spot(&at)[kProductsAtOnce]) {
+        const Rows gateRows = p.a.from(first), upRows = p.b.from(first), out = p.y.from(first);
+        const Codes gateCodes = p.first.from(first), upCodes = p.second.from(first);
+        Raw<T> gates[kProductsAtOnce], ups[kProductsAtOnce];
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) {
-            gates[n] = loadEight<T, WIDE>(p.a, p.aPitch, at[n], countOf(p, at[n]));
-            ups[n] = loadEight<T, WIDE>(p.b, p.bPitch, at[n], countOf(p, at[n]));
+        for (int n = 0; n < kProductsAtOnce; ++n) {
+            gates[n] = loadEight<T, WIDE>(gateRows, at[n], countOf<WIDE>(p, at[n]));
+            ups[n] = loadEight<T, WIDE>(upRows, at[n], countOf<WIDE>(p, at[n]));
         }
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) {
+        for (int n = 0; n < kProductsAtOnce; ++n) {
             if (!at[n].real) continue;
-            const int count = countOf(p, at[n]);
+            const int count = countOf<WIDE>(p, at[n]);
             Pair gate[kPairs], up[kPairs], y[kPairs], slope[kPairs];
             gates[n].unpack(gate);
             ups[n].unpack(up);
-            if (p.first.codes) {
-                keepEight<T>(p, p.first, at[n], count, gates[n], gate);
-                keepEight<T>(p, p.second, at[n], count, ups[n], up);
+            if (p.first.codes.at) {
+                keepEight<T>(p, gateCodes, at[n], count, gates[n], gate);
+                keepEight<T>(p, upCodes, at[n], count, ups[n], up);
             }
             activate<ACTIVATION, false, kSignificant<T>>(gate, y, slope);
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) y[i] = mul2(y[i], up[i]);
-            storeEight<T, WIDE>(p.y, p.width, at[n], count, y);
+            storeEight<T, WIDE>(out, at[n], count, y);
         }
     });
 }
@@ -241,19 +287,21 @@ template <class T, bool WIDE, int ACTIVATION>
 __global__ void __launch_bounds__(kThreads, 4) gatedProductBackward(const __grid_constant__ Pass p) {
     waitForPredecessor();
     letDependentsStart();
-    eachRowWord<kAtOnce>(p.rows, p.words, blockIdx.x, gridDim.x, [&](const RowWord(&at)[kAtOnce]) {
-        Raw<T> dys[kAtOnce];
-        Held gates[kAtOnce], ups[kAtOnce];
+    eachSpot<kGradientsAtOnce>(p, [&](int64_t first, const Spot(&at)[kGradientsAtOnce]) {
+        const Rows dyRows = p.a.from(first), dgate = p.y.from(first), dup = p.z.from(first);
+        const Codes gateCodes = p.first.from(first), upCodes = p.second.from(first);
+        Raw<T> dys[kGradientsAtOnce];
+        Held gates[kGradientsAtOnce], ups[kGradientsAtOnce];
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) {
-            const int count = countOf(p, at[n]);
-            dys[n] = loadEight<T, WIDE>(p.a, p.aPitch, at[n], count);
-            gates[n] = heldEight(p, p.first, at[n], count);
-            ups[n] = heldEight(p, p.second, at[n], count);
+        for (int n = 0; n < kGradientsAtOnce; ++n) {
+            const int count = countOf<WIDE>(p, at[n]);
+            dys[n] = loadEight<T, WIDE>(dyRows, at[n], count);
+            gates[n] = heldEight(gateCodes, at[n], count);
+            ups[n] = heldEight(upCodes, at[n], count);
         }
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) {
-            const int count = countOf(p, at[n]);
+        for (int n = 0; n < kGradientsAtOnce; ++n) {
+            const int count = countOf<WIDE>(p, at[n]);
             Pair dy[kPairs], gate[kPairs], up[kPairs], y[kPairs], slope[kPairs];
             dys[n].unpack(dy);
             valuesOfEight(gates[n], gate);
@@ -264,8 +312,8 @@ __global__ void __launch_bounds__(kThreads, 4) gatedProductBackward(const __grid
                 y[i] = mul2(y[i], dy[i]);
                 slope[i] = mul2(slope[i], mul2(up[i], dy[i]));
             }
-            if (p.z) storeEight<T, WIDE>(p.z, p.width, at[n], count, y);
-            if (p.y) storeEight<T, WIDE>(p.y, p.width, at[n], count, slope);
+            if (p.z.at) storeEight<T, WIDE>(dup, at[n], count, y);
+            if (p.y.at) storeEight<T, WIDE>(dgate, at[n], count, slope);
         }
     });
 }
@@ -283,9 +331,17 @@ Pass passOf(int64_t rows, int width, int type, const char *what) {
     p.lowest = lowestExponent(type);
     return p;
 }
-void requireCodes(const Pass &p, const void *codes, const void *exponents, const char *what) {
+// Rows `pitch` elements apart; the distance of a single row's next one does not matter.
+Rows rowsOf(const Pass &p, const void *data, int64_t pitch, size_t size, const char *what) {
+    if (p.rows == 1) pitch = 0;
+    RXMET_REQUIRE(pitch >= 0, "%s: rows %lld elements apart", what, static_cast<long long>(pitch));
+    if (pitch > static_cast<int64_t>(INT32_MAX / size)) fail(RXMET_ERR_UNSUPPORTED, "%s: rows %lld elements apart, at most %lld", what, static_cast<long long>(pitch), static_cast<long long>(INT32_MAX / size));
+    return {static_cast<uint8_t *>(const_cast<void *>(data)), static_cast<uint32_t>(pitch * static_cast<int64_t>(size))};
+}
+Codes codeRowsOf(const Pass &p, const void *codes, const void *exponents, int64_t pitch, const char *what) {
     RXMET_REQUIRE(codes && exponents, "%s: null pointer", what);
-    RXMET_REQUIRE(alignedTo(codes, 16) && p.codesPitch % 16 == 0 && (p.rows == 1 || p.codesPitch >= p.width), "%s: rows of codes must start on 16 bytes, and apart", what);
+    RXMET_REQUIRE(alignedTo(codes, 16) && (p.rows == 1 || (pitch % 16 == 0 && pitch >= p.width)), "%s: rows of codes must start on 16 bytes, and apart", what);
+    return {rowsOf(p, codes, pitch, 1, what), rowsOf(p, exponents, p.words / 4, 1, what)};
 }
 
 // f(the activation as a constant).
@@ -298,8 +354,9 @@ void withActivation(int activation, F f) {
 }
 
 template <class F>
-void launch(F kernel, const char *name, const Pass &p, cudaStream_t st) {
-    const int blocks = rowWordBlocks(p.rows, p.words, kAtOnce, kThreads, currentDevice().sms * residentPerSm(reinterpret_cast<const void *>(kernel), kThreads, 0));
+void launch(F kernel, int atOnce, const char *name, const Pass &p, cudaStream_t st) {
+    const int64_t rowsOf = std::max<int64_t>(1, atOnce * kThreads / p.words), chunks = (p.rows + rowsOf - 1) / rowsOf;
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(chunks, currentDevice().sms * residentPerSm(reinterpret_cast<const void *>(kernel), kThreads, 0)));
     {
         KernelTimer timer__(name, st);
         launchDependent(kernel, blocks, kThreads, 0, st, p);
@@ -317,16 +374,13 @@ extern "C" int rxmet_keep_codes(int64_t rows, int width, int type, const void *x
     return guarded([&] {
         kept::Pass p = kept::passOf(rows, width, type, "keep_codes");
         if (rows == 0) return;
-        p.codesPitch = codes_pitch;
         RXMET_REQUIRE(x, "keep_codes: null pointer");
-        kept::requireCodes(p, codes, exponents, "keep_codes");
-        p.a = x;
-        p.aPitch = x_pitch;
-        p.first = {codes, exponents};
+        p.a = kept::rowsOf(p, x, x_pitch, typeBytes(type), "keep_codes");
+        p.first = kept::codeRowsOf(p, codes, exponents, codes_pitch, "keep_codes");
         const bool wide = width % 8 == 0 && kept::wideRows(x, rows, x_pitch, typeBytes(type));
         withType(type, [&](auto t) {
             using T = decltype(t);
-            kept::launch(wide ? kept::keepCodes<T, true> : kept::keepCodes<T, false>, "keepCodes", p, static_cast<cudaStream_t>(stream));
+            kept::launch(wide ? kept::keepCodes<T, true> : kept::keepCodes<T, false>, kept::kCodesAtOnce, "keepCodes", p, static_cast<cudaStream_t>(stream));
         });
     });
 }
@@ -335,15 +389,13 @@ extern "C" int rxmet_kept_values(int64_t rows, int width, int type, const int8_t
     return guarded([&] {
         kept::Pass p = kept::passOf(rows, width, type, "kept_values");
         if (rows == 0) return;
-        p.codesPitch = codes_pitch;
         RXMET_REQUIRE(out, "kept_values: null pointer");
-        kept::requireCodes(p, codes, exponents, "kept_values");
-        p.y = out;
-        p.first = {const_cast<int8_t *>(codes), const_cast<int8_t *>(exponents)};
+        p.y = kept::rowsOf(p, out, width, typeBytes(type), "kept_values");
+        p.first = kept::codeRowsOf(p, codes, exponents, codes_pitch, "kept_values");
         const bool wide = width % 8 == 0 && alignedTo(out, 16);
         withType(type, [&](auto t) {
             using T = decltype(t);
-            kept::launch(wide ? kept::keptValues<T, true> : kept::keptValues<T, false>, "keptValues", p, static_cast<cudaStream_t>(stream));
+            kept::launch(wide ? kept::keptValues<T, true> : kept::keptValues<T, false>, kept::kValuesAtOnce, "keptValues", p, static_cast<cudaStream_t>(stream));
         });
     });
 }
@@ -354,26 +406,21 @@ extern "C" int rxmet_gated_product(int64_t rows, int width, int type, int activa
         kept::Pass p = kept::passOf(rows, width, type, "gated_product");
         RXMET_REQUIRE(activation >= RXMET_ACTIVATION_NONE && activation <= RXMET_ACTIVATION_GELU, "gated_product: unknown activation %d", activation);
         if (rows == 0) return;
-        p.codesPitch = codes_pitch;
         RXMET_REQUIRE(gate && up && y, "gated_product: null pointer");
         if (gate_codes || gate_exponents || up_codes || up_exponents) {
-            kept::requireCodes(p, gate_codes, gate_exponents, "gated_product");
-            kept::requireCodes(p, up_codes, up_exponents, "gated_product");
+            p.first = kept::codeRowsOf(p, gate_codes, gate_exponents, codes_pitch, "gated_product");
+            p.second = kept::codeRowsOf(p, up_codes, up_exponents, codes_pitch, "gated_product");
         }
-        p.a = gate;
-        p.aPitch = gate_pitch;
-        p.b = up;
-        p.bPitch = up_pitch;
-        p.y = y;
-        p.first = {gate_codes, gate_exponents};
-        p.second = {up_codes, up_exponents};
         const size_t size = typeBytes(type);
+        p.a = kept::rowsOf(p, gate, gate_pitch, size, "gated_product");
+        p.b = kept::rowsOf(p, up, up_pitch, size, "gated_product");
+        p.y = kept::rowsOf(p, y, width, size, "gated_product");
         const bool wide = width % 8 == 0 && kept::wideRows(gate, rows, gate_pitch, size) && kept::wideRows(up, rows, up_pitch, size) && alignedTo(y, 16);
         withType(type, [&](auto t) {
             using T = decltype(t);
             kept::withActivation(activation, [&](auto a) {
                 constexpr int kActivation = decltype(a)::value;
-                kept::launch(wide ? kept::gatedProduct<T, true, kActivation> : kept::gatedProduct<T, false, kActivation>, "gatedProduct", p, static_cast<cudaStream_t>(stream));
+                kept::launch(wide ? kept::gatedProduct<T, true, kActivation> : kept::gatedProduct<T, false, kActivation>, kept::kProductsAtOnce, "gatedProduct", p, static_cast<cudaStream_t>(stream));
             });
         });
     });
@@ -385,22 +432,19 @@ extern "C" int rxmet_gated_product_backward(int64_t rows, int width, int type, i
         kept::Pass p = kept::passOf(rows, width, type, "gated_product backward");
         RXMET_REQUIRE(activation >= RXMET_ACTIVATION_NONE && activation <= RXMET_ACTIVATION_GELU, "gated_product backward: unknown activation %d", activation);
         if (rows == 0 || (!dgate && !dup)) return;
-        p.codesPitch = codes_pitch;
         RXMET_REQUIRE(dy, "gated_product backward: null pointer");
-        kept::requireCodes(p, gate_codes, gate_exponents, "gated_product backward");
-        kept::requireCodes(p, up_codes, up_exponents, "gated_product backward");
-        p.a = dy;
-        p.aPitch = dy_pitch;
-        p.y = dgate;
-        p.z = dup;
-        p.first = {const_cast<int8_t *>(gate_codes), const_cast<int8_t *>(gate_exponents)};
-        p.second = {const_cast<int8_t *>(up_codes), const_cast<int8_t *>(up_exponents)};
+        const size_t size = typeBytes(type);
+        p.a = kept::rowsOf(p, dy, dy_pitch, size, "gated_product backward");
+        p.y = kept::rowsOf(p, dgate, width, size, "gated_product backward");
+        p.z = kept::rowsOf(p, dup, width, size, "gated_product backward");
+        p.first = kept::codeRowsOf(p, gate_codes, gate_exponents, codes_pitch, "gated_product backward");
+        p.second = kept::codeRowsOf(p, up_codes, up_exponents, codes_pitch, "gated_product backward");
         const bool wide = width % 8 == 0 && kept::wideRows(dy, rows, dy_pitch, typeBytes(type)) && alignedTo(dgate, 16) && alignedTo(dup, 16);
         withType(type, [&](auto t) {
             using T = decltype(t);
             kept::withActivation(activation, [&](auto a) {
                 constexpr int kActivation = decltype(a)::value;
-                kept::launch(wide ? kept::gatedProductBackward<T, true, kActivation> : kept::gatedProductBackward<T, false, kActivation>, "gatedProductBackward", p, static_cast<cudaStream_t>(stream));
+                kept::launch(wide ? kept::gatedProductBackward<T, true, kActivation> : kept::gatedProductBackward<T, false, kActivation>, kept::kGradientsAtOnce, "gatedProductBackward", p, static_cast<cudaStream_t>(stream));
             });
         });
     });

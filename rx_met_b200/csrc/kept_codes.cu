@@ -37,25 +37,45 @@ struct Spot {
     uint32_t row, word;
     bool real;
 };
-// The walk of the CTAs over all words: COUNT a thread at a time, so that it can ask for all operands before it uses the first; f(first row of the chunk, spots).  Rows and words of a chunk are 32-bit numbers,
-// and 64-bit addresses are worked out once a chunk.
-template <int COUNT, class F>
-__device__ __forceinline__ void eachSpot(const Pass &p, F f) {
+// The walk of the CTAs over all words, COUNT a thread at a time: load(first row of the chunk, spots) asks for the operands of a round, and use(first, spots, operands) works on them once those of the next
+// round have been asked for.  Rows and words of a chunk are 32-bit numbers, and 64-bit addresses are worked out once a round.
+template <int COUNT, class Load, class Use>
+__device__ __forceinline__ void eachSpot(const Pass &p, Load load, Use use) {
     const uint32_t words = p.words, per = COUNT * kThreads, rowsOf = max(1u, per / words), wordsOf = rowsOf * words;   // of a chunk
     const uint32_t magic = 0xffffffffu / words + 1;   // i / words = high word of i * magic for i < 2^32 / words; at most 16384 words here
     const int64_t chunks = (p.rows + rowsOf - 1) / rowsOf;
-    for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-        const int64_t first = chunk * rowsOf;
-        const uint32_t end = static_cast<uint32_t>(min(static_cast<int64_t>(rowsOf), p.rows - first)) * words;
-        for (uint32_t base = threadIdx.x; base < wordsOf; base += per) {
-            Spot at[COUNT];
+    struct Round {
+        int64_t chunk, first;
+        uint32_t base, end;
+        Spot at[COUNT];
+    };
+    auto place = [&](Round &r) {
+        r.first = r.chunk * rowsOf;
+        r.end = r.chunk < chunks ? static_cast<uint32_t>(min(static_cast<int64_t>(rowsOf), p.rows - r.first)) * words : 0u;
 #pragma unroll
-            for (int n = 0; n < COUNT; ++n) {
-                const uint32_t i = base + n * kThreads, r = __umulhi(i, magic);
-                at[n] = {r, i - r * words, i < end};
-            }
-            f(first, at);
+        for (int n = 0; n < COUNT; ++n) {
+            const uint32_t i = r.base + n * kThreads + threadIdx.x, row = __umulhi(i, magic);
+            r.at[n] = {row, i - row * words, i < r.end};
         }
+    };
+    Round now;
+    now.chunk = blockIdx.x;
+    now.base = 0;
+    place(now);
+    auto operands = load(now.first, now.at);
+    while (now.chunk < chunks) {
+        Round next;
+        next.base = now.base + per;
+        next.chunk = now.chunk;
+        if (next.base >= wordsOf) {
+            next.base = 0;
+            next.chunk += gridDim.x;
+        }
+        place(next);
+        auto later = load(next.first, next.at);
+        use(now.first, now.at, operands);
+        now = next;
+        operands = later;
     }
 }
 
@@ -214,18 +234,24 @@ template <class T, bool WIDE>
 __global__ void __launch_bounds__(kThreads) keepCodes(const __grid_constant__ Pass p) {
     waitForPredecessor();
     letDependentsStart();
-    eachSpot<kCodesAtOnce>(p, [&](int64_t first, const Spot(&at)[kCodesAtOnce]) {
+    struct Operands {
+        Raw<T> x[kCodesAtOnce];
+    };
+    auto load = [&](int64_t first, const Spot(&at)[kCodesAtOnce]) {
         const Rows x = p.a.from(first);
-        const Codes to = p.first.from(first);
-        Raw<T> raw[kCodesAtOnce];
+        Operands o;
 #pragma unroll
-        for (int n = 0; n < kCodesAtOnce; ++n) raw[n] = loadEight<T, WIDE>(x, at[n], countOf<WIDE>(p, at[n]));
+        for (int n = 0; n < kCodesAtOnce; ++n) o.x[n] = loadEight<T, WIDE>(x, at[n], countOf<WIDE>(p, at[n]));
+        return o;
+    };
+    eachSpot<kCodesAtOnce>(p, load, [&](int64_t first, const Spot(&at)[kCodesAtOnce], const Operands &o) {
+        const Codes to = p.first.from(first);
 #pragma unroll
         for (int n = 0; n < kCodesAtOnce; ++n) {
             if (!at[n].real) continue;
             Pair v[kPairs];
-            raw[n].unpack(v);
-            keepEight<T>(p, to, at[n], countOf<WIDE>(p, at[n]), raw[n], v);
+            o.x[n].unpack(v);
+            keepEight<T>(p, to, at[n], countOf<WIDE>(p, at[n]), o.x[n], v);
         }
     });
 }
@@ -234,16 +260,22 @@ template <class T, bool WIDE>
 __global__ void __launch_bounds__(kThreads) keptValues(const __grid_constant__ Pass p) {
     waitForPredecessor();
     letDependentsStart();
-    eachSpot<kValuesAtOnce>(p, [&](int64_t first, const Spot(&at)[kValuesAtOnce]) {
+    struct Operands {
+        Held x[kValuesAtOnce];
+    };
+    auto load = [&](int64_t first, const Spot(&at)[kValuesAtOnce]) {
         const Codes from = p.first.from(first);
-        const Rows out = p.y.from(first);
-        Held held[kValuesAtOnce];
+        Operands o;
 #pragma unroll
-        for (int n = 0; n < kValuesAtOnce; ++n) held[n] = heldEight(from, at[n], countOf<WIDE>(p, at[n]));
+        for (int n = 0; n < kValuesAtOnce; ++n) o.x[n] = heldEight(from, at[n], countOf<WIDE>(p, at[n]));
+        return o;
+    };
+    eachSpot<kValuesAtOnce>(p, load, [&](int64_t first, const Spot(&at)[kValuesAtOnce], const Operands &o) {
+        const Rows out = p.y.from(first);
 #pragma unroll
         for (int n = 0; n < kValuesAtOnce; ++n) {
             Pair v[kPairs];
-            valuesOfEight(held[n], v);
+            valuesOfEight(o.x[n], v);
             storeEight<T, WIDE>(out, at[n], countOf<WIDE>(p, at[n]), v);
         }
     });
@@ -251,28 +283,35 @@ __global__ void __launch_bounds__(kThreads) keptValues(const __grid_constant__ P
 
 // a: gate, b: up.
 template <class T, bool WIDE, int ACTIVATION>
-__global__ void __launch_bounds__(kThreads, 4) gatedProduct(const __grid_constant__ Pass p) {
+__global__ void __launch_bounds__(kThreads, 3) gatedProduct(const __grid_constant__ Pass p) {
     waitForPredecessor();
     letDependentsStart();
-    eachSpot<kProductsAtOnce>(p, [&](int64_t first, const Spot(&at)[kProductsAtOnce]) {
-        const Rows gateRows = p.a.from(first), upRows = p.b.from(first), out = p.y.from(first);
-        const Codes gateCodes = p.first.from(first), upCodes = p.second.from(first);
-        Raw<T> gates[kProductsAtOnce], ups[kProductsAtOnce];
+    struct Operands {
+        Raw<T> gate[kProductsAtOnce], up[kProductsAtOnce];
+    };
+    auto load = [&](int64_t first, const Spot(&at)[kProductsAtOnce]) {
+        const Rows gate = p.a.from(first), up = p.b.from(first);
+        Operands o;
 #pragma unroll
         for (int n = 0; n < kProductsAtOnce; ++n) {
-            gates[n] = loadEight<T, WIDE>(gateRows, at[n], countOf<WIDE>(p, at[n]));
-            ups[n] = loadEight<T, WIDE>(upRows, at[n], countOf<WIDE>(p, at[n]));
+            o.gate[n] = loadEight<T, WIDE>(gate, at[n], countOf<WIDE>(p, at[n]));
+            o.up[n] = loadEight<T, WIDE>(up, at[n], countOf<WIDE>(p, at[n]));
         }
+        return o;
+    };
+    eachSpot<kProductsAtOnce>(p, load, [&](int64_t first, const Spot(&at)[kProductsAtOnce], const Operands &o) {
+        const Rows out = p.y.from(first);
+        const Codes gateCodes = p.first.from(first), upCodes = p.second.from(first);
 #pragma unroll
         for (int n = 0; n < kProductsAtOnce; ++n) {
             if (!at[n].real) continue;
             const int count = countOf<WIDE>(p, at[n]);
             Pair gate[kPairs], up[kPairs], y[kPairs], slope[kPairs];
-            gates[n].unpack(gate);
-            ups[n].unpack(up);
+            o.gate[n].unpack(gate);
+            o.up[n].unpack(up);
             if (p.first.codes.at) {
-                keepEight<T>(p, gateCodes, at[n], count, gates[n], gate);
-                keepEight<T>(p, upCodes, at[n], count, ups[n], up);
+                keepEight<T>(p, gateCodes, at[n], count, o.gate[n], gate);
+                keepEight<T>(p, upCodes, at[n], count, o.up[n], up);
             }
             activate<ACTIVATION, false, kSignificant<T>>(gate, y, slope);
 #pragma unroll
@@ -284,28 +323,35 @@ __global__ void __launch_bounds__(kThreads, 4) gatedProduct(const __grid_constan
 
 // a: dy, y: dgate, z: dup.
 template <class T, bool WIDE, int ACTIVATION>
-__global__ void __launch_bounds__(kThreads, 4) gatedProductBackward(const __grid_constant__ Pass p) {
+__global__ void __launch_bounds__(kThreads, 3) gatedProductBackward(const __grid_constant__ Pass p) {
     waitForPredecessor();
     letDependentsStart();
-    eachSpot<kGradientsAtOnce>(p, [&](int64_t first, const Spot(&at)[kGradientsAtOnce]) {
-        const Rows dyRows = p.a.from(first), dgate = p.y.from(first), dup = p.z.from(first);
-        const Codes gateCodes = p.first.from(first), upCodes = p.second.from(first);
-        Raw<T> dys[kGradientsAtOnce];
-        Held gates[kGradientsAtOnce], ups[kGradientsAtOnce];
+    struct Operands {
+        Raw<T> dy[kGradientsAtOnce];
+        Held gate[kGradientsAtOnce], up[kGradientsAtOnce];
+    };
+    auto load = [&](int64_t first, const Spot(&at)[kGradientsAtOnce]) {
+        const Rows dy = p.a.from(first);
+        const Codes gate = p.first.from(first), up = p.second.from(first);
+        Operands o;
 #pragma unroll
         for (int n = 0; n < kGradientsAtOnce; ++n) {
             const int count = countOf<WIDE>(p, at[n]);
-            dys[n] = loadEight<T, WIDE>(dyRows, at[n], count);
-            gates[n] = heldEight(gateCodes, at[n], count);
-            ups[n] = heldEight(upCodes, at[n], count);
+            o.dy[n] = loadEight<T, WIDE>(dy, at[n], count);
+            o.gate[n] = heldEight(gate, at[n], count);
+            o.up[n] = heldEight(up, at[n], count);
         }
+        return o;
+    };
+    eachSpot<kGradientsAtOnce>(p, load, [&](int64_t first, const Spot(&at)[kGradientsAtOnce], const Operands &o) {
+        const Rows dgate = p.y.from(first), dup = p.z.from(first);
 #pragma unroll
         for (int n = 0; n < kGradientsAtOnce; ++n) {
             const int count = countOf<WIDE>(p, at[n]);
             Pair dy[kPairs], gate[kPairs], up[kPairs], y[kPairs], slope[kPairs];
-            dys[n].unpack(dy);
-            valuesOfEight(gates[n], gate);
-            valuesOfEight(ups[n], up);
+            o.dy[n].unpack(dy);
+            valuesOfEight(o.gate[n], gate);
+            valuesOfEight(o.up[n], up);
             activate<ACTIVATION, true, 8>(gate, y, slope);   // a code has eight bits, times a power of two
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) {

@@ -3,8 +3,9 @@
 //
 // On tcgen05 kind::f16 with 32-bit sums in tensor memory.  A code times its power of two is a number of bfloat16 and of half, so that one product a term is exact; dy in 32 bits comes as
 // its three runs of eight bits, each a number of bfloat16.
-// A pair of CTAs computes tiles of 256 output channels x 256 input channels, 64 tokens at a time; each CTA holds half of both operands.  dy arrives by TMA in the order in which
-// the tensor cores read it across its rows.  Eight warps load the codes, a few chunks ahead, and turn them into 16-bit values in that order: ten instructions for four codes.  Four warps store a tile while the next one is summed, two accumulators in turn.
+// A pair of CTAs computes tiles of 256 input channels x 512 output channels, 64 tokens at a time; each CTA holds half of both operands.  The values of the codes serve two products, which fill the tensor
+// memory: with one (256 x 256) shared memory had 80 kB to move for a chunk of 512 cycles, 16384 tokens of 4096 x 4096 took 450 us.  dy arrives by TMA in the order in which the tensor cores read it
+// across its rows.  Sixteen warps load the codes, a few chunks ahead, and turn them into 16-bit values in that order: ten instructions for four codes.  The same warps store a tile's sums.
 // Few tiles leave SMs without work, so the tokens are cut into parts, whose sums another kernel adds up in their order.
 #include "kept_codes.cuh"
 
@@ -17,11 +18,12 @@ namespace {
 
 using namespace ummatiles;
 
-constexpr int kTile = 256, kHalf = kTile / 2, kTokens = 64, kBlock = 64;   // kBlock: 16-bit elements of a swizzled row
-constexpr int kStages = 7, kConvertWarps = 16, kTeams = 4, kStoreWarps = 4;   // teams of converting warps take chunks in turn
-constexpr int kThreads = 32 * (kConvertWarps + kStoreWarps + 2);
+constexpr int kTile = 256, kHalf = kTile / 2, kTokens = 64, kBlock = 64;   // kTile: input channels, and output channels of one product; kBlock: 16-bit elements of a swizzled row
+constexpr int kOuter = 2 * kTile;                                          // output channels of a tile: two products, which share the codes' values
+constexpr int kStages = 4, kConvertWarps = 16, kTeams = 4;   // teams of converting warps take chunks in turn
+constexpr int kThreads = 32 * (kConvertWarps + 2);
 constexpr uint32_t kBlockBytes = kTokens * kBlock * 2, kOperandBytes = kHalf / kBlock * kBlockBytes;
-constexpr uint32_t kStageBytes = 2 * kOperandBytes;
+constexpr uint32_t kStageBytes = 3 * kOperandBytes;   // the codes' values, and dy of two products
 constexpr uint32_t kShared = 231936;   // cluster::leastShared(512): one CTA an SM
 static_assert(kStages * kStageBytes + 1024 <= kShared, "the stages fit");
 
@@ -95,7 +97,7 @@ template <class T, class OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     keptWeightGradient(const __grid_constant__ Problem p, const __grid_constant__ CUtensorMap dyMap, int *status) {
     extern __shared__ uint8_t raw[];
-    __shared__ __align__(8) uint64_t dyFull[kStages], converted[kStages], freed[kStages], accFull[2], accFree[2];
+    __shared__ __align__(8) uint64_t dyFull[kStages], converted[kStages], freed[kStages], accFull, accFree;
     __shared__ uint32_t tmemSlot;
     const uint32_t stages = (smemAddr(raw) + 1023u) & ~1023u;
     const int warp = warpIndex(), lane = threadIdx.x & 31;
@@ -106,10 +108,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             cluster::initBarrier(&converted[i], 2 * kConvertWarps / kTeams);
             cluster::initBarrier(&freed[i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
-            cluster::initBarrier(&accFull[i], 1);
-            cluster::initBarrier(&accFree[i], 2 * kStoreWarps);
-        }
+        cluster::initBarrier(&accFull, 1);
+        cluster::initBarrier(&accFree, 2 * kConvertWarps);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         prefetchMap(&dyMap);
     }
@@ -122,20 +122,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     waitForPredecessor();
     letDependentsStart();
 
-    const int outerTiles = (p.outer + kTile - 1) / kTile, innerTiles = (p.inner + kTile - 1) / kTile;
+    const int outerTiles = (p.outer + kOuter - 1) / kOuter, innerTiles = (p.inner + kTile - 1) / kTile;
     const int tiles = outerTiles * innerTiles, pairs = gridDim.x / 2;
     const int64_t items = static_cast<int64_t>(tiles) * p.parts;
-    // A part's tiles are neighbours, in columns of eight outer tiles, so that the pairs at work at the same time share both operands.
+    // A part's tiles are neighbours, in columns of four outer tiles, so that the pairs at work at the same time share both operands.
     struct Place {
-        int part, n0, k0, first, count;   // count: chunks of a term
+        int part, n0, k0, products, first, count;   // count: chunks of a term
     };
     auto place = [&](int64_t item) {
         Place at;
         at.part = static_cast<int>(item / tiles);
         const int tile = static_cast<int>(item - static_cast<int64_t>(at.part) * tiles);
-        const int group = tile / (8 * innerTiles), row0 = group * 8, rows = min(8, outerTiles - row0), in = tile - group * 8 * innerTiles;
+        const int group = tile / (4 * innerTiles), row0 = group * 4, rows = min(4, outerTiles - row0), in = tile - group * 4 * innerTiles;
         at.k0 = in / rows * kTile;
-        at.n0 = (row0 + in % rows) * kTile;
+        at.n0 = (row0 + in % rows) * kOuter;
+        at.products = p.outer - at.n0 > kTile ? 2 : 1;
         at.first = static_cast<int>(static_cast<int64_t>(p.chunks) * at.part / p.parts);
         at.count = static_cast<int>(static_cast<int64_t>(p.chunks) * (at.part + 1) / p.parts) - at.first;
         return at;
@@ -145,7 +146,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (alive) alive = __all_sync(0xffffffffu, waitSuspended(smemAddr(bar), parity));
     };
 
-    if (warp == kConvertWarps + kStoreWarps) {   // copies
+    if (warp == kConvertWarps) {   // copies
         Turn turn;
         for (int64_t item = blockIdx.x / 2; item < items; item += pairs) {
             const Place at = place(item);
@@ -155,8 +156,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (alive && electOne()) {
                         const uint32_t to = stages + turn.at * kStageBytes, m = (at.first + c) * kTokens;
                         const uint32_t bar = smemAddr(&dyFull[turn.at]);
-                        if (rank == 0) cluster::arriveExpect(bar, 2 * kOperandBytes);
-                        for (int block = 0; block < kHalf / kBlock; ++block) copyTile3Pair(to + block * kBlockBytes, &dyMap, at.n0 + rank * kHalf + block * kBlock, m, term, bar);
+                        if (rank == 0) cluster::arriveExpect(bar, 2 * at.products * kOperandBytes);
+                        for (int i = 0; i < at.products; ++i)
+                            for (int block = 0; block < kHalf / kBlock; ++block)
+                                copyTile3Pair(to + (1 + i) * kOperandBytes + block * kBlockBytes, &dyMap, at.n0 + i * kTile + rank * kHalf + block * kBlock, m, term, bar);
                     }
                     __syncwarp();
                 }
@@ -164,15 +167,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         // nothing is left in flight: the last use of each stage is read before this CTA ends
         for (int i = 0; i < kStages; ++i, turn.step(kStages))
             if (turn.again) waitSuspended(smemAddr(&freed[turn.at]), turn.parity ^ 1u);
-    } else if (warp == kConvertWarps + kStoreWarps + 1) {   // products, issued by the first CTA for both
+    } else if (warp == kConvertWarps + 1) {   // products, issued by the first CTA for both
         if (rank == 0) {
             Turn turn;
             int done = 0;
             constexpr uint32_t kIdesc = pairHalves(std::is_same_v<T, __nv_bfloat16>);
             for (int64_t item = blockIdx.x / 2; item < items; item += pairs, ++done) {
                 const Place at = place(item);
-                const uint32_t buf = done & 1;
-                if (done > 1) wait(&accFree[buf], ((done >> 1) - 1) & 1);
+                if (done > 0) wait(&accFree, (done - 1) & 1);
                 fenceAfter();
                 const int chunks = p.terms * at.count;
                 for (int c = 0; c < chunks; ++c, turn.step(kStages)) {
@@ -181,24 +183,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (alive && electOne()) {
                         fenceAfter();
                         const uint32_t from = stages + turn.at * kStageBytes;
-                        const uint64_t a = swizzledDescriptor(from, kBlockBytes), b = swizzledDescriptor(from + kOperandBytes, kBlockBytes);
+                        const uint64_t values = swizzledDescriptor(from, kBlockBytes);
+                        for (int i = 0; i < at.products; ++i) {
+                            const uint64_t dy = swizzledDescriptor(from + (1 + i) * kOperandBytes, kBlockBytes);
 #pragma unroll
-                        for (int k = 0; k < kTokens / 16; ++k) productPair(tmem + buf * kTile, a + k * (2048 >> 4), b + k * (2048 >> 4), kIdesc, c + k > 0 ? 1u : 0u);
+                            for (int k = 0; k < kTokens / 16; ++k) productPair(tmem + i * kTile, values + k * (2048 >> 4), dy + k * (2048 >> 4), kIdesc, c + k > 0 ? 1u : 0u);
+                        }
                         commitPair(smemAddr(&freed[turn.at]));
-                        if (c + 1 == chunks) commitPair(smemAddr(&accFull[buf]));
+                        if (c + 1 == chunks) commitPair(smemAddr(&accFull));
                     }
                     __syncwarp();
                 }
             }
         }
-    } else if (warp < kConvertWarps) {   // codes to values: a thread takes sixteen codes of a token at a time; teams take chunks in turn
+    } else {   // codes to values: a thread takes sixteen codes of a token at a time; teams take chunks in turn
         constexpr int kThreadsOfTeam = 32 * kConvertWarps / kTeams, kRows = kThreadsOfTeam / 8, kPieces = kTokens / kRows;
         // Eight neighbouring lanes store two rows of a block at once: the swizzle keeps an even row and the odd one behind it apart in the banks.
         const int team = threadIdx.x / kThreadsOfTeam, index = threadIdx.x % kThreadsOfTeam;
         const int column = index & 3, block = (index >> 3) & 1, row = ((index >> 2) & 1) + 2 * (index >> 4);
         const int inRow = block * kBlock + column * 16, groups = groupsOf(p.inner);
-        const uint32_t place0 = kOperandBytes + block * kBlockBytes;
+        const uint32_t place0 = block * kBlockBytes;
         int64_t seen = 0;   // chunks of the tiles so far
+        uint32_t done = 0;
         Turn turn;
         turn.step(kStages, team);
         for (int64_t item = blockIdx.x / 2; item < items; item += pairs) {
@@ -206,106 +212,89 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const int k = at.k0 + rank * kHalf + inRow, real = p.inner - k, chunks = p.terms * at.count;
             const int begin = static_cast<int>((team + kTeams - seen % kTeams) % kTeams);
             seen += chunks;
-            if (begin >= chunks) continue;
-            uint4 codes[kPieces];
-            int exponents[kPieces];
-            int chunk = begin % at.count;   // of the tokens, for what is asked for next
-            const int8_t *codesAt, *exponentsAt;
-            int left;                       // of its tokens, those that there are
-            auto turnTo = [&] {
-                const int64_t m = static_cast<int64_t>(at.first + chunk) * kTokens + row;
-                codesAt = p.codes + m * p.codesPitch + k;
-                exponentsAt = p.exponents + m * groups + k / kGroup;
-                left = real > 0 ? static_cast<int>(min(static_cast<int64_t>(kTokens), p.tokens - m)) : 0;
-            };
-            auto ask = [&](int i) {
-                codes[i] = make_uint4(0, 0, 0, 0);
-                exponents[i] = 0;
-                if (i * kRows < left) {
-                    codes[i] = __ldg(reinterpret_cast<const uint4 *>(codesAt));
-                    exponents[i] = __ldg(exponentsAt);
-                }
-                codesAt += kRows * p.codesPitch;
-                exponentsAt += kRows * groups;
-            };
-            turnTo();
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) ask(i);
-            for (int c = begin; c < chunks; c += kTeams, turn.step(kStages, kTeams)) {
-                if (turn.again) wait(&freed[turn.at], turn.parity ^ 1u);
-                const uint32_t values = stages + turn.at * kStageBytes + place0 + row * 128;
-                for (chunk += kTeams; chunk >= at.count;) chunk -= at.count;
-                turnTo();
-                if (c + kTeams >= chunks) left = 0;
-#pragma unroll
-                for (int i = 0; i < kPieces; ++i) {
-                    const uint32_t step = Convert<T>::step(exponents[i]);
-                    uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w}, v[8];
-                    if (real < 16) {   // what lies between a row's end and the next row may be anything
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int within = min(4, max(0, real - 4 * j));
-                            w[j] = within == 4 ? w[j] : w[j] & ((1u << (8 * within)) - 1);
-                        }
+            if (begin < chunks) {
+                uint4 codes[kPieces];
+                int exponents[kPieces];
+                int chunk = begin % at.count;   // of the tokens, for what is asked for next
+                const int8_t *codesAt, *exponentsAt;
+                int left;                       // of its tokens, those that there are
+                auto turnTo = [&] {
+                    const int64_t m = static_cast<int64_t>(at.first + chunk) * kTokens + row;
+                    codesAt = p.codes + m * p.codesPitch + k;
+                    exponentsAt = p.exponents + m * groups + k / kGroup;
+                    left = real > 0 ? static_cast<int>(min(static_cast<int64_t>(kTokens), p.tokens - m)) : 0;
+                };
+                auto ask = [&](int i) {
+                    codes[i] = make_uint4(0, 0, 0, 0);
+                    exponents[i] = 0;
+                    if (i * kRows < left) {
+                        codes[i] = __ldg(reinterpret_cast<const uint4 *>(codesAt));
+                        exponents[i] = __ldg(exponentsAt);
                     }
-                    ask(i);
+                    codesAt += kRows * p.codesPitch;
+                    exponentsAt += kRows * groups;
+                };
+                turnTo();
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) Convert<T>::four(w[j], step, v[2 * j], v[2 * j + 1]);
-                    // rows of a thread are kRows apart, a multiple of eight: one swizzle for all
+                for (int i = 0; i < kPieces; ++i) ask(i);
+                for (int c = begin; c < chunks; c += kTeams, turn.step(kStages, kTeams)) {
+                    if (turn.again) wait(&freed[turn.at], turn.parity ^ 1u);
+                    const uint32_t values = stages + turn.at * kStageBytes + place0 + row * 128;
+                    for (chunk += kTeams; chunk >= at.count;) chunk -= at.count;
+                    turnTo();
+                    if (c + kTeams >= chunks) left = 0;
 #pragma unroll
-                    for (int half = 0; half < 2; ++half)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(values + i * kRows * 128 + (((2 * column + half) ^ (row & 7)) << 4)), "r"(v[4 * half]),
-                                     "r"(v[4 * half + 1]), "r"(v[4 * half + 2]), "r"(v[4 * half + 3])
-                                     : "memory");
+                    for (int i = 0; i < kPieces; ++i) {
+                        const uint32_t step = Convert<T>::step(exponents[i]);
+                        uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w}, v[8];
+                        if (real < 16) {   // what lies between a row's end and the next row may be anything
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int within = min(4, max(0, real - 4 * j));
+                                w[j] = within == 4 ? w[j] : w[j] & ((1u << (8 * within)) - 1);
+                            }
+                        }
+                        ask(i);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) Convert<T>::four(w[j], step, v[2 * j], v[2 * j + 1]);
+                        // rows of a thread are kRows apart, a multiple of eight: one swizzle for all
+#pragma unroll
+                        for (int half = 0; half < 2; ++half)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(values + i * kRows * 128 + (((2 * column + half) ^ (row & 7)) << 4)), "r"(v[4 * half]),
+                                         "r"(v[4 * half + 1]), "r"(v[4 * half + 2]), "r"(v[4 * half + 3])
+                                         : "memory");
+                    }
+                    fenceAsyncProxy();
+                    __syncwarp();
+                    if (lane == 0) arrivePair(smemAddr(&converted[turn.at]));
                 }
-                fenceAsyncProxy();
-                __syncwarp();
-                if (lane == 0) arrivePair(smemAddr(&converted[turn.at]));
             }
-        }
-    } else {   // stores
-        const int quarter = warp & 3;
-        int done = 0;
-        for (int64_t item = blockIdx.x / 2; item < items; item += pairs, ++done) {
-            const Place at = place(item);
-            const uint32_t buf = done & 1;
-            const int n = at.n0 + rank * kHalf + 32 * quarter + lane, count = min(kTile, p.inner - at.k0);
+            // the tile's sums: a lane of tensor memory is an input channel, and for one output channel the lanes of a warp store neighbours
+            constexpr int kColumns = kOuter / (kConvertWarps / 4);
+            const int quarter = warp & 3, group = warp >> 2;   // of input channels, of output channels
+            const int kOut = at.k0 + rank * kHalf + 32 * quarter + lane, n = at.n0 + group * kColumns, count = min(kColumns, p.outer - n);
             OUT *to = nullptr;
             if constexpr (std::is_same_v<OUT, float>) to = p.parts > 1 ? p.partial + static_cast<int64_t>(at.part) * p.outer * p.inner : static_cast<float *>(p.out);
             else to = static_cast<OUT *>(p.out);
-            to += static_cast<int64_t>(n) * p.inner + at.k0;
-            constexpr int kPer = 16 / sizeof(OUT);
-            const bool wide = p.inner % kPer == 0 && reinterpret_cast<uintptr_t>(to) % 16 == 0;
-            wait(&accFull[buf], (done >> 1) & 1);
+            to += static_cast<int64_t>(n) * p.inner + kOut;
+            wait(&accFull, done & 1);
+            ++done;
             fenceAfter();
-            const uint32_t from = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + buf * kTile;
+            const uint32_t from = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + group * kColumns;
 #pragma unroll 1
-            for (int col = 0; col < kTile; col += 32) {
-                uint32_t acc[32];
+            for (int col = 0; col < count; col += 16) {
+                uint32_t acc[16];
                 __syncwarp();
-                loadTmem32(from + col, acc);
+                loadTmem16(from + col, acc);
                 loadsDone();
-                if (col + 32 == kTile) {
-                    fenceBefore();
-                    __syncwarp();
-                    if (lane == 0) arriveRemote(cluster::remote(smemAddr(&accFree[buf]), 0));
-                }
-                if (!alive || n >= p.outer) continue;
-                if (wide) {
+                if (!alive || kOut >= p.inner) continue;
 #pragma unroll
-                    for (int j = 0; j < 32; j += kPer) {
-                        if (col + j >= count) break;
-                        Pack<OUT, kPer> pack;
-#pragma unroll
-                        for (int i = 0; i < kPer; ++i) pack.v[i] = fromFloat<OUT>(__uint_as_float(acc[j + i]));
-                        *reinterpret_cast<Pack<OUT, kPer> *>(to + col + j) = pack;
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (col + j < count) to[col + j] = fromFloat<OUT>(__uint_as_float(acc[j]));
-                }
+                for (int j = 0; j < 16; ++j, to += p.inner)
+                    if (col + j < count) *to = fromFloat<OUT>(__uint_as_float(acc[j]));
             }
+            fenceBefore();
+            __syncwarp();
+            if (lane == 0) arriveRemote(cluster::remote(smemAddr(&accFree), 0));
         }
     }
     if (!alive && lane == 0) atomicExch(status, 1);
@@ -315,6 +304,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (warp == 0) freeTmem<2>(tmem, 512);
 }
 
+constexpr int kLayRows = 4;   // rows of dy that a thread asks for at once
+
 // dy in rows that TMA can copy, [term][token][pitch]: a copy of 16-bit elements, or the three runs of eight bits of a float, from the top.
 template <class T, int TERMS>
 __global__ void __launch_bounds__(256) layGradient(const T *dy, int64_t dyPitch, int64_t tokens, int outer, uint16_t *to, int pitch) {
@@ -322,27 +313,35 @@ __global__ void __launch_bounds__(256) layGradient(const T *dy, int64_t dyPitch,
     waitForPredecessor();
     letDependentsStart();
     if (n >= outer) return;
-    for (int64_t m = blockIdx.y; m < tokens; m += gridDim.y) {
-        uint32_t out[TERMS] = {};
+    for (int64_t m0 = static_cast<int64_t>(blockIdx.y) * kLayRows; m0 < tokens; m0 += static_cast<int64_t>(gridDim.y) * kLayRows) {
+        T in[kLayRows][2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (n + i >= outer) break;
-            if constexpr (TERMS == 1) {
-                out[0] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(dy + m * dyPitch + n + i)) << (16 * i);
-            } else {
-                float left = dy[m * dyPitch + n + i];
-                const bool finite = (__float_as_uint(left) & 0x7f800000u) != 0x7f800000u;
-                if (isnan(left)) left = __int_as_float(0x7fc00000);   // whose upper half is one, too
+        for (int r = 0; r < kLayRows; ++r)
 #pragma unroll
-                for (int t = 0; t < TERMS; ++t) {
-                    const uint32_t top = __float_as_uint(left) & 0xffff0000u;
-                    out[t] |= (top >> 16) << (16 * i);
-                    left = finite ? left - __uint_as_float(top) : 0.f;
+            for (int i = 0; i < 2; ++i) in[r][i] = m0 + r < tokens && n + i < outer ? dy[(m0 + r) * dyPitch + n + i] : fromFloat<T>(0.f);
+#pragma unroll
+        for (int r = 0; r < kLayRows; ++r) {
+            uint32_t out[TERMS] = {};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if constexpr (TERMS == 1) {
+                    out[0] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&in[r][i])) << (16 * i);
+                } else {
+                    float left = in[r][i];
+                    const bool finite = (__float_as_uint(left) & 0x7f800000u) != 0x7f800000u;
+                    if (isnan(left)) left = __int_as_float(0x7fc00000);   // whose upper half is one, too
+#pragma unroll
+                    for (int t = 0; t < TERMS; ++t) {
+                        const uint32_t top = __float_as_uint(left) & 0xffff0000u;
+                        out[t] |= (top >> 16) << (16 * i);
+                        left = finite ? left - __uint_as_float(top) : 0.f;
+                    }
                 }
             }
-        }
+            if (m0 + r >= tokens) break;
 #pragma unroll
-        for (int t = 0; t < TERMS; ++t) *reinterpret_cast<uint32_t *>(to + (static_cast<int64_t>(t) * tokens + m) * pitch + n) = out[t];
+            for (int t = 0; t < TERMS; ++t) *reinterpret_cast<uint32_t *>(to + (static_cast<int64_t>(t) * tokens + m0 + r) * pitch + n) = out[t];
+        }
     }
 }
 
@@ -353,10 +352,17 @@ __global__ void __launch_bounds__(256) sumParts(const float *partial, int parts,
     letDependentsStart();
     for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * W; i < total; i += static_cast<int64_t>(gridDim.x) * 256 * W) {
         float sum[W] = {};
-        for (int part = 0; part < parts; ++part) {
-            const Pack<float, W> v = *reinterpret_cast<const Pack<float, W> *>(partial + part * total + i);
+        constexpr int kAtOnce = 8;
+        for (int part = 0; part < parts; part += kAtOnce) {
+            Pack<float, W> v[kAtOnce];
 #pragma unroll
-            for (int j = 0; j < W; ++j) sum[j] += v.v[j];
+            for (int q = 0; q < kAtOnce; ++q)
+                if (part + q < parts) v[q] = *reinterpret_cast<const Pack<float, W> *>(partial + (part + q) * total + i);
+#pragma unroll
+            for (int q = 0; q < kAtOnce; ++q)
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    if (part + q < parts) sum[j] += v[q].v[j];
         }
         Pack<OUT, W> r;
 #pragma unroll
@@ -379,7 +385,7 @@ struct Plan {
     int terms, pitch, parts, chunks;
     bool copied;
 };
-// The least of these estimates, in microseconds: 0.3 for a chunk, 3 to begin and end a tile, and for several parts 2.5 and the writing and reading of their sums.
+// The least of these estimates, in microseconds: 0.3 for a product of a chunk, 4 to begin and end a tile, and for several parts 2.5 and the writing and reading of their sums.
 Plan planOf(int64_t tokens, int inner, int outer, int type, const void *dy, int64_t dyPitch) {
     Plan plan;
     plan.terms = type == RXMET_TYPE_F32 ? 3 : 1;
@@ -387,12 +393,13 @@ Plan planOf(int64_t tokens, int inner, int outer, int type, const void *dy, int6
     plan.pitch = static_cast<int>(alignUp(outer, 8));
     plan.chunks = static_cast<int>((tokens + kTokens - 1) / kTokens);
     const int pairs = std::max(1, currentDevice().sms / 2);
-    const int64_t tiles = static_cast<int64_t>((outer + kTile - 1) / kTile) * ((inner + kTile - 1) / kTile);
+    const int64_t tiles = static_cast<int64_t>((outer + kOuter - 1) / kOuter) * ((inner + kTile - 1) / kTile);
+    const int products = outer > kTile ? 2 : 1;
     double best = 0;
     plan.parts = 1;
     for (int q = 1; q <= std::min(plan.chunks, pairs); ++q) {
         const double rounds = static_cast<double>((tiles * q + pairs - 1) / pairs), chunks = (plan.chunks + q - 1) / q * plan.terms;
-        const double time = rounds * (0.3 * chunks + 3.0) + (q > 1 ? 2.5 + 8e-6 / 5 * q * outer * inner : 0.0);
+        const double time = rounds * (0.3 * products * chunks + 4.0) + (q > 1 ? 2.5 + 8e-6 / 5 * q * outer * inner : 0.0);
         if (q == 1 || time < best) {
             best = time;
             plan.parts = q;
@@ -423,7 +430,7 @@ template <class T, class OUT>
 void launchProduct(const Problem &p, const CUtensorMap &dy, cudaStream_t st) {
     const auto kernel = keptWeightGradient<T, OUT>;
     ensureDynamicSmem(reinterpret_cast<const void *>(kernel), kShared);
-    const int64_t items = static_cast<int64_t>((p.outer + kTile - 1) / kTile) * ((p.inner + kTile - 1) / kTile) * p.parts;
+    const int64_t items = static_cast<int64_t>((p.outer + kOuter - 1) / kOuter) * ((p.inner + kTile - 1) / kTile) * p.parts;
     {
         KernelTimer timer__("keptWeightGradient", st);
         launchDependent(kernel, 2 * static_cast<unsigned>(std::min<int64_t>(currentDevice().sms / 2, items)), kThreads, kShared, st, p, dy, waitStatus());
@@ -467,7 +474,7 @@ extern "C" int rxmet_kept_weight_gradient(int64_t tokens, int inner, int outer, 
         uint16_t *laid = nullptr;
         kept::takeBuffers(Workspace(workspace, workspace_bytes), plan, tokens, inner, outer, &laid, &p.partial);
         if (plan.copied) {
-            const dim3 grid((outer + 511) / 512, static_cast<unsigned>(std::min<int64_t>(tokens, std::max(1, 16 * currentDevice().sms / ((outer + 511) / 512)))));
+            const dim3 grid((outer + 511) / 512, static_cast<unsigned>(std::min<int64_t>((tokens + kept::kLayRows - 1) / kept::kLayRows, std::max(1, 16 * currentDevice().sms / ((outer + 511) / 512)))));
             {
                 KernelTimer timer__("layGradient", st);
                 if (type == RXMET_TYPE_F32) launchDependent(kept::layGradient<float, 3>, grid, 256, 0, st, static_cast<const float *>(dy), dy_pitch, tokens, outer, laid, plan.pitch);

@@ -1,0 +1,177 @@
+"""The gated mixer's operators together: a block that trains with activations kept in 8 bits and serves in 8-bit codes."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+import gated_lib as gl
+
+pytestmark = pytest.mark.gpu
+
+WIDTH, INNER, HIDDEN = 192, 160, 400
+
+
+def block(dtype, seed=0):
+    from rx_met_b200.gated_block import GatedBlock
+    torch.manual_seed(seed)
+    return GatedBlock(WIDTH, INNER, HIDDEN, dtype=dtype)
+
+
+def norm(t, scale):
+    return t * torch.rsqrt((t ** 2).mean(dim=-1, keepdim=True) + 1e-6) * scale
+
+
+def recur(forget, value, state):
+    """Differentiable, in 64 bits."""
+    f, h, out = torch.sigmoid(forget), state, []
+    for t in range(forget.shape[1]):
+        h = f[:, t] * h + torch.sigmoid(-forget[:, t]) * value[:, t]
+        out.append(h)
+    return torch.stack(out, dim=1)
+
+
+def kept(x):
+    """What the codes of x stand for, with the gradient of x."""
+    return x + (gl.values(*gl.keep(x.detach().float())) - x).detach()
+
+
+def linear(x, weight, bias=None):
+    """The product, with the gradient of the weight from kept codes."""
+    k = kept(x.detach())
+    y = F.linear(x, weight.detach()) + F.linear(k, weight) - F.linear(k, weight.detach())
+    return y if bias is None else y + bias
+
+
+def gated(gate, up):
+    """The product, with the gradients at the values of kept codes."""
+    s = F.silu(kept(gate)) * kept(up)
+    return s + (F.silu(gate) * up - s).detach()
+
+
+def plain(x, w, state):
+    f, v, g = linear(norm(x, w["norm1"]), w["w_in"], w["bias"]).chunk(3, dim=-1)
+    h = x + linear(gated(g, recur(f, v, state)), w["w_mix"])
+    a, b = linear(norm(h, w["norm2"]), w["w_up"]).chunk(2, dim=-1)
+    return h + linear(gated(a, b), w["w_down"])
+
+
+def off(got, want):
+    return float((got.detach().double() - want.detach()).norm() / want.detach().norm())
+
+
+# relative, over the whole output: eight roundings of 2^-9 to 2^-8 of their type's values in a row for 16 bits; 8-bit codes are off by 127^-1 / sqrt(12) of a row's largest value, four times its mean for
+# normal values and eight times for products of two, on both sides of a product: 1.3 and 2.6 %, of which a half of the block has three
+@pytest.mark.parametrize("dtype,floats,codes", [(torch.float32, 1e-5, 0.06), (torch.bfloat16, 0.02, 0.06), (torch.float16, 0.003, 0.06)])
+def test_block_against_its_formula(dtype, floats, codes):
+    b = block(dtype)
+    x = torch.randn(3, 150, WIDTH, device="cuda").to(dtype)
+    state = torch.randn(3, INNER, device="cuda")
+    lengths = torch.tensor([150, 0, 77], device="cuda")
+    w = {n: p.detach().double() for n, p in b.named_parameters()}
+    want = plain(x.double(), w, state.double())
+    y, last = b(x, state)
+    assert y.dtype == dtype and off(y, want) < floats
+    f, v, _ = F.linear(norm(x.double(), w["norm1"]), w["w_in"], w["bias"]).chunk(3, dim=-1)
+    _, wanted_last, *_ = gl.recur(f, v, state=state, lengths=lengths)
+    c = b.coded()
+    for call, allowed in ((b, floats), (c.prefill, codes)):
+        _, ragged = call(x, state, lengths)
+        assert off(ragged, wanted_last) < allowed
+    y, _ = c.prefill(x, state)
+    assert y.dtype == dtype and off(y, want) < codes
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_prompt_and_its_tokens(dtype):
+    """A prompt at once, and its last tokens one by one behind the rest of it."""
+    c = block(dtype, seed=1).coded()
+    x = torch.randn(2, 140, WIDTH, device="cuda").to(dtype)
+    whole, last = c.prefill(x)
+    first, state = c.prefill(x[:, :132])
+    tail = torch.stack([c.step(x[:, t], state) for t in range(132, 140)], dim=1)
+    # the two ways round differently, and a code may fall on the other side of a half
+    assert off(tail, whole[:, 132:].double()) < 0.02 and off(state, last.double()) < 0.02 and torch.isfinite(tail).all()
+    assert off(first, whole[:, :132].double()) < 0.02
+
+
+def test_block_trains():
+    """Gradients of all parameters, of the input and of the state against automatic differentiation of the formulas in 64 bits."""
+    b = block(torch.float32, seed=2)
+    x, state = torch.randn(2, 70, WIDTH, device="cuda").requires_grad_(), torch.randn(2, INNER, device="cuda").requires_grad_()
+    dy = torch.randn(2, 70, WIDTH, device="cuda")
+    params = {n: p.detach().double().requires_grad_() for n, p in b.named_parameters()}
+    ends = [x.detach().double().requires_grad_(), state.detach().double().requires_grad_()]
+    wants = torch.autograd.grad(plain(ends[0], params, ends[1]), [*params.values(), *ends], dy.double())
+    grads = torch.autograd.grad(b(x, state)[0], [*b.parameters(), x, state], dy)
+    for name, got, want in zip([*params, "x", "state"], grads, wants):
+        # activations that are off by 1e-6 of a group's largest fall on the other side of a half in 2.5e-4 of all cases, by a step of 1 / 127 of it: 2.5e-4 of their norm, a few times over
+        assert off(got, want) < 1e-3, name
+
+
+def test_a_captured_training_step():
+    """The same gradients from a graph as from the calls, on inputs that change."""
+    b = block(torch.bfloat16, seed=3)
+    x, dy = (torch.randn(2, 200, WIDTH, device="cuda").bfloat16() for _ in range(2))
+    params = list(b.parameters())
+
+    def step(t):
+        return torch.autograd.grad(b(t)[0], params, dy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(x)
+    torch.cuda.current_stream().wait_stream(side)
+    held = torch.zeros_like(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(held)
+    for seed in range(2):
+        torch.manual_seed(seed)
+        other = torch.randn_like(x)
+        held.copy_(other)
+        graph.replay()
+        kept_grads = [g.clone() for g in got]
+        # torch's products may differ in their order of sums between a graph's workspace and another
+        assert all(off(a, w.double()) < 0.02 for a, w in zip(kept_grads, step(other)))
+
+
+def test_block_in_a_graph():
+    """A decoding step of the coded block, captured and replayed on new tokens."""
+    c = block(torch.bfloat16, seed=4).coded()
+    x = torch.randn(4, WIDTH, device="cuda").bfloat16()
+    state = torch.zeros(4, INNER, device="cuda")
+    c.step(x, state.clone())
+    held = torch.empty_like(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = c.step(held, state)
+    state.zero_()
+    other = torch.zeros_like(state)
+    for seed in range(3):
+        torch.manual_seed(seed)
+        token = torch.randn(4, WIDTH, device="cuda").bfloat16()
+        held.copy_(token)
+        graph.replay()
+        assert torch.equal(y, c.step(token, other)) and torch.equal(state, other)
+
+
+def test_what_a_block_keeps():
+    """Between the passes: codes of the inputs of four products and of four factors, the norms' inputs, and the gates and values of the recurrence."""
+    b = block(torch.bfloat16, seed=5)
+    rows = 4 * 2048
+    x = torch.randn(4, 2048, WIDTH, device="cuda").bfloat16()
+    b(x)[0].sum().backward()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y, last = b(x)
+    held = torch.cuda.memory_allocated() - before - y.numel() * 2
+    codes = sum(n + n // 32 + 32 for n in (WIDTH, INNER, WIDTH, HIDDEN, INNER, INNER, HIDDEN, HIDDEN))
+    # the norms keep x, the mixed stream and a float each; the recurrence a projection's result, and with it the gate; marks and a MB of rounding
+    floats = 2 * (WIDTH + WIDTH) + 2 * 3 * INNER + 8
+    assert held <= rows * (codes + floats) + (4 << 20)
+
+
+def test_no_wait_gave_up():
+    import rx_met_b200
+    assert rx_met_b200.wait_gave_up() is False

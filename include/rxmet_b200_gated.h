@@ -62,8 +62,8 @@ RXMET_API int rxmet_gated_product_backward(int64_t rows, int width, int type, in
 
 /* ---- gradient of a weight from kept codes ---------------------------------------------------------
  * out[n][k] = sum_m dy[m][n] * codes[m][k] * 2^exponents[m][k / 32], dy of `type` with rows dy_pitch elements apart, the codes those of an activation of that type;
- * out [outer][inner] contiguous in out_type.  Products are exact, sums in 32 bits.  tokens and outer at most 2^30, inner at most 131071. */
-RXMET_API size_t rxmet_kept_weight_gradient_workspace_bytes(int64_t tokens, int inner, int outer, int type, const void *dy_dev, int64_t dy_pitch);
+ * out [outer][inner] contiguous in out_type.  Products are exact, sums in 32 bits (long ones in parts of 512 tokens, where the sums of the tensor cores alone would show in out).  tokens and outer at most 2^30, inner at most 131071. */
+RXMET_API size_t rxmet_kept_weight_gradient_workspace_bytes(int64_t tokens, int inner, int outer, int type, const void *dy_dev, int64_t dy_pitch, int out_type);
 RXMET_API int rxmet_kept_weight_gradient(int64_t tokens, int inner, int outer, int type, const void *dy_dev, int64_t dy_pitch, const int8_t *codes_dev,
                                          int64_t codes_pitch, const int8_t *exponents_dev, int out_type, void *out_dev, void *workspace_dev,
                                          size_t workspace_bytes, void *stream);

@@ -1051,7 +1051,7 @@ Tensor keptWeightGradient(const Tensor &dy, const Tensor &codes, const Tensor &e
     TORCH_CHECK(d.type == type, "dy must be of the type of the activation that was kept");
     const c10::cuda::CUDAGuard guard(codes.device());
     const Tensor out = emptyLike(codes, {d.width, h.width}, kElementTypes[outType]);
-    const size_t bytes = rxmet_kept_weight_gradient_workspace_bytes(d.count, h.width, d.width, d.type, d.data(), d.pitch());
+    const size_t bytes = rxmet_kept_weight_gradient_workspace_bytes(d.count, h.width, d.width, d.type, d.data(), d.pitch(), outType);
     const Tensor ws = bytes > 0 ? emptyLike(codes, {static_cast<int64_t>(bytes)}, at::kByte) : Tensor();
     checkStatus(rxmet_kept_weight_gradient(d.count, h.width, d.width, d.type, d.data(), d.pitch(), h.data(), h.pitch(), h.powers(), outType, mutableOf(out), mutableOf(ws), bytes,
                                            streamOf(codes)),

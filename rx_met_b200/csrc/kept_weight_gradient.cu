@@ -19,13 +19,18 @@ namespace {
 using namespace ummatiles;
 
 constexpr int kTile = 256, kHalf = kTile / 2, kTokens = 64, kBlock = 64;   // kTile: input channels, and output channels of one product; kBlock: 16-bit elements of a swizzled row
-constexpr int kOuter = 2 * kTile;                                          // output channels of a tile: two products, which share the codes' values
-constexpr int kStages = 4, kConvertWarps = 16, kTeams = 4;   // teams of converting warps take chunks in turn
+constexpr int kConvertWarps = 16, kTeams = 4;                              // teams of converting warps take chunks in turn
+// A tile's output channels: two products, which share the codes' values, or, with sums in parts, one.
+__host__ __device__ constexpr int outerOf(bool fine) { return fine ? kTile : 2 * kTile; }
+__host__ __device__ constexpr int stagesOf(bool fine) { return fine ? 7 : 4; }
+// Chunks that are summed in tensor memory before the sum is taken over to registers.  A product's step cuts its sum to 24 bits, towards zero: n steps leave about n 2^-25 of it, where roundings would
+// leave the root of that (65536 tokens at 112 steps a part: 1.7e-6 of the gradient, in segments of 32 steps 0.4e-6; torch's products in 32 bits: 0.6e-6).
+constexpr int kSegment = 8, kSteps = kTokens / 16;
 constexpr int kThreads = 32 * (kConvertWarps + 2);
 constexpr uint32_t kBlockBytes = kTokens * kBlock * 2, kOperandBytes = kHalf / kBlock * kBlockBytes;
-constexpr uint32_t kStageBytes = 3 * kOperandBytes;   // the codes' values, and dy of two products
+__host__ __device__ constexpr uint32_t stageBytes(bool fine) { return (fine ? 2 : 3) * kOperandBytes; }   // the codes' values, and dy of the products
 constexpr uint32_t kShared = 231936;   // cluster::leastShared(512): one CTA an SM
-static_assert(kStages * kStageBytes + 1024 <= kShared, "the stages fit");
+static_assert(stagesOf(true) * stageBytes(true) + 1024 <= kShared && stagesOf(false) * stageBytes(false) + 1024 <= kShared, "the stages fit");
 
 struct Problem {
     int64_t tokens;
@@ -92,12 +97,14 @@ struct Convert<__half> {
     }
 };
 
-// T: the products' type; OUT: that of what is stored (parts: floats).
-template <class T, class OUT>
+// T: the products' type; OUT: that of what is stored (parts: floats); FINE: sums in segments.
+template <class T, class OUT, bool FINE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     keptWeightGradient(const __grid_constant__ Problem p, const __grid_constant__ CUtensorMap dyMap, int *status) {
+    constexpr int kStages = stagesOf(FINE), kOuter = outerOf(FINE), kProducts = FINE ? 1 : 2;
+    constexpr uint32_t kStageBytes = stageBytes(FINE);
     extern __shared__ uint8_t raw[];
-    __shared__ __align__(8) uint64_t dyFull[kStages], converted[kStages], freed[kStages], accFull, accFree;
+    __shared__ __align__(8) uint64_t dyFull[kStages], converted[kStages], freed[kStages], accFull[2], accFree[2];   // a second accumulator where sums are in segments
     __shared__ uint32_t tmemSlot;
     const uint32_t stages = (smemAddr(raw) + 1023u) & ~1023u;
     const int warp = warpIndex(), lane = threadIdx.x & 31;
@@ -108,8 +115,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             cluster::initBarrier(&converted[i], 2 * kConvertWarps / kTeams);
             cluster::initBarrier(&freed[i], 1);
         }
-        cluster::initBarrier(&accFull, 1);
-        cluster::initBarrier(&accFree, 2 * kConvertWarps);
+        for (int i = 0; i < 2; ++i) {
+            cluster::initBarrier(&accFull[i], 1);
+            cluster::initBarrier(&accFree[i], 2 * kConvertWarps);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         prefetchMap(&dyMap);
     }
@@ -136,7 +145,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int group = tile / (4 * innerTiles), row0 = group * 4, rows = min(4, outerTiles - row0), in = tile - group * 4 * innerTiles;
         at.k0 = in / rows * kTile;
         at.n0 = (row0 + in % rows) * kOuter;
-        at.products = p.outer - at.n0 > kTile ? 2 : 1;
+        at.products = kProducts == 2 && p.outer - at.n0 > kTile ? 2 : 1;
         at.first = static_cast<int>(static_cast<int64_t>(p.chunks) * at.part / p.parts);
         at.count = static_cast<int>(static_cast<int64_t>(p.chunks) * (at.part + 1) / p.parts) - at.first;
         return at;
@@ -150,7 +159,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         Turn turn;
         for (int64_t item = blockIdx.x / 2; item < items; item += pairs) {
             const Place at = place(item);
-            for (int term = 0; term < p.terms; ++term)
+            for (int term = p.terms - 1; term >= 0; --term)   // the least first, while the sum that they are cut to is small
                 for (int c = 0; c < at.count; ++c, turn.step(kStages)) {
                     if (turn.again) wait(&freed[turn.at], turn.parity ^ 1u);
                     if (alive && electOne()) {
@@ -170,14 +179,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     } else if (warp == kConvertWarps + 1) {   // products, issued by the first CTA for both
         if (rank == 0) {
             Turn turn;
-            int done = 0;
+            uint32_t sums = 0;   // so far: of tiles, or of their segments
             constexpr uint32_t kIdesc = pairHalves(std::is_same_v<T, __nv_bfloat16>);
-            for (int64_t item = blockIdx.x / 2; item < items; item += pairs, ++done) {
+            for (int64_t item = blockIdx.x / 2; item < items; item += pairs) {
                 const Place at = place(item);
-                if (done > 0) wait(&accFree, (done - 1) & 1);
-                fenceAfter();
                 const int chunks = p.terms * at.count;
                 for (int c = 0; c < chunks; ++c, turn.step(kStages)) {
+                    const bool begins = c == 0 || (FINE && c % kSegment == 0), ends = c + 1 == chunks || (FINE && (c + 1) % kSegment == 0);
+                    const uint32_t buf = FINE ? sums & 1 : 0, uses = FINE ? sums >> 1 : sums;   // of that accumulator, before this one
+                    if (begins && uses > 0) wait(&accFree[buf], (uses - 1) & 1);
                     wait(&dyFull[turn.at], turn.parity);
                     wait(&converted[turn.at], turn.parity);
                     if (alive && electOne()) {
@@ -187,12 +197,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         for (int i = 0; i < at.products; ++i) {
                             const uint64_t dy = swizzledDescriptor(from + (1 + i) * kOperandBytes, kBlockBytes);
 #pragma unroll
-                            for (int k = 0; k < kTokens / 16; ++k) productPair(tmem + i * kTile, values + k * (2048 >> 4), dy + k * (2048 >> 4), kIdesc, c + k > 0 ? 1u : 0u);
+                            for (int k = 0; k < kSteps; ++k) productPair(tmem + (buf + i) * kTile, values + k * (2048 >> 4), dy + k * (2048 >> 4), kIdesc, !begins || k > 0 ? 1u : 0u);
                         }
                         commitPair(smemAddr(&freed[turn.at]));
-                        if (c + 1 == chunks) commitPair(smemAddr(&accFull));
+                        if (ends) commitPair(smemAddr(&accFull[buf]));
                     }
                     __syncwarp();
+                    if (ends) ++sums;
                 }
             }
         }
@@ -204,7 +215,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int inRow = block * kBlock + column * 16, groups = groupsOf(p.inner);
         const uint32_t place0 = block * kBlockBytes;
         int64_t seen = 0;   // chunks of the tiles so far
-        uint32_t done = 0;
+        uint32_t sums = 0;
+        constexpr int kColumns = kOuter / (kConvertWarps / 4);
+        const int quarter = warp & 3, part = warp >> 2;   // of a tile's input channels, of its output channels
+        const uint32_t sumsAt = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + part * kColumns;
         Turn turn;
         turn.step(kStages, team);
         for (int64_t item = blockIdx.x / 2; item < items; item += pairs) {
@@ -212,6 +226,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const int k = at.k0 + rank * kHalf + inRow, real = p.inner - k, chunks = p.terms * at.count;
             const int begin = static_cast<int>((team + kTeams - seen % kTeams) % kTeams);
             seen += chunks;
+            float total[FINE ? kColumns : 1];
+            int segment = 0;
+            auto takeSegment = [&] {
+                const uint32_t buf = sums & 1;
+                wait(&accFull[buf], (sums >> 1) & 1);
+                fenceAfter();
+#pragma unroll
+                for (int col = 0; col < kColumns; col += 16) {
+                    uint32_t acc[16];
+                    loadTmem16(sumsAt + buf * kTile + col, acc);
+                    loadsDone();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (FINE) total[col + j] += __uint_as_float(acc[j]);
+                }
+                fenceBefore();
+                __syncwarp();
+                if (lane == 0) arrivePair(smemAddr(&accFree[buf]));
+                ++sums;
+                ++segment;
+            };
+            if (FINE) {
+#pragma unroll
+                for (int j = 0; j < (FINE ? kColumns : 1); ++j) total[j] = 0.f;
+            }
             if (begin < chunks) {
                 uint4 codes[kPieces];
                 int exponents[kPieces];
@@ -267,34 +306,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     fenceAsyncProxy();
                     __syncwarp();
                     if (lane == 0) arrivePair(smemAddr(&converted[turn.at]));
+                    // a segment whose products lie as far back as there are stages is there
+                    if (FINE && (segment + 1) * kSegment + kStages <= c) takeSegment();
                 }
             }
             // the tile's sums: a lane of tensor memory is an input channel, and for one output channel the lanes of a warp store neighbours
-            constexpr int kColumns = kOuter / (kConvertWarps / 4);
-            const int quarter = warp & 3, group = warp >> 2;   // of input channels, of output channels
-            const int kOut = at.k0 + rank * kHalf + 32 * quarter + lane, n = at.n0 + group * kColumns, count = min(kColumns, p.outer - n);
+            const int kOut = at.k0 + rank * kHalf + 32 * quarter + lane, n = at.n0 + part * kColumns, count = min(kColumns, p.outer - n);
             OUT *to = nullptr;
             if constexpr (std::is_same_v<OUT, float>) to = p.parts > 1 ? p.partial + static_cast<int64_t>(at.part) * p.outer * p.inner : static_cast<float *>(p.out);
             else to = static_cast<OUT *>(p.out);
             to += static_cast<int64_t>(n) * p.inner + kOut;
-            wait(&accFull, done & 1);
-            ++done;
-            fenceAfter();
-            const uint32_t from = tmem + (static_cast<uint32_t>(32 * quarter) << 16) + group * kColumns;
-#pragma unroll 1
-            for (int col = 0; col < count; col += 16) {
-                uint32_t acc[16];
-                __syncwarp();
-                loadTmem16(from + col, acc);
-                loadsDone();
-                if (!alive || kOut >= p.inner) continue;
+            if constexpr (FINE) {
+                while (segment * kSegment < chunks) takeSegment();
+                if (alive && kOut < p.inner) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j, to += p.inner)
-                    if (col + j < count) *to = fromFloat<OUT>(__uint_as_float(acc[j]));
+                    for (int j = 0; j < kColumns; ++j, to += p.inner)
+                        if (j < count) *to = fromFloat<OUT>(total[j]);
+                }
+            } else {
+                wait(&accFull[0], sums & 1);
+                ++sums;
+                fenceAfter();
+#pragma unroll 1
+                for (int col = 0; col < count; col += 16) {
+                    uint32_t acc[16];
+                    __syncwarp();
+                    loadTmem16(sumsAt + col, acc);
+                    loadsDone();
+                    if (!alive || kOut >= p.inner) continue;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j, to += p.inner)
+                        if (col + j < count) *to = fromFloat<OUT>(__uint_as_float(acc[j]));
+                }
+                fenceBefore();
+                __syncwarp();
+                if (lane == 0) arrivePair(smemAddr(&accFree[0]));
             }
-            fenceBefore();
-            __syncwarp();
-            if (lane == 0) arriveRemote(cluster::remote(smemAddr(&accFree), 0));
         }
     }
     if (!alive && lane == 0) atomicExch(status, 1);
@@ -380,29 +427,32 @@ CUtensorMap mapOf(CUtensorMapDataType type, int rank, const void *data, const cu
     return map;
 }
 
-// How a call is laid out: whether dy is copied, and into how many parts the tokens are cut.
+// How a call is laid out: whether dy is copied, into how many parts the tokens are cut, and whether their sums are in segments.
 struct Plan {
     int terms, pitch, parts, chunks;
-    bool copied;
+    bool copied, fine;
 };
-// The least of these estimates, in microseconds: 0.3 for a product of a chunk, 4 to begin and end a tile, and for several parts 2.5 and the writing and reading of their sums.
-Plan planOf(int64_t tokens, int inner, int outer, int type, const void *dy, int64_t dyPitch) {
+// The least of these estimates, in microseconds: 0.3 for a product of a chunk (0.45 with one product a tile), 4 to begin and end a tile, and for several parts 2.5 and the writing and reading of their sums.
+// Sums go by segments where a part's steps would leave more than a rounding of the output: 32 of floats, 2048 of 16 bits, whose roundings are 2^-12 and more.
+Plan planOf(int64_t tokens, int inner, int outer, int type, const void *dy, int64_t dyPitch, int outType) {
     Plan plan;
     plan.terms = type == RXMET_TYPE_F32 ? 3 : 1;
     plan.copied = plan.terms > 1 || !alignedTo(dy, 16) || (tokens > 1 && (dyPitch % 8 != 0 || dyPitch < outer));
     plan.pitch = static_cast<int>(alignUp(outer, 8));
     plan.chunks = static_cast<int>((tokens + kTokens - 1) / kTokens);
-    const int pairs = std::max(1, currentDevice().sms / 2);
-    const int64_t tiles = static_cast<int64_t>((outer + kOuter - 1) / kOuter) * ((inner + kTile - 1) / kTile);
-    const int products = outer > kTile ? 2 : 1;
+    const int pairs = std::max(1, currentDevice().sms / 2), mostSteps = outType == RXMET_TYPE_F32 ? 32 : 2048;
     double best = 0;
-    plan.parts = 1;
-    for (int q = 1; q <= std::min(plan.chunks, pairs); ++q) {
-        const double rounds = static_cast<double>((tiles * q + pairs - 1) / pairs), chunks = (plan.chunks + q - 1) / q * plan.terms;
-        const double time = rounds * (0.3 * products * chunks + 4.0) + (q > 1 ? 2.5 + 8e-6 / 5 * q * outer * inner : 0.0);
-        if (q == 1 || time < best) {
+    plan.parts = 0;
+    for (int q = 1; q <= std::max(1, std::min(plan.chunks, pairs)); ++q) {
+        const int chunks = (plan.chunks + q - 1) / q;
+        const bool fine = chunks * kSteps > mostSteps;
+        const int64_t tiles = static_cast<int64_t>((outer + outerOf(fine) - 1) / outerOf(fine)) * ((inner + kTile - 1) / kTile);
+        const double rounds = static_cast<double>((tiles * q + pairs - 1) / pairs), chunk = fine ? 0.45 : outer > kTile ? 0.6 : 0.45;
+        const double time = rounds * (chunk * chunks * plan.terms + 4.0) + (q > 1 ? 2.5 + 8e-6 / 5 * q * outer * inner : 0.0);
+        if (plan.parts == 0 || time < best) {
             best = time;
             plan.parts = q;
+            plan.fine = fine;
         }
     }
     return plan;
@@ -426,11 +476,11 @@ void requireSizes(int64_t tokens, int inner, int outer, int type) {
         fail(RXMET_ERR_UNSUPPORTED, "kept_weight_gradient: %lld tokens, inner %d, outer %d, at most %d, 131071 and %d", static_cast<long long>(tokens), inner, outer, 1 << 30, 1 << 30);
 }
 
-template <class T, class OUT>
+template <class T, class OUT, bool FINE>
 void launchProduct(const Problem &p, const CUtensorMap &dy, cudaStream_t st) {
-    const auto kernel = keptWeightGradient<T, OUT>;
+    const auto kernel = keptWeightGradient<T, OUT, FINE>;
     ensureDynamicSmem(reinterpret_cast<const void *>(kernel), kShared);
-    const int64_t items = static_cast<int64_t>((p.outer + kOuter - 1) / kOuter) * ((p.inner + kTile - 1) / kTile) * p.parts;
+    const int64_t items = static_cast<int64_t>((p.outer + outerOf(FINE) - 1) / outerOf(FINE)) * ((p.inner + kTile - 1) / kTile) * p.parts;
     {
         KernelTimer timer__("keptWeightGradient", st);
         launchDependent(kernel, 2 * static_cast<unsigned>(std::min<int64_t>(currentDevice().sms / 2, items)), kThreads, kShared, st, p, dy, waitStatus());
@@ -444,11 +494,11 @@ void launchProduct(const Problem &p, const CUtensorMap &dy, cudaStream_t st) {
 
 using namespace rxmet;
 
-extern "C" size_t rxmet_kept_weight_gradient_workspace_bytes(int64_t tokens, int inner, int outer, int type, const void *dy, int64_t dy_pitch) {
+extern "C" size_t rxmet_kept_weight_gradient_workspace_bytes(int64_t tokens, int inner, int outer, int type, const void *dy, int64_t dy_pitch, int out_type) {
     WorkspaceSizer sizer;
     guarded([&] {
         kept::requireSizes(tokens, inner, outer, type);
-        kept::takeBuffers(sizer, kept::planOf(tokens, inner, outer, type, dy, dy_pitch), tokens, inner, outer, nullptr, nullptr);
+        kept::takeBuffers(sizer, kept::planOf(tokens, inner, outer, type, dy, dy_pitch, out_type), tokens, inner, outer, nullptr, nullptr);
     });
     return sizer.used();
 }
@@ -468,7 +518,7 @@ extern "C" int rxmet_kept_weight_gradient(int64_t tokens, int inner, int outer, 
         RXMET_REQUIRE(alignedTo(codes, 16) && codes_pitch % 16 == 0 && (tokens == 1 || codes_pitch >= inner), "kept_weight_gradient: rows of codes must start on 16 bytes, and apart");
         if (encodeTiled() == nullptr) fail(RXMET_ERR_CUDA, "kept_weight_gradient: the driver encodes no tensor maps");
         bindContext();
-        const kept::Plan plan = kept::planOf(tokens, inner, outer, type, dy, dy_pitch);
+        const kept::Plan plan = kept::planOf(tokens, inner, outer, type, dy, dy_pitch, out_type);
         if (tokens == 1) codes_pitch = 0;   // the distance of a single row's next one does not matter
         kept::Problem p{tokens, inner, outer, plan.terms, plan.parts, plan.chunks, codes, exponents, codes_pitch, out, nullptr};
         uint16_t *laid = nullptr;
@@ -489,9 +539,13 @@ extern "C" int rxmet_kept_weight_gradient(int64_t tokens, int inner, int outer, 
         const CUtensorMap dyMap = kept::mapOf(type == RXMET_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, from, dyDims, dyStrides, dyBox, CU_TENSOR_MAP_SWIZZLE_128B);
         withType(out_type, [&](auto o) {
             using OUT = decltype(o);
+            auto product = [&](auto stored) {
+                using S = decltype(stored);
+                if (type == RXMET_TYPE_F16) plan.fine ? kept::launchProduct<__half, S, true>(p, dyMap, st) : kept::launchProduct<__half, S, false>(p, dyMap, st);
+                else plan.fine ? kept::launchProduct<__nv_bfloat16, S, true>(p, dyMap, st) : kept::launchProduct<__nv_bfloat16, S, false>(p, dyMap, st);
+            };
             if (p.parts > 1) {
-                if (type == RXMET_TYPE_F16) kept::launchProduct<__half, float>(p, dyMap, st);
-                else kept::launchProduct<__nv_bfloat16, float>(p, dyMap, st);
+                product(float{});
                 const bool wide = total % 4 == 0 && alignedTo(out, 4 * sizeof(OUT));
                 const int64_t blocks = (total / (wide ? 4 : 1) + 255) / 256;
                 {
@@ -500,10 +554,8 @@ extern "C" int rxmet_kept_weight_gradient(int64_t tokens, int inner, int outer, 
                                     static_cast<const float *>(p.partial), p.parts, total, static_cast<OUT *>(out));
                 }
                 afterLaunch("sumParts");
-            } else if (type == RXMET_TYPE_F16) {
-                kept::launchProduct<__half, OUT>(p, dyMap, st);
             } else {
-                kept::launchProduct<__nv_bfloat16, OUT>(p, dyMap, st);
+                product(OUT{});
             }
         });
     });

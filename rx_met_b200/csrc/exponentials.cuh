@@ -48,15 +48,19 @@ __device__ __forceinline__ Pair exponentials(Pair x) {
     const Pair e = pairOf(c, d);
     return fma2(e, left, e);
 }
-// sigmoid(x), and 1 - sigmoid(x) without the bits that a subtraction from one would lose, from exp(-x).
+// sigmoid(x), and 1 - sigmoid(x) without the bits that a subtraction from one would lose, from exp(-x).  The reciprocal is off by up to a unit, and to one side: over the hundreds of gates of a long memory
+// that adds up (gradient of a state 3000 tokens away: 8.7e-7), so that gates are REFINED by a step of Newton's (3.5e-7).
+template <bool REFINED>
 struct Sigmoids {
     Pair open, shut;
     __device__ __forceinline__ explicit Sigmoids(Pair e) {
-        const float2 sum = floatsOf(add2(e, bothOf(1.f)));
+        const Pair sum = add2(e, bothOf(1.f));
+        const float2 s = floatsOf(sum);
         float a, b;
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(sum.x));   // one unit in the last place
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(sum.y));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(s.x));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(s.y));
         open = pairOf(a, b);
+        if (REFINED) open = fma2(open, fma2(mul2(sum, bothOf(-1.f)), open, bothOf(1.f)), open);
         shut = mul2(e, open);
     }
 };

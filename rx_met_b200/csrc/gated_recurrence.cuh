@@ -79,9 +79,9 @@ __device__ __forceinline__ Pair clampRow(const uint8_t *row) {
 }
 // Both gates of two channels, from exp(-x) or from a row.
 template <class T>
-struct Gates : Sigmoids {
-    using Sigmoids::Sigmoids;
-    __device__ __forceinline__ explicit Gates(const uint8_t *row) : Sigmoids(exponentials<kSignificant<T>>(clampRow<T>(row))) {}
+struct Gates : Sigmoids<true> {
+    using Sigmoids<true>::Sigmoids;
+    __device__ __forceinline__ explicit Gates(const uint8_t *row) : Sigmoids<true>(exponentials<kSignificant<T>>(clampRow<T>(row))) {}
 };
 __device__ __forceinline__ Pair tanhOf(Pair x) {
     const float2 v = floatsOf(x);

@@ -213,7 +213,7 @@ __device__ __forceinline__ void activate(const Pair (&x)[kPairs], Pair (&y)[kPai
             auto step = [](float f) { return f > 0.f ? 1.f : f <= 0.f ? 0.f : f; };
             if (SLOPES) slope[i] = pairOf(step(v.x), step(v.y));
         } else if constexpr (ACTIVATION == RXMET_ACTIVATION_SILU) {
-            const Sigmoids s(exponentials<BITS>(clampPair(x[i])));
+            const Sigmoids<false> s(exponentials<BITS>(clampPair(x[i])));
             y[i] = mul2(x[i], s.open);
             if (SLOPES) slope[i] = fma2(y[i], s.shut, s.open);
         } else if constexpr (ACTIVATION == RXMET_ACTIVATION_GELU) {

@@ -3,7 +3,7 @@
  * counterpart in the reference.
  *
  * Conventions as in rxmet_b200_mixer.h: device pointers, a stream, a caller's workspace where one is named, status < 0 and rxmet_last_error() on
- * failure.  Every call only enqueues work; none allocates device memory.  No output may overlap an input unless it is said to. */
+ * failure.  Workspaces start on 16 bytes.  Every call only enqueues work; none allocates device memory.  No output may overlap an input unless it is said to. */
 #ifndef RXMET_B200_GATED_H_
 #define RXMET_B200_GATED_H_
 

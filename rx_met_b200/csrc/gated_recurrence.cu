@@ -180,7 +180,7 @@ Pass passOf(const rxmet_gated_recurrence &problem) {
     const int tokens = tokensOf(problem.type, problem.input.data != nullptr);
     p.chunks = std::max(1, (problem.tokens + tokens - 1) / tokens);
     p.groups = (p.chunks + kGroup - 1) / kGroup;
-    p.slabsOfRow = (problem.width + kChannels - 1) / kChannels;
+    p.slabsOfRow = (problem.width - 1) / kChannels + 1;
     const int64_t slabs = static_cast<int64_t>(p.batch) * p.slabsOfRow;
     if (slabs * p.chunks > INT32_MAX) fail(RXMET_ERR_UNSUPPORTED, "gated_recurrence: %lld runs of %d tokens of %d channels, at most %d", static_cast<long long>(slabs * p.chunks), tokens, kChannels, INT32_MAX);
     p.tiles = slabs * p.chunks;
@@ -201,6 +201,7 @@ void startChain(Pass &p, void *workspace, size_t bytes, cudaStream_t st) {
     p.chain.status = waitStatus();
     const int64_t units = chainUnits(p);
     if (units == 0) return;
+    RXMET_REQUIRE(alignedTo(workspace, 16), "gated_recurrence: the workspace must start on 16 bytes");
     uint4 *at = Workspace(workspace, bytes).take<uint4>(units);
     p.chain.ticket = reinterpret_cast<unsigned *>(at);
     p.chain.parts = reinterpret_cast<unsigned long long *>(at + 1);
@@ -239,7 +240,7 @@ void launchForward(Pass &p, int type, cudaStream_t st) {
 
 namespace {
 void launchStep(const Pass &p, int type, cudaStream_t st) {
-    const int pairs = (p.width + 1) / 2;
+    const int pairs = (p.width - 1) / 2 + 1;
     const int64_t blocks = (static_cast<int64_t>(p.batch) * pairs + kThreads - 1) / kThreads;
     withType(type, [&](auto t) {
         using T = decltype(t);

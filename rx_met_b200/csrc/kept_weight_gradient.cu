@@ -521,6 +521,7 @@ extern "C" int rxmet_kept_weight_gradient(int64_t tokens, int inner, int outer, 
         const kept::Plan plan = kept::planOf(tokens, inner, outer, type, dy, dy_pitch, out_type);
         if (tokens == 1) codes_pitch = 0;   // the distance of a single row's next one does not matter
         kept::Problem p{tokens, inner, outer, plan.terms, plan.parts, plan.chunks, codes, exponents, codes_pitch, out, nullptr};
+        RXMET_REQUIRE(alignedTo(workspace, 16), "kept_weight_gradient: the workspace must start on 16 bytes");
         uint16_t *laid = nullptr;
         kept::takeBuffers(Workspace(workspace, workspace_bytes), plan, tokens, inner, outer, &laid, &p.partial);
         if (plan.copied) {

@@ -72,7 +72,8 @@ class _Linear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         weight, codes, exponents = ctx.saved_tensors
-        dx = None if weight is None else dy @ weight
+        with torch.autocast("cuda", enabled=False):
+            dx = None if weight is None else dy @ weight
         dweight = None if codes is None else weight_gradient(dy, KeptCodes(codes, exponents, ctx.dtype))
         return dx, dweight, dy.flatten(0, -2).sum(dim=0) if ctx.biased else None
 

@@ -156,6 +156,38 @@ def test_block_in_a_graph():
         assert torch.equal(y, c.step(token, other)) and torch.equal(state, other)
 
 
+FIRST_CALLS = """
+import torch
+from rx_met_b200 import gated_recurrence, kept_codes
+x = torch.randn(2, 700, 256, device="cuda", dtype=torch.bfloat16)
+state, weight = torch.zeros(2, 256, device="cuda"), torch.randn(300, 700, device="cuda", dtype=torch.bfloat16)
+dy = torch.randn(1400, 96, device="cuda", dtype=torch.bfloat16)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out, last = gated_recurrence.gated_recurrence(x, x)
+    step = gated_recurrence.gated_recurrence_step(x[:, 0], x[:, 0], state)
+    kept = kept_codes.keep(x)
+    y = kept_codes.gated_product(kept_codes.values(kept), out)
+    dw = kept_codes.weight_gradient(dy.view(2, 700, 96), kept)
+graph.replay()
+held = [t.clone() for t in (out, last, step, y, dw)]
+want, wanted = gated_recurrence.gated_recurrence(x, x)
+kept = kept_codes.keep(x)
+assert torch.equal(held[0], want) and torch.equal(held[1], wanted) and torch.equal(held[4], kept_codes.weight_gradient(dy.view(2, 700, 96), kept))
+assert torch.equal(held[3], kept_codes.gated_product(kept_codes.values(kept), want)) and torch.equal(held[2], want[:, 0])
+print("first calls captured")
+"""
+
+
+def test_first_calls_of_a_process_in_a_graph():
+    import pathlib
+    import subprocess
+    import sys
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS], capture_output=True, text=True, timeout=300, cwd=pathlib.Path(__file__).resolve().parent.parent)
+    assert done.returncode == 0 and "first calls captured" in done.stdout, done.stderr[-2000:]
+
+
 def test_what_a_block_keeps():
     """Between the passes: codes of the inputs of four products and of four factors, the norms' inputs, and the gates and values of the recurrence."""
     b = block(torch.bfloat16, seed=5)

@@ -175,6 +175,42 @@ def test_strides_alignment_and_reproducibility():
     assert all(torch.equal(a, b) for g in grads[1:] for a, b in zip(g, grads[0]))
 
 
+@pytest.mark.parametrize("own,dtype", [(False, torch.bfloat16), (False, torch.float32), (True, torch.float16), (True, torch.float32)])
+def test_more_tiles_than_run_at_once(own, dtype):
+    """Thousands of tiles, of which every CTA takes several, in sequences of many groups; three times over."""
+    from rx_met_b200.gated_recurrence import gated_recurrence
+    batch, tokens, width = 8, 3000, 1024
+    forget, value, input = (None if t is None else t.detach().requires_grad_() for t in tensors(batch, tokens, width, dtype, own, seed=11))
+    dout = torch.randn(batch, tokens, width, device="cuda").to(dtype)
+    leaves = [t for t in (forget, value, input) if t is not None]
+    results = []
+    for _ in range(3):
+        out, last = gated_recurrence(forget, value, input=input)
+        results.append([out.detach(), last.detach(), *torch.autograd.grad(out, leaves, dout)])
+    assert all(torch.equal(a, b) for r in results[1:] for a, b in zip(r, results[0]))
+    plain = [None if t is None else t.detach() for t in (forget, value, input)]
+    check_forward(dtype, results[0][:2], gl.recur(*plain))
+    wants = [w for w in gl.recur_gradients(*plain, "none", None, None, dout, None)[:3] if w is not None]
+    for grad, (want, bound) in zip(results[0][2:], wants):
+        ml.within(grad, want, 1.01 * bound + want.abs() * ml.UNIT[dtype] + ml.TINY[dtype] + underflow(tokens))
+
+
+def test_calls_side_by_side():
+    """Two streams at once, each with a chain of tiles of its own."""
+    from rx_met_b200.gated_recurrence import gated_recurrence
+    inputs = [tensors(4, 2000, 512, torch.bfloat16, seed=s)[:2] for s in (12, 13)]
+    wants = [gated_recurrence(*t) for t in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in inputs]
+    for _ in range(5):
+        got = []
+        for stream, t in zip(streams, inputs):
+            with torch.cuda.stream(stream):
+                got.append(gated_recurrence(*t))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, wants) for a, b in zip(g, w))
+
+
 def test_empty_ones():
     from rx_met_b200.gated_recurrence import gated_recurrence, gated_recurrence_step
     state = torch.randn(3, 20, device="cuda")

@@ -18,6 +18,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
     __shared__ Tile tiles[kPlaces];
     __shared__ Pair front[32];
     __shared__ __align__(8) uint64_t full[kStages];
+    __shared__ uint32_t extra[kStages][Rows<T, OWN, COPY>::kExtra];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0 && COPY == Copy::Boxes) {
         for (int i = 0; i < kStages; ++i) cluster::initBarrier(&full[i], 1);
@@ -32,7 +33,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
             tickets.ask();
         }
     __syncthreads();
-    auto rows = [&](int stage) { return Rows<T, OWN, COPY>{umma::smemAddr(stages) + stage * kStageBytes, &full[stage]}; };
+    auto rows = [&](int stage) { return Rows<T, OWN, COPY>{umma::smemAddr(stages) + stage * kStageBytes, &full[stage], extra[stage]}; };
     constexpr unsigned kUsed = OWN ? 7 : 3;
     for (int i = 0; i < kStages; ++i) rows(i).ask(p, tiles[i], kUsed);
 
@@ -48,6 +49,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
         if (!rows(stage).arrived(tile, parities >> stage & 1)) gaveUp(p.chain);
         if (tile.live > 0) parities ^= 1u << stage;
         if (COPY != Copy::Boxes) __syncthreads();
+        rows(stage).shift(p, tile, kUsed);
 
         const uint8_t *from = stages + stage * kStageBytes + warp * S * kRow + lane * 2 * sizeof(T);
         Pair a[S], b[S];

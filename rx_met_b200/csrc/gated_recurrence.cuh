@@ -127,28 +127,64 @@ __device__ __forceinline__ void gaveUp(const Chain &c) {
     if ((threadIdx.x & 31) == 0) atomicExch(c.status, 1);   // the results are not to be used
 }
 // The rows of a stage, up to four tensors of a tile: a row of shared memory holds the tile's channels of one token.  TMA copies them as boxes, one instruction a tensor (its threads' own copies
-// took 1200 of 9500 cycles a tile), where rows start on 16 bytes; else threads do, in pieces of four bytes or of one element.
-enum class Copy { Boxes, Words, Elements };
+// took 1200 of 9500 cycles a tile), where rows start on 16 bytes; else threads do, in words of four bytes.  Rows of 16-bit elements may start in the middle of a word: the words around them are copied, and
+// shifted in place once they are there (8 x 2048 tokens of 2047 channels: 437 us element by element).
+enum class Copy { Boxes, Words, Halves };
 template <class T, bool OWN, Copy COPY>
 struct Rows {
+    static constexpr int kExtra = COPY == Copy::Halves ? 4 * kTokens<T, OWN> : 1;
     uint32_t to;
     uint64_t *bar;
+    uint32_t *extra;   // [kExtra]: of Halves, the word behind a row
     // Of the tensors forget, value, input and dout; without an input gate dout moves up.
     static __device__ __forceinline__ int slot(int tensor) { return tensor == 3 && !OWN ? 2 : tensor; }
+    // Whether a row of a tensor starts in the middle of a word.
+    static __device__ __forceinline__ bool halfway(const rxmet_token_tensor &t, const Tile &tile, int row) {
+        return ((reinterpret_cast<uintptr_t>(t.data) >> 1) + static_cast<uintptr_t>(tile.b * t.stride_b + row * t.stride_t)) & 1;   // tiles start at even channels and tokens
+    }
     // Copies by threads: the live tokens of one tensor.
     __device__ __forceinline__ void copy(int place, const rxmet_token_tensor &t, const Tile &tile, int width) const {
-        constexpr int kPer = COPY == Copy::Words ? 4 / static_cast<int>(sizeof(T)) : 1, kPieces = kChannels / kPer, kRow = kChannels * sizeof(T), kRows = kThreads / kPieces;
-        const int r0 = threadIdx.x / kPieces, piece = threadIdx.x % kPieces;
-        const int real = min(kPer, width - tile.d0 - piece * kPer);
-        if (real <= 0) return;
-        const T *from = static_cast<const T *>(t.data) + tile.b * t.stride_b + (static_cast<int64_t>(tile.first) + r0) * t.stride_t + tile.d0 + piece * kPer;
-        const int64_t step = kRows * t.stride_t;
-        uint32_t at = to + place * kTensorBytes<OWN> + r0 * kRow + piece * kPer * static_cast<int>(sizeof(T));
-        for (int r = r0; r < tile.live; r += kRows, from += step, at += kRows * kRow) {
-            if constexpr (COPY == Copy::Words) copyWord(at, from, real * static_cast<int>(sizeof(T)));
-            else {
-                const uint16_t v = *reinterpret_cast<const uint16_t *>(from);   // no asynchronous copy takes two bytes
-                asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(v) : "memory");
+        constexpr int kPer = 4 / static_cast<int>(sizeof(T)), kPieces = kChannels / kPer, kRow = kChannels * sizeof(T), kRows = kThreads / kPieces;
+        const int r0 = threadIdx.x / kPieces, piece = threadIdx.x % kPieces, real = width - tile.d0;
+        const T *from = static_cast<const T *>(t.data) + tile.b * t.stride_b + static_cast<int64_t>(tile.first) * t.stride_t + tile.d0;
+        uint32_t at = to + place * kTensorBytes<OWN> + r0 * kRow + piece * 4;
+        if constexpr (COPY == Copy::Words) {
+            const int bytes = min(4, (real - piece * kPer) * static_cast<int>(sizeof(T)));
+            if (bytes <= 0) return;
+            const int64_t step = kRows * t.stride_t;
+            from += r0 * t.stride_t + piece * kPer;
+            for (int r = r0; r < tile.live; r += kRows, from += step, at += kRows * kRow) copyWord(at, from, bytes);
+        } else {
+            // words that hold an element of the row, and nothing beyond the word
+            auto word = [&](int r, int w, uint32_t to) {
+                const T *row = from + r * t.stride_t;
+                const bool half = halfway(t, tile, r);
+                if (2 * w - half < real && (w < kPieces || half)) copyWord(to, row - half + 2 * w, 4);
+            };
+            for (int r = r0; r < tile.live; r += kRows, at += kRows * kRow) word(r, piece, at);
+            for (int r = threadIdx.x; r < tile.live; r += kThreads) word(r, kPieces, umma::smemAddr(extra + place * kTokens<T, OWN> + r));
+        }
+    }
+    // The rows of a warp, once they have arrived, from the start of a word on.
+    __device__ __forceinline__ void shift(const Pass &p, const Tile &tile, unsigned used) const {
+        if constexpr (COPY == Copy::Halves) {
+            constexpr int S = kSteps<T, OWN>;
+            const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+            const rxmet_token_tensor *tensors[4] = {&p.forget, &p.value, &p.input, &p.dout};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (!(used >> i & 1)) continue;
+#pragma unroll 4
+                for (int s = 0; s < S; ++s) {
+                    const int r = warp * S + s;
+                    if (r >= tile.live || !halfway(*tensors[i], tile, r)) continue;
+                    const uint32_t at = to + slot(i) * kTensorBytes<OWN> + (r * 32 + lane) * 4;
+                    uint32_t word, next;
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(word) : "r"(at) : "memory");
+                    next = __shfl_down_sync(0xffffffffu, word, 1);
+                    if (lane == 31) next = extra[slot(i) * kTokens<T, OWN> + r];
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(__byte_perm(word, next, 0x5432)) : "memory");
+                }
             }
         }
     }
@@ -372,7 +408,7 @@ inline Copy copyOf(const rxmet_token_tensor &t, int batch, int tokens, size_t si
         return alignedTo(t.data, bytes) && (batch == 1 || t.stride_b * static_cast<int64_t>(size) % bytes == 0) && (tokens == 1 || t.stride_t * static_cast<int64_t>(size) % bytes == 0);
     };
     const bool apart = (batch == 1 || t.stride_b > 0) && (tokens == 1 || t.stride_t > 0);   // a box has no strides of zero
-    return apart && fits(16) && encodeTiled() ? Copy::Boxes : fits(4) ? Copy::Words : Copy::Elements;
+    return apart && fits(16) && encodeTiled() ? Copy::Boxes : fits(4) ? Copy::Words : Copy::Halves;
 }
 inline CUtensorMap boxesOf(const rxmet_token_tensor &t, const Pass &p, int type, int boxTokens) {
     CUtensorMap map;
@@ -414,7 +450,7 @@ void withCopy(Pass &p, int type, bool own, F f) {
     }
     if (copy == Copy::Boxes) f(std::integral_constant<Copy, Copy::Boxes>{});
     else if (copy == Copy::Words || sizeof(T) == 4) f(std::integral_constant<Copy, Copy::Words>{});
-    else f(std::integral_constant<Copy, sizeof(T) == 4 ? Copy::Words : Copy::Elements>{});
+    else f(std::integral_constant<Copy, sizeof(T) == 4 ? Copy::Words : Copy::Halves>{});
 }
 
 // Launches of gated_recurrence.cu and gated_recurrence_backward.cu.

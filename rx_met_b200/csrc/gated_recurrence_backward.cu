@@ -23,6 +23,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
     __shared__ Pair front[32];
     __shared__ __align__(16) float starts[kStages][kChannels];
     __shared__ __align__(8) uint64_t full[kStages];
+    __shared__ uint32_t extra[kStages][Rows<T, OWN, COPY>::kExtra];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0 && COPY == Copy::Boxes) {
         for (int i = 0; i < kStages; ++i) cluster::initBarrier(&full[i], 1);
@@ -37,7 +38,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
             tickets.ask();
         }
     __syncthreads();
-    auto rows = [&](int stage) { return Rows<T, OWN, COPY>{umma::smemAddr(stages) + stage * kStageBytes, &full[stage]}; };
+    auto rows = [&](int stage) { return Rows<T, OWN, COPY>{umma::smemAddr(stages) + stage * kStageBytes, &full[stage], extra[stage]}; };
     constexpr int kDout = OWN ? 3 : 2;   // its place in a stage
     const unsigned used = 3u | (OWN ? 4u : 0u) | (p.dout.data ? 8u : 0u);
     if (!p.dout.data)   // zeros, which nothing writes over
@@ -67,6 +68,7 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
         if (tile.live > 0) parities ^= 1u << stage;
         if (COPY == Copy::Boxes) copiesArrived<0>();
         __syncthreads();
+        rows(stage).shift(p, tile, used);
         askState(stage ^ 1, next);
         if (tid == 0) storesRead();
         rows(stage ^ 1).ask(p, next, used);   // what it held was read in front of the barrier, or left by a store

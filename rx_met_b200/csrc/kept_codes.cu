@@ -122,14 +122,21 @@ __device__ __forceinline__ Raw<T> loadEight(const Rows &rows, const Spot &at, in
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4 *>(r.w)[i] = reinterpret_cast<const uint4 *>(from)[i];
     }
-    if (!WIDE) {
-        T one[kPer];
+    if constexpr (!WIDE && sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) one[i] = i < count ? from[i] : fromFloat<T>(0.f);
+        for (int i = 0; i < kPer; ++i) r.w[i] = i < count ? __float_as_uint(from[i]) : 0u;
+    }
+    if constexpr (!WIDE && sizeof(T) == 2) {
+        // words that hold an element; a row may start in the middle of one
+        const int half = (reinterpret_cast<uintptr_t>(from) >> 1) & 1;
+        const uint32_t *words = reinterpret_cast<const uint32_t *>(from - half);
+        uint32_t w[kPairs + 1];
 #pragma unroll
-        for (int i = 0; i < kPer * static_cast<int>(sizeof(T)) / 4; ++i) {
-            if constexpr (sizeof(T) == 4) r.w[i] = __float_as_uint(one[i]);
-            else r.w[i] = static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(one)[2 * i]) | static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(one)[2 * i + 1]) << 16;
+        for (int i = 0; i <= kPairs; ++i) w[i] = count > 0 && 2 * i < half + count ? words[i] : 0u;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            const uint32_t two = half ? __byte_perm(w[i], w[i + 1], 0x5432) : w[i];
+            r.w[i] = 2 * i + 1 < count ? two : 2 * i < count ? two & 0xffffu : 0u;
         }
     }
     return r;
@@ -152,10 +159,31 @@ __device__ __forceinline__ void storeEight(const Rows &rows, const Spot &at, int
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4 *>(to)[i] = reinterpret_cast<const uint4 *>(r.w)[i];
     }
-    if (!WIDE) {
+    if constexpr (!WIDE && sizeof(T) == 4) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-            if (i < count) to[i] = fromFloat<T>(i & 1 ? floatsOf(v[i / 2]).y : floatsOf(v[i / 2]).x);
+            if (i < count) to[i] = i & 1 ? floatsOf(v[i / 2]).y : floatsOf(v[i / 2]).x;
+    }
+    if constexpr (!WIDE && sizeof(T) == 2) {
+        uint32_t w[kPairs];
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) w[i] = pack2<T>(v[i]);
+        auto one = [&](int i) { reinterpret_cast<uint16_t *>(to)[i] = static_cast<uint16_t>(i & 1 ? w[i / 2] >> 16 : w[i / 2]); };
+        if (reinterpret_cast<uintptr_t>(to) & 2) {   // an element, three words, an element
+            if (count > 0) one(0);
+#pragma unroll
+            for (int i = 1; i < kPer - 1; i += 2) {
+                if (i + 1 < count) *reinterpret_cast<uint32_t *>(to + i) = __byte_perm(w[i / 2], w[i / 2 + 1], 0x5432);
+                else if (i < count) one(i);
+            }
+            if (count == kPer) one(kPer - 1);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; i += 2) {
+                if (i + 1 < count) *reinterpret_cast<uint32_t *>(to + i) = w[i / 2];
+                else if (i < count) one(i);
+            }
+        }
     }
 }
 

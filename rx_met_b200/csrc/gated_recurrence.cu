@@ -100,15 +100,15 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
         }
         if (warp == 0 && p.marks && tile.chunk > 0) writeFloats(p.marks + tile.mark + 2 * lane, h, real);
         h = ahead(h);
-        if (p.outBoxes) {
-            uint8_t *to = outputs + warp * S * kRow + lane * 2 * sizeof(T);
+        uint8_t *rowsOut = outputs + warp * S * kRow;
 #pragma unroll
-            for (int s = 0; s < S; ++s) {
-                h = fma2(a[s], h, b[s]);
-                keepRow<T>(to + s * kRow, h);
-            }
-            if (live < S)
-                for (int s = max(live, 0); s < S; ++s) keepRow<T>(to + s * kRow, bothOf(0.f));
+        for (int s = 0; s < S; ++s) {
+            h = fma2(a[s], h, b[s]);
+            keepRow<T>(rowsOut + s * kRow + lane * 2 * sizeof(T), h);
+        }
+        if (live < S)
+            for (int s = max(live, 0); s < S; ++s) keepRow<T>(rowsOut + s * kRow + lane * 2 * sizeof(T), bothOf(0.f));
+        if (p.outBoxes) {
             ummatiles::fenceAsyncProxy();
             __syncthreads();
             if (tid == 0) {
@@ -116,13 +116,11 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
                 commitStores();
             }
         } else {
-            const int here = min(p.tokens - tile.first - warp * S, S);   // tokens that have an output
-            T *to = static_cast<T *>(p.out) + tile.out + static_cast<int64_t>(warp * S) * p.width + 2 * lane;
-#pragma unroll
-            for (int s = 0; s < S; ++s, to += p.width) {
-                h = fma2(a[s], h, b[s]);
-                if (p.out && s < here) writeRow<T>(to, s < live ? h : bothOf(0.f), real, p.paired);
-            }
+            __syncwarp();
+            const int here = p.out ? min(p.tokens - tile.first - warp * S, S) : 0;   // tokens that have an output
+            T *to = static_cast<T *>(p.out) + tile.out + static_cast<int64_t>(warp * S) * p.width;
+#pragma unroll 4
+            for (int s = 0; s < here; ++s, to += p.width) giveRow<T>(to, rowsOut + s * kRow, p.width - tile.d0);
             __syncthreads();   // `parts` is written again
         }
         if (last && warp == kWarps - 1 && p.finalState) writeFloats(p.finalState + row, h, real);
@@ -291,7 +289,6 @@ extern "C" int rxmet_gated_recurrence_forward(const rxmet_gated_recurrence *prob
         p.out = out;
         p.finalState = final_state;
         p.marks = marks;
-        p.paired = p.width % 2 == 0 && alignedTo(out, 2 * typeBytes(problem->type));
         const auto st = static_cast<cudaStream_t>(stream);
         if (p.tokens == 1) return gated::launchStep(p, problem->type, st);
         gated::startChain(p, workspace, workspace_bytes, st);
@@ -316,8 +313,6 @@ extern "C" int rxmet_gated_recurrence_backward(const rxmet_gated_recurrence *pro
         p.dvalue = dvalue;
         p.dinput = dinput;
         p.dstate = dstate;
-        const size_t two = 2 * typeBytes(problem->type);
-        p.paired = p.width % 2 == 0 && alignedTo(dforget, two) && alignedTo(dvalue, two) && alignedTo(dinput, two);
         const auto st = static_cast<cudaStream_t>(stream);
         gated::startChain(p, workspace, workspace_bytes, st);
         gated::launchBackward(p, problem->type, st);

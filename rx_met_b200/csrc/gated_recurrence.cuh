@@ -52,7 +52,6 @@ __device__ __forceinline__ unsigned long long wholeWord(float h) { return (0xc00
 __device__ __forceinline__ bool isWhole(unsigned long long word) { return (word >> 62) == 3ull; }   // (or A is a NaN, and so is B)
 struct Pass {
     int batch, tokens, width, chunks, groups, slabsOfRow, tanhValue;   // chunks: tiles of a sequence
-    bool paired;   // two neighbours of a 16-bit output can be written at once
     int64_t tiles;
     rxmet_token_tensor forget, value, input, dout;
     CUtensorMap maps[4];   // of these, in this order, where rows can be copied by TMA
@@ -148,21 +147,22 @@ struct Rows {
         const int r0 = threadIdx.x / kPieces, piece = threadIdx.x % kPieces, real = width - tile.d0;
         const T *from = static_cast<const T *>(t.data) + tile.b * t.stride_b + static_cast<int64_t>(tile.first) * t.stride_t + tile.d0;
         uint32_t at = to + place * kTensorBytes<OWN> + r0 * kRow + piece * 4;
+        const int64_t step = kRows * t.stride_t;
         if constexpr (COPY == Copy::Words) {
             const int bytes = min(4, (real - piece * kPer) * static_cast<int>(sizeof(T)));
             if (bytes <= 0) return;
-            const int64_t step = kRows * t.stride_t;
             from += r0 * t.stride_t + piece * kPer;
             for (int r = r0; r < tile.live; r += kRows, from += step, at += kRows * kRow) copyWord(at, from, bytes);
         } else {
-            // words that hold an element of the row, and nothing beyond the word
-            auto word = [&](int r, int w, uint32_t to) {
-                const T *row = from + r * t.stride_t;
-                const bool half = halfway(t, tile, r);
-                if (2 * w - half < real && (w < kPieces || half)) copyWord(to, row - half + 2 * w, 4);
-            };
-            for (int r = r0; r < tile.live; r += kRows, at += kRows * kRow) word(r, piece, at);
-            for (int r = threadIdx.x; r < tile.live; r += kThreads) word(r, kPieces, umma::smemAddr(extra + place * kTokens<T, OWN> + r));
+            // words that hold an element of the row, and nothing beyond the word; a thread's rows are an even number apart
+            const int half = halfway(t, tile, r0);
+            if (2 * piece - half < real) {
+                const T *word = from + r0 * t.stride_t - half + 2 * piece;
+                for (int r = r0; r < tile.live; r += kRows, word += step, at += kRows * kRow) copyWord(at, word, 4);
+            }
+            const int r = threadIdx.x;
+            static_assert(kTokens<T, OWN> <= kThreads);
+            if (r < tile.live && 2 * kPieces - 1 < real && halfway(t, tile, r)) copyWord(umma::smemAddr(extra + place * kTokens<T, OWN> + r), from + r * t.stride_t - 1 + 2 * kPieces, 4);
         }
     }
     // The rows of a warp, once they have arrived, from the start of a word on.
@@ -174,10 +174,11 @@ struct Rows {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (!(used >> i & 1)) continue;
+                const bool even = halfway(*tensors[i], tile, 0), odd = halfway(*tensors[i], tile, 1);   // of rows; a warp starts at an even one
 #pragma unroll 4
                 for (int s = 0; s < S; ++s) {
+                    if (!(s & 1 ? odd : even)) continue;
                     const int r = warp * S + s;
-                    if (r >= tile.live || !halfway(*tensors[i], tile, r)) continue;
                     const uint32_t at = to + slot(i) * kTensorBytes<OWN> + (r * 32 + lane) * 4;
                     uint32_t word, next;
                     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(word) : "r"(at) : "memory");
@@ -239,18 +240,26 @@ __device__ __forceinline__ Pair readRow(const uint8_t *row) {
         return pairOf(two.x, two.y);
     }
 }
-// `real`: of the two channels, those of the row; `paired`: both can be written at once.
+// A row from shared memory to an array whose rows may start anywhere, by one warp: its channels that there are, in words of four bytes.  What a tile shares a word with belongs to another one.
 template <class T>
-__device__ __forceinline__ void writeRow(T *to, Pair v, int real, bool paired) {
-    const float2 two = floatsOf(v);
-    if (paired) {
-        if (real > 0) {
-            if constexpr (sizeof(T) == 4) *reinterpret_cast<Pair *>(to) = v;
-            else *reinterpret_cast<uint32_t *>(to) = pack2<T>(v);
-        }
+__device__ __forceinline__ void giveRow(T *to, const uint8_t *row, int real) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (sizeof(T) == 4) {
+        const float *from = reinterpret_cast<const float *>(row);
+        if (lane < real) to[lane] = from[lane];
+        if (lane + 32 < real) to[lane + 32] = from[lane + 32];
     } else {
-        if (real > 0) to[0] = fromFloat<T>(two.x);
-        if (real > 1) to[1] = fromFloat<T>(two.y);
+        const uint32_t word = reinterpret_cast<const uint32_t *>(row)[lane], before = __shfl_up_sync(0xffffffffu, word, 1);
+        uint16_t *at = reinterpret_cast<uint16_t *>(to) + 2 * lane;
+        if ((reinterpret_cast<uintptr_t>(to) & 2) == 0) {
+            if (2 * lane + 1 < real) *reinterpret_cast<uint32_t *>(at) = word;
+            else if (2 * lane < real) *at = static_cast<uint16_t>(word);
+        } else {
+            if (lane == 0) *at = static_cast<uint16_t>(word);
+            else if (2 * lane < real) *reinterpret_cast<uint32_t *>(at - 1) = __byte_perm(before, word, 0x5432);
+            else if (2 * lane - 1 < real) at[-1] = static_cast<uint16_t>(before >> 16);
+            if (lane == 31 && real > 63) at[1] = static_cast<uint16_t>(word >> 16);
+        }
     }
 }
 __device__ __forceinline__ Pair readFloats(const float *from, int real) { return pairOf(from && real > 0 ? from[0] : 0.f, from && real > 1 ? from[1] : 0.f); }

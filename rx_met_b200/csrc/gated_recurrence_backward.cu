@@ -140,10 +140,8 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
             before[s] = h;
             h = next;   // behind the sequence's end nobody reads it
         }
-        const int here = min(p.tokens - tile.first - warp * S, S);
-        const int64_t to = tile.out + static_cast<int64_t>(warp * S) * p.width + 2 * lane;
         const Pair minus = bothOf(-1.f);
-        // gradients of a token take the place of what they come from, if a box of them can be stored
+        // gradients of a token take the place of what they come from
         auto giveTokens = [&](auto all) {
 #pragma unroll
             for (int s = S - 1; s >= 0; --s) {
@@ -164,20 +162,13 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
                     dvalue = mul2(G, z);
                     if (TANH) dvalue = mul2(dvalue, fma2(mul2(c, minus), c, bothOf(1.f)));
                 }
-                if (decltype(all)::value || p.outBoxes) {
-                    uint8_t *row = from + s * kRow;
-                    keepRow<T>(row, dforget);
-                    keepRow<T>(row + kTensorBytes<OWN>, dvalue);
-                    if (OWN) keepRow<T>(row + 2 * kTensorBytes<OWN>, dinput);
-                } else if (s < here) {
-                    const int64_t at = to + static_cast<int64_t>(s) * p.width;
-                    if (p.dforget) writeRow<T>(static_cast<T *>(p.dforget) + at, dforget, real, p.paired);
-                    if (p.dvalue) writeRow<T>(static_cast<T *>(p.dvalue) + at, dvalue, real, p.paired);
-                    if (OWN && p.dinput) writeRow<T>(static_cast<T *>(p.dinput) + at, dinput, real, p.paired);
-                }
+                uint8_t *row = from + s * kRow;
+                keepRow<T>(row, dforget);
+                keepRow<T>(row + kTensorBytes<OWN>, dvalue);
+                if (OWN) keepRow<T>(row + 2 * kTensorBytes<OWN>, dinput);
             }
         };
-        if (live >= S && p.outBoxes) giveTokens(std::true_type{});
+        if (live >= S) giveTokens(std::true_type{});
         else giveTokens(std::false_type{});
         if (p.outBoxes) {
             ummatiles::fenceAsyncProxy();
@@ -188,6 +179,18 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __g
                 if (p.dvalue) storeBox(&p.outMaps[1], at + kTensorBytes<OWN>, tile);
                 if (OWN && p.dinput) storeBox(&p.outMaps[2], at + 2 * kTensorBytes<OWN>, tile);
                 commitStores();
+            }
+        } else {
+            __syncwarp();
+            const int here = min(p.tokens - tile.first - warp * S, S);   // tokens that have gradients
+            const uint8_t *rowsOut = from - lane * 2 * sizeof(T);
+            int64_t to = tile.out + static_cast<int64_t>(warp * S) * p.width;
+            const int channels = p.width - tile.d0;
+#pragma unroll 2
+            for (int s = 0; s < here; ++s, to += p.width, rowsOut += kRow) {
+                if (p.dforget) giveRow<T>(static_cast<T *>(p.dforget) + to, rowsOut, channels);
+                if (p.dvalue) giveRow<T>(static_cast<T *>(p.dvalue) + to, rowsOut + kTensorBytes<OWN>, channels);
+                if (OWN && p.dinput) giveRow<T>(static_cast<T *>(p.dinput) + to, rowsOut + 2 * kTensorBytes<OWN>, channels);
             }
         }
         if (last && warp == 0 && p.dstate) writeFloats(p.dstate + row, R, real);

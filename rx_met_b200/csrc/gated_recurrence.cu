@@ -1,4 +1,4 @@
-// Gated linear recurrence: entry points, the forward pass over sequences, and single tokens.
+// Gated linear recurrence: entry points, the forward pass over sequences, and few tokens.
 //
 // Forward: a tile's gates are worked out once and stay in registers, (f, z c) of sixteen tokens a thread; the state in front of the tile comes from the chain, and a second walk over the
 // registers gives the outputs.  So every input is read once and every output written once, whatever the length.
@@ -128,38 +128,54 @@ __global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedForward(const __gr
     if (tid == 0) storesRead();
 }
 
-// Single tokens: a thread for two neighbouring channels of a row.
+// Few tokens: a thread takes two neighbouring channels of a row from token to token, four of which it asks for at once.
 template <class T, bool OWN>
-__global__ void __launch_bounds__(kThreads) gatedStep(const __grid_constant__ Pass p, const int pairsOfRow) {
+__global__ void __launch_bounds__(kThreads) gatedWalk(const __grid_constant__ Pass p, const int pairsOfRow) {
+    constexpr int kAtOnce = 4;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
     const int b = static_cast<int>(i / pairsOfRow), d = 2 * static_cast<int>(i - static_cast<int64_t>(b) * pairsOfRow);
     waitForPredecessor();
     letDependentsStart();
     if (b >= p.batch) return;
-    const bool live = !p.lengths || p.lengths[b] > 0;
-    auto at = [&](const rxmet_token_tensor &t, int v) { return static_cast<const T *>(t.data)[b * t.stride_b + d + v]; };
+    const int live = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
     const int64_t row = static_cast<int64_t>(b) * p.width + d;
     const int count = min(2, p.width - d);
-    alignas(8) T forget[2], input[2];
-    float value[2], h[2];
+    const int second = count - 1;   // of a row's last channel by itself, the same one twice
+    float h[2];
+    for (int v = 0; v < 2; ++v) h[v] = p.state ? p.state[row + v * second] : 0.f;
+    auto ask = [&](const rxmet_token_tensor &t, int token, T (&to)[2]) {
+        const T *from = static_cast<const T *>(t.data) + b * t.stride_b + token * t.stride_t + d;
+        to[0] = from[0];
+        to[1] = from[second];
+    };
+    T *to = static_cast<T *>(p.out) + static_cast<int64_t>(b) * p.tokens * p.width + d;
+    for (int first = 0; first < p.tokens; first += kAtOnce) {
+        alignas(8) T forget[kAtOnce][2], value[kAtOnce][2], input[kAtOnce][2];
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-        const int u = min(v, count - 1);
-        forget[v] = at(p.forget, u);
-        value[v] = toFloat(at(p.value, u));
-        if (OWN) input[v] = at(p.input, u);
-        h[v] = p.state ? p.state[row + u] : 0.f;
-    }
-    const Gates<T> forgets(reinterpret_cast<const uint8_t *>(forget));
-    const float2 f = floatsOf(forgets.open), z = floatsOf(OWN ? Gates<T>(reinterpret_cast<const uint8_t *>(input)).open : forgets.shut);
+        for (int s = 0; s < kAtOnce; ++s) {
+            if (first + s >= live) continue;
+            ask(p.forget, first + s, forget[s]);
+            ask(p.value, first + s, value[s]);
+            if (OWN) ask(p.input, first + s, input[s]);
+        }
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-        if (v >= count) continue;
-        const float c = p.tanhValue ? tanhf(value[v]) : value[v];
-        const float next = live ? fmaf(v ? f.y : f.x, h[v], (v ? z.y : z.x) * c) : h[v];
-        if (p.finalState) p.finalState[row + v] = next;
-        if (p.out) static_cast<T *>(p.out)[row + v] = fromFloat<T>(live ? next : 0.f);
+        for (int s = 0; s < kAtOnce; ++s) {
+            if (first + s >= p.tokens) break;
+            if (first + s < live) {
+                const Gates<T> forgets(reinterpret_cast<const uint8_t *>(forget[s]));
+                const float2 f = floatsOf(forgets.open), z = floatsOf(OWN ? Gates<T>(reinterpret_cast<const uint8_t *>(input[s])).open : forgets.shut);
+                float c[2] = {toFloat(value[s][0]), toFloat(value[s][1])};
+                if (p.tanhValue)
+                    for (int v = 0; v < 2; ++v) c[v] = tanhf(c[v]);
+                h[0] = fmaf(f.x, h[0], z.x * c[0]);
+                h[1] = fmaf(f.y, h[1], z.y * c[1]);
+            }
+            if (p.out)
+                for (int v = 0; v < count; ++v) to[static_cast<int64_t>(first + s) * p.width + v] = fromFloat<T>(first + s < live ? h[v] : 0.f);
+        }
     }
+    if (p.finalState)
+        for (int v = 0; v < count; ++v) p.finalState[row + v] = h[v];
 }
 
 // Words and ticket of a chain.
@@ -239,16 +255,18 @@ void launchForward(Pass &p, int type, cudaStream_t st) {
 }
 
 namespace {
-void launchStep(const Pass &p, int type, cudaStream_t st) {
+// Up to so many tokens one after another, when a tile's 64 or 128 would mostly be empty: 64 rows of 10 tokens of 1024 channels take WALK us here and 18.4 in tiles, of 16 tokens WALK16 and TILE16.
+constexpr int kWalk = 16;
+void launchWalk(const Pass &p, int type, cudaStream_t st) {
     const int pairs = (p.width - 1) / 2 + 1;
     const int64_t blocks = (static_cast<int64_t>(p.batch) * pairs + kThreads - 1) / kThreads;
     withType(type, [&](auto t) {
         using T = decltype(t);
         {
-            KernelTimer timer__("gatedStep", st);
-            launchDependent(p.input.data ? gatedStep<T, true> : gatedStep<T, false>, static_cast<unsigned>(blocks), kThreads, 0, st, p, pairs);
+            KernelTimer timer__("gatedWalk", st);
+            launchDependent(p.input.data ? gatedWalk<T, true> : gatedWalk<T, false>, static_cast<unsigned>(blocks), kThreads, 0, st, p, pairs);
         }
-        afterLaunch("gatedStep");
+        afterLaunch("gatedWalk");
     });
 }
 }  // namespace
@@ -290,7 +308,7 @@ extern "C" int rxmet_gated_recurrence_forward(const rxmet_gated_recurrence *prob
         p.finalState = final_state;
         p.marks = marks;
         const auto st = static_cast<cudaStream_t>(stream);
-        if (p.tokens == 1) return gated::launchStep(p, problem->type, st);
+        if (p.tokens <= gated::kWalk) return gated::launchWalk(p, problem->type, st);
         gated::startChain(p, workspace, workspace_bytes, st);
         gated::launchForward(p, problem->type, st);
     });

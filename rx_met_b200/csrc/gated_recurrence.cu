@@ -255,8 +255,9 @@ void launchForward(Pass &p, int type, cudaStream_t st) {
 }
 
 namespace {
-// Up to so many tokens one after another, when a tile's 64 or 128 would mostly be empty: 64 rows of 10 tokens of 1024 channels take WALK us here and 18.4 in tiles, of 16 tokens WALK16 and TILE16.
-constexpr int kWalk = 16;
+// Whether tokens go one after another.  A tile of 32 to 128 tokens is mostly empty then: with 64 rows of 2048 channels, 2048 tiles of which 296 run at once, 32 tokens take 19.5 us one by one and 27.6 in
+// tiles, 64 tokens 31.7 and 27.6; with few rows a token's latency counts: 4 rows of 512 channels take 13.3 us for 24 tokens one by one and 9.2 in tiles.
+bool walks(const Pass &p) { return p.tokens <= 8 || (p.tokens <= 32 && p.tiles >= 1024); }
 void launchWalk(const Pass &p, int type, cudaStream_t st) {
     const int pairs = (p.width - 1) / 2 + 1;
     const int64_t blocks = (static_cast<int64_t>(p.batch) * pairs + kThreads - 1) / kThreads;
@@ -308,7 +309,7 @@ extern "C" int rxmet_gated_recurrence_forward(const rxmet_gated_recurrence *prob
         p.finalState = final_state;
         p.marks = marks;
         const auto st = static_cast<cudaStream_t>(stream);
-        if (p.tokens <= gated::kWalk) return gated::launchWalk(p, problem->type, st);
+        if (gated::walks(p)) return gated::launchWalk(p, problem->type, st);
         gated::startChain(p, workspace, workspace_bytes, st);
         gated::launchForward(p, problem->type, st);
     });

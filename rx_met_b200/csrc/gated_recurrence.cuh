@@ -37,7 +37,7 @@ constexpr uint32_t kTensorBytes = kChannels * kWarps * (OWN ? 16 : 32);   // of 
 // either side waits for all that the thread has in flight.
 // The tiles come in groups of kGroup.  `parts` holds a tile's (A, B); `fronts` the state in front of a group, or, until that is known, the (A, B) of the whole group in front of it.  A state in front of
 // a tile is always that in front of its group, taken through the group's tiles one by one, and the next group's is always taken through the whole group at once, so that bits do not depend on who was
-// first.  65536 tokens of 512 channels are 512 tiles in a row: one tile at a time they took 486 us, with groups 60.
+// first.  65536 tokens of 512 channels are 512 tiles in a row: from tile to tile they took 335 us, in groups 81.
 struct Chain {
     unsigned *ticket;
     unsigned long long *parts;    // [slab][place in the chain][channels]

@@ -6,6 +6,7 @@
 // A pair of CTAs computes tiles of 256 input channels x 512 output channels, 64 tokens at a time; each CTA holds half of both operands.  The values of the codes serve two products, which fill the tensor
 // memory: with one (256 x 256) shared memory had 80 kB to move for a chunk of 512 cycles, 16384 tokens of 4096 x 4096 took 450 us.  dy arrives by TMA in the order in which the tensor cores read it
 // across its rows.  Sixteen warps load the codes, a few chunks ahead, and turn them into 16-bit values in that order: ten instructions for four codes.  The same warps store a tile's sums.
+// Bound: tensor cores: 16384 tokens of 4096 x 4096 bfloat16 354 us, 92 % of a library product's rate in 16 bits (1673 TFLOP/s), of which 1.73 rounds of tiles in two leave 86 %.
 // Few tiles leave SMs without work, so the tokens are cut into parts, whose sums another kernel adds up in their order.
 #include "kept_codes.cuh"
 

@@ -1,4 +1,6 @@
 """The gated mixer's plain forms agree with one another, and its entry points refuse what needs no GPU to be refused."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -81,3 +83,59 @@ def test_kept_codes_refuse_what_needs_no_gpu():
         kept_codes.gated_product(x, x, activation="tanh")
     with pytest.raises(RuntimeError, match="type"):
         kept_codes.values(kept._replace(dtype=torch.float64))
+
+
+class TokenTensor(C.Structure):
+    """``rxmet_token_tensor``."""
+    _fields_ = [("data", C.c_void_p), ("stride_b", C.c_int64), ("stride_t", C.c_int64)]
+
+
+class Problem(C.Structure):
+    """``rxmet_gated_recurrence``."""
+    _fields_ = [(n, C.c_int32) for n in ("batch", "tokens", "width", "type", "tanh_value")] + [(n, TokenTensor) for n in ("forget", "value", "input")] + [("lengths", C.c_void_p)]
+
+
+def library():
+    from rx_met_b200 import _cabi
+    lib = _cabi.load_library()
+    for name in ("rxmet_gated_recurrence_marks", "rxmet_gated_recurrence_workspace_bytes"):
+        getattr(lib, name).restype = C.c_size_t
+    return lib
+
+
+@pytest.mark.parametrize("sizes,message", [((1, 2 ** 30 + 1, 1, 0), b"tokens, at most"), ((2 ** 20, 2 ** 20, 2 ** 20, 1), b"runs of"), ((-1, 1, 1, 0), b"batch -1"), ((1, 1, 0, 0), b"width 0"),
+                                           ((1, 1, 1, 3), b"element type"), ((1, 40, 8, 0), b"null pointer")])
+def test_the_recurrence_refuses_sizes_that_it_cannot_place(sizes, message):
+    lib, none = library(), TokenTensor(None, 1, 1)
+    problem = Problem(*sizes, 0, none, none, none, None)
+    for call in (lambda: lib.rxmet_gated_recurrence_forward(C.byref(problem), None, None, None, None, None, C.c_size_t(0), None),
+                 lambda: lib.rxmet_gated_recurrence_backward(C.byref(problem), None, None, None, None, None, None, None, None, None, C.c_size_t(0), None)):
+        assert call() < 0 and message in lib.rxmet_last_error()
+
+
+def test_what_the_recurrence_asks_for():
+    """Marks of every tile but a sequence's first: 128 tokens of 16 bits, 64 beside an input gate, half of that of floats; a chain's words for tiles that wait for one another."""
+    lib, none, some = library(), TokenTensor(None, 1, 1), TokenTensor(16, 1, 1)
+    for kind, tile in ((1, 128), (2, 128), (0, 64)):
+        for own, gate in ((1, none), (2, some)):
+            for tokens in (0, 1, tile // own, tile // own + 1, 1000):
+                problem = Problem(3, tokens, 70, kind, 0, none, none, gate, None)
+                tiles = max(1, -(-tokens // (tile // own)))
+                assert lib.rxmet_gated_recurrence_marks(C.byref(problem)) == 3 * 70 * (tiles - 1)
+                groups = -(-tiles // 8)
+                words = 3 * 2 * (tiles + groups) * 64 * 8
+                assert lib.rxmet_gated_recurrence_workspace_bytes(C.byref(problem)) == (0 if tiles == 1 else -(-(words + 16) // 256) * 256)
+
+
+def test_kept_codes_refuse_rows_that_they_cannot_place():
+    lib = library()
+    one, far = C.c_int64(1), C.c_int64(1 << 40)
+    calls = [lambda: lib.rxmet_keep_codes(one, 131072, 1, None, one, None, one, None, None), lambda: lib.rxmet_keep_codes(one, 0, 1, None, one, None, one, None, None),
+             lambda: lib.rxmet_keep_codes(one, 8, 5, None, one, None, one, None, None), lambda: lib.rxmet_keep_codes(C.c_int64(2), 8, 1, C.c_void_p(16), far, C.c_void_p(16), C.c_int64(16), C.c_void_p(16), None),
+             lambda: lib.rxmet_keep_codes(C.c_int64(2), 8, 1, C.c_void_p(16), C.c_int64(8), C.c_void_p(16), C.c_int64(8), C.c_void_p(16), None),
+             lambda: lib.rxmet_gated_product(one, 8, 1, 4, C.c_void_p(16), one, C.c_void_p(16), one, C.c_void_p(16), None, None, None, None, one, None),
+             lambda: lib.rxmet_kept_weight_gradient(one, 131072, 8, 1, None, one, None, one, None, 0, None, None, C.c_size_t(0), None),
+             lambda: lib.rxmet_kept_weight_gradient(far, 8, 8, 1, None, one, None, one, None, 0, None, None, C.c_size_t(0), None)]
+    messages = [b"at most 131071", b"of 0 elements", b"element type", b"elements apart", b"16 bytes", b"activation", b"at most", b"at most"]
+    for call, message in zip(calls, messages):
+        assert call() < 0 and message in lib.rxmet_last_error(), (message, lib.rxmet_last_error())

@@ -213,13 +213,13 @@ struct Rows {
     }
     // The stage asked for first has arrived, before a barrier of all threads; `parity` changes with every tile that had live tokens.
     __device__ __forceinline__ bool arrived(const Tile &tile, uint32_t parity) const {
-        if constexpr (COPY == Copy::Boxes) return tile.live == 0 || umma::waitPhase(umma::smemAddr(bar), parity);
+        if constexpr (COPY == Copy::Boxes) return tile.live == 0 || umma::waitSuspended(umma::smemAddr(bar), parity);
         else copiesArrived<1>();
         return true;
     }
 };
 
-// A tile of an output from shared memory, by one thread; what lies beyond the array is left out.  Those that it began have been read once `stored` returns.
+// A tile of an output from shared memory, by one thread; what lies beyond the array is left out.  Those that it began have been read once storesRead() returns.
 __device__ __forceinline__ void storeBox(const CUtensorMap *map, uint32_t from, const Tile &tile) {
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(tile.d0), "r"(tile.first), "r"(tile.b), "r"(from) : "memory");
 }

@@ -14,7 +14,7 @@ namespace gated {
 namespace {
 
 template <class T, Copy COPY, bool OWN, bool TANH>
-__global__ void __launch_bounds__(kThreads, OWN ? 3 : 2) gatedBackward(const __grid_constant__ Pass p) {
+__global__ void __launch_bounds__(kThreads, 2) gatedBackward(const __grid_constant__ Pass p) {
     constexpr int S = kSteps<T, OWN>, kTensors = OWN ? 4 : 3;
     constexpr uint32_t kStageBytes = kTensors * kTensorBytes<OWN>;
     extern __shared__ __align__(128) uint8_t stages[];

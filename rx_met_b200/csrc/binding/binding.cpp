@@ -1003,7 +1003,6 @@ struct GatedProduct : torch::autograd::Function<GatedProduct> {
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({held.begin(), held.end()});
         ctx->saved_data["activation"] = activation;
-        ctx->saved_data["type"] = static_cast<int64_t>(a.gate.type);
         return {y};
     }
 

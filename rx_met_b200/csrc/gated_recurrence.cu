@@ -136,12 +136,13 @@ template <class T, bool OWN>
 __global__ void __launch_bounds__(kThreads) gatedWalk(const __grid_constant__ Pass p, const int pairsOfRow) {
     constexpr int kAtOnce = 4;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-    const int b = static_cast<int>(i / pairsOfRow), d = 2 * static_cast<int>(i - static_cast<int64_t>(b) * pairsOfRow);
+    const int64_t b = i / pairsOfRow;   // beyond 32 bits behind the last of 2^31 - 1 rows
+    const int d = 2 * static_cast<int>(i - b * pairsOfRow);
     waitForPredecessor();
     letDependentsStart();
     if (b >= p.batch) return;
     const int live = p.lengths ? min(max(p.lengths[b], 0), p.tokens) : p.tokens;
-    const int64_t row = static_cast<int64_t>(b) * p.width + d;
+    const int64_t row = b * p.width + d;
     const int count = min(2, p.width - d);
     const int second = count - 1;   // of a row's last channel by itself, the same one twice
     float h[2];
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(kThreads) gatedWalk(const __grid_constant__ Pa
         to[0] = from[0];
         to[1] = from[second];
     };
-    T *to = static_cast<T *>(p.out) + static_cast<int64_t>(b) * p.tokens * p.width + d;
+    T *to = static_cast<T *>(p.out) + b * p.tokens * p.width + d;
     for (int first = 0; first < p.tokens; first += kAtOnce) {
         alignas(8) T forget[kAtOnce][2], value[kAtOnce][2], input[kAtOnce][2];
 #pragma unroll

@@ -334,6 +334,17 @@ def test_a_captured_training_step():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_as_many_rows_as_there_can_be():
+    """One more row than a batch may have does not fit into 32 bits, and the last block has threads for it."""
+    rows = 2 ** 31 - 1
+    forget, value = torch.zeros(rows, 1, device="cuda", dtype=torch.float16), torch.ones(rows, 1, device="cuda", dtype=torch.float16)
+    state = torch.zeros(rows, 1, device="cuda")
+    out = gated_recurrence_step(forget, value, state)
+    assert all(t.amin().item() == 0.5 and t.amax().item() == 0.5 for t in (out, state))   # h = 0 / 2 + 1 / 2
+    del forget, value, state, out
+    torch.cuda.empty_cache()
+
+
 def test_refusals():
     from rx_met_b200.gated_recurrence import gated_recurrence, gated_recurrence_step
     x = torch.zeros(2, 8, 16, device="cuda", dtype=torch.bfloat16)

@@ -31,7 +31,7 @@ typedef struct rxmet_gated_recurrence {
 RXMET_API size_t rxmet_gated_recurrence_marks(const rxmet_gated_recurrence *problem);
 RXMET_API size_t rxmet_gated_recurrence_workspace_bytes(const rxmet_gated_recurrence *problem);
 /* out [batch][tokens][width] in the inputs' type (null: not wanted); state [batch][width] in 32 bits, null for zeros; final_state the same, may be null, may be
- * `state` itself; marks null where there will be no backward pass. */
+ * `state` itself for up to 32 tokens (more are refused); marks null where there will be no backward pass. */
 RXMET_API int rxmet_gated_recurrence_forward(const rxmet_gated_recurrence *problem, const float *state_dev, void *out_dev, float *final_state_dev,
                                              float *marks_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
 /* Gradients of forget, value, input (contiguous) and state, each null where it is not wanted, from those of out and of the final state (null, or

@@ -307,6 +307,8 @@ extern "C" int rxmet_gated_recurrence_forward(const rxmet_gated_recurrence *prob
         RXMET_REQUIRE(problem, "gated_recurrence: null pointer");
         gated::Pass p = gated::passOf(*problem);
         gated::requireData(*problem, p.tiles);
+        // A sequence's last tile may be done before all warps of its first one have read where it starts; a CTA's own barriers keep the two of one tile apart.
+        RXMET_REQUIRE(!state || state != final_state || p.tokens <= 32, "gated_recurrence: the final state of %d tokens in the place of the state, at most 32", p.tokens);
         if (p.tiles == 0) return;
         p.state = state;
         p.out = out;

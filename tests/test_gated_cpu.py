@@ -113,6 +113,15 @@ def test_the_recurrence_refuses_sizes_that_it_cannot_place(sizes, message):
         assert call() < 0 and message in lib.rxmet_last_error()
 
 
+@pytest.mark.parametrize("tokens", [33, 64, 1000])
+def test_the_recurrence_refuses_the_final_state_of_many_tokens_in_the_place_of_the_state(tokens):
+    """A sequence's first tile may still be reading the state when its last one is done."""
+    lib, none, some, state = library(), TokenTensor(None, 1, 1), TokenTensor(16, 8 * tokens, 8), C.c_void_p(16)
+    problem = Problem(1, tokens, 8, 1, 0, some, some, none, None)
+    assert lib.rxmet_gated_recurrence_forward(C.byref(problem), state, C.c_void_p(16), state, None, None, C.c_size_t(0), None) < 0
+    assert b"in the place of the state" in lib.rxmet_last_error()
+
+
 def test_what_the_recurrence_asks_for():
     """Marks of every tile but a sequence's first: 128 tokens of 16 bits, 64 beside an input gate, half of that of floats; a chain's words for tiles that wait for one another."""
     lib, none, some = library(), TokenTensor(None, 1, 1), TokenTensor(16, 1, 1)

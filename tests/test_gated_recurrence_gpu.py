@@ -336,6 +336,7 @@ def test_a_captured_training_step():
 
 def test_as_many_rows_as_there_can_be():
     """One more row than a batch may have does not fit into 32 bits, and the last block has threads for it."""
+    from rx_met_b200.gated_recurrence import gated_recurrence_step
     rows = 2 ** 31 - 1
     forget, value = torch.zeros(rows, 1, device="cuda", dtype=torch.float16), torch.ones(rows, 1, device="cuda", dtype=torch.float16)
     state = torch.zeros(rows, 1, device="cuda")
